@@ -453,6 +453,7 @@ int vtx_indexer_quest_fused_supported(int32_t head_dim, int32_t group_size);
 /* Output element types. */
 #define VTX_DTYPE_BF16 0
 #define VTX_DTYPE_F32 1
+#define VTX_DTYPE_F16 2
 
 /*
  * Page-finish reduction (CMean / CMax / CMin / CL2Norm).
@@ -635,6 +636,36 @@ int vtx_bf16_rounding_check(unsigned long long* counts, void* stream);
 int vtx_set_kv_buffer(void* k_cache, void* v_cache, int64_t cache_rows, const void* new_k,
                       const void* new_v, const int64_t* loc, int64_t nnz, int32_t num_kv_heads,
                       int32_t head_dim, int32_t elem_bytes, int32_t page_size, void* stream);
+
+/*
+ * vtx_set_kv_buffer with the position rotation on the way, and the queries'
+ * with it.  Token i < nnz takes row positions[i] of the table cos_sin
+ * ([table_rows, rotary_dim] fp32: rotary_dim / 2 cosines, then as many sines)
+ * and rotates its query and key rows in pairs j < rotary_dim / 2,
+ *   a' = a cos_j - b sin_j,  b' = b cos_j + a sin_j
+ * with (a, b) = columns (j, j + rotary_dim / 2), or (2j, 2j + 1) where
+ * interleaved; columns from rotary_dim on stay.  fp32, one rounding.  Queries
+ * go to q_out, keys and (unrotated) values to pool row
+ *   (loc / page_size) * (page_size * H) + h * page_size + loc % page_size
+ * of k_cache / v_cache ([pages * H, page_size, head_dim], dense).  A token
+ * whose pool row lies outside the pool (a negative loc: padding) stores no key
+ * or value; one whose position lies outside the table is skipped, its q_out
+ * rows left as they were.  Tokens that share a slot leave either's values there.
+ * dtype: the rows' and the pools' (VTX_DTYPE_BF16, _F16 or _F32).  strides:
+ * host array of eight, in elements: token and head strides of q, q_out, new_k
+ * and new_v, whose rows are dense (slices of one projection's output, for
+ * example).  q_out may be q with the same strides; other overlaps of outputs
+ * with inputs are not allowed.  q_heads 0: no queries (q and q_out NULL).
+ * Rows, strides and pointers of multiples of 16 bytes (and as much for half of
+ * rotary_dim, or for all of it where interleaved) take 16-byte accesses, others
+ * element-wide ones.
+ * No counterpart in the reference, whose runtime rotates before it stores.
+ */
+int vtx_set_kv_buffer_rope(void* k_cache, void* v_cache, int64_t cache_rows, const void* q, void* q_out,
+                           const void* new_k, const void* new_v, const int64_t* strides, const int64_t* loc,
+                           const int64_t* positions, const float* cos_sin, int64_t table_rows, int64_t nnz,
+                           int32_t q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                           int32_t dtype, int32_t page_size, int32_t interleaved, void* stream);
 
 /*
  * Paged decode attention over a block table (the consumer of the sparse

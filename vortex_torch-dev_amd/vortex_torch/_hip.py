@@ -123,6 +123,11 @@ _SIGNATURES = {
         [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp],
         ctypes.c_int,
     ),
+    "vtx_set_kv_buffer_rope": (
+        [_vp, _vp, _i64, _vp, _vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32,
+         _i32, _i32, _i32, _vp],
+        ctypes.c_int,
+    ),
     "vtx_paged_decode_attention": (
         [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp],
         ctypes.c_int,
@@ -148,7 +153,7 @@ EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 REDUCE_MEAN, REDUCE_MAX, REDUCE_MIN, REDUCE_L2NORM, REDUCE_SUM = 0, 1, 2, 3, 4
 ROWS_BATCHED, ROWS_PAGED, ROWS_RAGGED = 0, 1, 2
 SEGMENT_SOFTMAX, SEGMENT_NORMALIZE = 0, 1
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_F16 = 0, 1, 2
 FUSED_AUTO, FUSED_SEGMENT, FUSED_SPLIT = 0, 1, 2
 
 
@@ -1019,6 +1024,123 @@ def set_kv_buffer(k_cache, v_cache, new_k, new_v, loc, page_size: int) -> None:
                                    new_v.data_ptr(), loc.data_ptr(), nnz, H, D, new_k.element_size(),
                                    int(page_size), _stream(dev))
     _check(rc, "set_kv_buffer")
+
+
+_ROPE_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32, torch.float16: DTYPE_F16}
+_EightI64 = _i64 * 8
+
+
+def _span(t: torch.Tensor) -> tuple:
+    """First byte and byte past the last of a [tokens, heads, head_dim] tensor of dense rows."""
+    n, h, d = t.shape
+    first, size = t.data_ptr(), t.element_size()
+    if n == 0 or h == 0:
+        return first, first
+    return first, first + size * ((n - 1) * t.stride(0) + (h - 1) * t.stride(1) + d)
+
+
+def _tokens_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [tokens, heads, head_dim] tensors share no memory: apart as
+    a whole, or column ranges of the same rows (slices of one projection)."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    if a.shape[0] < 2 or b.shape[0] < 2 or a.stride(0) != b.stride(0) or a.element_size() != b.element_size():
+        return False
+    size, step = a.element_size(), a.element_size() * a.stride(0)
+    wide_a, wide_b = (size * ((t.shape[1] - 1) * t.stride(1) + t.shape[2]) for t in (a, b))
+    off = (b0 - a0) % step if step > 0 else 0
+    return wide_a <= off and off + wide_b <= step
+
+
+def _rows_distinct(t: torch.Tensor) -> bool:
+    """Whether no two rows of a [tokens, heads, head_dim] tensor of dense rows meet."""
+    n, h, d = t.shape
+    ts, hs = t.stride(0), t.stride(1)
+    if n == 1 or h == 1:
+        return (n == 1 or ts >= d) and (h == 1 or hs >= d)
+    return (hs >= d and ts >= (h - 1) * hs + d) or (ts >= d and hs >= (n - 1) * ts + d)
+
+
+@_plain_args
+def set_kv_buffer_rope(k_cache, v_cache, q, new_k, new_v, loc, page_size: int, positions, cos_sin_cache,
+                       interleaved: bool = False, q_out=None):
+    """set_kv_buffer with the position rotation of q [nnz, Hq, D] (or None) and
+    new_k on the way; returns the rotated queries (q_out, or a new tensor)."""
+    lib = load_library()
+    given = q_out is not None
+    if q is None and given:
+        raise RuntimeError("vortex_torch: q_out without q")
+    tensors = [k_cache, v_cache, new_k, new_v, loc, positions, cos_sin_cache]
+    if q is not None:
+        tensors.append(q)
+    if given:
+        tensors.append(q_out)
+    dev = _require_gpu(*tensors)
+    _req(loc, torch.int64, "loc")
+    _req(positions, torch.int64, "positions")
+    _req(cos_sin_cache, torch.float32, "cos_sin_cache")
+    if new_k.dim() != 3 or new_v.shape != new_k.shape:
+        raise RuntimeError("vortex_torch: new_k and new_v must both be [nnz, num_kv_heads, head_dim]")
+    dtype = new_k.dtype
+    if dtype not in _ROPE_DTYPES:
+        raise RuntimeError(f"vortex_torch: new_k must be bfloat16, float16 or float32, got {dtype}")
+    nnz, H, D = new_k.shape
+    named = [(k_cache, "k_cache"), (v_cache, "v_cache"), (new_v, "new_v")]
+    Hq = 0
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != nnz or q.shape[2] != D:
+            raise RuntimeError(f"vortex_torch: q must be [{nnz}, q_heads, {D}], got {tuple(q.shape)}")
+        Hq = q.shape[1]
+        named.append((q, "q"))
+        if given:
+            if q_out.shape != q.shape:
+                raise RuntimeError(f"vortex_torch: q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
+            named.append((q_out, "q_out"))
+    for t, n in named:
+        if t.dtype != dtype:
+            raise RuntimeError(f"vortex_torch: {n} is {t.dtype}, new_k is {dtype}")
+    for t, n in [(new_k, "new_k")] + named[2:]:
+        if D > 1 and t.stride(2) != 1:
+            raise RuntimeError(f"vortex_torch: {n} must have dense rows (a last stride of 1)")
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise RuntimeError("vortex_torch: k_cache and v_cache must be contiguous")
+    if k_cache.dim() != 3 or k_cache.shape != v_cache.shape or k_cache.shape[2] != D or k_cache.shape[1] != page_size:
+        raise RuntimeError(f"vortex_torch: k_cache and v_cache must be [pages * H, {page_size}, {D}]")
+    if k_cache.shape[0] % max(H, 1):
+        raise RuntimeError(f"vortex_torch: the pools' {k_cache.shape[0]} rows are not pages of {H} kv heads")
+    if loc.numel() < nnz or positions.numel() < nnz:
+        raise RuntimeError("vortex_torch: loc or positions shorter than the new tokens")
+    if cos_sin_cache.dim() != 2:
+        raise RuntimeError("vortex_torch: cos_sin_cache must be [positions, rotary_dim]")
+    kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
+    pool = k_cache.numel() * k_cache.element_size()
+    if pool and -pool < kp - vp < pool:
+        raise RuntimeError("vortex_torch: k_cache and v_cache share memory")
+    for t, n in [(new_k, "new_k")] + named[2:]:
+        p = t.data_ptr()
+        if kp <= p < kp + pool or vp <= p < vp + pool:
+            raise RuntimeError(f"vortex_torch: {n} lies in the pools that the call writes")
+    if q is not None:
+        if not given:
+            q_out = torch.empty((nnz, Hq, D), dtype=dtype, device=dev)
+        elif nnz and Hq:
+            if not _rows_distinct(q_out):
+                raise RuntimeError("vortex_torch: q_out has rows that share memory")
+            in_place = q_out.data_ptr() == q.data_ptr() and q_out.stride() == q.stride()
+            for t, n in ((q, "q"), (new_k, "new_k"), (new_v, "new_v")):
+                if not (in_place and t is q) and not _tokens_apart(q_out, t):
+                    raise RuntimeError(f"vortex_torch: q_out shares memory with {n}")
+    strides = _EightI64(*(q.stride()[:2] if Hq else (0, 0)), *(q_out.stride()[:2] if Hq else (0, 0)),
+                        *new_k.stride()[:2], *new_v.stride()[:2])
+    with _on_device(dev):
+        rc = lib.vtx_set_kv_buffer_rope(
+            kp, vp, k_cache.shape[0] * k_cache.shape[1], q.data_ptr() if Hq else None,
+            q_out.data_ptr() if Hq else None, new_k.data_ptr(), new_v.data_ptr(), strides, loc.data_ptr(),
+            positions.data_ptr(), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], nnz, Hq, H, D,
+            cos_sin_cache.shape[1], _ROPE_DTYPES[dtype], int(page_size), 1 if interleaved else 0, _stream(dev))
+    _check(rc, "set_kv_buffer_rope")
+    return q_out
 
 
 def _scratch(floats: int, dev: torch.device, stream: int):
