@@ -716,6 +716,49 @@ int64_t vtx_paged_decode_attention_workspace_len(int32_t batch_size, int32_t num
 int vtx_paged_decode_attention_supported(int32_t head_dim, int32_t group_size);
 
 /*
+ * Planner of vtx_shared_prefix_decode_attention: which requests of a block
+ * table share leading pages, and how the attention's work is divided; once per
+ * table, for every layer that reads it.  Per kv head, consecutive requests with
+ * pages form a run while their group_ids ([B] int32) are equal; group_ids NULL:
+ * while their first entries are equal.  A run of several requests shares its
+ * longest common prefix of entries, less than each one's page count (a request
+ * keeps its last page to itself); a run of one shares nothing.  A segment whose
+ * range lies outside kv_indices counts as empty and ends a run.
+ * plan: vtx_shared_prefix_plan_len int32, 32-byte aligned.  With S = B * H,
+ * plan[16 + s] receives the first request of segment s's run and
+ * plan[16 + (S rounded up to 8) + s] the pages it shares; the rest is the
+ * attention's.  No counterpart in the reference.
+ */
+int64_t vtx_shared_prefix_plan_len(int32_t batch_size, int32_t num_kv_heads, int32_t group_size, int32_t head_dim);
+int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* kv_indices, int64_t kv_indices_len,
+                           const int32_t* group_ids, int32_t batch_size, int32_t num_kv_heads, int32_t group_size,
+                           int32_t head_dim, int32_t page_size, int32_t* plan, int64_t plan_len, void* stream);
+
+/*
+ * vtx_paged_decode_attention's result over the block table that `plan` was made
+ * of (with the same sizes), every shared page read once for its run instead of
+ * once for each request, and the scores and outputs on the matrix cores: the
+ * probabilities are rounded to bf16 (and sum to one as rounded), the rest is
+ * fp32.  A NaN score gives NaN (there: zeros).  kv_last_page_len may have changed since the plan was made; after any
+ * other change of the table plan anew (the results are undefined otherwise, but
+ * no access leaves a buffer).  workspace: vtx_shared_prefix_workspace_len
+ * floats, 16-byte aligned, its contents neither read nor kept across calls;
+ * calls that may overlap need one each.  A request's last bits depend on the
+ * other requests of the table (how its tokens are divided).
+ * head_dim 64, 128 or 256; group_size 1..8; at most 2^24 segments and 2^32
+ * pool tokens (pool rows x page_size).
+ */
+int64_t vtx_shared_prefix_workspace_len(int32_t batch_size, int32_t num_kv_heads, int32_t group_size,
+                                        int32_t head_dim);
+int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o, const uint16_t* k_cache,
+                                       const uint16_t* v_cache, int64_t cache_rows, const int32_t* kv_indptr,
+                                       const int32_t* kv_indices, int64_t kv_indices_len,
+                                       const int32_t* kv_last_page_len, const int32_t* plan, int64_t plan_len,
+                                       int32_t batch_size, int32_t num_kv_heads, int32_t group_size,
+                                       int32_t head_dim, int32_t page_size, float sm_scale, float* workspace,
+                                       int64_t workspace_len, void* stream);
+
+/*
  * Bandwidth probes (measurement only; no counterpart in the reference).
  * vtx_probe_read reads `bytes` of src sequentially (16-byte nontemporal
  * loads, grid-stride over four 512-thread workgroups per compute unit).

@@ -1,0 +1,550 @@
+// Decode attention for requests that share leading pages, for gfx950: the
+// result of paged decode attention over the same block table, with a shared
+// page read once for all requests of its run instead of once for each.
+//
+// For a query row and the tokens t of its segment,
+//   o = sum_t p_t V[t] / sum_t p_t,  p_t = 2^(c q.K[t] - m),  c = scale log2 e
+// over any partition of the tokens into chunks, each with its own m, the joint
+// sums follow from the chunks' (m, sum p, sum p V) weighted by 2^(m - max m).
+// So the plan's items (vtx_shared_prefix.h) are independent: the rows of a run
+// against a chunk of its shared pages, or those of a request against a chunk
+// of its own; a second launch joins the partial results (fp32).
+//
+// Both products run on the matrix cores (v_mfma_f32_32x32x16_bf16), transposed
+// so that a lane holds one query row: S^T = K Q^T (32 tokens x 32 rows per
+// step, fp32) leaves lane l with row l % 32 and half of the 32 tokens, so the
+// softmax is in the lane but for one exchange of halves; rounded to bf16, those
+// registers are the B operand of O^T = V^T P^T as they stand, if V^T's tokens
+// are taken in the same order, which is the transposing LDS read's addressing.
+// P is rounded to bf16 for the matrix cores; the sums are taken of the rounded
+// values, so the weights sum to one and a mean of V is not shifted.
+//
+// 4 waves.  Up to 32 rows (a request's own pages): every wave takes tiles of 32
+// tokens of its own.  More: tiles of 64 tokens for all waves, of which each
+// takes 32 rows (or 32 rows and 32 tokens where there are up to 64 rows), two
+// buffers.  K and V go through registers to LDS, requested one tile ahead.
+#include "vtx_shared_prefix.h"
+
+#include "vtx_device.h"
+#include "vtx_host.h"
+
+namespace {
+
+using namespace vtx_prefix;
+
+struct SharedArgs {
+  const uint16_t* q;
+  uint16_t* o;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t rows;  // pool rows (page * H + h)
+  const int32_t* indptr;
+  const int32_t* indices;
+  int64_t indices_len;
+  const int32_t* last_len;
+  const int32_t* head;     // plan header
+  const Item* items;
+  const int32_t* combine;  // [segments][kCombineInts]
+  int32_t max_items;
+  int32_t B, H, G, P, p_shift;
+  float c;          // |scale| log2 e, or 1 for a scale of 0
+  uint32_t q_sign;  // flips the queries' signs for a negative scale
+  uint32_t q_keep;  // 0 for a scale of 0: no scores
+  float* acc;       // [max_rows, D]
+  float2* ml;       // [max_rows]
+  int64_t max_rows;
+};
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// LDS rows of a tile are kD bf16 in 16-byte pieces; piece c of token t lies at
+// c ^ swizzle(t), so that the 8 (or 16) tokens of a K read, at one c, and the
+// 8 tokens x 4 pieces of a transposing V read spread over all banks.
+template <int kD>
+__device__ __forceinline__ int swizzle(int t) {
+  if constexpr (kD == 64) return (((t >> 1) & 1) << 2) | (((t >> 2) & 1) << 1) | ((t >> 3) & 1);
+  return ((t & 3) << 2) | ((t >> 2) & 3);
+}
+
+// Orders a wave's LDS accesses around it (its lanes read what others wrote;
+// the hardware keeps a wave's LDS operations in order).
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A wave's 32 query rows: their fragments, running maximum (scaled, base 2),
+// sum (this lane's half of the tokens) and output.
+template <int kD>
+struct Rows {
+  vtx::U4 q[kD / 16];
+  float m, l;
+  f32x16 o[kD / 32];
+};
+
+// kN x 32 tokens at kt / vt in LDS; bit i of mask: token i counts.
+template <int kD, int kN>
+__device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, const unsigned char* vt, uint64_t mask,
+                                       float c) {
+  constexpr int kRow = kD * 2;
+  const int lane = vtx::lane_id(), r = lane % 32, half = lane / 32;
+  f32x16 s[kN];
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
+  const int ksw = swizzle<kD>(r);
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int kk = 0; kk < kD / 16; ++kk) {
+      const vtx::U4 f = vtx::ld16(kt + (n * 32 + r) * kRow + (((2 * kk + half) ^ ksw) << 4));
+      s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, w.q[kk]),
+                                                     s[n], 0, 0, 0);
+    }
+  constexpr uint64_t kAll = kN == 2 ? ~0ull : 0xffffffffull;
+  if ((mask & kAll) != kAll) {  // uniform
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!((mask >> (n * 32 + 8 * (i / 4) + 4 * half + i % 4)) & 1)) s[n][i] = -INFINITY;
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+  mx = fmaxf(mx, vtx::xshfl(mx, 32)) * c;
+  if (__ballot(mx > w.m)) {  // uniform
+    const float nm = fmaxf(w.m, mx);
+    const float f = nm == -INFINITY ? 1.f : exp2_fast(w.m - nm);
+    w.l *= f;
+#pragma unroll
+    for (int d = 0; d < kD / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w.o[d][i] *= f;
+    w.m = nm;
+  }
+  const float base = w.m == -INFINITY ? 0.f : w.m;
+  uint32_t p[kN][8];
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[n][i] = vtx::bf16_pair(exp2_fast(fmaf(s[n][2 * i], c, -base)), exp2_fast(fmaf(s[n][2 * i + 1], c, -base)));
+      w.l = vtx::dot2_bf16(p[n][i], 0x3f803f80u, w.l);
+    }
+  // V^T: 16 lanes take 4 tokens x 16 columns per read
+  typedef __attribute__((address_space(3))) s16x4 lds4;
+  const int g16 = lane / 16, i16 = lane % 16;
+  const int vrow = 4 * half + i16 / 4;
+  const int vcol = (g16 & 1) * 2 + (i16 % 4) / 2;
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const vtx::U4 b = vtx::U4{p[n][4 * kk], p[n][4 * kk + 1], p[n][4 * kk + 2], p[n][4 * kk + 3]};
+#pragma unroll
+      for (int d = 0; d < kD / 32; ++d) {
+        s16x4 f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int t = vrow + 8 * e;  // (+ 32 n + 16 kk, which the swizzle does not see)
+          const unsigned char* at =
+              vt + (n * 32 + kk * 16 + t) * kRow + (((d * 4 + vcol) ^ swizzle<kD>(t)) << 4) + (i16 % 2) * 8;
+          f[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
+        }
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 a = __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                         w.o[d], 0, 0, 0);
+      }
+    }
+}
+
+// The tokens of an item: where they lie in the table, and how many.
+struct Tokens {
+  const int32_t* pages;
+  int count;
+};
+
+// Pool token row (page row * P + slot) of token t, and whether it exists and
+// lies inside the pool; 0 (a valid row) where it does not.  In two steps, the
+// table entry requested a tile before it is needed.
+struct Entry {
+  int page, slot;  // page: the table's entry, -1 past the last token
+};
+__device__ __forceinline__ Entry entry_of(const SharedArgs& a, const Tokens& tk, int t) {
+  Entry e{-1, 0};
+  if (t < tk.count) {
+    const int pg = a.p_shift >= 0 ? t >> a.p_shift : t / a.P;
+    e.slot = t - pg * a.P;
+    e.page = tk.pages[pg];
+  }
+  return e;
+}
+__device__ __forceinline__ bool resolve(const SharedArgs& a, const Entry& e, uint32_t& row) {
+  const bool ok = e.page >= 0 && e.page < a.rows;
+  row = ok ? (uint32_t)e.page * (uint32_t)a.P + (uint32_t)e.slot : 0u;
+  return ok;
+}
+
+template <int kD>
+constexpr int kMinBlocks = kD == 64 ? 3 : (kD == 128 ? 2 : 1);
+
+template <int kD>
+__global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attention_kernel(SharedArgs a) {
+  constexpr int kRow = kD * 2;
+  constexpr int kPieces = kD / 8;
+  __shared__ alignas(16) unsigned char s_tile[256 * kRow];  // two buffers of 64 tokens, or four of 32; then the rows' outputs
+  __shared__ float s_m[kWaves][32];
+  __shared__ float s_l[kWaves][32];
+
+  const int run_items = a.head[kHeadRunItems], items = run_items + a.head[kHeadOwnItems];
+  if ((int)blockIdx.x >= items || items > a.max_items) return;  // uniform
+  const Item it = a.items[blockIdx.x];
+  const int tid = threadIdx.x, lane = vtx::lane_id();
+  const int wave = vtx::uniform(tid / vtx::kWave);
+  const int seg = vtx::uniform(it.segment), S = a.B * a.H;
+  if (seg < 0 || seg >= S) return;
+  const int b0 = seg / a.H, h = seg - b0 * a.H;
+  const int rows = min(max(it.rows, 0), kTileRows);
+
+  // the item's tokens, within what the table holds now
+  Tokens tk{nullptr, 0};
+  {
+    const int start = a.indptr[seg];
+    const long long end = a.indptr[seg + 1];
+    const int n = start >= 0 && end > start && end <= a.indices_len && a.rows > 0 ? (int)(end - start) : 0;
+    const int p0 = max(it.page0, 0), p1 = min(it.page1, n);
+    if (p1 > p0) {
+      const int ll = a.last_len[seg], last = ll < 0 ? 0 : (ll > a.P ? a.P : ll);
+      const long long t = (long long)(p1 - p0 - 1) * a.P + (p1 == n ? last : a.P);
+      tk.pages = a.indices + start + p0;
+      tk.count = (int)(t < 0x3fffffff ? t : 0x3fffffff);
+    }
+  }
+
+  const int wr = rows > 64 ? 4 : (rows > 32 ? 2 : 1);  // blocks of 32 rows, a power of two
+  const int rb = wave % wr, tb = wave / wr, wt = kWaves / wr;
+  Rows<kD> w;
+  w.m = -INFINITY;
+  w.l = 0.f;
+#pragma unroll
+  for (int d = 0; d < kD / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w.o[d][i] = 0.f;
+  {
+    const int r = rb * 32 + lane % 32, at = it.row0 + r;
+    const int b = b0 + at / a.G, g = at % a.G;
+    const bool ok = r < rows && at >= 0 && b < a.B;
+    const uint16_t* q = a.q + (((long long)(ok ? b : b0) * a.H + h) * a.G + (ok ? g : 0)) * kD + (lane / 32) * 8;
+    const uint32_t keep = ok ? a.q_keep : 0u;
+#pragma unroll
+    for (int kk = 0; kk < kD / 16; ++kk) {
+      const vtx::U4 x = vtx::ld16(q + kk * 16);
+      w.q[kk] = vtx::U4{(x.x & keep) ^ a.q_sign, (x.y & keep) ^ a.q_sign, (x.z & keep) ^ a.q_sign,
+                        (x.w & keep) ^ a.q_sign};
+    }
+  }
+
+  if (wr == 1) {  // uniform: tiles of 32 tokens, wave w those of index w, w + 4, ...
+    constexpr int kPass = vtx::kWave / kPieces;  // tokens per wave-wide load
+    constexpr int kLoads = 32 / kPass;
+    unsigned char* kt = s_tile + wave * 64 * kRow;
+    unsigned char* vt = kt + 32 * kRow;
+    const int piece = lane % kPieces, sub = lane / kPieces;
+    const int tiles = (tk.count + 31) / 32;
+    const int n = tiles > wave ? (tiles - wave + kWaves - 1) / kWaves : 0;
+    vtx::U4 kr[kLoads], vr[kLoads];
+    uint64_t next_mask = 0;
+    Entry e = entry_of(a, tk, n > 0 ? wave * 32 + lane % 32 : 0x7fffffff);
+    auto request = [&](int j) {  // tile j's rows, and the entries of tile j + 1
+      uint32_t row;
+      const bool ok = resolve(a, e, row);
+      next_mask = __ballot(ok) & 0xffffffffull;
+      e = entry_of(a, tk, j + 1 < n ? (wave + kWaves * (j + 1)) * 32 + lane % 32 : 0x7fffffff);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t tr = (uint32_t)__shfl((int)row, i * kPass + sub);
+        kr[i] = vtx::ld16_stream(a.k + (uint64_t)tr * kD + piece * 8);
+        vr[i] = vtx::ld16_stream(a.v + (uint64_t)tr * kD + piece * 8);
+      }
+    };
+    if (n > 0) request(0);
+    for (int j = 0; j < n; ++j) {
+      const uint64_t mask = next_mask;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int t = i * kPass + sub;
+        const int at = t * kRow + ((piece ^ swizzle<kD>(t)) << 4);
+        const uint32_t live = (mask >> t) & 1 ? ~0u : 0u;  // (what lies in a masked row may be NaN)
+        vtx::st16(kt + at, kr[i]);
+        vtx::st16(vt + at, vtx::U4{vr[i].x & live, vr[i].y & live, vr[i].z & live, vr[i].w & live});
+      }
+      wave_lds_fence();
+      if (j + 1 < n) request(j + 1);
+      attend<kD, 1>(w, kt, vt, mask, a.c);
+      wave_lds_fence();
+    }
+  } else {  // uniform: tiles of 64 tokens for all waves
+    constexpr int kPass = kThreads / kPieces;
+    constexpr int kLoads = 64 / kPass;
+    const int piece = tid % kPieces, sub = tid / kPieces;
+    const int tiles = (tk.count + 63) / 64;
+    const bool busy = rb * 32 < rows;
+    vtx::U4 kr[kLoads], vr[kLoads];
+    uint64_t next_mask = 0;
+    Entry e = entry_of(a, tk, lane);
+    auto request = [&](int j) {
+      uint32_t row;
+      const bool ok = resolve(a, e, row);
+      next_mask = __ballot(ok);
+      e = entry_of(a, tk, (j + 1) * 64 + lane);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t tr = (uint32_t)__shfl((int)row, i * kPass + sub);
+        kr[i] = vtx::ld16(a.k + (uint64_t)tr * kD + piece * 8);
+        vr[i] = vtx::ld16(a.v + (uint64_t)tr * kD + piece * 8);
+      }
+    };
+    auto put = [&](int j) {
+      unsigned char* kt = s_tile + (j & 1) * 128 * kRow;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int t = i * kPass + sub;
+        const int at = t * kRow + ((piece ^ swizzle<kD>(t)) << 4);
+        const uint32_t live = (next_mask >> t) & 1 ? ~0u : 0u;
+        vtx::st16(kt + at, kr[i]);
+        vtx::st16(kt + 64 * kRow + at, vtx::U4{vr[i].x & live, vr[i].y & live, vr[i].z & live, vr[i].w & live});
+      }
+    };
+    if (tiles > 0) {
+      request(0);
+      put(0);
+      __syncthreads();
+      for (int j = 0; j < tiles; ++j) {
+        const uint64_t mask = next_mask;
+        if (j + 1 < tiles) request(j + 1);
+        const unsigned char* kt = s_tile + (j & 1) * 128 * kRow;
+        const unsigned char* vt = kt + 64 * kRow;
+        if (busy) {  // uniform over the wave
+          if (wr == 4) attend<kD, 2>(w, kt, vt, mask, a.c);
+          else attend<kD, 1>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c);
+        }
+        if (j + 1 < tiles) put(j + 1);  // (the other buffer: read last before the barrier before this tile)
+        __syncthreads();
+      }
+    }
+  }
+
+  // The waves' results meet in LDS (rows in 16-byte pieces, piece x of row r at
+  // x ^ r), and leave it joined and in whole rows.
+  __syncthreads();
+  constexpr int kOut = kD / 4;  // pieces of an output row
+  float* s_o = reinterpret_cast<float*>(s_tile) + wave * 32 * kD;
+  {
+    const int r = lane % 32, half = lane / 32;
+    const float l = w.l + vtx::xshfl(w.l, 32);
+    if (half == 0) {
+      s_m[wave][r] = w.m;
+      s_l[wave][r] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < kD / 32; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int pc = (d * 8 + x * 2 + half) ^ (r % kOut);
+        *reinterpret_cast<float4*>(s_o + r * kD + pc * 4) =
+            float4{w.o[d][4 * x], w.o[d][4 * x + 1], w.o[d][4 * x + 2], w.o[d][4 * x + 3]};
+      }
+  }
+  __syncthreads();
+  const bool direct = it.out < 0;
+  if (!direct && (long long)it.out + rows > a.max_rows) return;  // uniform
+  for (int x = tid; x < rows * kOut; x += kThreads) {
+    const int r = x / kOut, pc = x - r * kOut, rl = r % 32, blk = r / 32;
+    float M = -INFINITY;
+    for (int i = 0; i < wt; ++i) M = fmaxf(M, s_m[i * wr + blk][rl]);
+    float L = 0.f;
+    float4 O{0.f, 0.f, 0.f, 0.f};
+    if (M != -INFINITY) {
+      for (int i = 0; i < wt; ++i) {
+        const int v = i * wr + blk;
+        const float f = exp2_fast(s_m[v][rl] - M);
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(s_tile) + (v * 32 + rl) * kD +
+                                                          ((pc ^ (rl % kOut)) * 4));
+        L = fmaf(s_l[v][rl], f, L);
+        O.x = fmaf(y.x, f, O.x);
+        O.y = fmaf(y.y, f, O.y);
+        O.z = fmaf(y.z, f, O.z);
+        O.w = fmaf(y.w, f, O.w);
+      }
+    }
+    if (direct) {
+      const int at = it.row0 + r, b = b0 + at / a.G, g = at % a.G;
+      if (at < 0 || b >= a.B) continue;
+      const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN);
+      uint2 y{vtx::bf16_pair(O.x * inv, O.y * inv), vtx::bf16_pair(O.z * inv, O.w * inv)};
+      *reinterpret_cast<uint2*>(a.o + (((long long)b * a.H + h) * a.G + g) * kD + pc * 4) = y;
+    } else {
+      *reinterpret_cast<float4*>(a.acc + ((long long)it.out + r) * kD + pc * 4) = O;
+      if (pc == 0) a.ml[(long long)it.out + r] = float2{M, L};
+    }
+  }
+}
+
+// One wave per query row: the row's partial results, weighted.
+constexpr int kJoinRows = 4;
+template <int kD>
+__global__ __launch_bounds__(kJoinRows* vtx::kWave) void shared_prefix_join_kernel(SharedArgs a) {
+  constexpr int kCols = kD / vtx::kWave;
+  const int row = blockIdx.x * kJoinRows + vtx::uniform(threadIdx.x / vtx::kWave);
+  const int lane = vtx::lane_id();
+  if (row >= a.B * a.H * a.G) return;
+  const int seg = row / a.G, g = row - seg * a.G;
+  const int32_t* info = a.combine + (long long)kCombineInts * seg;
+  const int run_row = info[0], run_n = info[1], run_step = info[2], own_row = info[3], own_n = info[4];
+  if (run_n + own_n == 1 && run_n == 0) return;  // written by its item
+  auto at = [&](int i) -> long long {
+    return i < run_n ? run_row + (long long)i * run_step + g : own_row + (long long)(i - run_n) * a.G + g;
+  };
+  const int n = run_n + own_n;
+  float M = -INFINITY, L = 0.f, O[kCols];
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) O[j] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += vtx::kWave) {  // 64 at a time, lane i the (max, sum) of the i-th
+    const int live = min(n - i0, vtx::kWave);
+    const long long mine = at(i0 + min(lane, live - 1));
+    const float2 ml = mine >= 0 && mine < a.max_rows ? a.ml[mine] : float2{-INFINITY, 0.f};
+    float mx = ml.x;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) mx = fmaxf(mx, vtx::xshfl(mx, d));
+    const float nm = fmaxf(M, mx);
+    if (nm == -INFINITY) continue;
+    const float f = exp2_fast(M - nm);
+    const float wgt = lane < live ? exp2_fast(ml.x - nm) : 0.f;
+    L = fmaf(L, f, vtx::wave_sum(wgt * ml.y));
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) O[j] *= f;
+    M = nm;
+    constexpr int kAhead = 8;
+    for (int i = 0; i < live; i += kAhead) {
+      float x[kAhead][kCols];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        long long r = at(i0 + min(i + u, live - 1));
+        r = r >= 0 && r < a.max_rows ? r : 0;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) x[u][j] = a.acc[r * kD + j * vtx::kWave + lane];
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float wu = i + u < live ? __uint_as_float(vtx::lane_value(__float_as_uint(wgt), min(i + u, 63))) : 0.f;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) O[j] = i + u < live ? fmaf(x[u][j], wu, O[j]) : O[j];
+      }
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN);
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) a.o[(long long)row * kD + j * vtx::kWave + lane] = (uint16_t)vtx::f32_to_bf16(O[j] * inv);
+}
+
+template <int kD>
+int launch(const SharedArgs& a, hipStream_t s) {
+  shared_prefix_attention_kernel<kD><<<a.max_items, kThreads, 0, s>>>(a);
+  const int rows = a.B * a.H * a.G;
+  shared_prefix_join_kernel<kD><<<(rows + kJoinRows - 1) / kJoinRows, kJoinRows * vtx::kWave, 0, s>>>(a);
+  return vtx::check_launch("shared_prefix_decode_attention");
+}
+
+}  // namespace
+
+extern "C" int64_t vtx_shared_prefix_workspace_len(int32_t batch_size, int32_t num_kv_heads, int32_t group_size,
+                                                   int32_t head_dim) {
+  const int cus = vtx::device_cu_count();
+  if (batch_size < 0 || num_kv_heads < 1 || cus <= 0 || !vtx_paged_decode_attention_supported(head_dim, group_size))
+    return 0;
+  const int64_t S = (int64_t)batch_size * num_kv_heads;
+  return S > kMaxSegments ? 0 : most_rows(S, group_size, aimed_items(head_dim, cus)) * (head_dim + 2);
+}
+
+extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o, const uint16_t* k_cache,
+                                                  const uint16_t* v_cache, int64_t cache_rows,
+                                                  const int32_t* kv_indptr, const int32_t* kv_indices,
+                                                  int64_t kv_indices_len, const int32_t* kv_last_page_len,
+                                                  const int32_t* plan, int64_t plan_len, int32_t batch_size,
+                                                  int32_t num_kv_heads, int32_t group_size, int32_t head_dim,
+                                                  int32_t page_size, float sm_scale, float* workspace,
+                                                  int64_t workspace_len, void* stream) {
+  vtx::clear_error();
+  const char* what = "shared_prefix_decode_attention";
+  if (batch_size < 0 || num_kv_heads < 1 || page_size < 1 || cache_rows < 0 || kv_indices_len < 0)
+    return vtx::fail(VTX_E_INVALID, "%s: bad sizes", what);
+  if (!vtx_paged_decode_attention_supported(head_dim, group_size))
+    return vtx::fail(VTX_E_INVALID, "%s: head_dim %d with %d query heads per kv head not supported", what, head_dim,
+                     group_size);
+  const int64_t S = (int64_t)batch_size * num_kv_heads;
+  if (S > kMaxSegments) return vtx::fail(VTX_E_INVALID, "%s: too many segments", what);
+  if (S == 0) return VTX_OK;
+  if (cache_rows > 0x7fffffffLL || cache_rows * page_size > 0xffffffffLL)
+    return vtx::fail(VTX_E_INVALID, "%s: pools of more than 2^32 tokens x heads", what);
+  if (!q || !o || !k_cache || !v_cache || !kv_indptr || !kv_last_page_len || !plan || !workspace ||
+      (kv_indices_len > 0 && !kv_indices))
+    return vtx::fail(VTX_E_INVALID, "%s: null pointer", what);
+  if (!vtx::aligned16(q) || !vtx::aligned16(o) || !vtx::aligned16(k_cache) || !vtx::aligned16(v_cache))
+    return vtx::fail(VTX_E_INVALID, "%s: q, o, k_cache and v_cache must be 16-byte aligned", what);
+  const int cus = vtx::device_cu_count();
+  if (cus <= 0) return vtx::fail(VTX_E_DEVICE, "%s: device query failed", what);
+  const int64_t slots = aimed_items(head_dim, cus);
+  const Layout at = layout_of(S, most_items(S, group_size, slots));
+  if (plan_len < at.size || reinterpret_cast<uintptr_t>(plan) % 32)
+    return vtx::fail(VTX_E_INVALID, "%s: plan of %lld int32 (32-byte aligned) needed, got %lld", what,
+                     (long long)at.size, (long long)plan_len);
+  const int64_t rows = most_rows(S, group_size, slots);
+  if (workspace_len < rows * (head_dim + 2) || !vtx::aligned16(workspace))
+    return vtx::fail(VTX_E_INVALID, "%s: workspace of %lld floats (16-byte aligned) needed, got %lld", what,
+                     (long long)(rows * (head_dim + 2)), (long long)workspace_len);
+  SharedArgs a;
+  a.q = q;
+  a.o = o;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.rows = cache_rows;
+  a.indptr = kv_indptr;
+  a.indices = kv_indices;
+  a.indices_len = kv_indices_len;
+  a.last_len = kv_last_page_len;
+  a.head = plan;
+  a.items = reinterpret_cast<const Item*>(plan + at.items);
+  a.combine = plan + at.combine;
+  a.max_items = (int32_t)most_items(S, group_size, slots);
+  a.B = batch_size;
+  a.H = num_kv_heads;
+  a.G = group_size;
+  a.P = page_size;
+  a.p_shift = vtx::log2_exact(page_size);
+  const float log2e = 1.44269504088896340736f;
+  a.c = sm_scale == 0.f ? 1.f : (sm_scale < 0.f ? -sm_scale : sm_scale) * log2e;
+  a.q_sign = sm_scale < 0.f ? 0x80008000u : 0u;
+  a.q_keep = sm_scale == 0.f ? 0u : ~0u;
+  a.acc = workspace;
+  a.ml = reinterpret_cast<float2*>(workspace + rows * head_dim);
+  a.max_rows = rows;
+  hipStream_t s = vtx::as_stream(stream);
+  switch (head_dim) {
+    case 64: return launch<64>(a, s);
+    case 128: return launch<128>(a, s);
+    default: return launch<256>(a, s);
+  }
+}

@@ -2,9 +2,11 @@
 
 Every wrapper validates dtypes, devices, contiguity and sizes of its torch
 tensors, then launches on torch's current HIP stream of the tensors' device.
-No kernel wrapper synchronises or reads device memory, and none but
-``paged_decode_attention`` allocates (scratch, where that lasts: see there), so
-they can be recorded into a HIP graph (``torch.cuda.graph``).
+No kernel wrapper synchronises or reads device memory, and none allocates but
+``paged_decode_attention`` and ``shared_prefix_decode_attention`` (scratch,
+where that lasts: see there), ``plan_shared_prefix`` and ``set_kv_buffer_rope``
+(their results, where the caller gives no tensor for them), so they can be
+recorded into a HIP graph (``torch.cuda.graph``).
 
 There is no CPU fallback: a tensor that is not on a GPU, or a missing
 library, raises ``RuntimeError``.
@@ -138,6 +140,17 @@ _SIGNATURES = {
     ),
     "vtx_paged_decode_attention_workspace_len": ([_i32, _i32, _i32, _i32, _i32, _i64], ctypes.c_int64),
     "vtx_paged_decode_attention_supported": ([_i32, _i32], ctypes.c_int),
+    "vtx_shared_prefix_plan_len": ([_i32, _i32, _i32, _i32], ctypes.c_int64),
+    "vtx_plan_shared_prefix": (
+        [_vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp],
+        ctypes.c_int,
+    ),
+    "vtx_shared_prefix_workspace_len": ([_i32, _i32, _i32, _i32], ctypes.c_int64),
+    "vtx_shared_prefix_decode_attention": (
+        [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp,
+         _i64, _vp],
+        ctypes.c_int,
+    ),
     "vtx_bf16_rounding_check": ([_vp, _vp], ctypes.c_int),
     "vtx_stream_capture_id": ([_vp, ctypes.POINTER(ctypes.c_ulonglong)], ctypes.c_int),
     "vtx_probe_read": ([_vp, _i64, _vp, _i64, ctypes.c_uint32, _vp], ctypes.c_int),
@@ -1188,6 +1201,82 @@ def paged_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_las
             kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr(), B, H, G, D, P, float(sm_scale),
             None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream)
     _check(rc, "paged_decode_attention")
+
+
+@_plain_args
+def plan_shared_prefix(kv_indptr, kv_indices, group_ids, batch_size: int, num_kv_heads: int, group_size: int,
+                       head_dim: int, page_size: int, plan=None):
+    """Writes the shared-prefix plan of a block table into `plan` (int32), or
+    into a new tensor; returns it."""
+    lib = load_library()
+    more = [t for t in (group_ids, plan) if t is not None]
+    dev = _require_gpu(kv_indptr, kv_indices, *more)
+    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (group_ids, "group_ids"), (plan, "plan")):
+        if t is not None:
+            _req(t, torch.int32, n)
+    B, H, G, D = int(batch_size), int(num_kv_heads), int(group_size), int(head_dim)
+    if B < 0 or H < 1 or int(page_size) < 1:
+        raise RuntimeError("vortex_torch: batch_size, num_kv_heads and page_size must be positive")
+    if not paged_decode_attention_supported(D, G):
+        raise RuntimeError(f"vortex_torch: head_dim {D} with {G} query heads per kv head not supported")
+    if kv_indptr.numel() < B * H + 1:
+        raise RuntimeError(f"vortex_torch: kv_indptr needs {B * H + 1} entries")
+    if group_ids is not None and group_ids.numel() < B:
+        raise RuntimeError(f"vortex_torch: group_ids needs {B} entries")
+    with _on_device(dev):
+        stream = _stream(dev)
+        if plan is None:
+            from . import _deferred
+
+            if not _deferred.scratch_lasts(stream):
+                raise RuntimeError("vortex_torch: a capture that torch did not begin needs a plan made before it")
+            plan = torch.empty(max(lib.vtx_shared_prefix_plan_len(B, H, G, D), 16), dtype=torch.int32, device=dev)
+        rc = lib.vtx_plan_shared_prefix(
+            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
+            None if group_ids is None else group_ids.data_ptr(), B, H, G, D, int(page_size), plan.data_ptr(),
+            plan.numel(), stream)
+    _check(rc, "plan_shared_prefix")
+    return plan
+
+
+@_plain_args
+def shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan,
+                                   batch_size: int, num_kv_heads: int, group_size: int, sm_scale: float) -> None:
+    """paged_decode_attention with the pages that a plan found shared read once
+    per run.  Its partial results need scratch from torch's allocator; without
+    (see _scratch) paged decode attention itself runs, which needs none."""
+    lib = load_library()
+    dev = _require_gpu(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan)
+    for t, n in ((q, "q"), (o, "o"), (k_cache, "k_cache"), (v_cache, "v_cache")):
+        _req(t, torch.bfloat16, n)
+    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (kv_last_page_len, "kv_last_page_len"),
+                 (plan, "plan")):
+        _req(t, torch.int32, n)
+    if k_cache.dim() != 3 or v_cache.shape != k_cache.shape:
+        raise RuntimeError("vortex_torch: k_cache and v_cache must both be [pages * H, page_size, head_dim]")
+    rows, P, D = k_cache.shape
+    B, H, G = int(batch_size), int(num_kv_heads), int(group_size)
+    if q.numel() != B * H * G * D or o.numel() != q.numel():
+        raise RuntimeError("vortex_torch: q and o must hold batch * kv heads * group rows of head_dim")
+    if kv_indptr.numel() < B * H + 1 or kv_last_page_len.numel() < B * H:
+        raise RuntimeError(f"vortex_torch: kv_indptr needs {B * H + 1} and kv_last_page_len {B * H} entries")
+    with _on_device(dev):
+        stream = _stream(dev)
+        args = (q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), rows, kv_indptr.data_ptr(),
+                kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr())
+        floats = lib.vtx_shared_prefix_workspace_len(B, H, G, D)
+        ws = _scratch(floats, dev, stream)
+        if ws is None and floats > 0:
+            rc = lib.vtx_paged_decode_attention(*args, B, H, G, D, P, float(sm_scale), stream)
+        else:
+            rc = lib.vtx_shared_prefix_decode_attention(
+                *args, plan.data_ptr(), plan.numel(), B, H, G, D, P, float(sm_scale),
+                None if ws is None else ws.data_ptr(), floats, stream)
+    _check(rc, "shared_prefix_decode_attention")
+
+
+def paged_decode_attention_supported(head_dim: int, group_size: int) -> bool:
+    return bool(load_library().vtx_paged_decode_attention_supported(int(head_dim), int(group_size)))
 
 
 def bf16_rounding_check(device="cuda") -> tuple:
