@@ -22,7 +22,7 @@
 // 4 waves.  Up to 32 rows (a request's own pages): every wave takes tiles of 32
 // tokens of its own.  More: tiles of 64 tokens for all waves, of which each
 // takes 32 rows (or 32 rows and 32 tokens where there are up to 64 rows), two
-// buffers.  K and V go through registers to LDS, requested one tile ahead.
+// buffers, copied straight to LDS one tile ahead.
 #include "vtx_shared_prefix.h"
 
 #include "vtx_device.h"
@@ -81,6 +81,14 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Copies 16 bytes per lane to LDS: lane l's to `to` (uniform) + 16 l.
+__device__ __forceinline__ void copy16(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+// Waits for this wave's copies (and other loads).
+__device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // A wave's 32 query rows: their fragments, running maximum (scaled, base 2),
 // sum (this lane's half of the tokens) and output.
 template <int kD>
@@ -89,6 +97,11 @@ struct Rows {
   float m, l;
   f32x16 o[kD / 32];
 };
+
+// The running maximum follows the scores only when they outgrow it by so much
+// (base 2): until then weights up to 2^8 are as exact as weights up to 1, and
+// most tiles leave the outputs as they are.
+constexpr float kGrowth = 8.f;
 
 // kN x 32 tokens at kt / vt in LDS; bit i of mask: token i counts.
 template <int kD, int kN>
@@ -112,11 +125,15 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
     }
   constexpr uint64_t kAll = kN == 2 ? ~0ull : 0xffffffffull;
   if ((mask & kAll) != kAll) {  // uniform
+    const uint64_t mine = mask >> (4 * half);
 #pragma unroll
-    for (int n = 0; n < kN; ++n)
+    for (int n = 0; n < kN; ++n) {
+      const uint32_t bits = (uint32_t)(mine >> (32 * n));
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (!((mask >> (n * 32 + 8 * (i / 4) + 4 * half + i % 4)) & 1)) s[n][i] = -INFINITY;
+        if (!(bits & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
+    }
+    asm volatile("" : "+v"(s[0][0]));  // (a branch, not selects in every tile)
   }
   float mx = s[0][0];
 #pragma unroll
@@ -124,7 +141,7 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
   mx = fmaxf(mx, vtx::xshfl(mx, 32)) * c;
-  if (__ballot(mx > w.m)) {  // uniform
+  if (__ballot(mx > w.m + kGrowth)) {  // uniform
     const float nm = fmaxf(w.m, mx);
     const float f = nm == -INFINITY ? 1.f : exp2_fast(w.m - nm);
     w.l *= f;
@@ -205,7 +222,11 @@ template <int kD>
 __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attention_kernel(SharedArgs a) {
   constexpr int kRow = kD * 2;
   constexpr int kPieces = kD / 8;
-  __shared__ alignas(16) unsigned char s_tile[256 * kRow];  // two buffers of 64 tokens, or four of 32; then the rows' outputs
+  // Two buffers of 64 tokens (their K and V), or every wave's 32; then the waves'
+  // outputs.  Arrays of their own, so that the compiler sees which of them a copy
+  // in flight writes and lets the reads of the others pass it.
+  __shared__ alignas(16) unsigned char s_k0[64 * kRow], s_v0[64 * kRow], s_k1[64 * kRow], s_v1[64 * kRow];
+  auto part = [&](int i) -> unsigned char* { return i == 0 ? s_k0 : (i == 1 ? s_v0 : (i == 2 ? s_k1 : s_v1)); };
   __shared__ float s_m[kWaves][32];
   __shared__ float s_l[kWaves][32];
 
@@ -260,7 +281,7 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
   if (wr == 1) {  // uniform: tiles of 32 tokens, wave w those of index w, w + 4, ...
     constexpr int kPass = vtx::kWave / kPieces;  // tokens per wave-wide load
     constexpr int kLoads = 32 / kPass;
-    unsigned char* kt = s_tile + wave * 64 * kRow;
+    unsigned char* kt = part(wave);
     unsigned char* vt = kt + 32 * kRow;
     const int piece = lane % kPieces, sub = lane / kPieces;
     const int tiles = (tk.count + 31) / 32;
@@ -297,52 +318,55 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
       wave_lds_fence();
     }
   } else {  // uniform: tiles of 64 tokens for all waves
-    constexpr int kPass = kThreads / kPieces;
-    constexpr int kLoads = 64 / kPass;
-    const int piece = tid % kPieces, sub = tid / kPieces;
+    constexpr int kPass = vtx::kWave / kPieces;  // tokens per wave-wide copy
+    constexpr int kCopies = 64 / (kPass * kWaves);
     const int tiles = (tk.count + 63) / 64;
     const bool busy = rb * 32 < rows;
-    vtx::U4 kr[kLoads], vr[kLoads];
     uint64_t next_mask = 0;
     Entry e = entry_of(a, tk, lane);
-    auto request = [&](int j) {
+    // Requests tile j: copies straight to LDS, every lane 16 bytes to its place in
+    // the wave's stretch, so it is the piece it reads that follows the swizzle.
+    auto request = [&](int j, unsigned char* kt, unsigned char* vt) {
       uint32_t row;
       const bool ok = resolve(a, e, row);
       next_mask = __ballot(ok);
       e = entry_of(a, tk, (j + 1) * 64 + lane);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const uint32_t tr = (uint32_t)__shfl((int)row, i * kPass + sub);
-        kr[i] = vtx::ld16(a.k + (uint64_t)tr * kD + piece * 8);
-        vr[i] = vtx::ld16(a.v + (uint64_t)tr * kD + piece * 8);
+      for (int i = 0; i < kCopies; ++i) {
+        const int t0 = (i * kWaves + wave) * kPass, t = t0 + lane / kPieces;
+        const uint64_t at = (uint64_t)(uint32_t)__shfl((int)row, t) * kD + ((lane % kPieces) ^ swizzle<kD>(t)) * 8;
+        copy16(a.k + at, kt + t0 * kRow);
+        copy16(a.v + at, vt + t0 * kRow);
       }
     };
-    auto put = [&](int j) {
-      unsigned char* kt = s_tile + (j & 1) * 128 * kRow;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int t = i * kPass + sub;
-        const int at = t * kRow + ((piece ^ swizzle<kD>(t)) << 4);
-        const uint32_t live = (next_mask >> t) & 1 ? ~0u : 0u;
-        vtx::st16(kt + at, kr[i]);
-        vtx::st16(kt + 64 * kRow + at, vtx::U4{vr[i].x & live, vr[i].y & live, vr[i].z & live, vr[i].w & live});
+    auto tile = [&](uint64_t mask, unsigned char* kt, unsigned char* vt) {
+      if (mask != ~0ull) {  // uniform: what lies in a masked row may be NaN
+        for (int x = tid; x < 64 * kPieces; x += kThreads)
+          if (!((mask >> (x / kPieces)) & 1)) vtx::st16(vt + x * 16, vtx::U4{0u, 0u, 0u, 0u});
+        __syncthreads();
+      }
+      if (busy) {  // uniform over the wave
+        if (wr == 4) attend<kD, 2>(w, kt, vt, mask, a.c);
+        else attend<kD, 1>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c);
       }
     };
     if (tiles > 0) {
-      request(0);
-      put(0);
+      request(0, s_k0, s_v0);
+      copies_done();
       __syncthreads();
-      for (int j = 0; j < tiles; ++j) {
-        const uint64_t mask = next_mask;
-        if (j + 1 < tiles) request(j + 1);
-        const unsigned char* kt = s_tile + (j & 1) * 128 * kRow;
-        const unsigned char* vt = kt + 64 * kRow;
-        if (busy) {  // uniform over the wave
-          if (wr == 4) attend<kD, 2>(w, kt, vt, mask, a.c);
-          else attend<kD, 1>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c);
-        }
-        if (j + 1 < tiles) put(j + 1);  // (the other buffer: read last before the barrier before this tile)
+      for (int j = 0; j < tiles; j += 2) {
+        uint64_t mask = next_mask;
+        if (j + 1 < tiles) request(j + 1, s_k1, s_v1);
+        tile(mask, s_k0, s_v0);
+        copies_done();
         __syncthreads();
+        if (j + 1 < tiles) {
+          mask = next_mask;
+          if (j + 2 < tiles) request(j + 2, s_k0, s_v0);
+          tile(mask, s_k1, s_v1);
+          copies_done();
+          __syncthreads();
+        }
       }
     }
   }
@@ -351,7 +375,7 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
   // x ^ r), and leave it joined and in whole rows.
   __syncthreads();
   constexpr int kOut = kD / 4;  // pieces of an output row
-  float* s_o = reinterpret_cast<float*>(s_tile) + wave * 32 * kD;
+  float* s_o = reinterpret_cast<float*>(part(wave));
   {
     const int r = lane % 32, half = lane / 32;
     const float l = w.l + vtx::xshfl(w.l, 32);
@@ -381,7 +405,7 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
       for (int i = 0; i < wt; ++i) {
         const int v = i * wr + blk;
         const float f = exp2_fast(s_m[v][rl] - M);
-        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(s_tile) + (v * 32 + rl) * kD +
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(part(v)) + rl * kD +
                                                           ((pc ^ (rl % kOut)) * 4));
         L = fmaf(s_l[v][rl], f, L);
         O.x = fmaf(y.x, f, O.x);
