@@ -25,6 +25,8 @@
 // buffers, copied straight to LDS one tile ahead.
 #include "vtx_shared_prefix.h"
 
+#include <type_traits>
+
 #include "vtx_device.h"
 #include "vtx_host.h"
 
@@ -57,10 +59,16 @@ struct SharedArgs {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
+constexpr int kXcds = 8;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds4;
+
+// Classes of instructions for the scheduler's groups.
+constexpr int kSchedValu = 0x2, kSchedMfma = 0x8, kSchedRead = 0x100;
 
 // LDS rows of a tile are kD bf16 in 16-byte pieces; piece c of token t lies at
 // c ^ swizzle(t), so that the 8 (or 16) tokens of a K read, at one c, and the
@@ -103,8 +111,9 @@ struct Rows {
 // most tiles leave the outputs as they are.
 constexpr float kGrowth = 8.f;
 
-// kN x 32 tokens at kt / vt in LDS; bit i of mask: token i counts.
-template <int kD, int kN>
+// kN x 32 tokens at kt / vt in LDS; bit i of mask: token i counts.  kAhead: the
+// LDS reads are kept ahead of the products that take them (registers allowing).
+template <int kD, int kN, bool kAhead>
 __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, const unsigned char* vt, uint64_t mask,
                                        float c) {
   constexpr int kRow = kD * 2;
@@ -116,13 +125,41 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
     for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
   const int ksw = swizzle<kD>(r);
 #pragma unroll
-  for (int n = 0; n < kN; ++n)
+  for (int kk = 0; kk < kD / 16; ++kk)
 #pragma unroll
-    for (int kk = 0; kk < kD / 16; ++kk) {
+    for (int n = 0; n < kN; ++n) {
       const vtx::U4 f = vtx::ld16(kt + (n * 32 + r) * kRow + (((2 * kk + half) ^ ksw) << 4));
       s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, w.q[kk]),
                                                      s[n], 0, 0, 0);
     }
+  // V^T of the first 16 tokens, on the way during the softmax: 16 lanes take 4
+  // tokens x 16 columns per read
+  const int g16 = lane / 16, i16 = lane % 16;
+  const int vrow = 4 * half + i16 / 4;
+  const int vcol = (g16 & 1) * 2 + (i16 % 4) / 2;
+  constexpr int kSteps = 2 * kN;  // 16 tokens each
+  s16x4 f[kAhead ? 2 : 1][kD / 32][2];
+  auto read_v = [&](int k, s16x4 (&to)[kD / 32][2]) {
+#pragma unroll
+    for (int d = 0; d < kD / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int t = vrow + 8 * e;  // (+ 16 k, which the swizzle does not see)
+        const unsigned char* at =
+            vt + (k * 16 + t) * kRow + (((d * 4 + vcol) ^ swizzle<kD>(t)) << 4) + (i16 % 2) * 8;
+        to[d][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
+      }
+  };
+  if constexpr (kAhead) {
+    read_v(0, f[0]);
+    constexpr int kReads = kN * (kD / 16), kLead = kReads < 8 ? kReads : 8;
+    __builtin_amdgcn_sched_group_barrier(kSchedRead, kLead, 0);
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedRead, 1, 0);
+    }
+  }
   constexpr uint64_t kAll = kN == 2 ? ~0ull : 0xffffffffull;
   if ((mask & kAll) != kAll) {  // uniform
     const uint64_t mine = mask >> (4 * half);
@@ -152,40 +189,30 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
     w.m = nm;
   }
   const float base = w.m == -INFINITY ? 0.f : w.m;
-  uint32_t p[kN][8];
 #pragma unroll
-  for (int n = 0; n < kN; ++n)
+  for (int k = 0; k < kSteps; ++k) {
+    if constexpr (!kAhead) read_v(k, f[0]);
+    else if (k + 1 < kSteps) read_v(k + 1, f[(k + 1) & 1]);
+    uint32_t p[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[n][i] = vtx::bf16_pair(exp2_fast(fmaf(s[n][2 * i], c, -base)), exp2_fast(fmaf(s[n][2 * i + 1], c, -base)));
-      w.l = vtx::dot2_bf16(p[n][i], 0x3f803f80u, w.l);
+    for (int i = 0; i < 4; ++i) {
+      const int x = 8 * (k & 1) + 2 * i;
+      p[i] = vtx::bf16_pair(exp2_fast(fmaf(s[k / 2][x], c, -base)), exp2_fast(fmaf(s[k / 2][x + 1], c, -base)));
+      w.l = vtx::dot2_bf16(p[i], 0x3f803f80u, w.l);
     }
-  // V^T: 16 lanes take 4 tokens x 16 columns per read
-  typedef __attribute__((address_space(3))) s16x4 lds4;
-  const int g16 = lane / 16, i16 = lane % 16;
-  const int vrow = 4 * half + i16 / 4;
-  const int vcol = (g16 & 1) * 2 + (i16 % 4) / 2;
+    const vtx::U4 b = vtx::U4{p[0], p[1], p[2], p[3]};
 #pragma unroll
-  for (int n = 0; n < kN; ++n)
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const vtx::U4 b = vtx::U4{p[n][4 * kk], p[n][4 * kk + 1], p[n][4 * kk + 2], p[n][4 * kk + 3]};
-#pragma unroll
-      for (int d = 0; d < kD / 32; ++d) {
-        s16x4 f[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int t = vrow + 8 * e;  // (+ 32 n + 16 kk, which the swizzle does not see)
-          const unsigned char* at =
-              vt + (n * 32 + kk * 16 + t) * kRow + (((d * 4 + vcol) ^ swizzle<kD>(t)) << 4) + (i16 % 2) * 8;
-          f[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
-        }
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 a = __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
-                                                         w.o[d], 0, 0, 0);
-      }
+    for (int d = 0; d < kD / 32; ++d) {
+      const s16x8 a = __builtin_shufflevector(f[kAhead ? k & 1 : 0][d][0], f[kAhead ? k & 1 : 0][d][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                       w.o[d], 0, 0, 0);
     }
+    if constexpr (kAhead) {
+      if (k + 1 < kSteps) __builtin_amdgcn_sched_group_barrier(kSchedRead, kD / 16, 1);
+      __builtin_amdgcn_sched_group_barrier(kSchedValu, 24, 1);
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kD / 32, 1);
+    }
+  }
 }
 
 // The tokens of an item: where they lie in the table, and how many.
@@ -232,7 +259,15 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
 
   const int run_items = a.head[kHeadRunItems], items = run_items + a.head[kHeadOwnItems];
   if ((int)blockIdx.x >= items || items > a.max_items) return;  // uniform
-  const Item it = a.items[blockIdx.x];
+  // Workgroup i runs on XCD i % 8: each XCD takes a stretch of the runs' items,
+  // the row tiles of a chunk side by side in it, so that a chunk's pages come
+  // into one L2 once.
+  int at_item = blockIdx.x;
+  if (at_item < run_items) {
+    const int x = at_item % kXcds, each = run_items / kXcds, more = run_items % kXcds;
+    at_item = x * each + min(x, more) + at_item / kXcds;
+  }
+  const Item it = a.items[at_item];
   const int tid = threadIdx.x, lane = vtx::lane_id();
   const int wave = vtx::uniform(tid / vtx::kWave);
   const int seg = vtx::uniform(it.segment), S = a.B * a.H;
@@ -289,7 +324,7 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
     vtx::U4 kr[kLoads], vr[kLoads];
     uint64_t next_mask = 0;
     Entry e = entry_of(a, tk, n > 0 ? wave * 32 + lane % 32 : 0x7fffffff);
-    auto request = [&](int j) {  // tile j's rows, and the entries of tile j + 1
+    auto request = [&](int j) __attribute__((always_inline)) {  // tile j's rows, and the entries of tile j + 1
       uint32_t row;
       const bool ok = resolve(a, e, row);
       next_mask = __ballot(ok) & 0xffffffffull;
@@ -314,7 +349,7 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
       }
       wave_lds_fence();
       if (j + 1 < n) request(j + 1);
-      attend<kD, 1>(w, kt, vt, mask, a.c);
+      attend<kD, 1, false>(w, kt, vt, mask, a.c);
       wave_lds_fence();
     }
   } else {  // uniform: tiles of 64 tokens for all waves
@@ -326,7 +361,7 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
     Entry e = entry_of(a, tk, lane);
     // Requests tile j: copies straight to LDS, every lane 16 bytes to its place in
     // the wave's stretch, so it is the piece it reads that follows the swizzle.
-    auto request = [&](int j, unsigned char* kt, unsigned char* vt) {
+    auto request = [&](int j, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
       uint32_t row;
       const bool ok = resolve(a, e, row);
       next_mask = __ballot(ok);
@@ -339,35 +374,39 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
         copy16(a.v + at, vt + t0 * kRow);
       }
     };
-    auto tile = [&](uint64_t mask, unsigned char* kt, unsigned char* vt) {
+    auto tile = [&](auto all, uint64_t mask, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
       if (mask != ~0ull) {  // uniform: what lies in a masked row may be NaN
         for (int x = tid; x < 64 * kPieces; x += kThreads)
           if (!((mask >> (x / kPieces)) & 1)) vtx::st16(vt + x * 16, vtx::U4{0u, 0u, 0u, 0u});
         __syncthreads();
       }
       if (busy) {  // uniform over the wave
-        if (wr == 4) attend<kD, 2>(w, kt, vt, mask, a.c);
-        else attend<kD, 1>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c);
+        if constexpr (decltype(all)::value) attend<kD, 2, true>(w, kt, vt, mask, a.c);
+        else attend<kD, 1, true>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c);
       }
     };
-    if (tiles > 0) {
+    auto all_tiles = [&](auto all) __attribute__((always_inline)) {  // all: every wave takes all tokens of a tile, for 32 rows of its own
       request(0, s_k0, s_v0);
       copies_done();
       __syncthreads();
       for (int j = 0; j < tiles; j += 2) {
         uint64_t mask = next_mask;
         if (j + 1 < tiles) request(j + 1, s_k1, s_v1);
-        tile(mask, s_k0, s_v0);
+        tile(all, mask, s_k0, s_v0);
         copies_done();
         __syncthreads();
         if (j + 1 < tiles) {
           mask = next_mask;
           if (j + 2 < tiles) request(j + 2, s_k0, s_v0);
-          tile(mask, s_k1, s_v1);
+          tile(all, mask, s_k1, s_v1);
           copies_done();
           __syncthreads();
         }
       }
+    };
+    if (tiles > 0) {  // (loops of their own: each one's registers)
+      if (wr == 4) all_tiles(std::true_type{});
+      else all_tiles(std::false_type{});
     }
   }
 
