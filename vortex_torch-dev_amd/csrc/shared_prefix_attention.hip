@@ -59,7 +59,6 @@ struct SharedArgs {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-constexpr int kXcds = 8;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -97,13 +96,22 @@ __device__ __forceinline__ void copy16(const void* from, void* to) {
 // Waits for this wave's copies (and other loads).
 __device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
+// Output columns of a wave: all, or half of 256 (two waves share 32 rows and
+// both compute their scores: with all columns the 256 outputs and queries of a
+// lane leave no registers, and took 30 us where this takes XX).
+template <int kD>
+constexpr int kCols = kD == 256 ? 128 : kD;
+// Tokens of a tile that all waves share.
+template <int kD>
+constexpr int kTile = kD == 256 ? 32 : 64;
+
 // A wave's 32 query rows: their fragments, running maximum (scaled, base 2),
 // sum (this lane's half of the tokens) and output.
 template <int kD>
 struct Rows {
   vtx::U4 q[kD / 16];
   float m, l;
-  f32x16 o[kD / 32];
+  f32x16 o[kCols<kD> / 32];
 };
 
 // The running maximum follows the scores only when they outgrow it by so much
@@ -113,10 +121,11 @@ constexpr float kGrowth = 8.f;
 
 // kN x 32 tokens at kt / vt in LDS; bit i of mask: token i counts.  kAhead: the
 // LDS reads are kept ahead of the products that take them (registers allowing).
+// col: the wave's first output column / 8.
 template <int kD, int kN, bool kAhead>
 __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, const unsigned char* vt, uint64_t mask,
-                                       float c) {
-  constexpr int kRow = kD * 2;
+                                       float c, int col) {
+  constexpr int kRow = kD * 2, kBlocks = kCols<kD> / 32;
   const int lane = vtx::lane_id(), r = lane % 32, half = lane / 32;
   f32x16 s[kN];
 #pragma unroll
@@ -136,12 +145,12 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
   // tokens x 16 columns per read
   const int g16 = lane / 16, i16 = lane % 16;
   const int vrow = 4 * half + i16 / 4;
-  const int vcol = (g16 & 1) * 2 + (i16 % 4) / 2;
+  const int vcol = col + (g16 & 1) * 2 + (i16 % 4) / 2;
   constexpr int kSteps = 2 * kN;  // 16 tokens each
-  s16x4 f[kAhead ? 2 : 1][kD / 32][2];
-  auto read_v = [&](int k, s16x4 (&to)[kD / 32][2]) {
+  s16x4 f[kAhead ? 2 : 1][kBlocks][2];
+  auto read_v = [&](int k, s16x4 (&to)[kBlocks][2]) {
 #pragma unroll
-    for (int d = 0; d < kD / 32; ++d)
+    for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int t = vrow + 8 * e;  // (+ 16 k, which the swizzle does not see)
@@ -183,7 +192,7 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
     const float f = nm == -INFINITY ? 1.f : exp2_fast(w.m - nm);
     w.l *= f;
 #pragma unroll
-    for (int d = 0; d < kD / 32; ++d)
+    for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) w.o[d][i] *= f;
     w.m = nm;
@@ -202,15 +211,15 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
     }
     const vtx::U4 b = vtx::U4{p[0], p[1], p[2], p[3]};
 #pragma unroll
-    for (int d = 0; d < kD / 32; ++d) {
+    for (int d = 0; d < kBlocks; ++d) {
       const s16x8 a = __builtin_shufflevector(f[kAhead ? k & 1 : 0][d][0], f[kAhead ? k & 1 : 0][d][1], 0, 1, 2, 3, 4, 5, 6, 7);
       w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
                                                        w.o[d], 0, 0, 0);
     }
     if constexpr (kAhead) {
-      if (k + 1 < kSteps) __builtin_amdgcn_sched_group_barrier(kSchedRead, kD / 16, 1);
+      if (k + 1 < kSteps) __builtin_amdgcn_sched_group_barrier(kSchedRead, 2 * kBlocks, 1);
       __builtin_amdgcn_sched_group_barrier(kSchedValu, 24, 1);
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kD / 32, 1);
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kBlocks, 1);
     }
   }
 }
@@ -243,60 +252,50 @@ __device__ __forceinline__ bool resolve(const SharedArgs& a, const Entry& e, uin
 }
 
 template <int kD>
-constexpr int kMinBlocks = kD == 64 ? 3 : (kD == 128 ? 2 : 1);
-
-template <int kD>
-__global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attention_kernel(SharedArgs a) {
+__global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_attention_kernel(SharedArgs a) {
   constexpr int kRow = kD * 2;
   constexpr int kPieces = kD / 8;
-  // Two buffers of 64 tokens (their K and V), or every wave's 32; then the waves'
+  constexpr int kBlocks = kCols<kD> / 32;
+  constexpr int kShare = kD / kCols<kD>;  // waves that share rows
+  constexpr int kGroups = kWaves / kShare;
+  // Two buffers of a tile (its K and V), or every wave's 32 tokens; then the waves'
   // outputs.  Arrays of their own, so that the compiler sees which of them a copy
   // in flight writes and lets the reads of the others pass it.
-  __shared__ alignas(16) unsigned char s_k0[64 * kRow], s_v0[64 * kRow], s_k1[64 * kRow], s_v1[64 * kRow];
+  __shared__ alignas(16) unsigned char s_k0[kTile<kD> * kRow], s_v0[kTile<kD> * kRow], s_k1[kTile<kD> * kRow],
+      s_v1[kTile<kD> * kRow];
   auto part = [&](int i) -> unsigned char* { return i == 0 ? s_k0 : (i == 1 ? s_v0 : (i == 2 ? s_k1 : s_v1)); };
   __shared__ float s_m[kWaves][32];
   __shared__ float s_l[kWaves][32];
 
-  const int run_items = a.head[kHeadRunItems], items = run_items + a.head[kHeadOwnItems];
+  const Item it = a.items[blockIdx.x];  // (room for as many; past the last one it is not used)
+  const int items = a.head[kHeadItems];
   if ((int)blockIdx.x >= items || items > a.max_items) return;  // uniform
-  // Workgroup i runs on XCD i % 8: each XCD takes a stretch of the runs' items,
-  // the row tiles of a chunk side by side in it, so that a chunk's pages come
-  // into one L2 once.
-  int at_item = blockIdx.x;
-  if (at_item < run_items) {
-    const int x = at_item % kXcds, each = run_items / kXcds, more = run_items % kXcds;
-    at_item = x * each + min(x, more) + at_item / kXcds;
-  }
-  const Item it = a.items[at_item];
   const int tid = threadIdx.x, lane = vtx::lane_id();
   const int wave = vtx::uniform(tid / vtx::kWave);
   const int seg = vtx::uniform(it.segment), S = a.B * a.H;
   if (seg < 0 || seg >= S) return;
   const int b0 = seg / a.H, h = seg - b0 * a.H;
-  const int rows = min(max(it.rows, 0), kTileRows);
+  const int rows = min(max(it.rows, 0), tile_rows(kD));
 
-  // the item's tokens, within what the table holds now
+  // the item's tokens
   Tokens tk{nullptr, 0};
-  {
-    const int start = a.indptr[seg];
-    const long long end = a.indptr[seg + 1];
-    const int n = start >= 0 && end > start && end <= a.indices_len && a.rows > 0 ? (int)(end - start) : 0;
-    const int p0 = max(it.page0, 0), p1 = min(it.page1, n);
-    if (p1 > p0) {
-      const int ll = a.last_len[seg], last = ll < 0 ? 0 : (ll > a.P ? a.P : ll);
-      const long long t = (long long)(p1 - p0 - 1) * a.P + (p1 == n ? last : a.P);
-      tk.pages = a.indices + start + p0;
-      tk.count = (int)(t < 0x3fffffff ? t : 0x3fffffff);
-    }
+  if (it.start >= 0 && it.pages > 0 && (long long)it.start + it.pages <= a.indices_len && a.rows > 0) {
+    int last = a.P;
+    if (it.last) last = min(max(a.last_len[seg], 0), a.P);
+    const long long t = (long long)(it.pages - 1) * a.P + last;
+    tk.pages = a.indices + it.start;
+    tk.count = (int)(t < 0x3fffffff ? t : 0x3fffffff);
   }
 
-  const int wr = rows > 64 ? 4 : (rows > 32 ? 2 : 1);  // blocks of 32 rows, a power of two
-  const int rb = wave % wr, tb = wave / wr, wt = kWaves / wr;
+  // blocks of 32 rows, a power of two; this wave's, its tokens among the waves
+  // that have the same rows, and its columns
+  const int wr = rows > 64 ? 4 : (rows > 32 ? 2 : 1);
+  const int half_col = wave % kShare, rb = (wave / kShare) % wr, tb = (wave / kShare) / wr, wt = kGroups / wr;
   Rows<kD> w;
   w.m = -INFINITY;
   w.l = 0.f;
 #pragma unroll
-  for (int d = 0; d < kD / 32; ++d)
+  for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) w.o[d][i] = 0.f;
   {
@@ -313,7 +312,9 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
     }
   }
 
-  if (wr == 1) {  // uniform: tiles of 32 tokens, wave w those of index w, w + 4, ...
+  bool alone = false;  // tiles of 32 tokens, wave w those of index w, w + 4, ...
+  if constexpr (kShare == 1) alone = wr == 1;
+  if (alone) {  // uniform
     constexpr int kPass = vtx::kWave / kPieces;  // tokens per wave-wide load
     constexpr int kLoads = 32 / kPass;
     unsigned char* kt = part(wave);
@@ -349,23 +350,26 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
       }
       wave_lds_fence();
       if (j + 1 < n) request(j + 1);
-      attend<kD, 1, false>(w, kt, vt, mask, a.c);
+      attend<kD, 1, false>(w, kt, vt, mask, a.c, 0);
       wave_lds_fence();
     }
-  } else {  // uniform: tiles of 64 tokens for all waves
+  } else {  // uniform: tiles of kTile tokens for all waves
+    constexpr int kT = kTile<kD>;
+    constexpr uint64_t kFull = kT == 64 ? ~0ull : (1ull << kT) - 1;
     constexpr int kPass = vtx::kWave / kPieces;  // tokens per wave-wide copy
-    constexpr int kCopies = 64 / (kPass * kWaves);
-    const int tiles = (tk.count + 63) / 64;
-    const bool busy = rb * 32 < rows;
+    constexpr int kCopies = kT / (kPass * kWaves);
+    const int tiles = (tk.count + kT - 1) / kT;
+    const int col = half_col * (kCols<kD> / 8);
+    const bool busy = rb * 32 < rows && tb * 32 < kT;
     uint64_t next_mask = 0;
-    Entry e = entry_of(a, tk, lane);
+    Entry e = entry_of(a, tk, lane % kT);
     // Requests tile j: copies straight to LDS, every lane 16 bytes to its place in
     // the wave's stretch, so it is the piece it reads that follows the swizzle.
     auto request = [&](int j, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
       uint32_t row;
       const bool ok = resolve(a, e, row);
-      next_mask = __ballot(ok);
-      e = entry_of(a, tk, (j + 1) * 64 + lane);
+      next_mask = __ballot(ok) & kFull;
+      e = entry_of(a, tk, (j + 1) * kT + lane % kT);
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
         const int t0 = (i * kWaves + wave) * kPass, t = t0 + lane / kPieces;
@@ -375,14 +379,14 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
       }
     };
     auto tile = [&](auto all, uint64_t mask, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
-      if (mask != ~0ull) {  // uniform: what lies in a masked row may be NaN
-        for (int x = tid; x < 64 * kPieces; x += kThreads)
+      if (mask != kFull) {  // uniform: what lies in a masked row may be NaN
+        for (int x = tid; x < kT * kPieces; x += kThreads)
           if (!((mask >> (x / kPieces)) & 1)) vtx::st16(vt + x * 16, vtx::U4{0u, 0u, 0u, 0u});
         __syncthreads();
       }
       if (busy) {  // uniform over the wave
-        if constexpr (decltype(all)::value) attend<kD, 2, true>(w, kt, vt, mask, a.c);
-        else attend<kD, 1, true>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c);
+        if constexpr (decltype(all)::value) attend<kD, kT / 32, true>(w, kt, vt, mask, a.c, col);
+        else attend<kD, 1, true>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c, col);
       }
     };
     auto all_tiles = [&](auto all) __attribute__((always_inline)) {  // all: every wave takes all tokens of a tile, for 32 rows of its own
@@ -405,17 +409,17 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
       }
     };
     if (tiles > 0) {  // (loops of their own: each one's registers)
-      if (wr == 4) all_tiles(std::true_type{});
-      else all_tiles(std::false_type{});
+      if (kShare > 1 || wr == 4) all_tiles(std::true_type{});
+      else if constexpr (kShare == 1) all_tiles(std::false_type{});
     }
   }
 
   // The waves' results meet in LDS (rows in 16-byte pieces, piece x of row r at
   // x ^ r), and leave it joined and in whole rows.
   __syncthreads();
-  constexpr int kOut = kD / 4;  // pieces of an output row
-  float* s_o = reinterpret_cast<float*>(part(wave));
+  constexpr int kOut = kCols<kD> / 4;  // pieces of a wave's part of an output row
   {
+    float* s_o = reinterpret_cast<float*>(part(wave));
     const int r = lane % 32, half = lane / 32;
     const float l = w.l + vtx::xshfl(w.l, 32);
     if (half == 0) {
@@ -423,29 +427,29 @@ __global__ __launch_bounds__(kThreads, kMinBlocks<kD>) void shared_prefix_attent
       s_l[wave][r] = l;
     }
 #pragma unroll
-    for (int d = 0; d < kD / 32; ++d)
+    for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int pc = (d * 8 + x * 2 + half) ^ (r % kOut);
-        *reinterpret_cast<float4*>(s_o + r * kD + pc * 4) =
+        *reinterpret_cast<float4*>(s_o + (r * kOut + pc) * 4) =
             float4{w.o[d][4 * x], w.o[d][4 * x + 1], w.o[d][4 * x + 2], w.o[d][4 * x + 3]};
       }
   }
   __syncthreads();
   const bool direct = it.out < 0;
   if (!direct && (long long)it.out + rows > a.max_rows) return;  // uniform
-  for (int x = tid; x < rows * kOut; x += kThreads) {
-    const int r = x / kOut, pc = x - r * kOut, rl = r % 32, blk = r / 32;
+  for (int x = tid; x < rows * (kD / 4); x += kThreads) {
+    const int r = x / (kD / 4), pc = x - r * (kD / 4), rl = r % 32, blk = r / 32;
+    const int share = pc / kOut, pw = pc % kOut;
     float M = -INFINITY;
-    for (int i = 0; i < wt; ++i) M = fmaxf(M, s_m[i * wr + blk][rl]);
+    for (int i = 0; i < wt; ++i) M = fmaxf(M, s_m[(i * wr + blk) * kShare + share][rl]);
     float L = 0.f;
     float4 O{0.f, 0.f, 0.f, 0.f};
     if (M != -INFINITY) {
       for (int i = 0; i < wt; ++i) {
-        const int v = i * wr + blk;
+        const int v = (i * wr + blk) * kShare + share;
         const float f = exp2_fast(s_m[v][rl] - M);
-        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(part(v)) + rl * kD +
-                                                          ((pc ^ (rl % kOut)) * 4));
+        const float4 y = reinterpret_cast<const float4*>(part(v))[rl * kOut + (pw ^ (rl % kOut))];
         L = fmaf(s_l[v][rl], f, L);
         O.x = fmaf(y.x, f, O.x);
         O.y = fmaf(y.y, f, O.y);
@@ -539,7 +543,7 @@ extern "C" int64_t vtx_shared_prefix_workspace_len(int32_t batch_size, int32_t n
   if (batch_size < 0 || num_kv_heads < 1 || cus <= 0 || !vtx_paged_decode_attention_supported(head_dim, group_size))
     return 0;
   const int64_t S = (int64_t)batch_size * num_kv_heads;
-  return S > kMaxSegments ? 0 : most_rows(S, group_size, aimed_items(head_dim, cus)) * (head_dim + 2);
+  return S > kMaxSegments ? 0 : most_rows(S, group_size, head_dim, aimed_items(head_dim, cus)) * (head_dim + 2);
 }
 
 extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o, const uint16_t* k_cache,
@@ -570,11 +574,11 @@ extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o
   const int cus = vtx::device_cu_count();
   if (cus <= 0) return vtx::fail(VTX_E_DEVICE, "%s: device query failed", what);
   const int64_t slots = aimed_items(head_dim, cus);
-  const Layout at = layout_of(S, most_items(S, group_size, slots));
+  const Layout at = layout_of(S, most_items(S, group_size, head_dim, slots));
   if (plan_len < at.size || reinterpret_cast<uintptr_t>(plan) % 32)
     return vtx::fail(VTX_E_INVALID, "%s: plan of %lld int32 (32-byte aligned) needed, got %lld", what,
                      (long long)at.size, (long long)plan_len);
-  const int64_t rows = most_rows(S, group_size, slots);
+  const int64_t rows = most_rows(S, group_size, head_dim, slots);
   if (workspace_len < rows * (head_dim + 2) || !vtx::aligned16(workspace))
     return vtx::fail(VTX_E_INVALID, "%s: workspace of %lld floats (16-byte aligned) needed, got %lld", what,
                      (long long)(rows * (head_dim + 2)), (long long)workspace_len);
@@ -591,7 +595,7 @@ extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o
   a.head = plan;
   a.items = reinterpret_cast<const Item*>(plan + at.items);
   a.combine = plan + at.combine;
-  a.max_items = (int32_t)most_items(S, group_size, slots);
+  a.max_items = (int32_t)most_items(S, group_size, head_dim, slots);
   a.B = batch_size;
   a.H = num_kv_heads;
   a.G = group_size;

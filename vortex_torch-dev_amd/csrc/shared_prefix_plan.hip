@@ -9,12 +9,13 @@
 // that each keeps at least its last page (the only one that may be partial).
 // The table decides: what ids promise is checked against the entries.
 //
-// Two launches: one workgroup per segment finds the length of the prefix it
-// has in common with the request before (the minimum of these over a run is
-// the run's); one workgroup then scans the segments, head by head, into runs,
-// and writes the work items of the attention: (rows of a run or a request) x
-// (pages of a chunk), at most kTileRows rows each, chunks sized so that all
-// items together are a few per workgroup slot of the device.
+// Two launches.  One wave per segment finds the length of the prefix that it
+// has in common with the request before (the minimum of these over a run is the
+// run's).  One workgroup then scans the segments, head by head, into runs, and
+// writes the work items of the attention: (rows of a run or a request) x
+// (entries of a chunk), tile_rows rows at most, chunks sized so that all items
+// together are one per workgroup slot of the device.  The second launch keeps
+// its tables in LDS (up to kLdsSegments segments; in the plan beyond).
 #include "vtx_shared_prefix.h"
 
 #include "vtx_device.h"
@@ -30,9 +31,9 @@ struct PlanArgs {
   int64_t indices_len;
   const int32_t* ids;
   int32_t B, H, G, P;
+  int32_t tile;       // rows of an item, at most
   int32_t slots;      // items aimed at
   int32_t max_items;  // room for
-  int32_t min_tokens; // of a chunk
   Layout at;
   int32_t* plan;
 };
@@ -46,44 +47,43 @@ __device__ __forceinline__ int pages_of(const PlanArgs& a, int s, int& start) {
 
 // common[s]: entries that segment (b, h) has in common with (b - 1, h), or -1
 // where no run goes through the two.
-constexpr int kCompareThreads = 256;
-constexpr int kAhead = 4;  // entries per thread and pass
-__global__ __launch_bounds__(kCompareThreads) void prefix_compare_kernel(PlanArgs a) {
-  __shared__ int s_first;
-  const int s = blockIdx.x, b = s / a.H;
-  int* out = a.plan + a.at.common + s;
+constexpr int kCompareWaves = 4;
+constexpr int kAhead = 8;  // entries per lane and pass
+__global__ __launch_bounds__(kCompareWaves* vtx::kWave) void prefix_compare_kernel(PlanArgs a) {
+  const int s = blockIdx.x * kCompareWaves + vtx::uniform(threadIdx.x / vtx::kWave), lane = vtx::lane_id();
+  if (s >= a.B * a.H) return;
+  const int b = s / a.H;
   int start, before;
   const int n = pages_of(a, s, start);
   const int m = b > 0 ? pages_of(a, s - a.H, before) : 0;
-  bool linked = n > 0 && m > 0;
-  if (linked)
-    linked = a.ids ? a.ids[b] == a.ids[b - 1] : a.indices[start] == a.indices[before];
-  if (!linked) {  // uniform
-    if (threadIdx.x == 0) *out = -1;
-    return;
-  }
-  const int len = min(n, m);
-  if (threadIdx.x == 0) s_first = len;
-  __syncthreads();
-  for (int at = 0; at < len; at += kCompareThreads * kAhead) {
-    int x[kAhead], y[kAhead];
+  const bool named = a.ids && b > 0;
+  const bool same = named ? a.ids[b] == a.ids[b - 1] : true;
+  int common = -1;
+  if (n > 0 && m > 0 && same) {  // uniform over the wave
+    const int len = min(n, m);
+    common = len;
+    for (int at = 0; at < len; at += vtx::kWave * kAhead) {
+      int x[kAhead], y[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = min(at + k * kCompareThreads + (int)threadIdx.x, len - 1);
-      x[k] = a.indices[start + (long long)i];
-      y[k] = a.indices[before + (long long)i];
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = min(at + k * vtx::kWave + lane, len - 1);
+        x[k] = a.indices[start + (long long)i];
+        y[k] = a.indices[before + (long long)i];
+      }
+      uint64_t differ[kAhead], any = 0;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) any |= differ[k] = __ballot(x[k] != y[k]);
+      if (any) {
+#pragma unroll
+        for (int k = kAhead - 1; k >= 0; --k)
+          if (differ[k]) common = at + k * vtx::kWave + __builtin_ctzll(differ[k]);
+        common = min(common, len - 1);  // (lanes past the end compare the last entry)
+        break;
+      }
     }
-    int first = len;
-#pragma unroll
-    for (int k = kAhead - 1; k >= 0; --k)
-      if (x[k] != y[k]) first = min(at + k * kCompareThreads + (int)threadIdx.x, len - 1);
-    if (first < len) atomicMin(&s_first, first);
-    __syncthreads();
-    const bool found = s_first < len;
-    __syncthreads();
-    if (found) break;  // uniform
+    if (!named && common == 0) common = -1;  // other first entries: another run
   }
-  if (threadIdx.x == 0) *out = s_first;
+  if (lane == 0) a.plan[a.at.common + s] = common;
 }
 
 constexpr int kPlanThreads = 1024;
@@ -132,7 +132,28 @@ __device__ __forceinline__ int chunks(int n, int per, int& pages) {
   return c > 0 ? (n + pages - 1) / pages : 0;
 }
 
+constexpr int kLdsSegments = 4096;
+
+// Per element i = h * B + b (a request's segment of a head; a run's numbers at
+// its first element), in LDS or in the plan.
+struct Tables {
+  int32_t *start, *pages, *first, *size, *shared, *run_items, *own_items, *run_rows, *own_rows;
+};
+__device__ __forceinline__ Tables tables_at(int32_t* p, int S) {
+  return Tables{p,         p + S,     p + 2 * S,     p + 3 * S,     p + 4 * S, p + 5 * S,
+                p + 6 * S + 1, p + 7 * S + 2, p + 8 * S + 2};
+}
+
+// How an element's work is cut: its run's (counted at the first element) and its own.
+struct Cut {
+  int tiles, run_chunks, run_pages;
+  int own_chunks, own_pages;
+  int used, size;  // shared pages that are read once; the run's requests
+};
+
+template <bool kLds>
 __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
+  __shared__ int32_t s_tables[kLds ? kScratchInts * kLdsSegments + 2 : 1];
   __shared__ int s_scan[kPlanWaves][4];
   __shared__ int s_run[kPlanWaves][2];
   __shared__ unsigned long long s_total;
@@ -140,21 +161,32 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
   const int each = (S + kPlanThreads - 1) / kPlanThreads;
   const int i0 = min(S, tid * each), i1 = min(S, i0 + each);
   int32_t* plan = a.plan;
-  const int32_t* common = plan + a.at.common;
-  int32_t* first = plan + a.at.scratch;  // of an element's run
-  int32_t* info = plan + a.at.segments;
-  auto seg = [&](int i) { return (i % a.B) * a.H + i / a.B; };  // element i = h * B + b
+  const Tables t = tables_at(kLds ? s_tables : plan + a.at.scratch, S);
+  auto segment = [&](int i) {
+    const int h = (int)((uint32_t)i / (uint32_t)a.B);
+    return (i - h * a.B) * a.H + h;
+  };
 
-  // 1. Runs.  Every element's run so far; a run's last element then has the
-  // run's minimum, and publishes (elements, pages) where its first one reads.
-  Run mine{-1, 0x7fffffff};
-  for (int i = i0; i < i1; ++i) {
-    const int s = seg(i);
+  // 1. What each element holds, and in `first` for now what it has in common
+  // with the one before.
+  if (tid == 0) s_total = 0;
+  for (int i = tid; i < S; i += kPlanThreads) {
+    const int s = segment(i);
     int start;
-    const int limit = pages_of(a, s, start) - 1;
-    const int c = i % a.B == 0 ? -1 : common[s];
-    mine = join(mine, c < 0 ? Run{i, limit} : Run{-1, min(c, limit)});
+    t.pages[i] = pages_of(a, s, start);
+    t.start[i] = start;
+    t.first[i] = plan[a.at.common + s];
   }
+  __syncthreads();
+
+  // 2. Runs, by a scan; a run's last element then has the run's minimum and
+  // leaves (requests, shared pages) at its first.
+  auto step = [&](int i) {
+    const int limit = t.pages[i] - 1, c = t.first[i];
+    return c < 0 ? Run{i, limit} : Run{-1, min(c, limit)};
+  };
+  Run mine{-1, 0x7fffffff};
+  for (int i = i0; i < i1; ++i) mine = join(mine, step(i));
   Run inc = mine;
 #pragma unroll
   for (int d = 1; d < vtx::kWave; d <<= 1) {
@@ -165,7 +197,7 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
     s_run[wave][0] = inc.start;
     s_run[wave][1] = inc.shared;
   }
-  if (tid == 0) s_total = 0;
+  const bool next_starts = i1 >= S || t.first[i1] < 0;  // (read before its thread writes over it)
   __syncthreads();
   Run at{-1, 0x7fffffff};
   for (int w = 0; w < wave; ++w) at = join(at, Run{s_run[w][0], s_run[w][1]});
@@ -174,144 +206,121 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
     if (lane > 0) at = join(at, o);
   }
   for (int i = i0; i < i1; ++i) {
-    const int s = seg(i);
-    int start;
-    const int limit = pages_of(a, s, start) - 1;
-    const int c = i % a.B == 0 ? -1 : common[s];
-    at = join(at, c < 0 ? Run{i, limit} : Run{-1, min(c, limit)});
-    first[i] = at.start;
-    const bool last = i + 1 == S || (i + 1) % a.B == 0 || common[seg(i + 1)] < 0;
-    if (last) {
-      const int n = i + 1 - at.start, h8 = kSegmentInts * at.start;
-      info[h8 + 0] = n;
-      info[h8 + 1] = n > 1 ? max(0, at.shared) : 0;
+    at = join(at, step(i));
+    t.first[i] = at.start;
+    if (i + 1 < i1 ? t.first[i + 1] < 0 : next_starts) {
+      const int n = i + 1 - at.start;
+      t.size[at.start] = n;
+      t.shared[at.start] = n > 1 ? max(0, at.shared) : 0;
     }
   }
   __syncthreads();
 
-  // 2. What is shared; the work in tokens x row tiles, and from it the chunks.
+  // 3. What is shared; the work in tokens x row tiles, and from it the chunks.
+  auto tiles_of = [&](int n) { return (int)(((long long)n * a.G + a.tile - 1) / a.tile); };
+  auto used_of = [&](int e) { return (long long)e * a.P >= kMinShared ? e : 0; };
   unsigned long long work = 0;
-  for (int i = i0; i < i1; ++i) {
-    const int s = seg(i), f = first[i], n = info[kSegmentInts * f], e = info[kSegmentInts * f + 1];
-    int start;
-    const int pages = pages_of(a, s, start);
+  for (int i = tid; i < S; i += kPlanThreads) {
+    const int s = segment(i), f = t.first[i], n = t.size[f], e = t.shared[f], used = used_of(e);
     plan[a.at.leaders + s] = f % a.B;
     plan[a.at.shared + s] = e;
-    const int used = (long long)e * a.P >= kMinShared ? e : 0;
-    const int tiles = (int)(((long long)n * a.G + kTileRows - 1) / kTileRows);
-    if (f == i) work += (unsigned long long)tiles * used * a.P;
-    work += (unsigned long long)(pages - used) * a.P;
+    if (f == i) work += (unsigned long long)tiles_of(n) * used * a.P;
+    work += (unsigned long long)(t.pages[i] - used) * a.P;
   }
   atomicAdd(&s_total, work);
   __syncthreads();
   const unsigned long long even = (s_total + a.slots - 1) / a.slots;
-  const int tokens = (int)min(max(even, (unsigned long long)a.min_tokens), 0x3fffffffull);
-  const int per = (int)((tokens + (long long)a.P - 1) / a.P);
+  const long long tokens = (long long)min(max(even, (unsigned long long)kMinChunk), 0x3fffffffull);
+  const int per = (int)((tokens + a.P - 1) / a.P);
 
-  // 3. Items and partial rows of every element: its run's (first element only)
-  // and its own.
-  Four count{{0, 0, 0, 0}};  // run items, own items, partial rows of runs, of requests
-  auto measure = [&](int i, int& tiles, int& rc, int& rp, int& oc, int& op, int& used, int& n) {
-    const int s = seg(i), f = first[i];
-    n = info[kSegmentInts * f];
-    const int e = info[kSegmentInts * f + 1];
-    int start;
-    const int pages = pages_of(a, s, start);
-    used = (long long)e * a.P >= kMinShared ? e : 0;
-    tiles = (int)(((long long)n * a.G + kTileRows - 1) / kTileRows);
-    rc = chunks(used, per, rp);
-    oc = chunks(pages - used, per, op);
+  // 4. Items and partial rows of every element, and their places by a scan.
+  auto cut = [&](int i) {
+    Cut c;
+    const int f = t.first[i];
+    c.size = t.size[f];
+    c.used = used_of(t.shared[f]);
+    c.tiles = tiles_of(c.size);
+    c.run_chunks = chunks(c.used, per, c.run_pages);
+    c.own_chunks = chunks(t.pages[i] - c.used, per, c.own_pages);
+    return c;
   };
+  auto count_of = [&](int i, const Cut& c) {
+    const bool head = t.first[i] == i, joined = c.run_chunks + c.own_chunks > 1;
+    return Four{{head ? c.tiles * c.run_chunks : 0, c.own_chunks, head ? c.size * a.G * c.run_chunks : 0,
+                 joined ? c.own_chunks * a.G : 0}};  // (a single partial result is the result)
+  };
+  Four count{{0, 0, 0, 0}};
   for (int i = i0; i < i1; ++i) {
-    int tiles, rc, rp, oc, op, used, n;
-    measure(i, tiles, rc, rp, oc, op, used, n);
-    if (first[i] == i) {
-      count.v[0] += tiles * rc;
-      count.v[2] += n * a.G * rc;
-    }
-    count.v[1] += oc;
-    count.v[3] += rc + oc > 1 ? oc * a.G : 0;  // (a single partial result is the result)
+    const Four x = count_of(i, cut(i));
+    for (int k = 0; k < 4; ++k) count.v[k] += x.v[k];
   }
   Four all;
   Four off = block_scan(count, s_scan, all);
-  int32_t* item_at = plan + a.at.offsets;  // run items before element i, own items before element i
   for (int i = i0; i < i1; ++i) {
-    int tiles, rc, rp, oc, op, used, n;
-    measure(i, tiles, rc, rp, oc, op, used, n);
-    item_at[i] = off.v[0];
-    item_at[S + 1 + i] = off.v[1];
-    int32_t* run_row = plan + a.at.rows + i;  // partial rows of the run, at its first element; of the request
-    if (first[i] == i) {
-      run_row[0] = off.v[2];
-      off.v[0] += tiles * rc;
-      off.v[2] += n * a.G * rc;
-    }
-    run_row[S] = all.v[2] + off.v[3];
-    off.v[1] += oc;
-    off.v[3] += rc + oc > 1 ? oc * a.G : 0;
+    const Four x = count_of(i, cut(i));
+    t.run_items[i] = off.v[0];
+    t.own_items[i] = off.v[1];
+    t.run_rows[i] = off.v[2];
+    t.own_rows[i] = all.v[2] + off.v[3];
+    for (int k = 0; k < 4; ++k) off.v[k] += x.v[k];
   }
-  const bool fits = all.v[0] + all.v[1] <= a.max_items;  // (always: slots and max_items belong together)
+  const int total = all.v[0] + all.v[1];
+  const bool fits = total <= a.max_items;  // (always: slots and max_items belong together)
   if (tid == 0) {
-    item_at[S] = all.v[0];
-    item_at[2 * S + 1] = all.v[1];
-    plan[kHeadRunItems] = fits ? all.v[0] : 0;
-    plan[kHeadOwnItems] = fits ? all.v[1] : 0;
-    plan[kHeadRows] = all.v[2] + all.v[3];
-  }
-  __syncthreads();
-
-  // 4. The items, every thread some of both kinds; the element by bisection.
-  if (fits) {
-    const int total = all.v[0] + all.v[1];
-    for (int k = tid; k < total; k += kPlanThreads) {
-      const bool run = k < all.v[0];
-      const int32_t* list = run ? item_at : item_at + S + 1;
-      const int j = run ? k : k - all.v[0];
-      int lo = 0, hi = S;  // list[lo] <= j < list[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (list[mid] <= j) lo = mid;
-        else hi = mid;
-      }
-      const int i = lo, in = j - list[i];
-      int tiles, rc, rp, oc, op, used, n;
-      measure(i, tiles, rc, rp, oc, op, used, n);
-      int start;
-      const int pages = pages_of(a, seg(i), start);
-      Item it;
-      it.segment = seg(i);
-      if (run) {  // the tiles of a chunk side by side: they read the same pages
-        const int c = in / tiles, t = in - c * tiles, rows = n * a.G;
-        it.row0 = t * kTileRows;
-        it.rows = min(rows - it.row0, kTileRows);
-        it.page0 = c * rp;
-        it.page1 = min(used, it.page0 + rp);
-        it.out = plan[a.at.rows + i] + c * rows + it.row0;
-      } else {
-        it.row0 = 0;
-        it.rows = a.G;
-        it.page0 = used + in * op;
-        it.page1 = min(pages, it.page0 + op);
-        it.out = rc + oc > 1 ? plan[a.at.rows + S + i] + in * a.G : -1;
-      }
-      it.reserved = 0;
-      it.last = it.page1 == pages ? 1 : 0;
-      reinterpret_cast<Item*>(plan + a.at.items)[k] = it;
-    }
+    t.run_items[S] = all.v[0];
+    t.own_items[S] = all.v[1];
+    plan[kHeadItems] = fits ? total : 0;
   }
   __syncthreads();
 
   // 5. Where the combine launch finds a segment's partial rows.
-  for (int i = i0; i < i1; ++i) {
-    int tiles, rc, rp, oc, op, used, n;
-    measure(i, tiles, rc, rp, oc, op, used, n);
-    const int f = first[i];
-    int32_t* to = plan + a.at.combine + (long long)kCombineInts * seg(i);
-    to[0] = plan[a.at.rows + f] + (i - f) * a.G;
-    to[1] = rc;
-    to[2] = n * a.G;
-    to[3] = plan[a.at.rows + S + i];
-    to[4] = oc;
+  for (int i = tid; i < S; i += kPlanThreads) {
+    const Cut c = cut(i);
+    const int f = t.first[i];
+    int4* to = reinterpret_cast<int4*>(plan + a.at.combine + (long long)kCombineInts * segment(i));
+    to[0] = int4{t.run_rows[f] + (i - f) * a.G, c.run_chunks, c.size * a.G, t.own_rows[i]};
+    to[1] = int4{c.own_chunks, 0, 0, 0};
+  }
+
+  // 6. The items, every thread some of both kinds; the element by bisection.
+  // Workgroup k of the attention runs on XCD k % 8: each XCD takes a stretch of
+  // the runs' items, the row tiles of a chunk side by side in it, so that a
+  // chunk's pages come into one L2 once.
+  const int per_xcd = all.v[0] / kXcds, more = all.v[0] % kXcds;
+  for (int k = tid; fits && k < total; k += kPlanThreads) {
+    const bool run = k < all.v[0];
+    const int x = k % kXcds;
+    const int32_t* list = run ? t.run_items : t.own_items;
+    const int j = run ? x * per_xcd + min(x, more) + k / kXcds : k - all.v[0];
+    int lo = 0, hi = S;  // list[lo] <= j < list[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (list[mid] <= j) lo = mid;
+      else hi = mid;
+    }
+    const int i = lo, in = j - list[i];
+    const Cut c = cut(i);
+    Item it;
+    it.segment = segment(i);
+    int page0;
+    if (run) {
+      const int chunk = in / c.tiles, tile = in - chunk * c.tiles, rows = c.size * a.G;
+      it.row0 = tile * a.tile;
+      it.rows = min(rows - it.row0, a.tile);
+      page0 = chunk * c.run_pages;
+      it.pages = min(c.used - page0, c.run_pages);
+      it.out = t.run_rows[i] + chunk * rows + it.row0;
+    } else {
+      it.row0 = 0;
+      it.rows = a.G;
+      page0 = c.used + in * c.own_pages;
+      it.pages = min(t.pages[i] - page0, c.own_pages);
+      it.out = c.run_chunks + c.own_chunks > 1 ? t.own_rows[i] + in * a.G : -1;
+    }
+    it.start = t.start[i] + page0;
+    it.last = page0 + it.pages == t.pages[i] ? 1 : 0;
+    it.reserved = 0;
+    reinterpret_cast<Item*>(plan + a.at.items)[k] = it;
   }
 }
 
@@ -319,20 +328,22 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
 
 namespace vtx_prefix {
 
-// Workgroups of the attention that the device holds at a time, and the items
-// that a plan aims at.
-int aimed_items(int head_dim, int cus) { return cus * (head_dim == 64 ? 6 : (head_dim == 128 ? 4 : 2)); }
+// Items that a plan aims at: the attention's workgroups that the device holds at
+// a time (chunks half as long: 256 requests of 8 heads each behind 16k tokens 225
+// us either way, 48 of one behind 32k, D 64, 47.4 us for 35.3, 64 of 4 behind 32k
+// 82.2 for 69.0: more partial results).
+int aimed_items(int head_dim, int cus) { return cus * (head_dim == 64 ? 3 : 2); }
 
-int64_t most_items(int64_t segments, int group_size, int64_t slots) {
+int64_t most_items(int64_t segments, int group_size, int head_dim, int64_t slots) {
   // Runs: tiles x ceil(pages / per) <= tiles x pages / per + tiles, at most one
   // run per two segments; requests: pages / per + 1 each.  The sums of x / per
   // are at most `slots` together.
-  return slots + segments + segments / 2 + segments * group_size / kTileRows + 1;
+  return slots + segments + segments / 2 + segments * group_size / tile_rows(head_dim) + 1;
 }
 
-int64_t most_rows(int64_t segments, int group_size, int64_t slots) {
-  // n * G rows per chunk of a run (at most kTileRows per tile), G per chunk of a request.
-  return slots * kTileRows + 2 * segments * group_size;
+int64_t most_rows(int64_t segments, int group_size, int head_dim, int64_t slots) {
+  // n * G rows per chunk of a run (at most tile_rows per tile), G per chunk of a request.
+  return slots * tile_rows(head_dim) + 2 * segments * group_size;
 }
 
 Layout layout_of(int64_t segments, int64_t items) {
@@ -348,10 +359,7 @@ Layout layout_of(int64_t segments, int64_t items) {
   l.combine = take(kCombineInts * segments);
   l.items = take((int64_t)(sizeof(Item) / sizeof(int32_t)) * items);
   l.common = take(segments);
-  l.scratch = take(segments);
-  l.segments = take(kSegmentInts * segments);
-  l.offsets = take(2 * (segments + 1));
-  l.rows = take(2 * segments);
+  l.scratch = take(segments > kLdsSegments ? kScratchInts * segments + 2 : 0);
   l.size = at;
   return l;
 }
@@ -365,7 +373,7 @@ extern "C" int64_t vtx_shared_prefix_plan_len(int32_t batch_size, int32_t num_kv
     return 0;
   const int64_t S = (int64_t)batch_size * num_kv_heads;
   if (S > kMaxSegments) return 0;
-  return layout_of(S, most_items(S, group_size, aimed_items(head_dim, cus))).size;
+  return layout_of(S, most_items(S, group_size, head_dim, aimed_items(head_dim, cus))).size;
 }
 
 extern "C" int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* kv_indices, int64_t kv_indices_len,
@@ -387,7 +395,7 @@ extern "C" int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* k
   if (cus <= 0) return vtx::fail(VTX_E_DEVICE, "plan_shared_prefix: device query failed");
   PlanArgs a;
   a.slots = aimed_items(head_dim, cus);
-  a.max_items = (int32_t)most_items(S, group_size, a.slots);
+  a.max_items = (int32_t)most_items(S, group_size, head_dim, a.slots);
   a.at = layout_of(S, a.max_items);
   if (plan_len < a.at.size || reinterpret_cast<uintptr_t>(plan) % 32)
     return vtx::fail(VTX_E_INVALID, "plan_shared_prefix: plan of %lld int32 (32-byte aligned) needed, got %lld",
@@ -400,10 +408,13 @@ extern "C" int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* k
   a.H = num_kv_heads;
   a.G = group_size;
   a.P = page_size;
-  a.min_tokens = kMinChunk;
+  a.tile = tile_rows(head_dim);
   a.plan = plan;
   hipStream_t s = vtx::as_stream(stream);
-  prefix_compare_kernel<<<(int)S, kCompareThreads, 0, s>>>(a);
-  prefix_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+  prefix_compare_kernel<<<(int)((S + kCompareWaves - 1) / kCompareWaves), kCompareWaves * vtx::kWave, 0, s>>>(a);
+  if (S <= kLdsSegments)
+    prefix_plan_kernel<true><<<1, kPlanThreads, 0, s>>>(a);
+  else
+    prefix_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(a);
   return vtx::check_launch("plan_shared_prefix");
 }
