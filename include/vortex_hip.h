@@ -745,7 +745,7 @@ int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* kv_indices, 
  * floats, 16-byte aligned, its contents neither read nor kept across calls;
  * calls that may overlap need one each.  A request's last bits depend on the
  * other requests of the table (how its tokens are divided).
- * head_dim 64, 128 or 256; group_size 1..8; at most 2^24 segments and 2^32
+ * head_dim 64, 128 or 256; group_size 1..8; at most 2^22 segments and 2^32
  * pool tokens (pool rows x page_size).
  */
 int64_t vtx_shared_prefix_workspace_len(int32_t batch_size, int32_t num_kv_heads, int32_t group_size,

@@ -44,17 +44,17 @@ struct SharedArgs {
   const int32_t* indices;
   int64_t indices_len;
   const int32_t* last_len;
-  const int32_t* head;     // plan header
+  const int32_t* counts;   // items of a head
   const Item* items;
   const int32_t* combine;  // [segments][kCombineInts]
-  int32_t max_items;
+  int32_t most_items;
   int32_t B, H, G, P, p_shift;
   float c;          // |scale| log2 e, or 1 for a scale of 0
   uint32_t q_sign;  // flips the queries' signs for a negative scale
   uint32_t q_keep;  // 0 for a scale of 0: no scores
   float* acc;       // [max_rows, D]
   float2* ml;       // [max_rows]
-  int64_t max_rows;
+  int64_t max_rows;  // of all heads
 };
 
 constexpr int kThreads = 256;
@@ -267,14 +267,14 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
   __shared__ float s_m[kWaves][32];
   __shared__ float s_l[kWaves][32];
 
-  const Item it = a.items[blockIdx.x];  // (room for as many; past the last one it is not used)
-  const int items = a.head[kHeadItems];
-  if ((int)blockIdx.x >= items || items > a.max_items) return;  // uniform
+  const int h = blockIdx.x % (uint32_t)a.H, nth = blockIdx.x / (uint32_t)a.H;
+  const Item it = a.items[(int64_t)h * a.most_items + nth];  // (past the head's last one not used)
+  if (nth >= a.counts[h]) return;  // uniform
   const int tid = threadIdx.x, lane = vtx::lane_id();
   const int wave = vtx::uniform(tid / vtx::kWave);
   const int seg = vtx::uniform(it.segment), S = a.B * a.H;
   if (seg < 0 || seg >= S) return;
-  const int b0 = seg / a.H, h = seg - b0 * a.H;
+  const int b0 = seg / a.H;
   const int rows = min(max(it.rows, 0), tile_rows(kD));
 
   // the item's tokens
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(kJoinRows* vtx::kWave) void shared_prefix_join_kern
 
 template <int kD>
 int launch(const SharedArgs& a, hipStream_t s) {
-  shared_prefix_attention_kernel<kD><<<a.max_items, kThreads, 0, s>>>(a);
+  shared_prefix_attention_kernel<kD><<<a.H * a.most_items, kThreads, 0, s>>>(a);
   const int rows = a.B * a.H * a.G;
   shared_prefix_join_kernel<kD><<<(rows + kJoinRows - 1) / kJoinRows, kJoinRows * vtx::kWave, 0, s>>>(a);
   return vtx::check_launch("shared_prefix_decode_attention");
@@ -542,8 +542,8 @@ extern "C" int64_t vtx_shared_prefix_workspace_len(int32_t batch_size, int32_t n
   const int cus = vtx::device_cu_count();
   if (batch_size < 0 || num_kv_heads < 1 || cus <= 0 || !vtx_paged_decode_attention_supported(head_dim, group_size))
     return 0;
-  const int64_t S = (int64_t)batch_size * num_kv_heads;
-  return S > kMaxSegments ? 0 : most_rows(S, group_size, head_dim, aimed_items(head_dim, cus)) * (head_dim + 2);
+  if ((int64_t)batch_size * num_kv_heads > kMaxSegments) return 0;
+  return layout_of(batch_size, num_kv_heads, group_size, head_dim, cus).most_rows * num_kv_heads * (head_dim + 2);
 }
 
 extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o, const uint16_t* k_cache,
@@ -573,12 +573,11 @@ extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o
     return vtx::fail(VTX_E_INVALID, "%s: q, o, k_cache and v_cache must be 16-byte aligned", what);
   const int cus = vtx::device_cu_count();
   if (cus <= 0) return vtx::fail(VTX_E_DEVICE, "%s: device query failed", what);
-  const int64_t slots = aimed_items(head_dim, cus);
-  const Layout at = layout_of(S, most_items(S, group_size, head_dim, slots));
+  const Layout at = layout_of(batch_size, num_kv_heads, group_size, head_dim, cus);
   if (plan_len < at.size || reinterpret_cast<uintptr_t>(plan) % 32)
     return vtx::fail(VTX_E_INVALID, "%s: plan of %lld int32 (32-byte aligned) needed, got %lld", what,
                      (long long)at.size, (long long)plan_len);
-  const int64_t rows = most_rows(S, group_size, head_dim, slots);
+  const int64_t rows = at.most_rows * num_kv_heads;
   if (workspace_len < rows * (head_dim + 2) || !vtx::aligned16(workspace))
     return vtx::fail(VTX_E_INVALID, "%s: workspace of %lld floats (16-byte aligned) needed, got %lld", what,
                      (long long)(rows * (head_dim + 2)), (long long)workspace_len);
@@ -592,10 +591,10 @@ extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o
   a.indices = kv_indices;
   a.indices_len = kv_indices_len;
   a.last_len = kv_last_page_len;
-  a.head = plan;
+  a.counts = plan + at.counts;
   a.items = reinterpret_cast<const Item*>(plan + at.items);
   a.combine = plan + at.combine;
-  a.max_items = (int32_t)most_items(S, group_size, head_dim, slots);
+  a.most_items = (int32_t)at.most_items;
   a.B = batch_size;
   a.H = num_kv_heads;
   a.G = group_size;

@@ -11,11 +11,11 @@
 //
 // Two launches.  One wave per segment finds the length of the prefix that it
 // has in common with the request before (the minimum of these over a run is the
-// run's).  One workgroup then scans the segments, head by head, into runs, and
-// writes the work items of the attention: (rows of a run or a request) x
-// (entries of a chunk), tile_rows rows at most, chunks sized so that all items
-// together are one per workgroup slot of the device.  The second launch keeps
-// its tables in LDS (up to kLdsSegments segments; in the plan beyond).
+// run's).  One workgroup per kv head then scans its requests into runs and
+// writes the head's work items: (rows of a run or a request) x (entries of a
+// chunk), tile_rows rows at most, chunks sized so that a head has its share of
+// the device's workgroup slots.  (One workgroup for all heads is bound by its
+// instructions: 2048 segments 21 us, 512 11.)
 #include "vtx_shared_prefix.h"
 
 #include "vtx_device.h"
@@ -31,9 +31,7 @@ struct PlanArgs {
   int64_t indices_len;
   const int32_t* ids;
   int32_t B, H, G, P;
-  int32_t tile;       // rows of an item, at most
-  int32_t slots;      // items aimed at
-  int32_t max_items;  // room for
+  int32_t tile_shift;  // log2 of an item's rows, at most
   Layout at;
   int32_t* plan;
 };
@@ -86,92 +84,88 @@ __global__ __launch_bounds__(kCompareWaves* vtx::kWave) void prefix_compare_kern
   if (lane == 0) a.plan[a.at.common + s] = common;
 }
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;
 constexpr int kPlanWaves = kPlanThreads / vtx::kWave;
 
 // Exclusive scan over the workgroup of four sums at a time; `all`: the totals.
 struct Four {
   int v[4];
 };
-__device__ __forceinline__ Four block_scan(Four x, int (*lds)[4], Four& all) {
+__device__ __forceinline__ Four block_scan(const Four& x, int (*lds)[4], Four& all) {
   const int wave = threadIdx.x / vtx::kWave, lane = vtx::lane_id();
-  Four inc = x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) inc.v[i] = (int)vtx::wave_prefix_sum((uint32_t)x.v[i]);
-  if (lane == vtx::kWave - 1)
-    for (int i = 0; i < 4; ++i) lds[wave][i] = inc.v[i];
-  __syncthreads();
   Four r;
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    int before = 0, total = 0;
-    for (int w = 0; w < kPlanWaves; ++w) {
-      before += w < wave ? lds[w][i] : 0;
-      total += lds[w][i];
-    }
-    r.v[i] = before + inc.v[i] - x.v[i];
-    all.v[i] = total;
+    const int inc = (int)vtx::wave_prefix_sum((uint32_t)x.v[i]);
+    if (lane == vtx::kWave - 1) lds[wave][i] = inc;
+    r.v[i] = inc - x.v[i];
+    all.v[i] = 0;
   }
   __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int y = lds[w][i];
+      r.v[i] += w < wave ? y : 0;
+      all.v[i] += y;
+    }
   return r;
 }
 
-// A stretch of segments in head-major order as the scan sees it: the run that
-// its last element lies in.
+// A stretch of a head's requests as the scan sees it: the run that its last
+// request lies in.
 struct Run {
-  int start;   // first element of that run, -1: before the stretch
-  int shared;  // minimum over the run's elements seen so far
+  int start;   // first request of that run, -1: before the stretch
+  int shared;  // minimum over the run's requests seen so far
 };
 __device__ __forceinline__ Run join(const Run& a, const Run& b) {
   return b.start >= 0 ? b : Run{a.start, min(a.shared, b.shared)};
 }
 
-// Units of up to `per` pages of n: their count, each of ceil(n / count) pages.
-__device__ __forceinline__ int chunks(int n, int per, int& pages) {
-  const int c = n > 0 ? (n + per - 1) / per : 0;
-  pages = c > 0 ? (n + c - 1) / c : 0;
-  return c > 0 ? (n + pages - 1) / pages : 0;
+// Chunks of up to `per` pages of n: their count, each of ceil(n / count) pages.
+__device__ __forceinline__ uint32_t chunks(uint32_t n, uint32_t per, uint32_t& pages) {
+  pages = 0;
+  if (n == 0) return 0;
+  const uint32_t c = (n + per - 1) / per;
+  pages = c == 1 ? n : (n + c - 1) / c;
+  return c == 1 ? 1 : (n + pages - 1) / pages;
 }
 
-constexpr int kLdsSegments = 4096;
+constexpr int kLdsRequests = 2048;
 
-// Per element i = h * B + b (a request's segment of a head; a run's numbers at
-// its first element), in LDS or in the plan.
+// Per request of the head (a run's numbers at its first one), in LDS or in the plan.
 struct Tables {
   int32_t *start, *pages, *first, *size, *shared, *run_items, *own_items, *run_rows, *own_rows;
 };
-__device__ __forceinline__ Tables tables_at(int32_t* p, int S) {
-  return Tables{p,         p + S,     p + 2 * S,     p + 3 * S,     p + 4 * S, p + 5 * S,
-                p + 6 * S + 1, p + 7 * S + 2, p + 8 * S + 2};
+__device__ __forceinline__ Tables tables_at(int32_t* p, int n) {
+  return Tables{p,         p + n,     p + 2 * n,     p + 3 * n,     p + 4 * n, p + 5 * n,
+                p + 6 * n + 1, p + 7 * n + 2, p + 8 * n + 2};
 }
 
-// How an element's work is cut: its run's (counted at the first element) and its own.
+// How a request's work is cut: its run's (counted at the first one) and its own.
 struct Cut {
-  int tiles, run_chunks, run_pages;
-  int own_chunks, own_pages;
+  uint32_t tiles, run_chunks, run_pages;
+  uint32_t own_chunks, own_pages;
   int used, size;  // shared pages that are read once; the run's requests
 };
 
 template <bool kLds>
 __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
-  __shared__ int32_t s_tables[kLds ? kScratchInts * kLdsSegments + 2 : 1];
+  __shared__ int32_t s_tables[kLds ? kScratchInts * kLdsRequests + 2 : 1];
   __shared__ int s_scan[kPlanWaves][4];
   __shared__ int s_run[kPlanWaves][2];
-  __shared__ unsigned long long s_total;
-  const int S = a.B * a.H, tid = threadIdx.x, wave = tid / vtx::kWave, lane = vtx::lane_id();
-  const int each = (S + kPlanThreads - 1) / kPlanThreads;
-  const int i0 = min(S, tid * each), i1 = min(S, i0 + each);
+  __shared__ unsigned long long s_total[kPlanWaves];
+  const int B = a.B, h = blockIdx.x, tid = threadIdx.x, wave = tid / vtx::kWave, lane = vtx::lane_id();
+  const int each = (B + kPlanThreads - 1) / kPlanThreads;
+  const int i0 = min(B, tid * each), i1 = min(B, i0 + each);
   int32_t* plan = a.plan;
-  const Tables t = tables_at(kLds ? s_tables : plan + a.at.scratch, S);
-  auto segment = [&](int i) {
-    const int h = (int)((uint32_t)i / (uint32_t)a.B);
-    return (i - h * a.B) * a.H + h;
-  };
+  const Tables t = tables_at(kLds ? s_tables : plan + a.at.scratch + (int64_t)h * (kScratchInts * (int64_t)B + 2), B);
 
-  // 1. What each element holds, and in `first` for now what it has in common
+  // 1. What each request holds, and in `first` for now what it has in common
   // with the one before.
-  if (tid == 0) s_total = 0;
-  for (int i = tid; i < S; i += kPlanThreads) {
-    const int s = segment(i);
+  for (int i = tid; i < B; i += kPlanThreads) {
+    const int s = i * a.H + h;
     int start;
     t.pages[i] = pages_of(a, s, start);
     t.start[i] = start;
@@ -179,7 +173,7 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
   }
   __syncthreads();
 
-  // 2. Runs, by a scan; a run's last element then has the run's minimum and
+  // 2. Runs, by a scan; a run's last request then has the run's minimum and
   // leaves (requests, shared pages) at its first.
   auto step = [&](int i) {
     const int limit = t.pages[i] - 1, c = t.first[i];
@@ -197,10 +191,12 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
     s_run[wave][0] = inc.start;
     s_run[wave][1] = inc.shared;
   }
-  const bool next_starts = i1 >= S || t.first[i1] < 0;  // (read before its thread writes over it)
+  const bool next_starts = i1 >= B || t.first[i1] < 0;  // (read before its thread writes over it)
   __syncthreads();
   Run at{-1, 0x7fffffff};
-  for (int w = 0; w < wave; ++w) at = join(at, Run{s_run[w][0], s_run[w][1]});
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w)
+    if (w < wave) at = join(at, Run{s_run[w][0], s_run[w][1]});
   {
     const Run o{__shfl_up(inc.start, 1), __shfl_up(inc.shared, 1)};
     if (lane > 0) at = join(at, o);
@@ -217,23 +213,28 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
   __syncthreads();
 
   // 3. What is shared; the work in tokens x row tiles, and from it the chunks.
-  auto tiles_of = [&](int n) { return (int)(((long long)n * a.G + a.tile - 1) / a.tile); };
+  auto tiles_of = [&](int n) { return (uint32_t)(n * a.G + (1 << a.tile_shift) - 1) >> a.tile_shift; };
   auto used_of = [&](int e) { return (long long)e * a.P >= kMinShared ? e : 0; };
-  unsigned long long work = 0;
-  for (int i = tid; i < S; i += kPlanThreads) {
-    const int s = segment(i), f = t.first[i], n = t.size[f], e = t.shared[f], used = used_of(e);
-    plan[a.at.leaders + s] = f % a.B;
+  unsigned long long work = 0;  // in pages
+  for (int i = tid; i < B; i += kPlanThreads) {
+    const int s = i * a.H + h, f = t.first[i], e = t.shared[f], used = used_of(e);
+    plan[a.at.leaders + s] = f;
     plan[a.at.shared + s] = e;
-    if (f == i) work += (unsigned long long)tiles_of(n) * used * a.P;
-    work += (unsigned long long)(t.pages[i] - used) * a.P;
+    if (f == i) work += (unsigned long long)tiles_of(t.size[f]) * used;
+    work += (unsigned long long)(t.pages[i] - used);
   }
-  atomicAdd(&s_total, work);
+#pragma unroll
+  for (int d = 1; d < vtx::kWave; d <<= 1) work += __shfl_xor(work, d);
+  if (lane == 0) s_total[wave] = work;
   __syncthreads();
-  const unsigned long long even = (s_total + a.slots - 1) / a.slots;
-  const long long tokens = (long long)min(max(even, (unsigned long long)kMinChunk), 0x3fffffffull);
-  const int per = (int)((tokens + a.P - 1) / a.P);
+  work = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) work += s_total[w];
+  // (rounded up: most_items counts on no fewer pages a chunk than work / slots)
+  const double even = (double)work / (double)a.at.slots * (1 + 1e-9) + 1;
+  const uint32_t per = max((uint32_t)(even < 1e9 ? even : 1e9), (uint32_t)(kMinChunk + a.P - 1) / (uint32_t)a.P);
 
-  // 4. Items and partial rows of every element, and their places by a scan.
+  // 4. Items and partial rows of every request, and their places by a scan.
   auto cut = [&](int i) {
     Cut c;
     const int f = t.first[i];
@@ -246,53 +247,64 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
   };
   auto count_of = [&](int i, const Cut& c) {
     const bool head = t.first[i] == i, joined = c.run_chunks + c.own_chunks > 1;
-    return Four{{head ? c.tiles * c.run_chunks : 0, c.own_chunks, head ? c.size * a.G * c.run_chunks : 0,
-                 joined ? c.own_chunks * a.G : 0}};  // (a single partial result is the result)
+    return Four{{head ? (int)(c.tiles * c.run_chunks) : 0, (int)c.own_chunks,
+                 head ? c.size * a.G * (int)c.run_chunks : 0,
+                 joined ? (int)c.own_chunks * a.G : 0}};  // (a single partial result is the result)
   };
   Four count{{0, 0, 0, 0}};
   for (int i = i0; i < i1; ++i) {
     const Four x = count_of(i, cut(i));
+#pragma unroll
     for (int k = 0; k < 4; ++k) count.v[k] += x.v[k];
   }
   Four all;
   Four off = block_scan(count, s_scan, all);
+  const int row0 = (int)(h * a.at.most_rows);
+  off.v[2] += row0;
+  off.v[3] += row0 + all.v[2];
   for (int i = i0; i < i1; ++i) {
-    const Four x = count_of(i, cut(i));
     t.run_items[i] = off.v[0];
     t.own_items[i] = off.v[1];
     t.run_rows[i] = off.v[2];
-    t.own_rows[i] = all.v[2] + off.v[3];
-    for (int k = 0; k < 4; ++k) off.v[k] += x.v[k];
+    t.own_rows[i] = off.v[3];
+    if (i + 1 < i1) {
+      const Four x = count_of(i, cut(i));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) off.v[k] += x.v[k];
+    }
   }
   const int total = all.v[0] + all.v[1];
-  const bool fits = total <= a.max_items;  // (always: slots and max_items belong together)
+  const bool fits = total <= a.at.most_items;  // (always: slots and most_items belong together)
   if (tid == 0) {
-    t.run_items[S] = all.v[0];
-    t.own_items[S] = all.v[1];
-    plan[kHeadItems] = fits ? total : 0;
+    t.run_items[B] = all.v[0];
+    t.own_items[B] = all.v[1];
+    plan[a.at.counts + h] = fits ? total : 0;
   }
   __syncthreads();
 
   // 5. Where the combine launch finds a segment's partial rows.
-  for (int i = tid; i < S; i += kPlanThreads) {
+  for (int i = tid; i < B; i += kPlanThreads) {
     const Cut c = cut(i);
     const int f = t.first[i];
-    int4* to = reinterpret_cast<int4*>(plan + a.at.combine + (long long)kCombineInts * segment(i));
-    to[0] = int4{t.run_rows[f] + (i - f) * a.G, c.run_chunks, c.size * a.G, t.own_rows[i]};
-    to[1] = int4{c.own_chunks, 0, 0, 0};
+    int4* to = reinterpret_cast<int4*>(plan + a.at.combine + (long long)kCombineInts * (i * a.H + h));
+    to[0] = int4{t.run_rows[f] + (i - f) * a.G, (int)c.run_chunks, c.size * a.G, t.own_rows[i]};
+    to[1] = int4{(int)c.own_chunks, 0, 0, 0};
   }
 
-  // 6. The items, every thread some of both kinds; the element by bisection.
-  // Workgroup k of the attention runs on XCD k % 8: each XCD takes a stretch of
-  // the runs' items, the row tiles of a chunk side by side in it, so that a
-  // chunk's pages come into one L2 once.
-  const int per_xcd = all.v[0] / kXcds, more = all.v[0] % kXcds;
+  // 6. The items, every thread some of both kinds; the request by bisection.
+  // Item k of head h is workgroup k * H + h of the attention, on XCD (k * H + h)
+  // % 8: the head's items go round `rounds` XCDs, and each of these takes a
+  // stretch of the runs' items, the row tiles of a chunk side by side in it, so
+  // that a chunk's pages come into one L2 once.
+  const int rounds = kXcds / ((a.H & -a.H) < kXcds ? (a.H & -a.H) : kXcds);
+  const int stretch = all.v[0] / rounds, more = all.v[0] % rounds;
+  Item* items = reinterpret_cast<Item*>(plan + a.at.items) + h * a.at.most_items;
   for (int k = tid; fits && k < total; k += kPlanThreads) {
     const bool run = k < all.v[0];
-    const int x = k % kXcds;
+    const int x = k & (rounds - 1);
     const int32_t* list = run ? t.run_items : t.own_items;
-    const int j = run ? x * per_xcd + min(x, more) + k / kXcds : k - all.v[0];
-    int lo = 0, hi = S;  // list[lo] <= j < list[hi]
+    const int j = run ? x * stretch + min(x, more) + k / rounds : k - all.v[0];
+    int lo = 0, hi = B;  // list[lo] <= j < list[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (list[mid] <= j) lo = mid;
@@ -301,26 +313,26 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
     const int i = lo, in = j - list[i];
     const Cut c = cut(i);
     Item it;
-    it.segment = segment(i);
+    it.segment = i * a.H + h;
     int page0;
     if (run) {
-      const int chunk = in / c.tiles, tile = in - chunk * c.tiles, rows = c.size * a.G;
-      it.row0 = tile * a.tile;
-      it.rows = min(rows - it.row0, a.tile);
+      const int chunk = (uint32_t)in / c.tiles, tile = in - chunk * c.tiles, rows = c.size * a.G;
+      it.row0 = tile << a.tile_shift;
+      it.rows = min(rows - it.row0, 1 << a.tile_shift);
       page0 = chunk * c.run_pages;
-      it.pages = min(c.used - page0, c.run_pages);
+      it.pages = min(c.used - page0, (int)c.run_pages);
       it.out = t.run_rows[i] + chunk * rows + it.row0;
     } else {
       it.row0 = 0;
       it.rows = a.G;
       page0 = c.used + in * c.own_pages;
-      it.pages = min(t.pages[i] - page0, c.own_pages);
+      it.pages = min(t.pages[i] - page0, (int)c.own_pages);
       it.out = c.run_chunks + c.own_chunks > 1 ? t.own_rows[i] + in * a.G : -1;
     }
     it.start = t.start[i] + page0;
     it.last = page0 + it.pages == t.pages[i] ? 1 : 0;
     it.reserved = 0;
-    reinterpret_cast<Item*>(plan + a.at.items)[k] = it;
+    items[k] = it;
   }
 }
 
@@ -328,26 +340,21 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
 
 namespace vtx_prefix {
 
-// Items that a plan aims at: the attention's workgroups that the device holds at
-// a time (chunks half as long: 256 requests of 8 heads each behind 16k tokens 225
-// us either way, 48 of one behind 32k, D 64, 47.4 us for 35.3, 64 of 4 behind 32k
-// 82.2 for 69.0: more partial results).
-int aimed_items(int head_dim, int cus) { return cus * (head_dim == 64 ? 3 : 2); }
-
-int64_t most_items(int64_t segments, int group_size, int head_dim, int64_t slots) {
-  // Runs: tiles x ceil(pages / per) <= tiles x pages / per + tiles, at most one
-  // run per two segments; requests: pages / per + 1 each.  The sums of x / per
-  // are at most `slots` together.
-  return slots + segments + segments / 2 + segments * group_size / tile_rows(head_dim) + 1;
-}
-
-int64_t most_rows(int64_t segments, int group_size, int head_dim, int64_t slots) {
-  // n * G rows per chunk of a run (at most tile_rows per tile), G per chunk of a request.
-  return slots * tile_rows(head_dim) + 2 * segments * group_size;
-}
-
-Layout layout_of(int64_t segments, int64_t items) {
+Layout layout_of(int64_t batch, int64_t heads, int group_size, int head_dim, int cus) {
   Layout l;
+  const int64_t segments = batch * heads, tile = tile_rows(head_dim);
+  // All heads' items together: the workgroups that the device holds at a time.
+  // (Twice as many, each half as long: 256 requests of 8 heads each behind 16k
+  // tokens 225 us either way, 48 of one behind 32k, D 64, 47.4 us for 35.3, 64 of
+  // 4 behind 32k 82.2 for 69.0: more partial results.)
+  const int64_t slots = cus * (head_dim == 64 ? 3 : 2);
+  l.slots = (slots + heads - 1) / heads;
+  // Runs: tiles x ceil(pages / per) <= tiles x pages / per + tiles, at most one run
+  // per two requests; requests: pages / per + 1 each.  The sums of x / per are at
+  // most `slots` together.
+  l.most_items = l.slots + batch + batch / 2 + batch * group_size / tile + 2;
+  // n * G rows per chunk of a run (at most `tile` per tile), G per chunk of a request.
+  l.most_rows = l.slots * tile + 2 * batch * group_size;
   int64_t at = kHeadInts;
   auto take = [&](int64_t n) {
     const int64_t r = at;
@@ -357,9 +364,10 @@ Layout layout_of(int64_t segments, int64_t items) {
   l.leaders = take(segments);
   l.shared = take(segments);
   l.combine = take(kCombineInts * segments);
-  l.items = take((int64_t)(sizeof(Item) / sizeof(int32_t)) * items);
+  l.counts = take(heads);
+  l.items = take((int64_t)(sizeof(Item) / sizeof(int32_t)) * l.most_items * heads);
   l.common = take(segments);
-  l.scratch = take(segments > kLdsSegments ? kScratchInts * segments + 2 : 0);
+  l.scratch = take(batch > kLdsRequests ? kScratchInts * segments + 2 * heads : 0);
   l.size = at;
   return l;
 }
@@ -371,9 +379,8 @@ extern "C" int64_t vtx_shared_prefix_plan_len(int32_t batch_size, int32_t num_kv
   const int cus = vtx::device_cu_count();
   if (batch_size < 0 || num_kv_heads < 1 || cus <= 0 || !vtx_paged_decode_attention_supported(head_dim, group_size))
     return 0;
-  const int64_t S = (int64_t)batch_size * num_kv_heads;
-  if (S > kMaxSegments) return 0;
-  return layout_of(S, most_items(S, group_size, head_dim, aimed_items(head_dim, cus))).size;
+  if ((int64_t)batch_size * num_kv_heads > kMaxSegments) return 0;
+  return layout_of(batch_size, num_kv_heads, group_size, head_dim, cus).size;
 }
 
 extern "C" int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* kv_indices, int64_t kv_indices_len,
@@ -394,9 +401,7 @@ extern "C" int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* k
   const int cus = vtx::device_cu_count();
   if (cus <= 0) return vtx::fail(VTX_E_DEVICE, "plan_shared_prefix: device query failed");
   PlanArgs a;
-  a.slots = aimed_items(head_dim, cus);
-  a.max_items = (int32_t)most_items(S, group_size, head_dim, a.slots);
-  a.at = layout_of(S, a.max_items);
+  a.at = layout_of(batch_size, num_kv_heads, group_size, head_dim, cus);
   if (plan_len < a.at.size || reinterpret_cast<uintptr_t>(plan) % 32)
     return vtx::fail(VTX_E_INVALID, "plan_shared_prefix: plan of %lld int32 (32-byte aligned) needed, got %lld",
                      (long long)a.at.size, (long long)plan_len);
@@ -408,13 +413,11 @@ extern "C" int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* k
   a.H = num_kv_heads;
   a.G = group_size;
   a.P = page_size;
-  a.tile = tile_rows(head_dim);
+  a.tile_shift = vtx::log2_exact(tile_rows(head_dim));
   a.plan = plan;
   hipStream_t s = vtx::as_stream(stream);
   prefix_compare_kernel<<<(int)((S + kCompareWaves - 1) / kCompareWaves), kCompareWaves * vtx::kWave, 0, s>>>(a);
-  if (S <= kLdsSegments)
-    prefix_plan_kernel<true><<<1, kPlanThreads, 0, s>>>(a);
-  else
-    prefix_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(a);
+  if (batch_size <= kLdsRequests) prefix_plan_kernel<true><<<num_kv_heads, kPlanThreads, 0, s>>>(a);
+  else prefix_plan_kernel<false><<<num_kv_heads, kPlanThreads, 0, s>>>(a);
   return vtx::check_launch("plan_shared_prefix");
 }

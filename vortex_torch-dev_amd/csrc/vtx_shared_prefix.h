@@ -12,11 +12,9 @@ constexpr int tile_rows(int head_dim) { return head_dim == 256 ? 64 : 128; }
 constexpr int kMinShared = 128;  // tokens from which a run's pages are read once for all
 constexpr int kMinChunk = 128;   // tokens of a chunk, at least
 constexpr int kXcds = 8;
-constexpr int64_t kMaxSegments = 1 << 24;
+constexpr int64_t kMaxSegments = 1 << 22;
 
-// Header, int32 each.
-constexpr int kHeadItems = 0;
-constexpr int kHeadInts = 16;
+constexpr int kHeadInts = 16;  // before everything else
 
 // One workgroup's work: `rows` query rows of the requests from the segment's
 // on (row0 + r: request (row0 + r) / G after it, head (row0 + r) % G) against
@@ -33,18 +31,16 @@ struct alignas(32) Item {
 // Per segment: first partial row of its run's chunks, their count, rows from one
 // to the next, first partial row of its own chunks (G rows each), their count.
 constexpr int kCombineInts = 8;
-constexpr int kScratchInts = 9;  // per segment, and 2 more (planner only)
+constexpr int kScratchInts = 9;  // per segment, and 2 more per head (planner only)
 
-// Places in the plan, in int32.
+// Sizes and places (in int32) of a plan.  Each kv head has a list of items of its
+// own, item k of head h at items + 8 (h * most_items + k), and rows of its own.
 struct Layout {
-  int64_t leaders, shared, combine, items;
+  int64_t leaders, shared, combine, counts, items;
   int64_t common, scratch;  // planner only
   int64_t size;
+  int64_t slots, most_items, most_rows;  // of a head
 };
-
-int aimed_items(int head_dim, int cus);
-int64_t most_items(int64_t segments, int group_size, int head_dim, int64_t slots);
-int64_t most_rows(int64_t segments, int group_size, int head_dim, int64_t slots);
-Layout layout_of(int64_t segments, int64_t items);
+Layout layout_of(int64_t batch, int64_t heads, int group_size, int head_dim, int cus);
 
 }  // namespace vtx_prefix
