@@ -470,29 +470,44 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
   }
 }
 
-// One wave per query row: the row's partial results, weighted.
-constexpr int kJoinRows = 4;
-template <int kD>
-__global__ __launch_bounds__(kJoinRows* vtx::kWave) void shared_prefix_join_kernel(SharedArgs a) {
-  constexpr int kCols = kD / vtx::kWave;
-  const int row = blockIdx.x * kJoinRows + vtx::uniform(threadIdx.x / vtx::kWave);
-  const int lane = vtx::lane_id();
-  if (row >= a.B * a.H * a.G) return;
+// A query row's partial results, weighted: by one wave, or by four that take
+// every fourth batch of them and meet in LDS (few rows have many: 384 rows of 64
+// columns with about 60 each XX us by one wave, XX by four; 16,384 of 128 with 5
+// XX and XX).  A partial row is read in 16-byte pieces, kAtOnce rows side by side
+// in the wave; before it reads them, lane i weighs the i-th of up to 64 rows.
+constexpr int kJoinWaves = 4;
+constexpr int kJoinRowsOfFour = 2048;  // query rows up to which four waves take one
+template <int kD, bool kFour>
+__global__ __launch_bounds__(kJoinWaves* vtx::kWave) void shared_prefix_join_kernel(SharedArgs a) {
+  constexpr int kPieces = kD / 4, kAtOnce = vtx::kWave / kPieces;
+  constexpr int kAhead = 8;  // loads in flight
+  constexpr int kBatch = kFour ? kAtOnce * kAhead : vtx::kWave;
+  __shared__ float s_ml[kFour ? kJoinWaves : 1][2];
+  __shared__ float4 s_o[kFour ? kJoinWaves : 1][kPieces];
+  const int wave = vtx::uniform(threadIdx.x / vtx::kWave), lane = vtx::lane_id();
+  const int row = kFour ? blockIdx.x : blockIdx.x * kJoinWaves + wave;
+  if (row >= a.B * a.H * a.G) return;  // uniform over the waves that meet
   const int seg = row / a.G, g = row - seg * a.G;
   const int32_t* info = a.combine + (long long)kCombineInts * seg;
   const int run_row = info[0], run_n = info[1], run_step = info[2], own_row = info[3], own_n = info[4];
-  if (run_n + own_n == 1 && run_n == 0) return;  // written by its item
+  if (run_n == 0 && own_n == 1) return;  // written by its item
+  const int n = run_n + own_n, sub = lane / kPieces, piece = lane % kPieces;
   auto at = [&](int i) -> long long {
-    return i < run_n ? run_row + (long long)i * run_step + g : own_row + (long long)(i - run_n) * a.G + g;
+    const long long r = i < run_n ? run_row + (long long)i * run_step + g : own_row + (long long)(i - run_n) * a.G + g;
+    return r >= 0 && r < a.max_rows ? r : 0;
   };
-  const int n = run_n + own_n;
-  float M = -INFINITY, L = 0.f, O[kCols];
+  float M = -INFINITY, L = 0.f;
+  float4 O{0.f, 0.f, 0.f, 0.f};
+  for (int i0 = kFour ? wave * kBatch : 0; i0 < n; i0 += kFour ? kJoinWaves * kBatch : kBatch) {
+    const int live = min(n - i0, kBatch);
+    float4 x[kAhead];
+    auto read = [&](int c) {
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) O[j] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += vtx::kWave) {  // 64 at a time, lane i the (max, sum) of the i-th
-    const int live = min(n - i0, vtx::kWave);
-    const long long mine = at(i0 + min(lane, live - 1));
-    const float2 ml = mine >= 0 && mine < a.max_rows ? a.ml[mine] : float2{-INFINITY, 0.f};
+      for (int u = 0; u < kAhead; ++u)
+        x[u] = reinterpret_cast<const float4*>(a.acc)[at(i0 + min(c + u * kAtOnce + sub, live - 1)) * kPieces + piece];
+    };
+    const float2 ml = a.ml[at(i0 + min(lane, live - 1))];
+    read(0);
     float mx = ml.x;
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) mx = fmaxf(mx, vtx::xshfl(mx, d));
@@ -501,37 +516,73 @@ __global__ __launch_bounds__(kJoinRows* vtx::kWave) void shared_prefix_join_kern
     const float f = exp2_fast(M - nm);
     const float wgt = lane < live ? exp2_fast(ml.x - nm) : 0.f;
     L = fmaf(L, f, vtx::wave_sum(wgt * ml.y));
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) O[j] *= f;
+    O.x *= f;
+    O.y *= f;
+    O.z *= f;
+    O.w *= f;
     M = nm;
-    constexpr int kAhead = 8;
-    for (int i = 0; i < live; i += kAhead) {
-      float x[kAhead][kCols];
+    for (int c = 0; c < live; c += kAtOnce * kAhead) {
+      if (c > 0) read(c);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        long long r = at(i0 + min(i + u, live - 1));
-        r = r >= 0 && r < a.max_rows ? r : 0;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) x[u][j] = a.acc[r * kD + j * vtx::kWave + lane];
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const float wu = i + u < live ? __uint_as_float(vtx::lane_value(__float_as_uint(wgt), min(i + u, 63))) : 0.f;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) O[j] = i + u < live ? fmaf(x[u][j], wu, O[j]) : O[j];
+        const int i = c + u * kAtOnce + sub;
+        const float wu = __shfl(wgt, min(i, vtx::kWave - 1));
+        const bool on = i < live;  // (an unwritten row may hold anything)
+        O.x = on ? fmaf(x[u].x, wu, O.x) : O.x;
+        O.y = on ? fmaf(x[u].y, wu, O.y) : O.y;
+        O.z = on ? fmaf(x[u].z, wu, O.z) : O.z;
+        O.w = on ? fmaf(x[u].w, wu, O.w) : O.w;
       }
     }
   }
-  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN);
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) a.o[(long long)row * kD + j * vtx::kWave + lane] = (uint16_t)vtx::f32_to_bf16(O[j] * inv);
+  for (int d = kPieces; d < vtx::kWave; d <<= 1) {
+    O.x += vtx::xshfl(O.x, d);
+    O.y += vtx::xshfl(O.y, d);
+    O.z += vtx::xshfl(O.z, d);
+    O.w += vtx::xshfl(O.w, d);
+  }
+  if constexpr (kFour) {
+    if (lane == 0) {
+      s_ml[wave][0] = M;
+      s_ml[wave][1] = L;
+    }
+    if (lane < kPieces) s_o[wave][lane] = O;
+    __syncthreads();
+    if (threadIdx.x >= kPieces) return;
+    M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) M = fmaxf(M, s_ml[w][0]);
+    L = 0.f;
+    O = float4{0.f, 0.f, 0.f, 0.f};
+    if (M != -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < kJoinWaves; ++w) {
+        const float f = exp2_fast(s_ml[w][0] - M);
+        const float4 y = s_o[w][threadIdx.x];
+        L = fmaf(s_ml[w][1], f, L);
+        O.x = fmaf(y.x, f, O.x);
+        O.y = fmaf(y.y, f, O.y);
+        O.z = fmaf(y.z, f, O.z);
+        O.w = fmaf(y.w, f, O.w);
+      }
+    }
+  } else {
+    if (lane >= kPieces) return;
+  }
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN);
+  reinterpret_cast<uint2*>(a.o + (long long)row * kD)[kFour ? threadIdx.x : lane] =
+      uint2{vtx::bf16_pair(O.x * inv, O.y * inv), vtx::bf16_pair(O.z * inv, O.w * inv)};
 }
 
 template <int kD>
 int launch(const SharedArgs& a, hipStream_t s) {
   shared_prefix_attention_kernel<kD><<<a.H * a.most_items, kThreads, 0, s>>>(a);
   const int rows = a.B * a.H * a.G;
-  shared_prefix_join_kernel<kD><<<(rows + kJoinRows - 1) / kJoinRows, kJoinRows * vtx::kWave, 0, s>>>(a);
+  if (rows <= kJoinRowsOfFour)
+    shared_prefix_join_kernel<kD, true><<<rows, kJoinWaves * vtx::kWave, 0, s>>>(a);
+  else
+    shared_prefix_join_kernel<kD, false><<<(rows + kJoinWaves - 1) / kJoinWaves, kJoinWaves * vtx::kWave, 0, s>>>(a);
   return vtx::check_launch("shared_prefix_decode_attention");
 }
 
