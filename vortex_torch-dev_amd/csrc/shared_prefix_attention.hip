@@ -480,7 +480,7 @@ constexpr int kJoinRowsOfFour = 2048;  // query rows up to which four waves take
 template <int kD, bool kFour>
 __global__ __launch_bounds__(kJoinWaves* vtx::kWave) void shared_prefix_join_kernel(SharedArgs a) {
   constexpr int kPieces = kD / 4, kAtOnce = vtx::kWave / kPieces;
-  constexpr int kAhead = 8;  // loads in flight
+  constexpr int kAhead = kFour ? 8 : 4;  // loads in flight
   constexpr int kBatch = kFour ? kAtOnce * kAhead : vtx::kWave;
   __shared__ float s_ml[kFour ? kJoinWaves : 1][2];
   __shared__ float4 s_o[kFour ? kJoinWaves : 1][kPieces];

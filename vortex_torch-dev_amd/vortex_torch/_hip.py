@@ -296,6 +296,46 @@ def device_cu_count(dev: torch.device) -> int:
     return _cu_counts[idx]
 
 
+_PLAIN_TYPES = frozenset({torch.Tensor, int, float, bool, type(None)})
+
+
+def _plain_positional(fn):
+    """_plain_args for wrappers that take positional arguments only: a call
+    without tensor subclasses costs one look at each argument's type."""
+    import functools
+
+    @functools.wraps(fn)
+    def wrapper(*args):
+        for a in args:
+            if type(a) not in _PLAIN_TYPES:
+                return fn(*[_plain(x) for x in args])
+        return fn(*args)
+
+    return wrapper
+
+
+def _device_index(*tensors: torch.Tensor) -> int:
+    """_require_gpu, as the tensors' device index."""
+    index = tensors[0].get_device()
+    if index >= 0:
+        for t in tensors:
+            if t.get_device() != index:
+                break
+        else:
+            if _pre_launch is not None:
+                _pre_launch()
+            return index
+    dev = _require_gpu(*tensors)
+    return -1 if dev is None or dev.index is None else dev.index
+
+
+def _elsewhere(index: int, call):
+    """call(the current stream of device `index`) with that device current."""
+    dev = torch.device("cuda", index)
+    with _on_device(dev):
+        return call(_stream(dev))
+
+
 class _on_device:
     """Makes `dev` current for the duration of a launch (no-op if it already is)."""
 
@@ -1075,85 +1115,132 @@ def _rows_distinct(t: torch.Tensor) -> bool:
     return (hs >= d and ts >= (h - 1) * hs + d) or (ts >= d and hs >= (n - 1) * ts + d)
 
 
-@_plain_args
-def set_kv_buffer_rope(k_cache, v_cache, q, new_k, new_v, loc, page_size: int, positions, cos_sin_cache,
-                       interleaved: bool = False, q_out=None):
-    """set_kv_buffer with the position rotation of q [nnz, Hq, D] (or None) and
-    new_k on the way; returns the rotated queries (q_out, or a new tensor)."""
-    lib = load_library()
-    given = q_out is not None
-    if q is None and given:
-        raise RuntimeError("vortex_torch: q_out without q")
-    tensors = [k_cache, v_cache, new_k, new_v, loc, positions, cos_sin_cache]
+def _rope_fits(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache) -> bool:
+    """Whether a call without q_out is well-formed beyond doubt, in one look
+    (otherwise _rope_refusal says what is wrong, if anything)."""
+    new, pools, dtype = new_k.shape, k_cache.shape, new_k.dtype
+    if len(new) != 3 or len(pools) != 3 or new_v.shape != new or v_cache.shape != pools or dtype not in _ROPE_DTYPES:
+        return False
+    nnz, H, D = new
+    kp, vp, pool = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() * k_cache.element_size()
     if q is not None:
-        tensors.append(q)
-    if given:
-        tensors.append(q_out)
-    dev = _require_gpu(*tensors)
-    _req(loc, torch.int64, "loc")
-    _req(positions, torch.int64, "positions")
-    _req(cos_sin_cache, torch.float32, "cos_sin_cache")
+        like = q.shape
+        if len(like) != 3 or like[0] != nnz or like[2] != D or q.dtype is not dtype or q.stride(2) != 1 \
+                or kp <= q.data_ptr() < kp + pool or vp <= q.data_ptr() < vp + pool:
+            return False
+    return (H > 0 and D > 0 and pools[2] == D and pools[1] == page_size and pools[0] % H == 0
+            and new_v.dtype is dtype and k_cache.dtype is dtype and v_cache.dtype is dtype
+            and new_k.stride(2) == 1 and new_v.stride(2) == 1 and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and loc.dtype is torch.int64 and positions.dtype is torch.int64 and cos_sin_cache.dtype is torch.float32
+            and loc.is_contiguous() and positions.is_contiguous() and cos_sin_cache.is_contiguous()
+            and loc.numel() >= nnz and positions.numel() >= nnz and cos_sin_cache.dim() == 2
+            and (kp + pool <= vp or vp + pool <= kp)
+            and not (kp <= new_k.data_ptr() < kp + pool or vp <= new_k.data_ptr() < vp + pool)
+            and not (kp <= new_v.data_ptr() < kp + pool or vp <= new_v.data_ptr() < vp + pool))
+
+
+def _rope_refusal(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache, q_out) -> str:
+    """What is wrong with the arguments of set_kv_buffer_rope ("": nothing)."""
+    for t, dtype, n in ((loc, torch.int64, "loc"), (positions, torch.int64, "positions"),
+                        (cos_sin_cache, torch.float32, "cos_sin_cache")):
+        if t.dtype != dtype:
+            return f"{n} must be {dtype}, got {t.dtype}"
+        if not t.is_contiguous():
+            return f"{n} must be contiguous"
     if new_k.dim() != 3 or new_v.shape != new_k.shape:
-        raise RuntimeError("vortex_torch: new_k and new_v must both be [nnz, num_kv_heads, head_dim]")
+        return "new_k and new_v must both be [nnz, num_kv_heads, head_dim]"
     dtype = new_k.dtype
     if dtype not in _ROPE_DTYPES:
-        raise RuntimeError(f"vortex_torch: new_k must be bfloat16, float16 or float32, got {dtype}")
+        return f"new_k must be bfloat16, float16 or float32, got {dtype}"
     nnz, H, D = new_k.shape
-    named = [(k_cache, "k_cache"), (v_cache, "v_cache"), (new_v, "new_v")]
-    Hq = 0
+    rows = [(new_k, "new_k"), (new_v, "new_v")]
     if q is not None:
         if q.dim() != 3 or q.shape[0] != nnz or q.shape[2] != D:
-            raise RuntimeError(f"vortex_torch: q must be [{nnz}, q_heads, {D}], got {tuple(q.shape)}")
-        Hq = q.shape[1]
-        named.append((q, "q"))
-        if given:
+            return f"q must be [{nnz}, q_heads, {D}], got {tuple(q.shape)}"
+        rows.append((q, "q"))
+        if q_out is not None:
             if q_out.shape != q.shape:
-                raise RuntimeError(f"vortex_torch: q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
-            named.append((q_out, "q_out"))
-    for t, n in named:
+                return f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}"
+            rows.append((q_out, "q_out"))
+    elif q_out is not None:
+        return "q_out without q"
+    for t, n in rows + [(k_cache, "k_cache"), (v_cache, "v_cache")]:
         if t.dtype != dtype:
-            raise RuntimeError(f"vortex_torch: {n} is {t.dtype}, new_k is {dtype}")
-    for t, n in [(new_k, "new_k")] + named[2:]:
+            return f"{n} is {t.dtype}, new_k is {dtype}"
+    for t, n in rows:
         if D > 1 and t.stride(2) != 1:
-            raise RuntimeError(f"vortex_torch: {n} must have dense rows (a last stride of 1)")
+            return f"{n} must have dense rows (a last stride of 1)"
     if not k_cache.is_contiguous() or not v_cache.is_contiguous():
-        raise RuntimeError("vortex_torch: k_cache and v_cache must be contiguous")
+        return "k_cache and v_cache must be contiguous"
     if k_cache.dim() != 3 or k_cache.shape != v_cache.shape or k_cache.shape[2] != D or k_cache.shape[1] != page_size:
-        raise RuntimeError(f"vortex_torch: k_cache and v_cache must be [pages * H, {page_size}, {D}]")
+        return f"k_cache and v_cache must be [pages * H, {page_size}, {D}]"
     if k_cache.shape[0] % max(H, 1):
-        raise RuntimeError(f"vortex_torch: the pools' {k_cache.shape[0]} rows are not pages of {H} kv heads")
+        return f"the pools' {k_cache.shape[0]} rows are not pages of {H} kv heads"
     if loc.numel() < nnz or positions.numel() < nnz:
-        raise RuntimeError("vortex_torch: loc or positions shorter than the new tokens")
+        return "loc or positions shorter than the new tokens"
     if cos_sin_cache.dim() != 2:
-        raise RuntimeError("vortex_torch: cos_sin_cache must be [positions, rotary_dim]")
-    kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
-    pool = k_cache.numel() * k_cache.element_size()
+        return "cos_sin_cache must be [positions, rotary_dim]"
+    kp, vp, pool = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() * k_cache.element_size()
     if pool and -pool < kp - vp < pool:
-        raise RuntimeError("vortex_torch: k_cache and v_cache share memory")
-    for t, n in [(new_k, "new_k")] + named[2:]:
-        p = t.data_ptr()
-        if kp <= p < kp + pool or vp <= p < vp + pool:
-            raise RuntimeError(f"vortex_torch: {n} lies in the pools that the call writes")
+        return "k_cache and v_cache share memory"
+    for t, n in rows:
+        if kp <= t.data_ptr() < kp + pool or vp <= t.data_ptr() < vp + pool:
+            return f"{n} lies in the pools that the call writes"
+    if q_out is not None and q_out.numel():
+        if not _rows_distinct(q_out):
+            return "q_out has rows that share memory"
+        in_place = q_out.data_ptr() == q.data_ptr() and q_out.stride() == q.stride()
+        for t, n in ((q, "q"), (new_k, "new_k"), (new_v, "new_v")):
+            if not (in_place and t is q) and not _tokens_apart(q_out, t):
+                return f"q_out shares memory with {n}"
+    return ""
+
+
+@_plain_positional
+def set_kv_buffer_rope(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache, interleaved, q_out):
+    """set_kv_buffer with the position rotation of q [nnz, Hq, D] (or None) and
+    new_k on the way; returns the rotated queries (q_out, or a new tensor)."""
+    lib = _lib or load_library()
+    if q is None:
+        index = _device_index(new_k, k_cache, v_cache, new_v, loc, positions, cos_sin_cache)
+    elif q_out is None:
+        index = _device_index(new_k, k_cache, v_cache, q, new_v, loc, positions, cos_sin_cache)
+    else:
+        index = _device_index(new_k, k_cache, v_cache, q, new_v, loc, positions, cos_sin_cache, q_out)
+    if q_out is not None or not _rope_fits(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache):
+        wrong = _rope_refusal(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache, q_out)
+        if wrong:
+            raise RuntimeError("vortex_torch: " + wrong)
+    nnz, H, D = new_k.shape
+    Hq, qp, op, q0, q1, o0, o1 = 0, None, None, 0, 0, 0, 0
     if q is not None:
-        if not given:
-            q_out = torch.empty((nnz, Hq, D), dtype=dtype, device=dev)
-        elif nnz and Hq:
-            if not _rows_distinct(q_out):
-                raise RuntimeError("vortex_torch: q_out has rows that share memory")
-            in_place = q_out.data_ptr() == q.data_ptr() and q_out.stride() == q.stride()
-            for t, n in ((q, "q"), (new_k, "new_k"), (new_v, "new_v")):
-                if not (in_place and t is q) and not _tokens_apart(q_out, t):
-                    raise RuntimeError(f"vortex_torch: q_out shares memory with {n}")
-    strides = _EightI64(*(q.stride()[:2] if Hq else (0, 0)), *(q_out.stride()[:2] if Hq else (0, 0)),
-                        *new_k.stride()[:2], *new_v.stride()[:2])
-    with _on_device(dev):
-        rc = lib.vtx_set_kv_buffer_rope(
-            kp, vp, k_cache.shape[0] * k_cache.shape[1], q.data_ptr() if Hq else None,
-            q_out.data_ptr() if Hq else None, new_k.data_ptr(), new_v.data_ptr(), strides, loc.data_ptr(),
-            positions.data_ptr(), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], nnz, Hq, H, D,
-            cos_sin_cache.shape[1], _ROPE_DTYPES[dtype], int(page_size), 1 if interleaved else 0, _stream(dev))
-    _check(rc, "set_kv_buffer_rope")
+        Hq = q.shape[1]
+        if q_out is None:
+            q_out = q.new_empty((nnz, Hq, D))
+        if Hq:
+            qp, op = q.data_ptr(), q_out.data_ptr()
+            q0, q1, _ = q.stride()
+            o0, o1, _ = q_out.stride()
+    k0, k1, _ = new_k.stride()
+    v0, v1, _ = new_v.stride()
+    table_rows, rotary = cos_sin_cache.shape
+    args = (k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() // D if D else 0, qp, op, new_k.data_ptr(),
+            new_v.data_ptr(), _EightI64(q0, q1, o0, o1, k0, k1, v0, v1), loc.data_ptr(), positions.data_ptr(),
+            cos_sin_cache.data_ptr(), table_rows, nnz, Hq, H, D, rotary, _ROPE_DTYPES[new_k.dtype], page_size,
+            1 if interleaved else 0)
+    if _raw_stream is not None and _current_device() == index:
+        rc = lib.vtx_set_kv_buffer_rope(*args, _raw_stream(index))
+    else:
+        rc = _elsewhere(index, lambda stream: lib.vtx_set_kv_buffer_rope(*args, stream))
+    if rc:
+        _check(rc, "set_kv_buffer_rope")
     return q_out
+
+
+def _scratch_lasts(stream: int) -> bool:
+    from . import _deferred
+
+    return _deferred.scratch_lasts(stream)
 
 
 def _scratch(floats: int, dev: torch.device, stream: int):
@@ -1161,9 +1248,7 @@ def _scratch(floats: int, dev: torch.device, stream: int):
     where the call does without: inside a capture that torch did not begin (the
     memory would be others' while the graph still uses it), or with no memory
     left (a call that is given its output needs none)."""
-    from . import _deferred
-
-    if floats <= 0 or not _deferred.scratch_lasts(stream):
+    if floats <= 0 or not _scratch_lasts(stream):
         return None
     try:
         return torch.empty(floats, dtype=torch.float32, device=dev)
@@ -1203,80 +1288,101 @@ def paged_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_las
     _check(rc, "paged_decode_attention")
 
 
-@_plain_args
-def plan_shared_prefix(kv_indptr, kv_indices, group_ids, batch_size: int, num_kv_heads: int, group_size: int,
-                       head_dim: int, page_size: int, plan=None):
+_BF16, _I32 = torch.bfloat16, torch.int32
+
+
+def _tables_fit(*tables) -> bool:
+    for t in tables:
+        if t.dtype is not _I32 or not t.is_contiguous():
+            return False
+    return True
+
+
+@_plain_positional
+def plan_shared_prefix(kv_indptr, kv_indices, group_ids, batch_size, num_kv_heads, group_size, head_dim, page_size,
+                       plan):
     """Writes the shared-prefix plan of a block table into `plan` (int32), or
     into a new tensor; returns it."""
-    lib = load_library()
-    more = [t for t in (group_ids, plan) if t is not None]
-    dev = _require_gpu(kv_indptr, kv_indices, *more)
-    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (group_ids, "group_ids"), (plan, "plan")):
-        if t is not None:
-            _req(t, torch.int32, n)
-    B, H, G, D = int(batch_size), int(num_kv_heads), int(group_size), int(head_dim)
-    if B < 0 or H < 1 or int(page_size) < 1:
+    lib = _lib or load_library()
+    given = [t for t in (kv_indptr, kv_indices, group_ids, plan) if t is not None]
+    index = _device_index(*given)
+    if not _tables_fit(*given):
+        for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (group_ids, "group_ids"), (plan, "plan")):
+            if t is not None:
+                _req(t, _I32, n)
+    B, H, G, D = batch_size, num_kv_heads, group_size, head_dim
+    if B < 0 or H < 1 or page_size < 1:
         raise RuntimeError("vortex_torch: batch_size, num_kv_heads and page_size must be positive")
-    if not paged_decode_attention_supported(D, G):
+    if plan is None and not lib.vtx_paged_decode_attention_supported(D, G):
         raise RuntimeError(f"vortex_torch: head_dim {D} with {G} query heads per kv head not supported")
     if kv_indptr.numel() < B * H + 1:
         raise RuntimeError(f"vortex_torch: kv_indptr needs {B * H + 1} entries")
     if group_ids is not None and group_ids.numel() < B:
         raise RuntimeError(f"vortex_torch: group_ids needs {B} entries")
-    with _on_device(dev):
-        stream = _stream(dev)
-        if plan is None:
-            from . import _deferred
 
-            if not _deferred.scratch_lasts(stream):
+    def launch(stream):
+        nonlocal plan
+        if plan is None:
+            if not _scratch_lasts(stream):
                 raise RuntimeError("vortex_torch: a capture that torch did not begin needs a plan made before it")
-            plan = torch.empty(max(lib.vtx_shared_prefix_plan_len(B, H, G, D), 16), dtype=torch.int32, device=dev)
-        rc = lib.vtx_plan_shared_prefix(
+            plan = kv_indptr.new_empty(max(lib.vtx_shared_prefix_plan_len(B, H, G, D), 16))
+        return lib.vtx_plan_shared_prefix(
             kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
-            None if group_ids is None else group_ids.data_ptr(), B, H, G, D, int(page_size), plan.data_ptr(),
-            plan.numel(), stream)
-    _check(rc, "plan_shared_prefix")
+            None if group_ids is None else group_ids.data_ptr(), B, H, G, D, page_size, plan.data_ptr(), plan.numel(),
+            stream)
+
+    if _raw_stream is not None and _current_device() == index:
+        rc = launch(_raw_stream(index))
+    else:
+        rc = _elsewhere(index, launch)
+    if rc:
+        _check(rc, "plan_shared_prefix")
     return plan
 
 
-@_plain_args
-def shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan,
-                                   batch_size: int, num_kv_heads: int, group_size: int, sm_scale: float) -> None:
+@_plain_positional
+def shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan, batch_size,
+                                   num_kv_heads, group_size, sm_scale) -> None:
     """paged_decode_attention with the pages that a plan found shared read once
     per run.  Its partial results need scratch from torch's allocator; without
     (see _scratch) paged decode attention itself runs, which needs none."""
-    lib = load_library()
-    dev = _require_gpu(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan)
-    for t, n in ((q, "q"), (o, "o"), (k_cache, "k_cache"), (v_cache, "v_cache")):
-        _req(t, torch.bfloat16, n)
-    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (kv_last_page_len, "kv_last_page_len"),
-                 (plan, "plan")):
-        _req(t, torch.int32, n)
-    if k_cache.dim() != 3 or v_cache.shape != k_cache.shape:
+    lib = _lib or load_library()
+    index = _device_index(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan)
+    if not (q.dtype is _BF16 and o.dtype is _BF16 and k_cache.dtype is _BF16 and v_cache.dtype is _BF16
+            and q.is_contiguous() and o.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and _tables_fit(kv_indptr, kv_indices, kv_last_page_len, plan)):
+        for t, n in ((q, "q"), (o, "o"), (k_cache, "k_cache"), (v_cache, "v_cache")):
+            _req(t, _BF16, n)
+        for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (kv_last_page_len, "kv_last_page_len"),
+                     (plan, "plan")):
+            _req(t, _I32, n)
+    pools = k_cache.shape
+    if len(pools) != 3 or v_cache.shape != pools:
         raise RuntimeError("vortex_torch: k_cache and v_cache must both be [pages * H, page_size, head_dim]")
-    rows, P, D = k_cache.shape
-    B, H, G = int(batch_size), int(num_kv_heads), int(group_size)
-    if q.numel() != B * H * G * D or o.numel() != q.numel():
+    rows, P, D = pools
+    B, H, G = batch_size, num_kv_heads, group_size
+    if q.numel() != B * H * G * D or o.numel() != B * H * G * D:
         raise RuntimeError("vortex_torch: q and o must hold batch * kv heads * group rows of head_dim")
     if kv_indptr.numel() < B * H + 1 or kv_last_page_len.numel() < B * H:
         raise RuntimeError(f"vortex_torch: kv_indptr needs {B * H + 1} and kv_last_page_len {B * H} entries")
-    with _on_device(dev):
-        stream = _stream(dev)
+
+    def launch(stream):
         args = (q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), rows, kv_indptr.data_ptr(),
                 kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr())
         floats = lib.vtx_shared_prefix_workspace_len(B, H, G, D)
-        ws = _scratch(floats, dev, stream)
+        ws = _scratch(floats, q.device, stream)
         if ws is None and floats > 0:
-            rc = lib.vtx_paged_decode_attention(*args, B, H, G, D, P, float(sm_scale), stream)
-        else:
-            rc = lib.vtx_shared_prefix_decode_attention(
-                *args, plan.data_ptr(), plan.numel(), B, H, G, D, P, float(sm_scale),
-                None if ws is None else ws.data_ptr(), floats, stream)
-    _check(rc, "shared_prefix_decode_attention")
+            return lib.vtx_paged_decode_attention(*args, B, H, G, D, P, sm_scale, stream)
+        return lib.vtx_shared_prefix_decode_attention(
+            *args, plan.data_ptr(), plan.numel(), B, H, G, D, P, sm_scale, None if ws is None else ws.data_ptr(),
+            floats, stream)
 
-
-def paged_decode_attention_supported(head_dim: int, group_size: int) -> bool:
-    return bool(load_library().vtx_paged_decode_attention_supported(int(head_dim), int(group_size)))
+    if _raw_stream is not None and _current_device() == index:
+        rc = launch(_raw_stream(index))
+    else:
+        rc = _elsewhere(index, launch)
+    if rc:
+        _check(rc, "shared_prefix_decode_attention")
 
 
 def bf16_rounding_check(device="cuda") -> tuple:

@@ -43,8 +43,8 @@ def set_kv_buffer_rope(k_cache: torch.Tensor, v_cache: torch.Tensor, q: Optional
     with a position outside the table is skipped, its ``q_out`` rows unwritten.
     Tokens of a call need slots of their own: where two share one, each value
     there is either's."""
-    return _hip.set_kv_buffer_rope(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache,
-                                   interleaved, q_out)
+    return _hip.set_kv_buffer_rope(k_cache, v_cache, q, new_k, new_v, loc, int(page_size), positions, cos_sin_cache,
+                                   bool(interleaved), q_out)
 
 
 __all__ = ["set_kv_buffer_launcher", "set_kv_buffer_rope"]
