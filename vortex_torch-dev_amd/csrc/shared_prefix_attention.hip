@@ -40,6 +40,7 @@ struct SharedArgs {
   const uint16_t* k;
   const uint16_t* v;
   int64_t rows;  // pool rows (page * H + h)
+  uint32_t pool_bytes;  // 0: over 4 GiB
   const int32_t* indptr;
   const int32_t* indices;
   int64_t indices_len;
@@ -68,6 +69,7 @@ typedef __attribute__((address_space(3))) s16x4 lds4;
 
 // Classes of instructions for the scheduler's groups.
 constexpr int kSchedValu = 0x2, kSchedMfma = 0x8, kSchedRead = 0x100;
+constexpr int kWeighOps = 24;  // instructions of a step's weights
 
 // LDS rows of a tile are kD bf16 in 16-byte pieces; piece c of token t lies at
 // c ^ swizzle(t), so that the 8 (or 16) tokens of a K read, at one c, and the
@@ -88,11 +90,29 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Copies 16 bytes per lane to LDS: lane l's to `to` (uniform) + 16 l.
-__device__ __forceinline__ void copy16(const void* from, void* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-}
+// Copies from a pool straight to LDS, 16 bytes per lane: lane l's, `at` elements
+// into the pool, to `to` (uniform) + 16 l.  Pools of up to 4 GiB (kFar false) take
+// buffer loads: 32-bit offsets, and LDS reads behind a copy in flight are waited
+// for one by one; behind the other form, which counts as an LDS operation too, the
+// compiler waits for all of them (256 requests of 8 heads each behind 16k tokens:
+// XX us a layer and XX).
+template <bool kFar>
+struct Pool {
+  const uint16_t* base;
+  __amdgpu_buffer_rsrc_t buffer;
+  __device__ __forceinline__ Pool(const uint16_t* p, uint32_t bytes) : base(p) {
+    if constexpr (!kFar) buffer = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x27000);
+  }
+  __device__ __forceinline__ void copy(uint32_t row, int log2_row, uint32_t within, void* to) const {
+    auto* lds = (__attribute__((address_space(3))) void*)to;
+    if constexpr (kFar) {
+      const uint16_t* from = base + (((uint64_t)row << log2_row) + within);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, lds, 16, 0, 0);
+    } else {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, lds, 16, (int)(((row << log2_row) + within) * 2u), 0, 0, 0);
+    }
+  }
+};
 // Waits for this wave's copies (and other loads).
 __device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
@@ -198,10 +218,8 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
     w.m = nm;
   }
   const float base = w.m == -INFINITY ? 0.f : w.m;
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    if constexpr (!kAhead) read_v(k, f[0]);
-    else if (k + 1 < kSteps) read_v(k + 1, f[(k + 1) & 1]);
+  // P of step k: 16 tokens
+  auto weigh = [&](int k) {
     uint32_t p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -209,17 +227,40 @@ __device__ __forceinline__ void attend(Rows<kD>& w, const unsigned char* kt, con
       p[i] = vtx::bf16_pair(exp2_fast(fmaf(s[k / 2][x], c, -base)), exp2_fast(fmaf(s[k / 2][x + 1], c, -base)));
       w.l = vtx::dot2_bf16(p[i], 0x3f803f80u, w.l);
     }
-    const vtx::U4 b = vtx::U4{p[0], p[1], p[2], p[3]};
+    return vtx::U4{p[0], p[1], p[2], p[3]};
+  };
+  auto product = [&](const vtx::U4& b, const s16x4 (&f)[kBlocks][2]) {
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d) {
-      const s16x8 a = __builtin_shufflevector(f[kAhead ? k & 1 : 0][d][0], f[kAhead ? k & 1 : 0][d][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      const s16x8 a = __builtin_shufflevector(f[d][0], f[d][1], 0, 1, 2, 3, 4, 5, 6, 7);
       w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
                                                        w.o[d], 0, 0, 0);
     }
-    if constexpr (kAhead) {
-      if (k + 1 < kSteps) __builtin_amdgcn_sched_group_barrier(kSchedRead, 2 * kBlocks, 1);
-      __builtin_amdgcn_sched_group_barrier(kSchedValu, 24, 1);
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kBlocks, 1);
+  };
+  if constexpr (kAhead) {
+    // The weights of a step between the products of the one before, its V reads
+    // before them.
+    if (kSteps > 1) read_v(1, f[1]);
+    vtx::U4 b = weigh(0);
+    __builtin_amdgcn_sched_group_barrier(kSchedRead, kSteps > 1 ? 2 * kBlocks : 0, 1);
+    __builtin_amdgcn_sched_group_barrier(kSchedValu, kWeighOps, 1);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      product(b, f[k & 1]);
+      if (k + 1 < kSteps) b = weigh(k + 1);
+      if (k + 2 < kSteps) read_v(k + 2, f[k & 1]);
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
+        if (k + 1 < kSteps) __builtin_amdgcn_sched_group_barrier(kSchedValu, kWeighOps / kBlocks, 1);
+      }
+      if (k + 2 < kSteps) __builtin_amdgcn_sched_group_barrier(kSchedRead, 2 * kBlocks, 1);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      read_v(k, f[0]);
+      product(weigh(k), f[0]);
     }
   }
 }
@@ -251,7 +292,7 @@ __device__ __forceinline__ bool resolve(const SharedArgs& a, const Entry& e, uin
   return ok;
 }
 
-template <int kD>
+template <int kD, bool kFar>
 __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_attention_kernel(SharedArgs a) {
   constexpr int kRow = kD * 2;
   constexpr int kPieces = kD / 8;
@@ -358,6 +399,8 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
     constexpr uint64_t kFull = kT == 64 ? ~0ull : (1ull << kT) - 1;
     constexpr int kPass = vtx::kWave / kPieces;  // tokens per wave-wide copy
     constexpr int kCopies = kT / (kPass * kWaves);
+    constexpr int kLog2 = kD == 64 ? 6 : (kD == 128 ? 7 : 8);
+    const Pool<kFar> pool_k(a.k, a.pool_bytes), pool_v(a.v, a.pool_bytes);
     const int tiles = (tk.count + kT - 1) / kT;
     const int col = half_col * (kCols<kD> / 8);
     const bool busy = rb * 32 < rows && tb * 32 < kT;
@@ -373,9 +416,9 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
         const int t0 = (i * kWaves + wave) * kPass, t = t0 + lane / kPieces;
-        const uint64_t at = (uint64_t)(uint32_t)__shfl((int)row, t) * kD + ((lane % kPieces) ^ swizzle<kD>(t)) * 8;
-        copy16(a.k + at, kt + t0 * kRow);
-        copy16(a.v + at, vt + t0 * kRow);
+        const uint32_t from = (uint32_t)__shfl((int)row, t), within = ((lane % kPieces) ^ swizzle<kD>(t)) * 8;
+        pool_k.copy(from, kLog2, within, kt + t0 * kRow);
+        pool_v.copy(from, kLog2, within, vt + t0 * kRow);
       }
     };
     auto tile = [&](auto all, uint64_t mask, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
@@ -577,7 +620,8 @@ __global__ __launch_bounds__(kJoinWaves* vtx::kWave) void shared_prefix_join_ker
 
 template <int kD>
 int launch(const SharedArgs& a, hipStream_t s) {
-  shared_prefix_attention_kernel<kD><<<a.H * a.most_items, kThreads, 0, s>>>(a);
+  if (a.pool_bytes) shared_prefix_attention_kernel<kD, false><<<a.H * a.most_items, kThreads, 0, s>>>(a);
+  else shared_prefix_attention_kernel<kD, true><<<a.H * a.most_items, kThreads, 0, s>>>(a);
   const int rows = a.B * a.H * a.G;
   if (rows <= kJoinRowsOfFour)
     shared_prefix_join_kernel<kD, true><<<rows, kJoinWaves * vtx::kWave, 0, s>>>(a);
@@ -638,6 +682,8 @@ extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o
   a.k = k_cache;
   a.v = v_cache;
   a.rows = cache_rows;
+  const int64_t bytes = cache_rows * page_size * head_dim * 2;
+  a.pool_bytes = bytes <= 0xffffffffLL ? (uint32_t)bytes : 0u;
   a.indptr = kv_indptr;
   a.indices = kv_indices;
   a.indices_len = kv_indices_len;
