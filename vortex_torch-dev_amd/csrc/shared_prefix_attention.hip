@@ -481,6 +481,32 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
   __syncthreads();
   const bool direct = it.out < 0;
   if (!direct && (long long)it.out + rows > a.max_rows) return;  // uniform
+  if (wt == 1) {  // uniform: nothing to join (and never direct: more than G rows)
+    auto leave = [&](const unsigned char* from, int v) __attribute__((always_inline)) {
+      const int r0 = (v / kShare) * 32, c0 = (v % kShare) * kCols<kD>;
+      if (direct || r0 >= rows) return;  // uniform
+      constexpr int kEach = 32 * kOut / kThreads;
+      float4 y[kEach];
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        const int x = u * kThreads + tid, rl = x / kOut, pw = x % kOut;
+        y[u] = reinterpret_cast<const float4*>(from)[rl * kOut + (pw ^ (rl % kOut))];
+      }
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        const int x = u * kThreads + tid, rl = x / kOut, pw = x % kOut;
+        if (r0 + rl < rows)
+          *reinterpret_cast<float4*>(a.acc + ((long long)it.out + r0 + rl) * kD + c0 + pw * 4) = y[u];
+      }
+    };
+    leave(s_k0, 0);
+    leave(s_v0, 1);
+    leave(s_k1, 2);
+    leave(s_v1, 3);
+    if (!direct && tid < rows) a.ml[(long long)it.out + tid] =
+        float2{s_m[tid / 32 * kShare][tid % 32], s_l[tid / 32 * kShare][tid % 32]};
+    return;
+  }
   for (int x = tid; x < rows * (kD / 4); x += kThreads) {
     const int r = x / (kD / 4), pc = x - r * (kD / 4), rl = r % 32, blk = r / 32;
     const int share = pc / kOut, pw = pc % kOut;
