@@ -56,6 +56,7 @@ struct SharedArgs {
   float* acc;       // [max_rows, D]
   float2* ml;       // [max_rows]
   int64_t max_rows;  // of all heads
+  bool join_four;
 };
 
 constexpr int kThreads = 256;
@@ -292,6 +293,49 @@ __device__ __forceinline__ bool resolve(const SharedArgs& a, const Entry& e, uin
   return ok;
 }
 
+// A result row: four columns of it from sums O and L.
+__device__ __forceinline__ uint2 result4(const float4& O, float L) {
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN);
+  return uint2{vtx::bf16_pair(O.x * inv, O.y * inv), vtx::bf16_pair(O.z * inv, O.w * inv)};
+}
+
+// A wave's output to its stretch of LDS: row r's 16-byte piece x at x ^ r.
+template <int kD>
+__device__ __forceinline__ void spread(const Rows<kD>& w, float* to) {
+  constexpr int kOut = kCols<kD> / 4;
+  const int r = vtx::lane_id() % 32, half = vtx::lane_id() / 32;
+#pragma unroll
+  for (int d = 0; d < kCols<kD> / 32; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int pc = (d * 8 + x * 2 + half) ^ (r % kOut);
+      *reinterpret_cast<float4*>(to + (r * kOut + pc) * 4) =
+          float4{w.o[d][4 * x], w.o[d][4 * x + 1], w.o[d][4 * x + 2], w.o[d][4 * x + 3]};
+    }
+}
+
+// The result of a wave that has a request of its own: its `rows` rows to
+// partial rows `out`, or finished to query rows q0 .. (out < 0).
+template <int kD>
+__device__ __forceinline__ void leave_apart(const SharedArgs& a, const Rows<kD>& w, float* lds, int rows, int out,
+                                            long long q0) {
+  constexpr int kOut = kD / 4;
+  const int lane = vtx::lane_id();
+  const float l = w.l + vtx::xshfl(w.l, 32);
+  spread<kD>(w, lds);
+  wave_lds_fence();
+  if (out >= 0 && (long long)out + rows > a.max_rows) return;
+  for (int x0 = 0; x0 < rows * kOut; x0 += vtx::kWave) {
+    const int x = x0 + lane, r = x / kOut, pc = x % kOut;
+    const float L = __shfl(l, r % 32);
+    if (r >= rows) continue;
+    const float4 O = reinterpret_cast<const float4*>(lds)[r * kOut + (pc ^ (r % kOut))];
+    if (out < 0) *reinterpret_cast<uint2*>(a.o + (q0 + r) * kD + pc * 4) = result4(O, L);
+    else *reinterpret_cast<float4*>(a.acc + ((long long)out + r) * kD + pc * 4) = O;
+  }
+  if (out >= 0 && lane < rows) a.ml[(long long)out + lane] = float2{w.m, l};
+}
+
 template <int kD, bool kFar>
 __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_attention_kernel(SharedArgs a) {
   constexpr int kRow = kD * 2;
@@ -315,16 +359,27 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
   const int wave = vtx::uniform(tid / vtx::kWave);
   const int seg = vtx::uniform(it.segment), S = a.B * a.H;
   if (seg < 0 || seg >= S) return;
-  const int b0 = seg / a.H;
-  const int rows = min(max(it.rows, 0), tile_rows(kD));
+  const bool apart = it.last == kApart;  // uniform
+  int b0 = seg / a.H, rows = min(max(it.rows, 0), tile_rows(kD)), out = it.out;
+  int start = it.start, pages = it.pages, last_of = it.last ? seg : -1;
+  if (apart) {  // this wave's request
+    b0 += wave;
+    if (wave >= pages || b0 >= a.B) return;  // (no barriers on this way)
+    last_of = b0 * a.H + h;
+    const int32_t* info = a.combine + (long long)kCombineInts * last_of;
+    if (vtx::uniform(info[4]) == 0) return;
+    out = info[1] == 0 ? -1 : info[3];
+    start = vtx::uniform(info[5]);
+    pages = vtx::uniform(info[6]);
+  }
 
   // the item's tokens
   Tokens tk{nullptr, 0};
-  if (it.start >= 0 && it.pages > 0 && (long long)it.start + it.pages <= a.indices_len && a.rows > 0) {
+  if (start >= 0 && pages > 0 && (long long)start + pages <= a.indices_len && a.rows > 0) {
     int last = a.P;
-    if (it.last) last = min(max(a.last_len[seg], 0), a.P);
-    const long long t = (long long)(it.pages - 1) * a.P + last;
-    tk.pages = a.indices + it.start;
+    if (last_of >= 0) last = min(max(a.last_len[last_of], 0), a.P);
+    const long long t = (long long)(pages - 1) * a.P + last;
+    tk.pages = a.indices + start;
     tk.count = (int)(t < 0x3fffffff ? t : 0x3fffffff);
   }
 
@@ -353,7 +408,8 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
     }
   }
 
-  bool alone = false;  // tiles of 32 tokens, wave w those of index w, w + 4, ...
+  // tiles of 32 tokens, wave w those of index w, w + 4, ...; or all, of its own request
+  bool alone = false;
   if constexpr (kShare == 1) alone = wr == 1;
   if (alone) {  // uniform
     constexpr int kPass = vtx::kWave / kPieces;  // tokens per wave-wide load
@@ -361,16 +417,16 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
     unsigned char* kt = part(wave);
     unsigned char* vt = kt + 32 * kRow;
     const int piece = lane % kPieces, sub = lane / kPieces;
-    const int tiles = (tk.count + 31) / 32;
-    const int n = tiles > wave ? (tiles - wave + kWaves - 1) / kWaves : 0;
+    const int t0 = apart ? 0 : wave * 32, step = apart ? 32 : kWaves * 32;
+    const int n = tk.count > t0 ? (tk.count - t0 + step - 1) / step : 0;
     vtx::U4 kr[kLoads], vr[kLoads];
     uint64_t next_mask = 0;
-    Entry e = entry_of(a, tk, n > 0 ? wave * 32 + lane % 32 : 0x7fffffff);
+    Entry e = entry_of(a, tk, t0 + lane % 32);
     auto request = [&](int j) __attribute__((always_inline)) {  // tile j's rows, and the entries of tile j + 1
       uint32_t row;
       const bool ok = resolve(a, e, row);
       next_mask = __ballot(ok) & 0xffffffffull;
-      e = entry_of(a, tk, j + 1 < n ? (wave + kWaves * (j + 1)) * 32 + lane % 32 : 0x7fffffff);
+      e = entry_of(a, tk, t0 + (j + 1) * step + lane % 32);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const uint32_t tr = (uint32_t)__shfl((int)row, i * kPass + sub);
@@ -457,30 +513,28 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
     }
   }
 
+  if constexpr (kShare == 1)
+    if (apart) {  // uniform
+      leave_apart(a, w, reinterpret_cast<float*>(part(wave)), rows, out, ((long long)b0 * a.H + h) * a.G);
+      return;
+    }
+
   // The waves' results meet in LDS (rows in 16-byte pieces, piece x of row r at
   // x ^ r), and leave it joined and in whole rows.
   __syncthreads();
   constexpr int kOut = kCols<kD> / 4;  // pieces of a wave's part of an output row
   {
-    float* s_o = reinterpret_cast<float*>(part(wave));
-    const int r = lane % 32, half = lane / 32;
+    const int r = lane % 32;
     const float l = w.l + vtx::xshfl(w.l, 32);
-    if (half == 0) {
+    if (lane < 32) {
       s_m[wave][r] = w.m;
       s_l[wave][r] = l;
     }
-#pragma unroll
-    for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int pc = (d * 8 + x * 2 + half) ^ (r % kOut);
-        *reinterpret_cast<float4*>(s_o + (r * kOut + pc) * 4) =
-            float4{w.o[d][4 * x], w.o[d][4 * x + 1], w.o[d][4 * x + 2], w.o[d][4 * x + 3]};
-      }
+    spread<kD>(w, reinterpret_cast<float*>(part(wave)));
   }
   __syncthreads();
-  const bool direct = it.out < 0;
-  if (!direct && (long long)it.out + rows > a.max_rows) return;  // uniform
+  const bool direct = out < 0;
+  if (!direct && (long long)out + rows > a.max_rows) return;  // uniform
   if (wt == 1) {  // uniform: nothing to join (and never direct: more than G rows)
     auto leave = [&](const unsigned char* from, int v) __attribute__((always_inline)) {
       const int r0 = (v / kShare) * 32, c0 = (v % kShare) * kCols<kD>;
@@ -496,14 +550,14 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
       for (int u = 0; u < kEach; ++u) {
         const int x = u * kThreads + tid, rl = x / kOut, pw = x % kOut;
         if (r0 + rl < rows)
-          *reinterpret_cast<float4*>(a.acc + ((long long)it.out + r0 + rl) * kD + c0 + pw * 4) = y[u];
+          *reinterpret_cast<float4*>(a.acc + ((long long)out + r0 + rl) * kD + c0 + pw * 4) = y[u];
       }
     };
     leave(s_k0, 0);
     leave(s_v0, 1);
     leave(s_k1, 2);
     leave(s_v1, 3);
-    if (!direct && tid < rows) a.ml[(long long)it.out + tid] =
+    if (!direct && tid < rows) a.ml[(long long)out + tid] =
         float2{s_m[tid / 32 * kShare][tid % 32], s_l[tid / 32 * kShare][tid % 32]};
     return;
   }
@@ -529,23 +583,23 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
     if (direct) {
       const int at = it.row0 + r, b = b0 + at / a.G, g = at % a.G;
       if (at < 0 || b >= a.B) continue;
-      const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN);
-      uint2 y{vtx::bf16_pair(O.x * inv, O.y * inv), vtx::bf16_pair(O.z * inv, O.w * inv)};
-      *reinterpret_cast<uint2*>(a.o + (((long long)b * a.H + h) * a.G + g) * kD + pc * 4) = y;
+      *reinterpret_cast<uint2*>(a.o + (((long long)b * a.H + h) * a.G + g) * kD + pc * 4) = result4(O, L);
     } else {
-      *reinterpret_cast<float4*>(a.acc + ((long long)it.out + r) * kD + pc * 4) = O;
-      if (pc == 0) a.ml[(long long)it.out + r] = float2{M, L};
+      *reinterpret_cast<float4*>(a.acc + ((long long)out + r) * kD + pc * 4) = O;
+      if (pc == 0) a.ml[(long long)out + r] = float2{M, L};
     }
   }
 }
 
 // A query row's partial results, weighted: by one wave, or by four that take
-// every fourth batch of them and meet in LDS (few rows have many: 384 rows of 64
-// columns with about 60 each XX us by one wave, XX by four; 16,384 of 128 with 5
-// XX and XX).  A partial row is read in 16-byte pieces, kAtOnce rows side by side
-// in the wave; before it reads them, lane i weighs the i-th of up to 64 rows.
+// every fourth batch of them and meet in LDS.  A partial row is read in 16-byte
+// pieces, kAtOnce rows side by side in the wave; before it reads them, lane i
+// weighs the i-th of up to 64 rows.  Four waves pay where a row has many (a layer
+// by one / four: 48 requests of one behind 32k, D 64, 60 and more each, 29.4 /
+// 27.2 us; 17 behind 5k, D 256, 40 each, 26.2 / 23.6) and cost where not (64 of 4
+// behind 8k, 32 each, 32.0 / 34.1; 16 of 4 behind 4k, D 64, 33 each, 10.8 / 12.7).
+constexpr int kJoinFour = 5120;  // partial rows x columns from which on
 constexpr int kJoinWaves = 4;
-constexpr int kJoinRowsOfFour = 2048;  // query rows up to which four waves take one
 template <int kD, bool kFour>
 __global__ __launch_bounds__(kJoinWaves* vtx::kWave) void shared_prefix_join_kernel(SharedArgs a) {
   constexpr int kPieces = kD / 4, kAtOnce = vtx::kWave / kPieces;
@@ -639,9 +693,7 @@ __global__ __launch_bounds__(kJoinWaves* vtx::kWave) void shared_prefix_join_ker
   } else {
     if (lane >= kPieces) return;
   }
-  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN);
-  reinterpret_cast<uint2*>(a.o + (long long)row * kD)[kFour ? threadIdx.x : lane] =
-      uint2{vtx::bf16_pair(O.x * inv, O.y * inv), vtx::bf16_pair(O.z * inv, O.w * inv)};
+  reinterpret_cast<uint2*>(a.o + (long long)row * kD)[kFour ? threadIdx.x : lane] = result4(O, L);
 }
 
 template <int kD>
@@ -649,7 +701,7 @@ int launch(const SharedArgs& a, hipStream_t s) {
   if (a.pool_bytes) shared_prefix_attention_kernel<kD, false><<<a.H * a.most_items, kThreads, 0, s>>>(a);
   else shared_prefix_attention_kernel<kD, true><<<a.H * a.most_items, kThreads, 0, s>>>(a);
   const int rows = a.B * a.H * a.G;
-  if (rows <= kJoinRowsOfFour)
+  if (a.join_four)
     shared_prefix_join_kernel<kD, true><<<rows, kJoinWaves * vtx::kWave, 0, s>>>(a);
   else
     shared_prefix_join_kernel<kD, false><<<(rows + kJoinWaves - 1) / kJoinWaves, kJoinWaves * vtx::kWave, 0, s>>>(a);
@@ -730,6 +782,11 @@ extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o
   a.acc = workspace;
   a.ml = reinterpret_cast<float2*>(workspace + rows * head_dim);
   a.max_rows = rows;
+  // A row's partial results, at most: its run's chunks, a slot each and kMinChunk
+  // tokens long, and its own.
+  const int64_t tiles = ((int64_t)batch_size * group_size + tile_rows(head_dim) - 1) / tile_rows(head_dim);
+  const int64_t parts = at.slots / tiles, longest = kv_indices_len * page_size / (S * kMinChunk) + 1;
+  a.join_four = (parts < longest ? parts : longest) * head_dim > kJoinFour;
   hipStream_t s = vtx::as_stream(stream);
   switch (head_dim) {
     case 64: return launch<64>(a, s);

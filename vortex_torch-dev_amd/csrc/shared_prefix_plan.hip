@@ -32,6 +32,7 @@ struct PlanArgs {
   const int32_t* ids;
   int32_t B, H, G, P;
   int32_t tile_shift;  // log2 of an item's rows, at most
+  int32_t apart;       // short_tokens
   Layout at;
   int32_t* plan;
 };
@@ -136,11 +137,11 @@ constexpr int kLdsRequests = 2048;
 
 // Per request of the head (a run's numbers at its first one), in LDS or in the plan.
 struct Tables {
-  int32_t *start, *pages, *first, *size, *shared, *run_items, *own_items, *run_rows, *own_rows;
+  int32_t *start, *pages, *first, *size, *shared, *run_items, *own_items, *run_rows, *own_rows, *apart;
 };
 __device__ __forceinline__ Tables tables_at(int32_t* p, int n) {
   return Tables{p,         p + n,     p + 2 * n,     p + 3 * n,     p + 4 * n, p + 5 * n,
-                p + 6 * n + 1, p + 7 * n + 2, p + 8 * n + 2};
+                p + 6 * n + 1, p + 7 * n + 2, p + 8 * n + 2, p + 9 * n + 2};
 }
 
 // How a request's work is cut: its run's (counted at the first one) and its own.
@@ -148,6 +149,7 @@ struct Cut {
   uint32_t tiles, run_chunks, run_pages;
   uint32_t own_chunks, own_pages;
   int used, size;  // shared pages that are read once; the run's requests
+  bool apart;      // with its three neighbours in one item
 };
 
 template <bool kLds>
@@ -216,12 +218,20 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
   auto tiles_of = [&](int n) { return (uint32_t)(n * a.G + (1 << a.tile_shift) - 1) >> a.tile_shift; };
   auto used_of = [&](int e) { return (long long)e * a.P >= kMinShared ? e : 0; };
   unsigned long long work = 0;  // in pages
-  for (int i = tid; i < B; i += kPlanThreads) {
-    const int s = i * a.H + h, f = t.first[i], e = t.shared[f], used = used_of(e);
-    plan[a.at.leaders + s] = f;
-    plan[a.at.shared + s] = e;
-    if (f == i) work += (unsigned long long)tiles_of(t.size[f]) * used;
-    work += (unsigned long long)(t.pages[i] - used);
+  for (int i0 = 0; i0 < B; i0 += kPlanThreads) {  // (all lanes: requests 4 j .. 4 j + 3 lie in one wave)
+    const int i = i0 + tid;
+    int own = 0;
+    if (i < B) {
+      const int s = i * a.H + h, f = t.first[i], e = t.shared[f], used = used_of(e);
+      plan[a.at.leaders + s] = f;
+      plan[a.at.shared + s] = e;
+      if (f == i) work += (unsigned long long)tiles_of(t.size[f]) * used;
+      own = t.pages[i] - used;
+      work += (unsigned long long)own;
+    }
+    const uint64_t few = __ballot((long long)own * a.P <= a.apart), some = __ballot(own > 0);
+    const int four = lane & ~3;
+    if (i < B) t.apart[i] = (few >> four & 15) == 15 && __builtin_popcountll(some >> four & 15) > 1;
   }
 #pragma unroll
   for (int d = 1; d < vtx::kWave; d <<= 1) work += __shfl_xor(work, d);
@@ -231,8 +241,13 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
 #pragma unroll
   for (int w = 0; w < kPlanWaves; ++w) work += s_total[w];
   // (rounded up: most_items counts on no fewer pages a chunk than work / slots)
-  const double even = (double)work / (double)a.at.slots * (1 + 1e-9) + 1;
-  const uint32_t per = max((uint32_t)(even < 1e9 ? even : 1e9), (uint32_t)(kMinChunk + a.P - 1) / (uint32_t)a.P);
+  auto share = [&](int64_t parts) {
+    const double x = (double)work / (double)parts * (1 + 1e-9) + 1;
+    return (uint32_t)(x < 1e9 ? x : 1e9);
+  };
+  const uint32_t least = (uint32_t)(kMinChunk + a.P - 1) / (uint32_t)a.P;
+  const uint32_t few = (uint32_t)(kFewChunk + a.P - 1) / (uint32_t)a.P;
+  const uint32_t per = max(max(share(a.at.slots), least), min(share(a.at.cus), few));
 
   // 4. Items and partial rows of every request, and their places by a scan.
   auto cut = [&](int i) {
@@ -243,11 +258,12 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
     c.tiles = tiles_of(c.size);
     c.run_chunks = chunks(c.used, per, c.run_pages);
     c.own_chunks = chunks(t.pages[i] - c.used, per, c.own_pages);
+    c.apart = t.apart[i];
     return c;
   };
   auto count_of = [&](int i, const Cut& c) {
     const bool head = t.first[i] == i, joined = c.run_chunks + c.own_chunks > 1;
-    return Four{{head ? (int)(c.tiles * c.run_chunks) : 0, (int)c.own_chunks,
+    return Four{{head ? (int)(c.tiles * c.run_chunks) : 0, c.apart ? i % 4 == 0 : (int)c.own_chunks,
                  head ? c.size * a.G * (int)c.run_chunks : 0,
                  joined ? (int)c.own_chunks * a.G : 0}};  // (a single partial result is the result)
   };
@@ -288,7 +304,7 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
     const int f = t.first[i];
     int4* to = reinterpret_cast<int4*>(plan + a.at.combine + (long long)kCombineInts * (i * a.H + h));
     to[0] = int4{t.run_rows[f] + (i - f) * a.G, (int)c.run_chunks, c.size * a.G, t.own_rows[i]};
-    to[1] = int4{(int)c.own_chunks, 0, 0, 0};
+    to[1] = int4{(int)c.own_chunks, t.start[i] + c.used, t.pages[i] - c.used, 0};
   }
 
   // 6. The items, every thread some of both kinds; the request by bisection.
@@ -331,6 +347,10 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
     }
     it.start = t.start[i] + page0;
     it.last = page0 + it.pages == t.pages[i] ? 1 : 0;
+    if (!run && c.apart) {
+      it.pages = min(B - i, 4);
+      it.last = kApart;
+    }
     it.reserved = 0;
     items[k] = it;
   }
@@ -349,6 +369,7 @@ Layout layout_of(int64_t batch, int64_t heads, int group_size, int head_dim, int
   // 4 behind 32k 82.2 for 69.0: more partial results.)
   const int64_t slots = cus * (head_dim == 64 ? 3 : 2);
   l.slots = (slots + heads - 1) / heads;
+  l.cus = (cus + heads - 1) / heads;
   // Runs: tiles x ceil(pages / per) <= tiles x pages / per + tiles, at most one run
   // per two requests; requests: pages / per + 1 each.  The sums of x / per are at
   // most `slots` together.
@@ -414,6 +435,7 @@ extern "C" int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* k
   a.G = group_size;
   a.P = page_size;
   a.tile_shift = vtx::log2_exact(tile_rows(head_dim));
+  a.apart = 2 * batch_size > a.at.slots ? short_tokens(head_dim) : 0;
   a.plan = plan;
   hipStream_t s = vtx::as_stream(stream);
   prefix_compare_kernel<<<(int)((S + kCompareWaves - 1) / kCompareWaves), kCompareWaves * vtx::kWave, 0, s>>>(a);

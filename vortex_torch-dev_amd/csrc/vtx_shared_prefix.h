@@ -9,8 +9,23 @@ namespace vtx_prefix {
 // Query rows of a workgroup, at most (rows of 256 columns: two waves share 32).
 constexpr int tile_rows(int head_dim) { return head_dim == 256 ? 64 : 128; }
 
-constexpr int kMinShared = 128;  // tokens from which a run's pages are read once for all
-constexpr int kMinChunk = 128;   // tokens of a chunk, at least
+// Tokens from which a run's pages are read once for all: fewer cost more in
+// partial results (64 tokens of eight requests, 32 runs of 8 heads each: 15.3 us a
+// layer read by each, 20.3 once; 200 tokens 35.1 and 22.7).
+constexpr int kMinShared = 128;
+// Tokens of a chunk: one item per compute unit from kMinChunk on, and only past
+// kFewChunk one per workgroup slot (32 requests of 8 heads each behind 8k: chunks
+// of 128 26.3 us a layer, of 256 20.6; 17 of 4 behind 5k, D 256, 23.6 and 21.3; 4 of
+// 8 behind 1k 9.0 and 10.3).
+constexpr int kMinChunk = 128, kFewChunk = 256;
+// Own tokens up to which four requests share a workgroup, a wave each, where a
+// head has more requests than half its workgroup slots (four waves to so few
+// tokens of one request are all latency: 256 requests of up to 128 own tokens
+// behind 4k, D 64, 26.6 us a layer, apart 19.2; 256 of 8 heads each with up to 16
+// behind 16k 176 and 163; but 4 behind 1k 9.0 and 10.0, 32 behind 4k, D 64, 12.8
+// and 13.8).
+constexpr int short_tokens(int head_dim) { return head_dim == 256 ? 0 : 128; }
+static_assert(short_tokens(64) <= kMinChunk, "one chunk each");
 constexpr int kXcds = 8;
 constexpr int64_t kMaxSegments = 1 << 22;
 
@@ -18,7 +33,9 @@ constexpr int kHeadInts = 16;  // before everything else
 
 // One workgroup's work: `rows` query rows of the requests from the segment's
 // on (row0 + r: request (row0 + r) / G after it, head (row0 + r) % G) against
-// `pages` entries of the table from `start` on.
+// `pages` entries of the table from `start` on.  Where last is kApart: `pages`
+// requests from the segment's on, one per wave, each against its own entries.
+constexpr int kApart = 2;
 struct alignas(32) Item {
   int32_t segment;
   int32_t row0, rows;
@@ -29,9 +46,10 @@ struct alignas(32) Item {
 };
 
 // Per segment: first partial row of its run's chunks, their count, rows from one
-// to the next, first partial row of its own chunks (G rows each), their count.
+// to the next, first partial row of its own chunks (G rows each), their count,
+// where its own entries start in the table, and how many there are.
 constexpr int kCombineInts = 8;
-constexpr int kScratchInts = 9;  // per segment, and 2 more per head (planner only)
+constexpr int kScratchInts = 10;  // per segment, and 2 more per head (planner only)
 
 // Sizes and places (in int32) of a plan.  Each kv head has a list of items of its
 // own, item k of head h at items + 8 (h * most_items + k), and rows of its own.
@@ -39,7 +57,7 @@ struct Layout {
   int64_t leaders, shared, combine, counts, items;
   int64_t common, scratch;  // planner only
   int64_t size;
-  int64_t slots, most_items, most_rows;  // of a head
+  int64_t slots, cus, most_items, most_rows;  // a head's share, and its lists
 };
 Layout layout_of(int64_t batch, int64_t heads, int group_size, int head_dim, int cus);
 
