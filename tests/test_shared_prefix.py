@@ -289,21 +289,62 @@ def test_attention_follows_last_page_lengths(gpu):
 
 
 @pytest.mark.gpu
-def test_attention_pool_past_32_bits(gpu):
-    P, D, H = 16, 128, 1
-    pages = (1 << 32) // (P * D * 2) + 40  # over 2^32 bytes each
+@pytest.mark.parametrize("D,requests,G", [(128, 2, 4), (64, 10, 4), (128, 20, 8), (256, 3, 8), (256, 12, 4)])
+def test_attention_pool_past_32_bits(gpu, D, requests, G):
+    """Pages at the end of pools of over 2^32 bytes, by rows of one tile and of several."""
+    P, shared = 16, 30
+    pages = (1 << 32) // (P * D * 2) + shared + requests
     k, v = (torch.zeros((pages, P, D), dtype=torch.bfloat16, device=gpu) for _ in range(2))
-    k[-40:].normal_()
-    v[-40:].normal_()
-    k[:40] = float("nan")
-    rows = torch.arange(pages - 40, pages, dtype=torch.int32)
-    indices = torch.cat([rows[:30], rows[30:35], rows[:30], rows[35:]])
-    indptr, last = torch.tensor([0, 35, 70], dtype=torch.int32), torch.tensor([4, 16], dtype=torch.int32)
-    q = torch.randn((2, 4, D), dtype=torch.bfloat16, device=gpu)
+    last_pages = shared + requests
+    k[-last_pages:].normal_()
+    v[-last_pages:].normal_()
+    k[:last_pages] = float("nan")
+    rows = torch.arange(pages - last_pages, pages, dtype=torch.int32)
+    indices = torch.cat([torch.cat([rows[:shared], rows[shared + i:shared + i + 1]]) for i in range(requests)])
+    indptr = torch.arange(requests + 1, dtype=torch.int32) * (shared + 1)
+    last = torch.tensor([1 + (5 * i) % P for i in range(requests)], dtype=torch.int32)
+    q = torch.randn((requests, G, D), dtype=torch.bfloat16, device=gpu)
     t = [x.to(gpu) for x in (indptr, indices, last)]
-    got = shared_prefix_decode_attention(q, k, v, *t, plan_shared_prefix(t[0], t[1], 2, H, 4, D, P))
+    plan = plan_shared_prefix(t[0], t[1], requests, 1, G, D, P)
+    assert plan.shared_pages.tolist() == [shared] * requests
+    got = shared_prefix_decode_attention(q, k, v, *t, plan)
     want, bound = _exact(q, k, v, indptr, t[1], last, D ** -0.5)
     assert bool(((got.view(-1, D).double() - want).abs() <= bound).all())
+
+
+# Short requests share workgroups where there are many: with a run's pages, without
+# (finished where they are), next to long and empty ones, at a batch's ragged end.
+MANY = {
+    "behind_one": [(20, [1 + i % 17 for i in range(90)])],
+    "alone": [(0, [1 + (37 * i) % 128]) for i in range(90)],
+    "mixed": [(10, [3, None, 128, 129, 1]), (0, [None, None, None]), (0, [5]), (0, [1000]), (12, [1, 2])] * 9,
+    "pairs": [(8, [16, 1]), (0, [None, 7, None, None])] * 15 + [(0, [9])],
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("name", MANY)
+def test_attention_many_short_requests(gpu, name, D):
+    _attention(_table(MANY[name], 16, 8, 3), 16, 8, 2, D, gpu)
+    _attention(_table(MANY[name], 16, 8, 3), 16, 8, 1, D, gpu, zero_queries=True)
+    _attention(_table(MANY[name], 8, 8, 3), 8, 8, 8, D, gpu)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [1, 3])
+def test_plan_and_attention_of_thousands_of_requests(gpu, H):
+    """More requests than the planner keeps in LDS."""
+    r = random.Random(5)
+    groups = [(r.choice([0, 1, 12]), [r.choice([1, 20, 40, None]) for _ in range(r.randint(1, 60))])
+              for _ in range(100)]
+    indptr, indices, last, pages = table = _table(groups, 16, H, 6)
+    B = (indptr.numel() - 1) // H
+    assert B > 2048
+    plan = plan_shared_prefix(indptr.to(gpu), indices.to(gpu), B, H, 2, 64, 16)
+    leaders, shared = _plain_plan(indptr, indices, B, H)
+    assert plan.leaders.tolist() == leaders and plan.shared_pages.tolist() == shared
+    _attention(table, 16, H, 2, 64, gpu)
 
 
 @pytest.mark.gpu

@@ -96,7 +96,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // buffer loads: 32-bit offsets, and LDS reads behind a copy in flight are waited
 // for one by one; behind the other form, which counts as an LDS operation too, the
 // compiler waits for all of them (256 requests of 8 heads each behind 16k tokens:
-// XX us a layer and XX).
+// 175 us a layer, 186 by the other form).
 template <bool kFar>
 struct Pool {
   const uint16_t* base;
@@ -118,8 +118,9 @@ struct Pool {
 __device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // Output columns of a wave: all, or half of 256 (two waves share 32 rows and
-// both compute their scores: with all columns the 256 outputs and queries of a
-// lane leave no registers, and took 30 us where this takes XX).
+// both compute their scores: with all columns a lane's outputs and queries leave
+// no registers for more, and the attention of 17 requests behind 5k tokens took
+// 30.3 us, this way 22.8).
 template <int kD>
 constexpr int kCols = kD == 256 ? 128 : kD;
 // Tokens of a tile that all waves share.
@@ -137,7 +138,8 @@ struct Rows {
 
 // The running maximum follows the scores only when they outgrow it by so much
 // (base 2): until then weights up to 2^8 are as exact as weights up to 1, and
-// most tiles leave the outputs as they are.
+// most tiles leave the outputs as they are (256 requests of 8 heads each behind
+// 16k tokens 168 us a layer, following every maximum 176).
 constexpr float kGrowth = 8.f;
 
 // kN x 32 tokens at kt / vt in LDS; bit i of mask: token i counts.  kAhead: the
@@ -395,9 +397,9 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
 #pragma unroll
     for (int i = 0; i < 16; ++i) w.o[d][i] = 0.f;
   {
-    const int r = rb * 32 + lane % 32, at = it.row0 + r;
-    const int b = b0 + at / a.G, g = at % a.G;
-    const bool ok = r < rows && at >= 0 && b < a.B;
+    const int r = rb * 32 + lane % 32, at = (int)((uint32_t)it.row0 + r);
+    const int b = (int)((uint32_t)b0 + (uint32_t)(at / a.G)), g = at % a.G;
+    const bool ok = r < rows && at >= 0 && (uint32_t)b < (uint32_t)a.B;
     const uint16_t* q = a.q + (((long long)(ok ? b : b0) * a.H + h) * a.G + (ok ? g : 0)) * kD + (lane / 32) * 8;
     const uint32_t keep = ok ? a.q_keep : 0u;
 #pragma unroll
@@ -477,12 +479,20 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
         pool_v.copy(from, kLog2, within, vt + t0 * kRow);
       }
     };
-    auto tile = [&](auto all, uint64_t mask, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
-      if (mask != kFull) {  // uniform: what lies in a masked row may be NaN
-        for (int x = tid; x < kT * kPieces; x += kThreads)
-          if (!((mask >> (x / kPieces)) & 1)) vtx::st16(vt + x * 16, vtx::U4{0u, 0u, 0u, 0u});
-        __syncthreads();
+    // The requested tile has arrived, this wave's part of it: what its copies left
+    // in masked rows of V may be NaN.
+    auto arrived = [&](unsigned char* vt) __attribute__((always_inline)) {
+      copies_done();
+      if (next_mask != kFull) {  // uniform
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int t0 = (i * kWaves + wave) * kPass;
+          if (!((next_mask >> (t0 + lane / kPieces)) & 1)) vtx::st16(vt + t0 * kRow + lane * 16, vtx::U4{0u, 0u, 0u, 0u});
+        }
       }
+      __syncthreads();
+    };
+    auto tile = [&](auto all, uint64_t mask, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
       if (busy) {  // uniform over the wave
         if constexpr (decltype(all)::value) attend<kD, kT / 32, true>(w, kt, vt, mask, a.c, col);
         else attend<kD, 1, true>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c, col);
@@ -490,20 +500,17 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
     };
     auto all_tiles = [&](auto all) __attribute__((always_inline)) {  // all: every wave takes all tokens of a tile, for 32 rows of its own
       request(0, s_k0, s_v0);
-      copies_done();
-      __syncthreads();
+      arrived(s_v0);
       for (int j = 0; j < tiles; j += 2) {
         uint64_t mask = next_mask;
         if (j + 1 < tiles) request(j + 1, s_k1, s_v1);
         tile(all, mask, s_k0, s_v0);
-        copies_done();
-        __syncthreads();
+        arrived(s_v1);  // (past the last tile: a barrier, and at most zeros)
         if (j + 1 < tiles) {
           mask = next_mask;
           if (j + 2 < tiles) request(j + 2, s_k0, s_v0);
           tile(all, mask, s_k1, s_v1);
-          copies_done();
-          __syncthreads();
+          arrived(s_v0);
         }
       }
     };
@@ -581,8 +588,8 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
       }
     }
     if (direct) {
-      const int at = it.row0 + r, b = b0 + at / a.G, g = at % a.G;
-      if (at < 0 || b >= a.B) continue;
+      const int at = (int)((uint32_t)it.row0 + r), b = (int)((uint32_t)b0 + (uint32_t)(at / a.G)), g = at % a.G;
+      if (at < 0 || (uint32_t)b >= (uint32_t)a.B) continue;
       *reinterpret_cast<uint2*>(a.o + (((long long)b * a.H + h) * a.G + g) * kD + pc * 4) = result4(O, L);
     } else {
       *reinterpret_cast<float4*>(a.acc + ((long long)out + r) * kD + pc * 4) = O;
@@ -612,7 +619,8 @@ __global__ __launch_bounds__(kJoinWaves* vtx::kWave) void shared_prefix_join_ker
   if (row >= a.B * a.H * a.G) return;  // uniform over the waves that meet
   const int seg = row / a.G, g = row - seg * a.G;
   const int32_t* info = a.combine + (long long)kCombineInts * seg;
-  const int run_row = info[0], run_n = info[1], run_step = info[2], own_row = info[3], own_n = info[4];
+  const int run_row = info[0], run_step = info[2], own_row = info[3];
+  const int run_n = min(max(info[1], 0), a.most_items), own_n = min(max(info[4], 0), a.most_items);
   if (run_n == 0 && own_n == 1) return;  // written by its item
   const int n = run_n + own_n, sub = lane / kPieces, piece = lane % kPieces;
   auto at = [&](int i) -> long long {

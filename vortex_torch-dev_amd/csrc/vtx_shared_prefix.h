@@ -13,11 +13,12 @@ constexpr int tile_rows(int head_dim) { return head_dim == 256 ? 64 : 128; }
 // partial results (64 tokens of eight requests, 32 runs of 8 heads each: 15.3 us a
 // layer read by each, 20.3 once; 200 tokens 35.1 and 22.7).
 constexpr int kMinShared = 128;
-// Tokens of a chunk: one item per compute unit from kMinChunk on, and only past
-// kFewChunk one per workgroup slot (32 requests of 8 heads each behind 8k: chunks
-// of 128 26.3 us a layer, of 256 20.6; 17 of 4 behind 5k, D 256, 23.6 and 21.3; 4 of
-// 8 behind 1k 9.0 and 10.3).
-constexpr int kMinChunk = 128, kFewChunk = 256;
+// Tokens of a chunk: one item per compute unit from kMinChunk on, and past
+// kFewChunk one per workgroup slot (us a layer, 128 from one per slot on / one per
+// compute unit up to 1024: 32 requests of 8 heads each behind 8k 26.3 / 21.1, 64 of
+// 4 heads behind 8k 33.5 / 27.6, 128 in eight runs of 4k 41.4 / 35.0; up to 2048: 48
+// of one behind 32k, D 64, 26.3 / 30.4).
+constexpr int kMinChunk = 128, kFewChunk = 1024;
 // Own tokens up to which four requests share a workgroup, a wave each, where a
 // head has more requests than half its workgroup slots (four waves to so few
 // tokens of one request are all latency: 256 requests of up to 128 own tokens
