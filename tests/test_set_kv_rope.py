@@ -221,7 +221,8 @@ _ROWS = torch.zeros((3, 8 * 16), dtype=torch.bfloat16).unflatten(1, (8, 16))
     (dict(new_k=torch.zeros((3, 2, 16), dtype=torch.float64), ), "must be bfloat16, float16 or float32"),
 ])
 def test_rope_append_refusals(monkeypatch, changes, says):
-    monkeypatch.setattr(_hip, "_require_gpu", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_hip, "_device_index", lambda *t: 0)
+    monkeypatch.setattr(_hip, "_current_device", lambda: 0)
     with pytest.raises(RuntimeError, match=says):
         set_kv_buffer_rope(**_arguments(**changes))
 

@@ -493,7 +493,8 @@ def test_capture_that_torch_did_not_begin_runs_paged_attention(gpu):
 
 # ------------------------------------------------------------- refusals (CPU)
 def _call(monkeypatch, **changes):
-    monkeypatch.setattr(_hip, "_require_gpu", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_hip, "_device_index", lambda *t: 0)
+    monkeypatch.setattr(_hip, "_current_device", lambda: 0)
     i32 = dict(dtype=torch.int32)
     a = dict(q=torch.zeros((4, 2, 64), dtype=torch.bfloat16), k_cache=torch.zeros((6, 16, 64), dtype=torch.bfloat16),
              v_cache=torch.zeros((6, 16, 64), dtype=torch.bfloat16), kv_indptr=torch.zeros(5, **i32),
@@ -534,7 +535,8 @@ def test_attention_refusals(monkeypatch, changes, says):
     (dict(plan=SharedPrefixPlan(torch.zeros(64, dtype=torch.int32), 2, 2, 1, 64, 16)), "plan is for"),
 ])
 def test_plan_refusals(monkeypatch, changes, says):
-    monkeypatch.setattr(_hip, "_require_gpu", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_hip, "_device_index", lambda *t: 0)
+    monkeypatch.setattr(_hip, "_current_device", lambda: 0)
     a = dict(kv_indptr=torch.zeros(5, dtype=torch.int32), kv_indices=torch.zeros(4, dtype=torch.int32), batch_size=2,
              num_kv_heads=2, group_size=2, head_dim=64, page_size=16)
     a.update(changes)

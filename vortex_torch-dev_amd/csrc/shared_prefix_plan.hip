@@ -44,45 +44,47 @@ __device__ __forceinline__ int pages_of(const PlanArgs& a, int s, int& start) {
   return start >= 0 && end > start && end <= a.indices_len ? (int)(end - start) : 0;
 }
 
-// common[s]: entries that segment (b, h) has in common with (b - 1, h), or -1
-// where no run goes through the two.
-constexpr int kCompareWaves = 4;
+// Entries that segment s = (b, h) has in common with (b - 1, h), or -1 where no
+// run goes through the two.  One wave.
 constexpr int kAhead = 8;  // entries per lane and pass
-__global__ __launch_bounds__(kCompareWaves* vtx::kWave) void prefix_compare_kernel(PlanArgs a) {
-  const int s = blockIdx.x * kCompareWaves + vtx::uniform(threadIdx.x / vtx::kWave), lane = vtx::lane_id();
-  if (s >= a.B * a.H) return;
-  const int b = s / a.H;
+__device__ __forceinline__ int common_entries(const PlanArgs& a, int s) {
+  const int lane = vtx::lane_id(), b = s / a.H;
   int start, before;
   const int n = pages_of(a, s, start);
   const int m = b > 0 ? pages_of(a, s - a.H, before) : 0;
   const bool named = a.ids && b > 0;
   const bool same = named ? a.ids[b] == a.ids[b - 1] : true;
-  int common = -1;
-  if (n > 0 && m > 0 && same) {  // uniform over the wave
-    const int len = min(n, m);
-    common = len;
-    for (int at = 0; at < len; at += vtx::kWave * kAhead) {
-      int x[kAhead], y[kAhead];
+  if (n == 0 || m == 0 || !same) return -1;  // uniform
+  const int len = min(n, m);
+  int common = len;
+  for (int at = 0; at < len; at += vtx::kWave * kAhead) {
+    int x[kAhead], y[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = min(at + k * vtx::kWave + lane, len - 1);
-        x[k] = a.indices[start + (long long)i];
-        y[k] = a.indices[before + (long long)i];
-      }
-      uint64_t differ[kAhead], any = 0;
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) any |= differ[k] = __ballot(x[k] != y[k]);
-      if (any) {
-#pragma unroll
-        for (int k = kAhead - 1; k >= 0; --k)
-          if (differ[k]) common = at + k * vtx::kWave + __builtin_ctzll(differ[k]);
-        common = min(common, len - 1);  // (lanes past the end compare the last entry)
-        break;
-      }
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = min(at + k * vtx::kWave + lane, len - 1);
+      x[k] = a.indices[start + (long long)i];
+      y[k] = a.indices[before + (long long)i];
     }
-    if (!named && common == 0) common = -1;  // other first entries: another run
+    uint64_t differ[kAhead], any = 0;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) any |= differ[k] = __ballot(x[k] != y[k]);
+    if (any) {
+#pragma unroll
+      for (int k = kAhead - 1; k >= 0; --k)
+        if (differ[k]) common = at + k * vtx::kWave + __builtin_ctzll(differ[k]);
+      common = min(common, len - 1);  // (lanes past the end compare the last entry)
+      break;
+    }
   }
-  if (lane == 0) a.plan[a.at.common + s] = common;
+  return !named && common == 0 ? -1 : common;  // (other first entries: another run)
+}
+
+constexpr int kCompareWaves = 4;
+__global__ __launch_bounds__(kCompareWaves* vtx::kWave) void prefix_compare_kernel(PlanArgs a) {
+  const int s = blockIdx.x * kCompareWaves + vtx::uniform(threadIdx.x / vtx::kWave);
+  if (s >= a.B * a.H) return;
+  const int common = common_entries(a, s);
+  if (vtx::lane_id() == 0) a.plan[a.at.common + s] = common;
 }
 
 constexpr int kPlanThreads = 256;
@@ -134,6 +136,10 @@ __device__ __forceinline__ uint32_t chunks(uint32_t n, uint32_t per, uint32_t& p
 }
 
 constexpr int kLdsRequests = 2048;
+// Requests up to which, in a table of one pass of entries each, the second launch
+// compares them itself (4 requests 8.5 us in two launches, 6.7 in one; 16 8.6 and
+// 8.9, and 2.9 us less of the host's time; 32 8.6 and 11.5).
+constexpr int kFewRequests = 16;
 
 // Per request of the head (a run's numbers at its first one), in LDS or in the plan.
 struct Tables {
@@ -152,7 +158,8 @@ struct Cut {
   bool apart;      // with its three neighbours in one item
 };
 
-template <bool kLds>
+// kCompare: finds the common entries itself, kPlanWaves requests at a time.
+template <bool kLds, bool kCompare>
 __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
   __shared__ int32_t s_tables[kLds ? kScratchInts * kLdsRequests + 2 : 1];
   __shared__ int s_scan[kPlanWaves][4];
@@ -171,8 +178,13 @@ __global__ __launch_bounds__(kPlanThreads) void prefix_plan_kernel(PlanArgs a) {
     int start;
     t.pages[i] = pages_of(a, s, start);
     t.start[i] = start;
-    t.first[i] = plan[a.at.common + s];
+    if constexpr (!kCompare) t.first[i] = plan[a.at.common + s];
   }
+  if constexpr (kCompare)
+    for (int i = vtx::uniform(wave); i < B; i += kPlanWaves) {
+      const int common = common_entries(a, i * a.H + h);
+      if (lane == 0) t.first[i] = common;
+    }
   __syncthreads();
 
   // 2. Runs, by a scan; a run's last request then has the run's minimum and
@@ -438,8 +450,12 @@ extern "C" int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* k
   a.apart = 2 * batch_size > a.at.slots ? short_tokens(head_dim) : 0;
   a.plan = plan;
   hipStream_t s = vtx::as_stream(stream);
-  prefix_compare_kernel<<<(int)((S + kCompareWaves - 1) / kCompareWaves), kCompareWaves * vtx::kWave, 0, s>>>(a);
-  if (batch_size <= kLdsRequests) prefix_plan_kernel<true><<<num_kv_heads, kPlanThreads, 0, s>>>(a);
-  else prefix_plan_kernel<false><<<num_kv_heads, kPlanThreads, 0, s>>>(a);
+  if (batch_size <= kFewRequests && kv_indices_len <= (int64_t)vtx::kWave * kAhead * S) {
+    prefix_plan_kernel<true, true><<<num_kv_heads, kPlanThreads, 0, s>>>(a);
+  } else {
+    prefix_compare_kernel<<<(int)((S + kCompareWaves - 1) / kCompareWaves), kCompareWaves * vtx::kWave, 0, s>>>(a);
+    if (batch_size <= kLdsRequests) prefix_plan_kernel<true, false><<<num_kv_heads, kPlanThreads, 0, s>>>(a);
+    else prefix_plan_kernel<false, false><<<num_kv_heads, kPlanThreads, 0, s>>>(a);
+  }
   return vtx::check_launch("plan_shared_prefix");
 }

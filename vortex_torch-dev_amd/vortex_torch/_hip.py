@@ -329,11 +329,9 @@ def _device_index(*tensors: torch.Tensor) -> int:
     return -1 if dev is None or dev.index is None else dev.index
 
 
-def _elsewhere(index: int, call):
-    """call(the current stream of device `index`) with that device current."""
-    dev = torch.device("cuda", index)
-    with _on_device(dev):
-        return call(_stream(dev))
+def _stream_of(index: int) -> int:
+    """The current stream's handle of device `index`."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 class _on_device:
@@ -1207,6 +1205,10 @@ def set_kv_buffer_rope(k_cache, v_cache, q, new_k, new_v, loc, page_size, positi
         index = _device_index(new_k, k_cache, v_cache, q, new_v, loc, positions, cos_sin_cache)
     else:
         index = _device_index(new_k, k_cache, v_cache, q, new_v, loc, positions, cos_sin_cache, q_out)
+    if _current_device() != index:
+        with _on_device(torch.device("cuda", index)):
+            return set_kv_buffer_rope(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache,
+                                      interleaved, q_out)
     if q_out is not None or not _rope_fits(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache):
         wrong = _rope_refusal(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache, q_out)
         if wrong:
@@ -1224,23 +1226,14 @@ def set_kv_buffer_rope(k_cache, v_cache, q, new_k, new_v, loc, page_size, positi
     k0, k1, _ = new_k.stride()
     v0, v1, _ = new_v.stride()
     table_rows, rotary = cos_sin_cache.shape
-    args = (k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() // D if D else 0, qp, op, new_k.data_ptr(),
-            new_v.data_ptr(), _EightI64(q0, q1, o0, o1, k0, k1, v0, v1), loc.data_ptr(), positions.data_ptr(),
-            cos_sin_cache.data_ptr(), table_rows, nnz, Hq, H, D, rotary, _ROPE_DTYPES[new_k.dtype], page_size,
-            1 if interleaved else 0)
-    if _raw_stream is not None and _current_device() == index:
-        rc = lib.vtx_set_kv_buffer_rope(*args, _raw_stream(index))
-    else:
-        rc = _elsewhere(index, lambda stream: lib.vtx_set_kv_buffer_rope(*args, stream))
+    rc = lib.vtx_set_kv_buffer_rope(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() // D if D else 0, qp, op, new_k.data_ptr(),
+        new_v.data_ptr(), _EightI64(q0, q1, o0, o1, k0, k1, v0, v1), loc.data_ptr(), positions.data_ptr(),
+        cos_sin_cache.data_ptr(), table_rows, nnz, Hq, H, D, rotary, _ROPE_DTYPES[new_k.dtype], page_size,
+        1 if interleaved else 0, _stream_of(index))
     if rc:
         _check(rc, "set_kv_buffer_rope")
     return q_out
-
-
-def _scratch_lasts(stream: int) -> bool:
-    from . import _deferred
-
-    return _deferred.scratch_lasts(stream)
 
 
 def _scratch(floats: int, dev: torch.device, stream: int):
@@ -1248,12 +1241,32 @@ def _scratch(floats: int, dev: torch.device, stream: int):
     where the call does without: inside a capture that torch did not begin (the
     memory would be others' while the graph still uses it), or with no memory
     left (a call that is given its output needs none)."""
-    if floats <= 0 or not _scratch_lasts(stream):
+    from . import _deferred
+
+    if floats <= 0 or not _deferred.scratch_lasts(stream):
         return None
     try:
         return torch.empty(floats, dtype=torch.float32, device=dev)
     except torch.OutOfMemoryError:
         return None
+
+
+_deferral = None
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
+
+
+def _scratch_lasts(stream: int) -> bool:
+    """_deferred.scratch_lasts of the current stream of the current GPU; out of
+    any capture, once that has seen to it that captures are told apart, one query
+    of torch's."""
+    global _deferral
+    if _deferral is None:
+        from . import _deferred
+
+        _deferral = _deferred
+    if _capturing is not None and "captures" in _deferral._hook_uses and not _capturing():
+        return True
+    return _deferral.scratch_lasts(stream)
 
 
 @_plain_args
@@ -1306,6 +1319,10 @@ def plan_shared_prefix(kv_indptr, kv_indices, group_ids, batch_size, num_kv_head
     lib = _lib or load_library()
     given = [t for t in (kv_indptr, kv_indices, group_ids, plan) if t is not None]
     index = _device_index(*given)
+    if _current_device() != index:
+        with _on_device(torch.device("cuda", index)):
+            return plan_shared_prefix(kv_indptr, kv_indices, group_ids, batch_size, num_kv_heads, group_size, head_dim,
+                                      page_size, plan)
     if not _tables_fit(*given):
         for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (group_ids, "group_ids"), (plan, "plan")):
             if t is not None:
@@ -1313,28 +1330,21 @@ def plan_shared_prefix(kv_indptr, kv_indices, group_ids, batch_size, num_kv_head
     B, H, G, D = batch_size, num_kv_heads, group_size, head_dim
     if B < 0 or H < 1 or page_size < 1:
         raise RuntimeError("vortex_torch: batch_size, num_kv_heads and page_size must be positive")
-    if plan is None and not lib.vtx_paged_decode_attention_supported(D, G):
-        raise RuntimeError(f"vortex_torch: head_dim {D} with {G} query heads per kv head not supported")
     if kv_indptr.numel() < B * H + 1:
         raise RuntimeError(f"vortex_torch: kv_indptr needs {B * H + 1} entries")
     if group_ids is not None and group_ids.numel() < B:
         raise RuntimeError(f"vortex_torch: group_ids needs {B} entries")
-
-    def launch(stream):
-        nonlocal plan
-        if plan is None:
-            if not _scratch_lasts(stream):
-                raise RuntimeError("vortex_torch: a capture that torch did not begin needs a plan made before it")
-            plan = kv_indptr.new_empty(max(lib.vtx_shared_prefix_plan_len(B, H, G, D), 16))
-        return lib.vtx_plan_shared_prefix(
-            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
-            None if group_ids is None else group_ids.data_ptr(), B, H, G, D, page_size, plan.data_ptr(), plan.numel(),
-            stream)
-
-    if _raw_stream is not None and _current_device() == index:
-        rc = launch(_raw_stream(index))
-    else:
-        rc = _elsewhere(index, launch)
+    if plan is None and not lib.vtx_paged_decode_attention_supported(D, G):
+        raise RuntimeError(f"vortex_torch: head_dim {D} with {G} query heads per kv head not supported")
+    stream = _stream_of(index)
+    if plan is None:
+        if not _scratch_lasts(stream):
+            raise RuntimeError("vortex_torch: a capture that torch did not begin needs a plan made before it")
+        plan = kv_indptr.new_empty(max(lib.vtx_shared_prefix_plan_len(B, H, G, D), 16))
+    rc = lib.vtx_plan_shared_prefix(
+        kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
+        None if group_ids is None else group_ids.data_ptr(), B, H, G, D, page_size, plan.data_ptr(), plan.numel(),
+        stream)
     if rc:
         _check(rc, "plan_shared_prefix")
     return plan
@@ -1348,6 +1358,10 @@ def shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices
     (see _scratch) paged decode attention itself runs, which needs none."""
     lib = _lib or load_library()
     index = _device_index(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan)
+    if _current_device() != index:
+        with _on_device(torch.device("cuda", index)):
+            return shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan,
+                                                  batch_size, num_kv_heads, group_size, sm_scale)
     if not (q.dtype is _BF16 and o.dtype is _BF16 and k_cache.dtype is _BF16 and v_cache.dtype is _BF16
             and q.is_contiguous() and o.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
             and _tables_fit(kv_indptr, kv_indices, kv_last_page_len, plan)):
@@ -1361,26 +1375,28 @@ def shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices
         raise RuntimeError("vortex_torch: k_cache and v_cache must both be [pages * H, page_size, head_dim]")
     rows, P, D = pools
     B, H, G = batch_size, num_kv_heads, group_size
-    if q.numel() != B * H * G * D or o.numel() != B * H * G * D:
+    S = B * H
+    if q.numel() != S * G * D or o.numel() != S * G * D:
         raise RuntimeError("vortex_torch: q and o must hold batch * kv heads * group rows of head_dim")
-    if kv_indptr.numel() < B * H + 1 or kv_last_page_len.numel() < B * H:
-        raise RuntimeError(f"vortex_torch: kv_indptr needs {B * H + 1} and kv_last_page_len {B * H} entries")
-
-    def launch(stream):
-        args = (q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), rows, kv_indptr.data_ptr(),
-                kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr())
-        floats = lib.vtx_shared_prefix_workspace_len(B, H, G, D)
-        ws = _scratch(floats, q.device, stream)
-        if ws is None and floats > 0:
-            return lib.vtx_paged_decode_attention(*args, B, H, G, D, P, sm_scale, stream)
-        return lib.vtx_shared_prefix_decode_attention(
-            *args, plan.data_ptr(), plan.numel(), B, H, G, D, P, sm_scale, None if ws is None else ws.data_ptr(),
-            floats, stream)
-
-    if _raw_stream is not None and _current_device() == index:
-        rc = launch(_raw_stream(index))
+    if kv_indptr.numel() < S + 1 or kv_last_page_len.numel() < S:
+        raise RuntimeError(f"vortex_torch: kv_indptr needs {S + 1} and kv_last_page_len {S} entries")
+    stream = _stream_of(index)
+    floats = lib.vtx_shared_prefix_workspace_len(B, H, G, D)
+    ws = None
+    if floats > 0 and _scratch_lasts(stream):
+        try:
+            ws = torch.empty(floats, dtype=torch.float32, device=q.device)
+        except torch.OutOfMemoryError:
+            pass
+    if ws is None and floats > 0:
+        rc = lib.vtx_paged_decode_attention(
+            q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), rows, kv_indptr.data_ptr(),
+            kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr(), B, H, G, D, P, sm_scale, stream)
     else:
-        rc = _elsewhere(index, launch)
+        rc = lib.vtx_shared_prefix_decode_attention(
+            q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), rows, kv_indptr.data_ptr(),
+            kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr(), plan.data_ptr(), plan.numel(), B, H,
+            G, D, P, sm_scale, None if ws is None else ws.data_ptr(), floats, stream)
     if rc:
         _check(rc, "shared_prefix_decode_attention")
 
