@@ -135,6 +135,40 @@ def test_rope_append_agrees_with_plain_store_bit_for_bit(gpu):
 
 
 @pytest.mark.gpu
+def test_rope_append_into_layout_tagged_pools_and_after_a_carried_mean(gpu):
+    """A flow's pools (vTensors), with the page-finish mean that forward_cache
+    left for the next launch: it sees the pool as it was before the call."""
+    import workloads as W
+    from vortex_torch import flow as vflow
+    from vortex_torch.abs import FORMAT, as_vtensor
+
+    batch = W.c1()
+    H, G, D, P = batch.num_kv_heads, batch.group_size, batch.head_dim, batch.page_size
+    ictx, cctx = W.make_contexts(batch, gpu)
+    flow = vflow.build_vflow("block_sparse_attention")
+    k = W.k_pool(batch, 10, gpu)
+    centroids = torch.zeros((batch.pool_pages * H, 1, D), device=gpu, dtype=torch.bfloat16)
+    cache = {"k": as_vtensor(k, FORMAT.PAGED), "v": as_vtensor(torch.zeros_like(k), FORMAT.PAGED),
+             "centroids": as_vtensor(centroids, FORMAT.PAGED)}
+    loc = torch.tensor([5 * P + P - 1], device=gpu)
+    for c in (ictx, cctx):
+        c.profile()
+    flow.forward_cache(cache, loc, cctx)
+    for c in (ictx, cctx):
+        c.execute()
+    before = k.view(-1, H, P, D)[5].float().mean(1)
+    flow.forward_cache(cache, loc, cctx)
+    gen = torch.Generator().manual_seed(4)
+    q, nk, nv = _tensors(1, (H * G, H, H), D, torch.bfloat16, "fused", gen, gpu)
+    table = _table(64, D, gpu)
+    set_kv_buffer_rope(cache["k"], cache["v"], q, nk, nv, loc, P, torch.tensor([9], device=gpu), table)
+    got = centroids.view(-1, H, D)[5].float()
+    assert bool(((got - before).abs() <= 2.0 ** -8 * before.abs() + 2.0 ** -20).all())
+    want, off = _rotated(nk, table, torch.tensor([9], device=gpu), False)
+    _close(k.view(-1, H, P, D)[5, :, P - 1], want[0], off[0], torch.bfloat16)
+
+
+@pytest.mark.gpu
 def test_rope_append_offsets_past_32_bits(gpu):
     """The last page of pools of over 2^32 bytes, the last row of a table as large."""
     D, P, pages = 128, 16, (1 << 32) // (16 * 128 * 2) + 9

@@ -348,6 +348,23 @@ def test_plan_and_attention_of_thousands_of_requests(gpu, H):
 
 
 @pytest.mark.gpu
+def test_attention_takes_layout_tagged_tensors(gpu):
+    """Pools and tables as a flow holds them (vTensors)."""
+    from vortex_torch.abs import FORMAT, as_vtensor
+
+    indptr, indices, last, _ = table = _table([(20, [40, 3, 77])], 16, 2, 7)
+    q, k, v = _inputs(table, 16, 2, 2, 128, 0, gpu)
+    t = [x.to(gpu) for x in (indptr, indices, last)]
+    want = shared_prefix_decode_attention(q, k, v, *t, plan_shared_prefix(t[0], t[1], 3, 2, 2, 128, 16))
+    tagged = as_vtensor(t[1].view(-1, 1, 1), FORMAT.RAGGED)
+    plan = plan_shared_prefix(t[0], tagged, 3, 2, 2, 128, 16)
+    got = shared_prefix_decode_attention(as_vtensor(q, FORMAT.BATCHED), as_vtensor(k, FORMAT.PAGED),
+                                         as_vtensor(v, FORMAT.PAGED), t[0], tagged, t[2], plan,
+                                         out=torch.zeros_like(q))
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_attention_streams_and_repeats(gpu):
     """Calls on two streams at once with one plan, and repeats, agree bit for bit."""
     table = _table([(60, [30 + i for i in range(16)])], 16, 4, 7)
@@ -542,6 +559,36 @@ def test_plan_refusals(monkeypatch, changes, says):
     a.update(changes)
     with pytest.raises(RuntimeError, match=says):
         plan_shared_prefix(**a)
+
+
+def test_calls_run_on_the_tensors_device(monkeypatch):
+    """With another device current, each call makes its tensors' one current and puts the other back."""
+    from vortex_torch.cache import set_kv_buffer_rope
+
+    now, seen = {"device": 1}, []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: seen.append((name, now["device"])) or (1024 if name.endswith("_len") else 0)
+
+    monkeypatch.setattr(_hip, "_lib", Lib())
+    monkeypatch.setattr(_hip, "_device_index", lambda *t: 0)
+    monkeypatch.setattr(_hip, "_current_device", lambda: now["device"])
+    monkeypatch.setattr(_hip, "_stream_of", lambda index: 0)
+    monkeypatch.setattr(_hip, "_scratch_lasts", lambda stream: True)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: now.update(device=d))
+    i32, bf = dict(dtype=torch.int32), dict(dtype=torch.bfloat16)
+    tables = torch.zeros(5, **i32), torch.zeros(4, **i32)
+    plan = plan_shared_prefix(*tables, 2, 2, 2, 64, 16, plan=SharedPrefixPlan(torch.zeros(512, **i32), 2, 2, 2, 64, 16))
+    pools = torch.zeros((2, 6, 16, 64), **bf)
+    shared_prefix_decode_attention(torch.zeros((4, 2, 64), **bf), pools[0], pools[1], *tables, torch.zeros(4, **i32), plan)
+    rows = torch.zeros((3, 2, 64), **bf)
+    set_kv_buffer_rope(pools[0], pools[1], rows, rows.clone(), rows.clone(), torch.arange(3), 16, torch.arange(3),
+                       torch.zeros((8, 64)))
+    assert now["device"] == 1 and {d for _, d in seen} == {0}
+    names = [n for n, _ in seen]
+    for n in ("vtx_plan_shared_prefix", "vtx_shared_prefix_decode_attention", "vtx_set_kv_buffer_rope"):
+        assert names.count(n) == 1
 
 
 def test_need_a_gpu():

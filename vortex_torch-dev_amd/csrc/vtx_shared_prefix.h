@@ -14,11 +14,11 @@ constexpr int tile_rows(int head_dim) { return head_dim == 256 ? 64 : 128; }
 // layer read by each, 20.3 once; 200 tokens 35.1 and 22.7).
 constexpr int kMinShared = 128;
 // Tokens of a chunk: one item per compute unit from kMinChunk on, and past
-// kFewChunk one per workgroup slot (us a layer, 128 from one per slot on / one per
-// compute unit up to 1024: 32 requests of 8 heads each behind 8k 26.3 / 21.1, 64 of
-// 4 heads behind 8k 33.5 / 27.6, 128 in eight runs of 4k 41.4 / 35.0; up to 2048: 48
-// of one behind 32k, D 64, 26.3 / 30.4).
-constexpr int kMinChunk = 128, kFewChunk = 1024;
+// kFewChunk one per workgroup slot (us a layer with 256 / 512 / 1024 for it: 64
+// requests of 8 x 4 heads behind 8k 33.0 / 28.1 / 29.4, 256 of 8 x 2 behind 8k 46.7 /
+// 43.8 / 40.0, 32 of 8 x 2 behind 16k 34.0 / 30.5 / 31.4, 48 of 8 x 1 behind 32k, D 64,
+// 29.7 / 29.1 / 31.8, 64 of 8 x 4 behind 32k 66.9 / 62.6 / 66.6).
+constexpr int kMinChunk = 128, kFewChunk = 512;
 // Own tokens up to which four requests share a workgroup, a wave each, where a
 // head has more requests than half its workgroup slots (four waves to so few
 // tokens of one request are all latency: 256 requests of up to 128 own tokens
