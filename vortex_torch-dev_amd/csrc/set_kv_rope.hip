@@ -12,11 +12,11 @@
 // lies outside the pool stores nothing there (its queries are still rotated);
 // one whose position lies outside the table is skipped altogether.
 //
-// Bound by memory (6 operations per pair): every row is read and written once.
+// Bound by memory (6 operations per pair): every row is read and written once
 // (65,536 tokens of 16 + 2 x 8 heads of 128 bf16 columns: 204 us, 5.4 TB/s; one
-// token 2.7 us.)  A unit of work is two 16-byte vectors of one row, both halves of its pairs,
-// so a pair's two columns meet in one thread and q_out may be q itself; rows
-// of other widths or alignments take element-wide units.
+// token 2.7 us).  A unit of work is two 16-byte vectors of one row, both halves
+// of its pairs, so a pair's two columns meet in one thread and q_out may be q
+// itself; rows of other widths or alignments take element-wide units.
 #include "vtx_device.h"
 #include "vtx_host.h"
 
