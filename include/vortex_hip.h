@@ -739,12 +739,13 @@ int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* kv_indices, 
  * of (with the same sizes), every shared page read once for its run instead of
  * once for each request, and the scores and outputs on the matrix cores: the
  * probabilities are rounded to bf16 (and sum to one as rounded), the rest is
- * fp32.  A NaN score gives NaN (there: zeros).  kv_last_page_len may have changed since the plan was made; after any
- * other change of the table plan anew (the results are undefined otherwise, but
- * no access leaves a buffer).  workspace: vtx_shared_prefix_workspace_len
- * floats, 16-byte aligned, its contents neither read nor kept across calls;
- * calls that may overlap need one each.  A request's last bits depend on the
- * other requests of the table (how its tokens are divided).
+ * fp32.  A NaN score gives NaN (there: zeros).  kv_last_page_len may have
+ * changed since the plan was made; after any other change of the table plan
+ * anew (the results are undefined otherwise, but no access leaves a buffer).
+ * workspace: vtx_shared_prefix_workspace_len floats, 16-byte aligned, its
+ * contents neither read nor kept across calls; calls that may overlap need one
+ * each.  A request's last bits depend on the other requests of the table (how
+ * its tokens are divided).
  * head_dim 64, 128 or 256; group_size 1..8; at most 2^22 segments and 2^32
  * pool tokens (pool rows x page_size).
  */

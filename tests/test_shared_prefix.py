@@ -147,8 +147,10 @@ def _exact(q, k, v, indptr, indices, last, scale):
         e_s = 2 * (D + 8) * 2.0 ** -24 * size + 2.0 ** -22
         exact_weights = (q[s].abs().amax(-1, keepdim=True) == 0) | (scale == 0)
         e_w = torch.where(exact_weights, 0.0, 1.01 * 2.0 ** -8 + e_s)
-        spread = torch.einsum("gt,gtd->gd", p, (vv[None] - o[:, None]).abs()) if vv.shape[0] * D * q.shape[1] < 1 << 25 \
-            else p @ vv.abs() + o.abs()
+        if vv.shape[0] * D * q.shape[1] < 1 << 25:
+            spread = torch.einsum("gt,gtd->gd", p, (vv[None] - o[:, None]).abs())
+        else:  # (a bound of it)
+            spread = p @ vv.abs() + o.abs()
         out[s] = o
         bound[s] = e_w * spread + (n + 64) * 2.0 ** -24 * (p @ vv.abs()) + 2.0 ** -8 * o.abs() * 1.01 + 1e-37
     return out.view(-1, D), bound.view(-1, D)
@@ -579,9 +581,11 @@ def test_calls_run_on_the_tensors_device(monkeypatch):
     monkeypatch.setattr(torch.cuda, "set_device", lambda d: now.update(device=d))
     i32, bf = dict(dtype=torch.int32), dict(dtype=torch.bfloat16)
     tables = torch.zeros(5, **i32), torch.zeros(4, **i32)
-    plan = plan_shared_prefix(*tables, 2, 2, 2, 64, 16, plan=SharedPrefixPlan(torch.zeros(512, **i32), 2, 2, 2, 64, 16))
+    plan = SharedPrefixPlan(torch.zeros(512, **i32), 2, 2, 2, 64, 16)
+    assert plan_shared_prefix(*tables, 2, 2, 2, 64, 16, plan=plan) is plan
     pools = torch.zeros((2, 6, 16, 64), **bf)
-    shared_prefix_decode_attention(torch.zeros((4, 2, 64), **bf), pools[0], pools[1], *tables, torch.zeros(4, **i32), plan)
+    shared_prefix_decode_attention(torch.zeros((4, 2, 64), **bf), pools[0], pools[1], *tables,
+                                   torch.zeros(4, **i32), plan)
     rows = torch.zeros((3, 2, 64), **bf)
     set_kv_buffer_rope(pools[0], pools[1], rows, rows.clone(), rows.clone(), torch.arange(3), 16, torch.arange(3),
                        torch.zeros((8, 64)))

