@@ -186,6 +186,30 @@ def test_rope_append_offsets_past_32_bits(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,P,D", [(1, 16, 128), (2, 16, 64), (3, 5, 7), (4, 16, 128), (8, 16, 128), (8, 1, 64)])
+def test_rope_append_slots_far_past_the_pool(gpu, H, P, D):
+    """A slot outside the pool stores nothing however large it is: a row of
+    heads x slot leaves 64 bits from 2^63 / H on.  Guards lie on both sides."""
+    pages, guard = 7, 130 * H * P
+    far = [pages * P, (1 << 31) - 1, 1 << 31, 1 << 32, 1 << 40, (1 << 63) // H - 1, (1 << 63) - 1, (1 << 63) - P,
+           *(1 << b for b in range(57, 63)), *((1 << b) + 3 * P + 2 for b in range(57, 63)), -1, -(1 << 63)]
+    loc = torch.tensor([pages * P - 1, *(min(x, (1 << 63) - 1) for x in far)], device=gpu)
+    n = loc.numel()
+    buffers = torch.full((2, guard + pages * H * P + guard, D), SENTINEL, dtype=torch.bfloat16, device=gpu)
+    kc, vc = (b[guard:-guard].view(pages * H, P, D) for b in buffers)
+    q, k, v = _tensors(n, (H, H, H), D, torch.bfloat16, "apart", torch.Generator().manual_seed(6), gpu)
+    table, positions = _table(64, D // 2 * 2, gpu), torch.arange(n, device=gpu)
+    got = set_kv_buffer_rope(kc, vc, q, k, v, loc, P, positions, table)
+    _close(got, *_rotated(q, table, positions, False), torch.bfloat16)  # (queries are rotated all the same)
+    want, off = _rotated(k, table, positions, False)
+    _close(kc.view(pages, H, P, D)[-1, :, -1], want[0], off[0], torch.bfloat16)
+    assert torch.equal(vc.view(pages, H, P, D)[-1, :, -1], v[0])
+    kc.view(pages, H, P, D)[-1, :, -1] = SENTINEL
+    vc.view(pages, H, P, D)[-1, :, -1] = SENTINEL
+    assert bool((buffers == SENTINEL).all())
+
+
+@pytest.mark.gpu
 def test_rope_append_streams_and_graphs(gpu):
     gen = torch.Generator().manual_seed(3)
     q, k, v = _tensors(24, (4, 2, 2), 128, torch.bfloat16, "fused", gen, gpu)

@@ -35,6 +35,7 @@ struct RopeArgs {
   const int64_t* pos;
   const float* table;
   int64_t cache_rows, table_rows;
+  int64_t last_page;  // the pool's last page, -1: none
   int64_t q_tok, q_head, qo_tok, qo_head, k_tok, k_head, v_tok, v_head;  // strides in elements
   uint32_t units, per_row, per_token;  // work units in all, of a row, of a token
   int32_t q_heads, heads, D, R, page;
@@ -139,9 +140,11 @@ __global__ __launch_bounds__(kThreads) void set_kv_rope_kernel(RopeArgs a) {
   }
   const long long loc = a.loc[i];
   if (loc < 0) return;
+  const long long page = loc / a.page;
+  if (page > a.last_page) return;  // (first of all: a far page's row leaves 64 bits and may come back inside)
   const bool key = slot < a.q_heads + a.heads;
   const int h = slot - a.q_heads - (key ? 0 : a.heads);
-  const long long row = (loc / a.page) * ((long long)a.page * a.heads) + (long long)h * a.page + loc % a.page;
+  const long long row = page * ((long long)a.page * a.heads) + (long long)h * a.page + (loc - page * a.page);
   if (row >= a.cache_rows) return;
   const T* x = key ? reinterpret_cast<const T*>(a.nk) + i * a.k_tok + h * a.k_head
                    : reinterpret_cast<const T*>(a.nv) + i * a.v_tok + h * a.v_head;
@@ -213,6 +216,7 @@ extern "C" int vtx_set_kv_buffer_rope(void* k_cache, void* v_cache, int64_t cach
   a.table = cos_sin;
   a.cache_rows = cache_rows;
   a.table_rows = table_rows;
+  a.last_page = cache_rows > 0 ? (cache_rows - 1) / ((int64_t)page_size * num_kv_heads) : -1;
   a.q_tok = q_heads > 0 ? strides[0] : 0;
   a.q_head = q_heads > 0 ? strides[1] : 0;
   a.qo_tok = q_heads > 0 ? strides[2] : 0;
