@@ -621,6 +621,29 @@ def test_set_kv_buffer_matches_oracle(gpu, dtype, D, kind):
     np.testing.assert_array_equal(bits(vd.cpu()), ev)
 
 
+@pytest.mark.parametrize("H,P,D,dtype", [(1, 16, 128, torch.bfloat16), (2, 16, 64, torch.bfloat16),
+                                         (3, 5, 7, torch.bfloat16), (4, 16, 2, torch.float32),
+                                         (8, 16, 128, torch.bfloat16), (8, 1, 64, torch.float32)])
+def test_set_kv_buffer_slots_far_past_the_pool(gpu, H, P, D, dtype):
+    """A slot outside the pool stores nothing however large it is: a row of
+    heads x slot leaves 64 bits from 2^63 / H on.  Guards lie on both sides."""
+    from vortex_torch.cache import set_kv_buffer_launcher
+
+    pages, guard = 7, 130 * H * P
+    far = [pages * P, (1 << 31) - 1, 1 << 31, 1 << 32, 1 << 40, (1 << 63) // H - 1, (1 << 63) - 1, (1 << 63) - P,
+           *(1 << b for b in range(57, 63)), *((1 << b) + 3 * P + 2 for b in range(57, 63)), -1, -(1 << 63)]
+    loc = torch.tensor([pages * P - 1, *(min(x, (1 << 63) - 1) for x in far)], device=gpu)
+    buffers = torch.full((2, guard + pages * H * P + guard, D), 7.0, dtype=dtype, device=gpu)
+    k, v = (b[guard:-guard].view(pages * H, P, D) for b in buffers)
+    nk, nv = torch.rand((2, loc.numel(), H, D), device=gpu).to(dtype)
+    set_kv_buffer_launcher(k, v, nk, nv, loc, P)
+    for pool, new in ((k, nk), (v, nv)):
+        last = pool.view(pages, H, P, D)[-1, :, -1]
+        assert torch.equal(last, new[0])
+        last.fill_(7.0)
+    assert bool((buffers == 7).all())
+
+
 def test_set_kv_then_cmean(gpu):
     """Decode step on the cache side: the new tokens go into the pool, then
     CMean of the pages they close equals the oracle's mean of the new pool."""

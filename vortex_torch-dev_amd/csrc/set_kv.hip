@@ -22,6 +22,7 @@ struct SetKvArgs {
   unsigned char* k;
   unsigned char* v;
   int64_t cache_rows;
+  int64_t last_page;  // the pool's last page, -1: none
   const unsigned char* nk;
   const unsigned char* nv;
   const int64_t* loc;
@@ -44,7 +45,9 @@ __global__ __launch_bounds__(kThreads) void set_kv_kernel(SetKvArgs a) {
     const int h = (int)(r - i * a.heads);
     const long long pos = a.loc[i];
     if (pos < 0) continue;
-    const long long dst = (pos / a.page) * ((long long)a.page * a.heads) + (long long)h * a.page + pos % a.page;
+    const long long page = pos / a.page;
+    if (page > a.last_page) continue;  // (first of all: a far page's row leaves 64 bits and may come back inside)
+    const long long dst = page * ((long long)a.page * a.heads) + (long long)h * a.page + (pos - page * a.page);
     if (dst >= a.cache_rows) continue;
     const long long so = r * a.row_bytes + u * kW;
     const long long d_o = dst * a.row_bytes + u * kW;
@@ -77,6 +80,7 @@ extern "C" int vtx_set_kv_buffer(void* k_cache, void* v_cache, int64_t cache_row
   a.k = static_cast<unsigned char*>(k_cache);
   a.v = static_cast<unsigned char*>(v_cache);
   a.cache_rows = cache_rows;
+  a.last_page = cache_rows > 0 ? (cache_rows - 1) / ((int64_t)page_size * num_kv_heads) : -1;
   a.nk = static_cast<const unsigned char*>(new_k);
   a.nv = static_cast<const unsigned char*>(new_v);
   a.loc = loc;
