@@ -274,6 +274,57 @@ def test_attention_nan_scores_give_nan(gpu):
     assert bool(nan[:2].all()) and not bool(nan[2].any())
 
 
+# (shared pages, own tokens): a request's only own token next to longer ones; workgroups of four
+# short requests; nothing shared, finished where they are or joined; several row tiles; four-wave joins
+NAN_TABLES = {
+    "few": [(20, [1, 40, 1])],
+    "many": [(20, [1] * 90)],
+    "alone": [(0, [1]), (0, [5])],
+    "many_alone": [(0, [1])] * 90,
+    "rows": [(12, [1 + 7 * (i % 5) for i in range(40)])],
+    "long": [(1200, [1, 9000])],
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("name", NAN_TABLES)
+def test_attention_keeps_nan_where_nothing_else_is_seen(gpu, name, D):
+    """A query of NaN, and a NaN key that is all a request holds of its own or
+    all it holds at all, give NaN in just the rows that see them, whatever way
+    the tokens are divided; all other rows keep their bits."""
+    H, G, P = (1, 2, 16) if name == "long" else (8, 2, 16)
+    indptr, indices, last, _ = table = _table(NAN_TABLES[name], P, H, 5)
+    q, k, v = _inputs(table, P, H, G, D, 0, gpu)
+    t = [x.to(gpu) for x in (indptr, indices, last)]
+    B = (indptr.numel() - 1) // H
+    plan = plan_shared_prefix(t[0], t[1], B, H, G, D, P)
+    clean = shared_prefix_decode_attention(q, k, v, *t, plan)
+    assert not bool(clean.isnan().any())
+
+    def check(q, k, rows):
+        got = shared_prefix_decode_attention(q, k, v, *t, plan)
+        assert bool(got[rows].isnan().all())
+        assert torch.equal(got[~rows], clean[~rows])
+
+    none = torch.zeros((B * H, G), dtype=torch.bool, device=gpu)
+    turned, rows = q.clone(), none.clone()
+    turned[0, 1] = turned[-1, 0] = float("nan")
+    rows[0, 1] = rows[-1, 0] = True
+    check(turned, k, rows)
+    keys, rows = k.clone(), none.clone()
+    keys[indices[indptr[1] - 1], 0] = float("nan")  # the first token that segment 0 does not share
+    rows[0] = True
+    check(q, keys, rows)
+    shared = int(plan.shared_pages[0])
+    keys, rows = k.clone(), none.clone()
+    keys[indices[indptr[0]:indptr[1]].long()] = float("nan")  # all of segment 0's, and who shares them
+    rows[0] = True
+    if shared:
+        rows[::H] = plan.leaders.view(B, H)[:, :1] == 0
+    check(q, keys, rows)
+
+
 @pytest.mark.gpu
 def test_attention_follows_last_page_lengths(gpu):
     """kv_last_page_len may change after the plan."""

@@ -307,6 +307,18 @@ __device__ __forceinline__ uint2 result4(const float4& O, float L) {
   return uint2{vtx::bf16_pair(O.x * inv, O.y * inv), vtx::bf16_pair(O.z * inv, O.w * inv)};
 }
 
+// A wave's maximum and sum, whole, as they leave it.  A maximum passes NaN scores
+// by, so rows of which nothing else was seen still have -inf, which the joins
+// take for "no tokens": they get a finite one, and their NaN stays in every sum.
+struct Stats {
+  float m, l;
+};
+template <int kD>
+__device__ __forceinline__ Stats stats_of(const Rows<kD>& w) {
+  const float l = w.l + vtx::xshfl(w.l, 32);
+  return Stats{l != l ? 0.f : w.m, l};
+}
+
 // A wave's output to its stretch of LDS: row r's 16-byte piece x at x ^ r.
 template <int kD>
 __device__ __forceinline__ void spread(const Rows<kD>& w, float* to) {
@@ -329,19 +341,19 @@ __device__ __forceinline__ void leave_apart(const SharedArgs& a, const Rows<kD>&
                                             long long q0) {
   constexpr int kOut = kD / 4;
   const int lane = vtx::lane_id();
-  const float l = w.l + vtx::xshfl(w.l, 32);
+  const Stats st = stats_of(w);
   spread<kD>(w, lds);
   wave_lds_fence();
   if (out >= 0 && (long long)out + rows > a.max_rows) return;
   for (int x0 = 0; x0 < rows * kOut; x0 += vtx::kWave) {
     const int x = x0 + lane, r = x / kOut, pc = x % kOut;
-    const float L = __shfl(l, r % 32);
+    const float L = __shfl(st.l, r % 32);
     if (r >= rows) continue;
     const float4 O = reinterpret_cast<const float4*>(lds)[r * kOut + (pc ^ (r % kOut))];
     if (out < 0) *reinterpret_cast<uint2*>(a.o + (q0 + r) * kD + pc * 4) = result4(O, L);
     else *reinterpret_cast<float4*>(a.acc + ((long long)out + r) * kD + pc * 4) = O;
   }
-  if (out >= 0 && lane < rows) a.ml[(long long)out + lane] = float2{w.m, l};
+  if (out >= 0 && lane < rows) a.ml[(long long)out + lane] = float2{st.m, st.l};
 }
 
 template <int kD, bool kFar>
@@ -540,10 +552,10 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
   constexpr int kOut = kCols<kD> / 4;  // pieces of a wave's part of an output row
   {
     const int r = lane % 32;
-    const float l = w.l + vtx::xshfl(w.l, 32);
+    const Stats st = stats_of(w);
     if (lane < 32) {
-      s_m[wave][r] = w.m;
-      s_l[wave][r] = l;
+      s_m[wave][r] = st.m;
+      s_l[wave][r] = st.l;
     }
     spread<kD>(w, reinterpret_cast<float*>(part(wave)));
   }
