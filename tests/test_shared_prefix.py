@@ -646,6 +646,27 @@ def test_calls_run_on_the_tensors_device(monkeypatch):
         assert names.count(n) == 1
 
 
+def test_attention_without_memory_for_its_scratch_raises(monkeypatch):
+    """No other operator takes its place: what a call gives does not depend on the memory that is free."""
+    called = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: called.append(name) or (1024 if name.endswith("_len") else 0)
+
+    def full(*a, **k):
+        raise torch.OutOfMemoryError("full")
+
+    monkeypatch.setattr(_hip, "_lib", Lib())
+    monkeypatch.setattr(_hip, "_stream_of", lambda index: 0)
+    monkeypatch.setattr(_hip, "_scratch_lasts", lambda stream: True)
+    out = torch.zeros((4, 2, 64), dtype=torch.bfloat16)
+    monkeypatch.setattr(torch, "empty", full)
+    with pytest.raises(torch.OutOfMemoryError):
+        _call(monkeypatch, out=out)
+    assert called == ["vtx_shared_prefix_workspace_len"]
+
+
 def test_need_a_gpu():
     with pytest.raises(RuntimeError, match="no CPU implementation"):
         plan_shared_prefix(torch.zeros(5, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), 2, 2, 2, 64, 16)

@@ -1354,8 +1354,11 @@ def plan_shared_prefix(kv_indptr, kv_indices, group_ids, batch_size, num_kv_head
 def shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan, batch_size,
                                    num_kv_heads, group_size, sm_scale) -> None:
     """paged_decode_attention with the pages that a plan found shared read once
-    per run.  Its partial results need scratch from torch's allocator; without
-    (see _scratch) paged decode attention itself runs, which needs none."""
+    per run.  Its partial results need scratch from torch's allocator, whose
+    OutOfMemoryError is the caller's (another operator in its place would make
+    the result a matter of free memory).  In a capture that torch did not begin
+    no scratch lasts: paged decode attention itself runs, which needs none, and
+    gives zeros where a score is NaN."""
     lib = _lib or load_library()
     index = _device_index(q, o, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, plan)
     if _current_device() != index:
@@ -1384,10 +1387,7 @@ def shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices
     floats = lib.vtx_shared_prefix_workspace_len(B, H, G, D)
     ws = None
     if floats > 0 and _scratch_lasts(stream):
-        try:
-            ws = torch.empty(floats, dtype=torch.float32, device=q.device)
-        except torch.OutOfMemoryError:
-            pass
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device)
     if ws is None and floats > 0:
         rc = lib.vtx_paged_decode_attention(
             q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), rows, kv_indptr.data_ptr(),
