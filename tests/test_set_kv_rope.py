@@ -247,6 +247,7 @@ def _arguments(**changes):
 
 
 _POOL = torch.zeros((4, 8, 16), dtype=torch.bfloat16)
+_ARENA = torch.zeros(1024, dtype=torch.bfloat16)
 _ROWS = torch.zeros((3, 8 * 16), dtype=torch.bfloat16).unflatten(1, (8, 16))
 
 
@@ -283,6 +284,39 @@ def test_rope_append_refusals(monkeypatch, changes, says):
     monkeypatch.setattr(_hip, "_current_device", lambda: 0)
     with pytest.raises(RuntimeError, match=says):
         set_kv_buffer_rope(**_arguments(**changes))
+
+
+@pytest.mark.parametrize("changes, says", [
+    (dict(k_cache=_ARENA[256:768].view(4, 8, 16), new_k=_ARENA[192:288].view(3, 2, 16)), "new_k lies in the pools"),
+    (dict(v_cache=_ARENA[256:768].view(4, 8, 16), new_v=_ARENA[161:257].view(3, 2, 16)), "new_v lies in the pools"),
+    (dict(k_cache=_ARENA[256:768].view(4, 8, 16), q=_ARENA[:192].view(3, 4, 16).as_strided((3, 4, 16), (128, 16, 1))),
+     "q lies in the pools"),
+    (dict(k_cache=_ARENA[256:768].view(4, 8, 16), q_out=_ARENA[65:257].view(3, 4, 16)), "q_out lies in the pools"),
+])
+def test_rope_append_refuses_rows_that_reach_into_a_pool(monkeypatch, changes, says):
+    """They begin before it."""
+    test_rope_append_refusals(monkeypatch, changes, says)
+
+
+def test_rope_append_takes_rows_that_end_where_a_pool_begins(monkeypatch):
+    """Rows up to a pool's first byte, and from its last one on, are answered."""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append(name) or 0
+
+    monkeypatch.setattr(_hip, "_lib", Lib())
+    monkeypatch.setattr(_hip, "_device_index", lambda *t: 0)
+    monkeypatch.setattr(_hip, "_current_device", lambda: 0)
+    monkeypatch.setattr(_hip, "_stream_of", lambda index: 0)
+    pool = _ARENA[256:768].view(4, 8, 16)
+    for at in (0, 64, 768, 800):  # (192 elements of q, 96 of new_k and of new_v)
+        q, rows = _ARENA[at:at + 192].view(3, 4, 16), _ARENA[at:at + 96].view(3, 2, 16)
+        for changes in (dict(q=q), dict(new_k=rows), dict(new_v=rows), dict(q_out=q)):
+            set_kv_buffer_rope(**_arguments(k_cache=pool, **changes))
+            set_kv_buffer_rope(**_arguments(v_cache=pool, **changes))
+    assert calls == ["vtx_set_kv_buffer_rope"] * 32
 
 
 def test_rope_append_needs_a_gpu():

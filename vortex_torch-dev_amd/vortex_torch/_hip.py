@@ -1090,6 +1090,11 @@ def _span(t: torch.Tensor) -> tuple:
     return first, first + size * ((n - 1) * t.stride(0) + (h - 1) * t.stride(1) + d)
 
 
+def _clear(first: int, end: int, kp: int, vp: int, pool: int) -> bool:
+    """Whether the bytes first .. end are clear of two pools of `pool` bytes at kp and vp."""
+    return (end <= kp or first >= kp + pool) and (end <= vp or first >= vp + pool)
+
+
 def _tokens_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two [tokens, heads, head_dim] tensors share no memory: apart as
     a whole, or column ranges of the same rows (slices of one projection)."""
@@ -1120,21 +1125,27 @@ def _rope_fits(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos
     if len(new) != 3 or len(pools) != 3 or new_v.shape != new or v_cache.shape != pools or dtype not in _ROPE_DTYPES:
         return False
     nnz, H, D = new
-    kp, vp, pool = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() * k_cache.element_size()
+    kp, vp, size = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.element_size()
+    pool = k_cache.numel() * size
     if q is not None:
-        like = q.shape
-        if len(like) != 3 or like[0] != nnz or like[2] != D or q.dtype is not dtype or q.stride(2) != 1 \
-                or kp <= q.data_ptr() < kp + pool or vp <= q.data_ptr() < vp + pool:
+        like, (s0, s1, dense) = q.shape, q.stride() if q.dim() == 3 else (0, 0, 0)
+        if dense != 1 or like[0] != nnz or like[2] != D or q.dtype is not dtype:
             return False
+        first = q.data_ptr()
+        if not _clear(first, first + size * ((nnz - 1) * s0 + (like[1] - 1) * s1 + D), kp, vp, pool):
+            return False
+    k0, k1, k2 = new_k.stride()
+    v0, v1, v2 = new_v.stride()
+    k, v = new_k.data_ptr(), new_v.data_ptr()
     return (H > 0 and D > 0 and pools[2] == D and pools[1] == page_size and pools[0] % H == 0
             and new_v.dtype is dtype and k_cache.dtype is dtype and v_cache.dtype is dtype
-            and new_k.stride(2) == 1 and new_v.stride(2) == 1 and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k2 == 1 and v2 == 1 and k_cache.is_contiguous() and v_cache.is_contiguous()
             and loc.dtype is torch.int64 and positions.dtype is torch.int64 and cos_sin_cache.dtype is torch.float32
             and loc.is_contiguous() and positions.is_contiguous() and cos_sin_cache.is_contiguous()
             and loc.numel() >= nnz and positions.numel() >= nnz and cos_sin_cache.dim() == 2
             and (kp + pool <= vp or vp + pool <= kp)
-            and not (kp <= new_k.data_ptr() < kp + pool or vp <= new_k.data_ptr() < vp + pool)
-            and not (kp <= new_v.data_ptr() < kp + pool or vp <= new_v.data_ptr() < vp + pool))
+            and _clear(k, k + size * ((nnz - 1) * k0 + (H - 1) * k1 + D), kp, vp, pool)
+            and _clear(v, v + size * ((nnz - 1) * v0 + (H - 1) * v1 + D), kp, vp, pool))
 
 
 def _rope_refusal(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, cos_sin_cache, q_out) -> str:
@@ -1182,7 +1193,8 @@ def _rope_refusal(k_cache, v_cache, q, new_k, new_v, loc, page_size, positions, 
     if pool and -pool < kp - vp < pool:
         return "k_cache and v_cache share memory"
     for t, n in rows:
-        if kp <= t.data_ptr() < kp + pool or vp <= t.data_ptr() < vp + pool:
+        first, end = _span(t)
+        if first < end and not _clear(first, end, kp, vp, pool):
             return f"{n} lies in the pools that the call writes"
     if q_out is not None and q_out.numel():
         if not _rows_distinct(q_out):
