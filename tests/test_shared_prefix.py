@@ -365,6 +365,95 @@ def test_attention_pool_past_32_bits(gpu, D, requests, G):
     assert bool(((got.view(-1, D).double() - want).abs() <= bound).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,requests,G", [(128, 2, 4), (64, 20, 8), (128, 20, 8), (256, 12, 4)])
+def test_attention_pool_past_31_bits(gpu, D, requests, G):
+    """Pages at the end of pools of 3.5 GiB, which 32 bits of offset still reach."""
+    P, shared = 16, 30
+    pages = (7 << 29) // (P * D * 2)
+    mine = shared + requests
+    k, v = (torch.zeros((pages, P, D), dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    k[-mine:].normal_()
+    v[-mine:].normal_()
+    k[:mine] = float("nan")
+    rows = torch.arange(pages - mine, pages, dtype=torch.int32)
+    indices = torch.cat([torch.cat([rows[:shared], rows[shared + i:shared + i + 1]]) for i in range(requests)])
+    indptr = torch.arange(requests + 1, dtype=torch.int32) * (shared + 1)
+    last = torch.tensor([1 + (5 * i) % P for i in range(requests)], dtype=torch.int32)
+    q = torch.randn((requests, G, D), dtype=torch.bfloat16, device=gpu)
+    t = [x.to(gpu) for x in (indptr, indices, last)]
+    plan = plan_shared_prefix(t[0], t[1], requests, 1, G, D, P)
+    got = shared_prefix_decode_attention(q, k, v, *t, plan)
+    want, bound = _exact(q, k, v, indptr, t[1], last, D ** -0.5)
+    assert bool(((got.view(-1, D).double() - want).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zero_queries", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_rows_of_many_partial_results(gpu, D, zero_queries):
+    """More than 5120 / D of them each on average, which four waves join; the
+    last batch of them is ragged, and one row's fewer than a batch."""
+    _attention(_table([(1200, [100, 20000])], 16, 1, 2), 16, 1, 4, D, gpu, zero_queries=zero_queries)
+    _attention(_table([(1500, [9000, 1, 4000]), (0, [40000])], 16, 1, 3), 16, 1, 1, D, gpu, zero_queries=zero_queries)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("name", ["few", "mixed", "long"])
+def test_table_with_room_behind_it(gpu, name, D):
+    """kv_indices as a server holds it, sized for the longest contexts: what lies
+    behind the last segment is not read, and the plan finds the same."""
+    groups, P = TABLES[name]
+    H, G = 2, 2
+    indptr, indices, last, pages = table = _table(groups, P, H, 5)
+    B = (indptr.numel() - 1) // H
+    q, k, v = _inputs(table, P, H, G, D, 1, gpu)
+    t = [x.to(gpu) for x in (indptr, indices, last)]
+    wide = torch.full((B * H * 8192,), -7, dtype=torch.int32, device=gpu)
+    wide[:indices.numel()] = t[1]
+    plan = plan_shared_prefix(t[0], wide, B, H, G, D, P)
+    leaders, shared = _plain_plan(indptr, indices, B, H)
+    assert plan.leaders.tolist() == leaders and plan.shared_pages.tolist() == shared
+    got = shared_prefix_decode_attention(q, k, v, t[0], wide, t[2], plan)
+    want, bound = _exact(q, k, v, indptr, t[1], last, D ** -0.5)
+    assert bool(((got.view(-1, D).double() - want).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+def test_prefixes_behind_a_common_page(gpu):
+    """Requests that all begin with one page and go on in groups: without ids
+    they are one run and share that page alone; ids give each group its own."""
+    H, G, D, P, longest = 2, 2, 128, 16, 40
+    r = random.Random(4)
+    sizes, own = [4, 1, 3, 2], 3  # requests of a group; pages of their own, at most
+    free = list(range(1, 1 + len(sizes) * longest + sum(sizes) * own))
+    r.shuffle(free)
+    rows, ids, lengths = [], [], []
+    for g, n in enumerate(sizes):
+        body = [free.pop() for _ in range(longest - 7 * g)]
+        lengths += [1 + len(body)] * n
+        ids += [g] * n
+        rows += [[0] + body + [free.pop() for _ in range(r.randint(1, own))] for _ in range(n)]
+    B = len(rows)
+    indices = torch.tensor([p * H + h for row in rows for h in range(H) for p in row], dtype=torch.int32)
+    indptr = torch.tensor([0] + [len(row) for row in rows for _ in range(H)], dtype=torch.int32).cumsum(0).int()
+    last = torch.tensor([r.randint(1, P) for _ in range(B)], dtype=torch.int32).repeat_interleave(H)
+    table = indptr, indices, last, len(free) + sum(sizes) * own + len(sizes) * longest + 1
+    t = [x.to(gpu) for x in (indptr, indices)]
+    plan = plan_shared_prefix(*t, B, H, G, D, P)
+    assert plan.leaders.tolist() == [0] * (B * H) and plan.shared_pages.tolist() == [1] * (B * H)
+    named = torch.tensor(ids, dtype=torch.int32, device=gpu)
+    plan = plan_shared_prefix(*t, B, H, G, D, P, group_ids=named)
+    first = [ids.index(g) for g in ids]
+    assert plan.leaders.view(B, H)[:, 0].tolist() == first == plan.leaders.view(B, H)[:, 1].tolist()
+    want = [0 if sizes[g] == 1 else n for g, n in zip(ids, lengths)]
+    assert plan.shared_pages.view(B, H)[:, 0].tolist() == want == plan.shared_pages.view(B, H)[:, 1].tolist()
+    for g in (None, named):
+        _attention(table, P, H, G, D, gpu, ids=g)
+        _attention(table, P, H, G, D, gpu, ids=g, zero_queries=True)
+
+
 # Short requests share workgroups where there are many: with a run's pages, without
 # (finished where they are), next to long and empty ones, at a batch's ragged end.
 MANY = {
