@@ -722,7 +722,9 @@ int vtx_paged_decode_attention_supported(int32_t head_dim, int32_t group_size);
  * pages form a run while their group_ids ([B] int32) are equal; group_ids NULL:
  * while their first entries are equal.  A run of several requests shares its
  * longest common prefix of entries, less than each one's page count (a request
- * keeps its last page to itself); a run of one shares nothing.  A segment whose
+ * keeps its last page to itself); a run of one shares nothing.  Sharing has one
+ * level: requests that all begin with one page are one run without ids, which
+ * shares what all of them do; ids keep groups behind that page apart.  A segment whose
  * range lies outside kv_indices counts as empty and ends a run.
  * plan: vtx_shared_prefix_plan_len int32, 32-byte aligned.  With S = B * H,
  * plan[16 + s] receives the first request of segment s's run and
@@ -739,13 +741,14 @@ int vtx_plan_shared_prefix(const int32_t* kv_indptr, const int32_t* kv_indices, 
  * of (with the same sizes), every shared page read once for its run instead of
  * once for each request, and the scores and outputs on the matrix cores: the
  * probabilities are rounded to bf16 (and sum to one as rounded), the rest is
- * fp32.  A NaN score gives NaN (there: zeros).  kv_last_page_len may have
+ * fp32.  A NaN score gives NaN (there: zeros).  kv_indptr is the plan's table's;
+ * where segments lie is read from the plan.  kv_last_page_len may have
  * changed since the plan was made; after any other change of the table plan
  * anew (the results are undefined otherwise, but no access leaves a buffer).
  * workspace: vtx_shared_prefix_workspace_len floats, 16-byte aligned, its
  * contents neither read nor kept across calls; calls that may overlap need one
  * each.  A request's last bits depend on the other requests of the table (how
- * its tokens are divided).
+ * its tokens are divided) and on kv_indices_len (how its results are joined).
  * head_dim 64, 128 or 256; group_size 1..8; at most 2^22 segments and 2^32
  * pool tokens (pool rows x page_size).
  */

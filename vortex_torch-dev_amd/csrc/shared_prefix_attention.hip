@@ -26,9 +26,8 @@
 // straight to LDS one tile ahead.
 //
 // Bound by HBM up to about 150 rows (5.7 TB/s in 32 runs of 8 requests behind 4k
-// tokens), by the matrix cores and exponentials beyond: 1.28 PFLOP/s inside a
-// long chunk of 128 rows x 128 columns, 860 TFLOP/s over the launch for 2048 rows
-// and 8 heads behind 16k tokens.
+// tokens), by the matrix cores, what feeds them and the exponentials beyond (886
+// TFLOP/s over both launches for 2048 rows and 8 heads behind 16k tokens, 155 us).
 #include "vtx_shared_prefix.h"
 
 #include <type_traits>
@@ -47,7 +46,6 @@ struct SharedArgs {
   const uint16_t* v;
   int64_t rows;  // pool rows (page * H + h)
   uint32_t pool_bytes;  // 0: over 4 GiB
-  const int32_t* indptr;
   const int32_t* indices;
   int64_t indices_len;
   const int32_t* last_len;
@@ -102,7 +100,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // buffer loads: 32-bit offsets, and LDS reads behind a copy in flight are waited
 // for one by one; behind the other form, which counts as an LDS operation too, the
 // compiler waits for all of them (256 requests of 8 heads each behind 16k tokens:
-// 175 us a layer, 186 by the other form).
+// 155 us a layer, 159 by the other form).
 template <bool kFar>
 struct Pool {
   const uint16_t* base;
@@ -125,8 +123,7 @@ __device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f7
 
 // Output columns of a wave: all, or half of 256 (two waves share 32 rows and
 // both compute their scores: with all columns a lane's outputs and queries leave
-// no registers for more, and the attention of 17 requests behind 5k tokens took
-// 30.3 us, this way 22.8).
+// no registers for more).
 template <int kD>
 constexpr int kCols = kD == 256 ? 128 : kD;
 // Tokens of a tile that all waves share.
@@ -145,7 +142,7 @@ struct Rows {
 // The running maximum follows the scores only when they outgrow it by so much
 // (base 2): until then weights up to 2^8 are as exact as weights up to 1, and
 // most tiles leave the outputs as they are (256 requests of 8 heads each behind
-// 16k tokens 168 us a layer, following every maximum 176).
+// 16k tokens 155 us a layer, following every maximum 159).
 constexpr float kGrowth = 8.f;
 
 // kN x 32 tokens at kt / vt in LDS; bit i of mask: token i counts.  kAhead: the
@@ -622,9 +619,9 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void shared_prefix_atte
 // every fourth batch of them and meet in LDS.  A partial row is read in 16-byte
 // pieces, kAtOnce rows side by side in the wave; before it reads them, lane i
 // weighs the i-th of up to 64 rows.  Four waves pay where a row has many (a layer
-// by one / four: 48 requests of one behind 32k, D 64, 60 and more each, 29.4 /
-// 27.2 us; 17 behind 5k, D 256, 40 each, 26.2 / 23.6) and cost where not (64 of 4
-// behind 8k, 32 each, 32.0 / 34.1; 16 of 4 behind 4k, D 64, 33 each, 10.8 / 12.7).
+// by one / four: 48 requests of one behind 32k, D 64, 65 each, 31.4 / 29.1 us; 17
+// behind 5k, D 256, 25 each, 24.3 / 22.0) and cost where not (64 of 4 behind 8k
+// 27.6 / 28.6; 16 of 4 behind 4k, D 64, 12.8 / 14.4).
 constexpr int kJoinFour = 5120;  // partial rows x columns from which on
 constexpr int kJoinWaves = 4;
 template <int kD, bool kFour>
@@ -790,7 +787,6 @@ extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o
   a.rows = cache_rows;
   const int64_t bytes = cache_rows * page_size * head_dim * 2;
   a.pool_bytes = bytes <= 0xffffffffLL ? (uint32_t)bytes : 0u;
-  a.indptr = kv_indptr;
   a.indices = kv_indices;
   a.indices_len = kv_indices_len;
   a.last_len = kv_last_page_len;
@@ -810,8 +806,12 @@ extern "C" int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o
   a.acc = workspace;
   a.ml = reinterpret_cast<float2*>(workspace + rows * head_dim);
   a.max_rows = rows;
-  // A row's partial results, at most: its run's chunks, a slot each and kMinChunk
-  // tokens long, and its own.
+  // A row's partial results, by what the host knows: one run's chunks, a slot each,
+  // or the segments' mean length, were the table's buffer full, in chunks of
+  // kMinChunk tokens.  A guess: a row of an uneven table can have more, one of a table
+  // with room behind it fewer (16 of 4 behind 4k, D 64, in a buffer for 128k tokens
+  // each 14.4 us a layer, 12.7 in one that fits).  Either join is right for any count;
+  // the order of its sums, and so a result's last bits, follow the buffer's length.
   const int64_t tiles = ((int64_t)batch_size * group_size + tile_rows(head_dim) - 1) / tile_rows(head_dim);
   const int64_t parts = at.slots / tiles, longest = kv_indices_len * page_size / (S * kMinChunk) + 1;
   a.join_four = (parts < longest ? parts : longest) * head_dim > kJoinFour;

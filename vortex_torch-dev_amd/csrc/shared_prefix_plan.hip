@@ -9,13 +9,21 @@
 // that each keeps at least its last page (the only one that may be partial).
 // The table decides: what ids promise is checked against the entries.
 //
-// Two launches.  One wave per segment finds the length of the prefix that it
-// has in common with the request before (the minimum of these over a run is the
-// run's).  One workgroup per kv head then scans its requests into runs and
-// writes the head's work items: (rows of a run or a request) x (entries of a
-// chunk), tile_rows rows at most, chunks sized so that a head has its share of
-// the device's workgroup slots.  (One workgroup for all heads is bound by its
-// instructions: 2048 segments 21 us, 512 11.)
+// Sharing has one level, the minimum over the run: where all requests begin
+// with a page and groups of them go on alike behind it, only ids tell the groups
+// apart (32 groups of eight behind 4k tokens, 8 x 2 heads, all behind one common
+// page: 315 us a layer without ids, 98 with).
+//
+// Two launches, or one for few requests.  One wave per segment finds the length
+// of the prefix that it has in common with the request before (the minimum of
+// these over a run is the run's).  One workgroup per kv head then scans its
+// requests into runs and writes the head's work items: (rows of a run or a
+// request) x (entries of a chunk), tile_rows rows at most, chunks sized so that a
+// head has its share of the device's workgroup slots.  (One workgroup for all
+// heads is bound by its instructions: plans of 265 requests of 8 heads 29.8 us,
+// this way 10.7; of 69 16.6 and 9.1.)  Latency bounds both: the loads of the
+// comparison, then a chain of steps in one workgroup.  More requests than fit
+// in LDS keep their numbers in the plan's memory (4096 of 8 heads 106 us).
 #include "vtx_shared_prefix.h"
 
 #include "vtx_device.h"
@@ -136,9 +144,10 @@ __device__ __forceinline__ uint32_t chunks(uint32_t n, uint32_t per, uint32_t& p
 }
 
 constexpr int kLdsRequests = 2048;
-// Requests up to which, in a table of one pass of entries each, the second launch
-// compares them itself (4 requests 8.5 us in two launches, 6.7 in one; 16 8.6 and
-// 8.9, and 2.9 us less of the host's time; 32 8.6 and 11.5).
+// Requests up to which, in a table whose buffer has room for no more than one pass
+// of entries a segment (the host does not know how many it holds), the second launch
+// compares them itself (4 requests 8.3 us in two launches, 6.6 in one; 16 8.4 and
+// 8.8, and a launch less of the host's time; 32 8.5 and 11.5).
 constexpr int kFewRequests = 16;
 
 // Per request of the head (a run's numbers at its first one), in LDS or in the plan.
@@ -377,8 +386,8 @@ Layout layout_of(int64_t batch, int64_t heads, int group_size, int head_dim, int
   const int64_t segments = batch * heads, tile = tile_rows(head_dim);
   // All heads' items together: the workgroups that the device holds at a time.
   // (Twice as many, each half as long: 256 requests of 8 heads each behind 16k
-  // tokens 225 us either way, 48 of one behind 32k, D 64, 47.4 us for 35.3, 64 of
-  // 4 behind 32k 82.2 for 69.0: more partial results.)
+  // tokens 165 us a layer for 158, 64 of 4 behind 32k 76 for 63: more partial
+  // results.)
   const int64_t slots = cus * (head_dim == 64 ? 3 : 2);
   l.slots = (slots + heads - 1) / heads;
   l.cus = (cus + heads - 1) / heads;

@@ -10,21 +10,21 @@ namespace vtx_prefix {
 constexpr int tile_rows(int head_dim) { return head_dim == 256 ? 64 : 128; }
 
 // Tokens from which a run's pages are read once for all: fewer cost more in
-// partial results (64 tokens of eight requests, 32 runs of 8 heads each: 15.3 us a
-// layer read by each, 20.3 once; 200 tokens 35.1 and 22.7).
+// partial results (a layer of 32 runs of eight requests of 8 x 2 heads, read by each
+// and once: behind up to 64 tokens 17.0 / 21.2 us, up to 200 35.0 / 24.3, of which
+// those past 128 alone once 29.4).  How many requests share them is not looked at.
 constexpr int kMinShared = 128;
 // Tokens of a chunk: one item per compute unit from kMinChunk on, and past
 // kFewChunk one per workgroup slot (us a layer with 256 / 512 / 1024 for it: 64
-// requests of 8 x 4 heads behind 8k 33.0 / 28.1 / 29.4, 256 of 8 x 2 behind 8k 46.7 /
-// 43.8 / 40.0, 32 of 8 x 2 behind 16k 34.0 / 30.5 / 31.4, 48 of 8 x 1 behind 32k, D 64,
-// 29.7 / 29.1 / 31.8, 64 of 8 x 4 behind 32k 66.9 / 62.6 / 66.6).
+// requests of 8 x 4 heads behind 8k 33.2 / 27.7 / 29.4, 256 of 8 x 2 behind 8k 46.0 /
+// 44.3 / 39.7, 32 of 8 x 2 behind 16k 34.2 / 30.5 / 31.4, 48 of 8 x 1 behind 32k, D 64,
+// 28.8 / 25.1 / 29.5, 64 of 8 x 4 behind 32k 64.9 / 61.8 / 60.6).
 constexpr int kMinChunk = 128, kFewChunk = 512;
 // Own tokens up to which four requests share a workgroup, a wave each, where a
 // head has more requests than half its workgroup slots (four waves to so few
 // tokens of one request are all latency: 256 requests of up to 128 own tokens
-// behind 4k, D 64, 26.6 us a layer, apart 19.2; 256 of 8 heads each with up to 16
-// behind 16k 176 and 163; but 4 behind 1k 9.0 and 10.0, 32 behind 4k, D 64, 12.8
-// and 13.8).
+// behind 4k, D 64, 24.7 us a layer, apart 20.6; 256 of 8 heads each with up to 16
+// behind 16k 163 and 155; but 4 behind 1k 10.2 and 10.8).
 constexpr int short_tokens(int head_dim) { return head_dim == 256 ? 0 : 128; }
 static_assert(short_tokens(64) <= kMinChunk, "one chunk each");
 constexpr int kXcds = 8;

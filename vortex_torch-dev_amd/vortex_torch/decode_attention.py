@@ -83,7 +83,10 @@ def plan_shared_prefix(kv_indptr: torch.Tensor, kv_indices: torch.Tensor, batch_
     consecutive requests form a run while their ``group_ids`` (int32 [batch])
     are equal, or without ids while their first pages are; the run shares its
     longest common prefix of entries (which is looked up: ids promise nothing),
-    except each request's own last page.  group_size: query heads per kv head.
+    except each request's own last page.  Sharing has one level: where all requests
+    begin with one page (a system prompt) and groups of them share what follows,
+    pass the groups' ids, or that page is all that is shared.  group_size: query
+    heads per kv head.
 
     Plan anew whenever entries or lengths in pages change (``kv_last_page_len``
     may).  ``plan``: an earlier plan of the same sizes to write into, as a
