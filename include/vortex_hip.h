@@ -455,6 +455,10 @@ int vtx_indexer_quest_fused_supported(int32_t head_dim, int32_t group_size);
 #define VTX_DTYPE_F32 1
 #define VTX_DTYPE_F16 2
 
+/* codes of the 8-bit pools */
+#define VTX_CODES_E4M3 0
+#define VTX_CODES_INT8 1
+
 /*
  * Page-finish reduction (CMean / CMax / CMin / CL2Norm).
  * x: bf16 pool [x_rows, rows_per_tile, cols]; row = (loc/page_size)*H + h.
@@ -761,6 +765,83 @@ int vtx_shared_prefix_decode_attention(const uint16_t* q, uint16_t* o, const uin
                                        int32_t batch_size, int32_t num_kv_heads, int32_t group_size,
                                        int32_t head_dim, int32_t page_size, float sm_scale, float* workspace,
                                        int64_t workspace_len, void* stream);
+
+/*
+ * The 8-bit paged cache (no counterpart in the reference, whose pools hold the
+ * model's type): pools [pages * H, page_size, head_dim] of codes, e4m3 (the
+ * finite kind: 448 the largest) or int8, and scales [pages * H, page_size, 2] of
+ * exponent bytes, K's and V's of every token and kv head.  A row holds the values
+ * code * 2^(b - 127), b the least byte of 1 and more by which the row's largest
+ * absolute value fits the codes' largest, 448 or 127; each value is rounded to
+ * the nearest code, ties to even.  A row with an infinity or a NaN is held as
+ * zeros with b = 255 and read as NaN throughout; b = 0, which no row is written
+ * with, reads as zeros.  Values of 2^127 and more may read as infinity.
+ *
+ * vtx_set_kv_buffer_quant: quantises new_k and new_v into the pools, at the rows
+ * of vtx_set_kv_buffer.  dtype: the new rows' (VTX_DTYPE_BF16, _F16 or _F32).
+ * strides: host array of four, in elements: token and head strides of new_k and
+ * new_v, whose rows are dense.  A token whose slot lies outside the pool (a
+ * negative loc: padding) is not stored.  Tokens that share a slot leave a mixture.
+ *
+ * vtx_read_kv_buffer_quant: the values at slots loc, rounded to dtype, to k_out
+ * and v_out ([nnz, H, head_dim] by their strides, as above); zeros where a slot
+ * lies outside the pool.
+ *
+ * head_dim a multiple of 8 up to 512, rows, strides of multiples of 16 bytes and
+ * pools of 8 take vector accesses, others element-wide ones.
+ */
+int vtx_set_kv_buffer_quant(void* k_cache, void* v_cache, void* scales, int64_t cache_rows, const void* new_k,
+                            const void* new_v, const int64_t* strides, const int64_t* loc, int64_t nnz,
+                            int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int32_t codes, int32_t page_size,
+                            void* stream);
+int vtx_read_kv_buffer_quant(const void* k_cache, const void* v_cache, const void* scales, int64_t cache_rows,
+                             void* k_out, void* v_out, const int64_t* strides, const int64_t* loc, int64_t nnz,
+                             int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int32_t codes, int32_t page_size,
+                             void* stream);
+
+/*
+ * vtx_page_reduce_multi, dim 1, over a pool of codes: x [x_rows, page_size, cols],
+ * its bytes scales[(row * page_size + slot) * 2] (pass scales + 1 for V's).  The
+ * outputs are those of the same reductions of a bf16 pool that holds the values,
+ * bit for bit where cols is 64, 128, 256 or 512 (else the sums' order may differ).
+ */
+int vtx_page_reduce_quant(const void* x, const void* scales, int64_t x_rows, int32_t page_size, int32_t cols,
+                          int32_t codes, int32_t n_out, void* const* outs, const int32_t* out_dtypes,
+                          const int32_t* reduce_types, int64_t out_rows, const int64_t* loc, int64_t nnz,
+                          int32_t num_kv_heads, void* stream);
+
+/*
+ * vtx_paged_decode_attention over the 8-bit pools, sparse tables or dense ones:
+ *   o[s * G + g] = sum_t softmax_t(f(sm_scale * q . K[t]) - slopes[h * G + g] * (n - 1 - t)) V[t]
+ * over the n tokens of segment s = b * H + h, t counted in the table's order; with
+ * f(y) = soft_cap * tanh(y / soft_cap), or y for a soft_cap of 0; slopes (fp32,
+ * H * G, may be NULL: none); and with window > 0 only the last `window` tokens.
+ * Products and sums are fp32, the weights exact to 2^-17.  q: bf16 or fp16 (dtype)
+ * rows q + b * q_strides[0] + h * q_strides[1] + g * q_strides[2] (elements); o the
+ * same type, [B * H * G, head_dim], dense.  A segment without tokens gets zeros,
+ * and so does one whose range lies outside kv_indices; entries outside the pool
+ * count as no tokens.  A NaN among a segment's scores or values gives NaN.
+ * kv_indptr is not to decrease (otherwise the results are undefined, but no access
+ * leaves a buffer).
+ * workspace: vtx_quant_decode_attention_workspace_len floats, 16-byte aligned, its
+ * contents neither read nor kept across calls; calls that may overlap need one
+ * each.  With it a table's pages are divided evenly over the card, and a second
+ * launch joins the parts of segments that lie in several divisions: a request's
+ * last bits follow the other requests of the table, and kv_indices_len.  NULL: a
+ * workgroup per segment, one launch, the same bits in every batch.
+ * head_dim 64, 128 or 256; group_size 1..16.
+ */
+int vtx_quant_decode_attention_supported(int32_t head_dim, int32_t group_size);
+int64_t vtx_quant_decode_attention_workspace_len(int32_t batch_size, int32_t num_kv_heads, int32_t group_size,
+                                                 int32_t head_dim, int32_t page_size, int32_t window,
+                                                 int64_t kv_indices_len);
+int vtx_quant_decode_attention(const void* q, const int64_t* q_strides, void* o, const void* k_cache,
+                               const void* v_cache, const void* scales, int64_t cache_rows, const int32_t* kv_indptr,
+                               const int32_t* kv_indices, int64_t kv_indices_len, const int32_t* kv_last_page_len,
+                               int32_t batch_size, int32_t num_kv_heads, int32_t group_size, int32_t head_dim,
+                               int32_t page_size, int32_t dtype, int32_t codes, float sm_scale, float soft_cap,
+                               int32_t window, const float* slopes, float* workspace, int64_t workspace_len,
+                               void* stream);
 
 /*
  * Bandwidth probes (measurement only; no counterpart in the reference).

@@ -4,7 +4,8 @@ Every wrapper validates dtypes, devices, contiguity and sizes of its torch
 tensors, then launches on torch's current HIP stream of the tensors' device.
 No kernel wrapper synchronises or reads device memory, and none allocates but
 ``paged_decode_attention`` and ``shared_prefix_decode_attention`` (scratch,
-where that lasts: see there), ``plan_shared_prefix`` and ``set_kv_buffer_rope``
+where that lasts: see there; ``quant_paged_decode_attention`` too),
+``plan_shared_prefix``, ``set_kv_buffer_rope`` and ``read_kv_buffer_quant``
 (their results, where the caller gives no tensor for them), so they can be
 recorded into a HIP graph (``torch.cuda.graph``).
 
@@ -14,6 +15,7 @@ library, raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import threading
 from pathlib import Path
@@ -151,6 +153,25 @@ _SIGNATURES = {
          _i64, _vp],
         ctypes.c_int,
     ),
+    "vtx_set_kv_buffer_quant": (
+        [_vp, _vp, _vp, _i64, _vp, _vp, ctypes.POINTER(_i64), _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp],
+        ctypes.c_int,
+    ),
+    "vtx_read_kv_buffer_quant": (
+        [_vp, _vp, _vp, _i64, _vp, _vp, ctypes.POINTER(_i64), _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp],
+        ctypes.c_int,
+    ),
+    "vtx_page_reduce_quant": (
+        [_vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp],
+        ctypes.c_int,
+    ),
+    "vtx_quant_decode_attention_supported": ([_i32, _i32], ctypes.c_int),
+    "vtx_quant_decode_attention_workspace_len": ([_i32, _i32, _i32, _i32, _i32, _i32, _i64], ctypes.c_int64),
+    "vtx_quant_decode_attention": (
+        [_vp, ctypes.POINTER(_i64), _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
+         _i32, ctypes.c_float, ctypes.c_float, _i32, _vp, _vp, _i64, _vp],
+        ctypes.c_int,
+    ),
     "vtx_bf16_rounding_check": ([_vp, _vp], ctypes.c_int),
     "vtx_stream_capture_id": ([_vp, ctypes.POINTER(ctypes.c_ulonglong)], ctypes.c_int),
     "vtx_probe_read": ([_vp, _i64, _vp, _i64, ctypes.c_uint32, _vp], ctypes.c_int),
@@ -167,6 +188,7 @@ REDUCE_MEAN, REDUCE_MAX, REDUCE_MIN, REDUCE_L2NORM, REDUCE_SUM = 0, 1, 2, 3, 4
 ROWS_BATCHED, ROWS_PAGED, ROWS_RAGGED = 0, 1, 2
 SEGMENT_SOFTMAX, SEGMENT_NORMALIZE = 0, 1
 DTYPE_BF16, DTYPE_F32, DTYPE_F16 = 0, 1, 2
+CODES_E4M3, CODES_INT8 = 0, 1
 FUSED_AUTO, FUSED_SEGMENT, FUSED_SPLIT = 0, 1, 2
 
 
@@ -1411,6 +1433,258 @@ def shared_prefix_decode_attention(q, o, k_cache, v_cache, kv_indptr, kv_indices
             G, D, P, sm_scale, None if ws is None else ws.data_ptr(), floats, stream)
     if rc:
         _check(rc, "shared_prefix_decode_attention")
+
+
+_CODES = {torch.float8_e4m3fn: CODES_E4M3, torch.int8: CODES_INT8}
+_SCALES = frozenset({torch.uint8, torch.float8_e8m0fnu})
+_ThreeI64, _FourI64 = _i64 * 3, _i64 * 4
+
+
+def _quant_pools_refusal(k_cache, v_cache, kv_scales) -> str:
+    """What is wrong with the pools of an 8-bit cache ("": nothing)."""
+    if k_cache.dtype not in _CODES:
+        return f"k_cache must hold float8_e4m3fn or int8 codes, got {k_cache.dtype}"
+    if k_cache.dim() != 3 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        return "k_cache and v_cache must both be [pages * H, page_size, head_dim] of the same codes"
+    if kv_scales.dtype not in _SCALES:
+        return f"kv_scales must be uint8 (or float8_e8m0fnu), got {kv_scales.dtype}"
+    want = (*k_cache.shape[:2], 2)
+    if tuple(kv_scales.shape) != want:
+        return f"kv_scales must be {want}, got {tuple(kv_scales.shape)}"
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and kv_scales.is_contiguous()):
+        return "k_cache, v_cache and kv_scales must be contiguous"
+    return ""
+
+
+def _apart(*tensors) -> bool:
+    """Whether no two of these contiguous tensors share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    return all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+
+
+def _quant_rows_refusal(k_cache, v_cache, kv_scales, k, v, loc, page_size, names, written: bool) -> str:
+    """What is wrong with rows k and v [nnz, H, D] (called names) that go into
+    the pools (written: that are read out of them), and their slots."""
+    wrong = _quant_pools_refusal(k_cache, v_cache, kv_scales)
+    if wrong:
+        return wrong
+    if not _apart(k_cache, v_cache, kv_scales):
+        return "k_cache, v_cache and kv_scales share memory"
+    if k.dim() != 3 or v.shape != k.shape:
+        return f"{names[0]} and {names[1]} must both be [nnz, num_kv_heads, head_dim]"
+    if k.dtype not in _ROPE_DTYPES or v.dtype != k.dtype:
+        return f"{names[0]} and {names[1]} must both be bfloat16, float16 or float32, got {k.dtype} and {v.dtype}"
+    nnz, H, D = k.shape
+    if H < 1 or D < 1:
+        return f"{names[0]} must have heads and columns, got {tuple(k.shape)}"
+    if k_cache.shape[1] != page_size or k_cache.shape[2] != D or page_size < 1:
+        return f"k_cache and v_cache must be [pages * H, {page_size}, {D}]"
+    if k_cache.shape[0] % H:
+        return f"the pools' {k_cache.shape[0]} rows are not pages of {H} kv heads"
+    if loc.dtype != torch.int64:
+        return f"loc must be {torch.int64}, got {loc.dtype}"
+    if not loc.is_contiguous():
+        return "loc must be contiguous"
+    if loc.numel() < nnz:
+        return "loc shorter than the tokens"
+    for t, n in ((k, names[0]), (v, names[1])):
+        if D > 1 and t.stride(2) != 1:
+            return f"{n} must have dense rows (a last stride of 1)"
+        first, end = _span(t)
+        for pool in (k_cache, v_cache, kv_scales):
+            p = pool.data_ptr()
+            if first < end and not (end <= p or p + pool.numel() * pool.element_size() <= first):
+                return f"{n} lies in the pools"
+        if written and nnz and not _rows_distinct(t):
+            return f"{n} has rows that share memory"
+    if written and nnz and not _tokens_apart(k, v):
+        return f"{names[0]} shares memory with {names[1]}"
+    return ""
+
+
+@_plain_positional
+def set_kv_buffer_quant(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size) -> None:
+    """Quantises new_k / new_v [nnz, H, D] into 8-bit pools at the slots loc."""
+    lib = _lib or load_library()
+    index = _device_index(new_k, new_v, k_cache, v_cache, kv_scales, loc)
+    if _current_device() != index:
+        with _on_device(torch.device("cuda", index)):
+            return set_kv_buffer_quant(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size)
+    wrong = _quant_rows_refusal(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size, ("new_k", "new_v"), False)
+    if wrong:
+        raise RuntimeError("vortex_torch: " + wrong)
+    nnz, H, D = new_k.shape
+    k0, k1 = (0 if n == 1 else t for n, t in zip((nnz, H), new_k.stride()))
+    v0, v1 = (0 if n == 1 else t for n, t in zip((nnz, H), new_v.stride()))
+    rc = lib.vtx_set_kv_buffer_quant(
+        k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), k_cache.shape[0] * page_size, new_k.data_ptr(),
+        new_v.data_ptr(), _FourI64(k0, k1, v0, v1), loc.data_ptr(), nnz, H, D, _ROPE_DTYPES[new_k.dtype],
+        _CODES[k_cache.dtype], page_size, _stream_of(index))
+    if rc:
+        _check(rc, "set_kv_buffer_quant")
+
+
+@_plain_positional
+def read_kv_buffer_quant(k_cache, v_cache, kv_scales, loc, page_size, num_kv_heads, dtype, k_out, v_out):
+    """The values of 8-bit pools at the slots loc: k, v [nnz, H, D] (k_out and
+    v_out, or new tensors of dtype)."""
+    lib = _lib or load_library()
+    given = [t for t in (k_out, v_out) if t is not None]
+    index = _device_index(loc, k_cache, v_cache, kv_scales, *given)
+    if _current_device() != index:
+        with _on_device(torch.device("cuda", index)):
+            return read_kv_buffer_quant(k_cache, v_cache, kv_scales, loc, page_size, num_kv_heads, dtype, k_out, v_out)
+    if len(given) == 1:
+        raise RuntimeError("vortex_torch: k_out and v_out go together")
+    if not given:
+        wrong = _quant_pools_refusal(k_cache, v_cache, kv_scales)
+        if not wrong and dtype not in _ROPE_DTYPES:
+            wrong = f"dtype must be bfloat16, float16 or float32, got {dtype}"
+        if not wrong and num_kv_heads < 1:
+            wrong = f"num_kv_heads must be positive, got {num_kv_heads}"
+        if wrong:
+            raise RuntimeError("vortex_torch: " + wrong)
+        shape = (loc.numel(), num_kv_heads, k_cache.shape[2])
+        k_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
+        v_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
+    elif k_out.dim() == 3 and (k_out.shape[0] != loc.numel() or k_out.shape[1] != num_kv_heads):
+        raise RuntimeError(
+            f"vortex_torch: k_out must be [{loc.numel()}, {num_kv_heads}, head_dim], got {tuple(k_out.shape)}")
+    wrong = _quant_rows_refusal(k_cache, v_cache, kv_scales, k_out, v_out, loc, page_size, ("k_out", "v_out"), True)
+    if wrong:
+        raise RuntimeError("vortex_torch: " + wrong)
+    nnz, H, D = k_out.shape
+    k0, k1 = (0 if n == 1 else t for n, t in zip((nnz, H), k_out.stride()))
+    v0, v1 = (0 if n == 1 else t for n, t in zip((nnz, H), v_out.stride()))
+    rc = lib.vtx_read_kv_buffer_quant(
+        k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), k_cache.shape[0] * page_size, k_out.data_ptr(),
+        v_out.data_ptr(), _FourI64(k0, k1, v0, v1), loc.data_ptr(), nnz, H, D, _ROPE_DTYPES[k_out.dtype],
+        _CODES[k_cache.dtype], page_size, _stream_of(index))
+    if rc:
+        _check(rc, "read_kv_buffer_quant")
+    return k_out, v_out
+
+
+@_plain_args
+def page_reduce_quant(x, kv_scales, of_values, outs, reduce_types, loc, num_kv_heads: int, page_size: int,
+                      dim: int) -> None:
+    """page_reduce_multi (dim 1) over codes x with kv_scales' exponents of the
+    keys (of_values: of the values)."""
+    lib = load_library()
+    outs, reduce_types = list(outs), [int(t) for t in reduce_types]
+    if not 1 <= len(outs) <= 4 or len(outs) != len(reduce_types):
+        raise RuntimeError("vortex_torch: page_reduce_quant needs 1..4 outputs, one type each")
+    dev = _require_gpu(x, kv_scales, loc, *outs)
+    wrong = _quant_pools_refusal(x, x, kv_scales)
+    if wrong:
+        raise RuntimeError("vortex_torch: " + wrong)
+    if dim != 1:
+        raise RuntimeError(f"vortex_torch: pools of codes are reduced over a page's tokens (dim 1), not dim {dim}")
+    rows, P, D = (int(s) for s in x.shape)
+    if P != page_size:
+        raise RuntimeError(f"vortex_torch: x must be [rows, {page_size}, head_dim], got {tuple(x.shape)}")
+    _req(loc, torch.int64, "loc")
+    out_rows = None
+    for o in outs:
+        if o.dtype not in _OUT_DTYPES:
+            raise RuntimeError(f"vortex_torch: reduce output must be bf16 or fp32, got {o.dtype}")
+        _req(o, o.dtype, "output")
+        if o.numel() % max(D, 1):
+            raise RuntimeError("vortex_torch: page reduce output size is not a multiple of its row")
+        r = o.numel() // max(D, 1)
+        out_rows = r if out_rows is None else min(out_rows, r)
+    if not _apart(x, kv_scales, *outs):
+        raise RuntimeError("vortex_torch: outputs share memory with each other or the pool")
+    n = len(outs)
+    ptrs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
+    dts = (ctypes.c_int32 * n)(*[_OUT_DTYPES[o.dtype] for o in outs])
+    tys = (ctypes.c_int32 * n)(*reduce_types)
+    with _on_device(dev):
+        rc = lib.vtx_page_reduce_quant(
+            x.data_ptr(), kv_scales.data_ptr() + (1 if of_values else 0), rows, P, D, _CODES[x.dtype], n, ptrs, dts,
+            tys, out_rows, loc.data_ptr(), loc.numel(), int(num_kv_heads), _stream(dev))
+    _check(rc, "page_reduce_quant")
+
+
+_QUERY_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+
+
+def _quant_attention_refusal(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B, H,
+                             soft_cap, window, slopes) -> str:
+    """What is wrong with the arguments of quant_paged_decode_attention ("": nothing)."""
+    wrong = _quant_pools_refusal(k_cache, v_cache, kv_scales)
+    if wrong:
+        return wrong
+    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (kv_last_page_len, "kv_last_page_len")):
+        if t.dtype != _I32:
+            return f"{n} must be {_I32}, got {t.dtype}"
+        if not t.is_contiguous():
+            return f"{n} must be contiguous"
+    if B < 0 or H < 1:
+        return "batch_size and num_kv_heads must be positive"
+    D = k_cache.shape[2]
+    if q.dtype not in _QUERY_DTYPES or o.dtype != q.dtype:
+        return f"q and out must both be bfloat16 or float16, got {q.dtype} and {o.dtype}"
+    if q.dim() != 3 or q.shape[2] != D or q.shape[0] not in (B, B * H) or q.shape[0] * q.shape[1] % max(B * H, 1):
+        return f"q must be [{B}, q_heads, {D}] or [{B * H}, group, {D}], got {tuple(q.shape)}"
+    if o.shape != q.shape or not o.is_contiguous():
+        return f"out must be a contiguous {tuple(q.shape)}, got {tuple(o.shape)}"
+    if q.stride(2) != 1:
+        return "q must have dense rows (a last stride of 1)"
+    if kv_indptr.numel() < B * H + 1 or kv_last_page_len.numel() < B * H:
+        return f"kv_indptr needs {B * H + 1} and kv_last_page_len {B * H} entries"
+    if not 0.0 <= soft_cap < math.inf:
+        return f"logits_soft_cap must be finite and not negative, got {soft_cap}"
+    if window < 0 or window > 0x7fffffff:
+        return f"window must be 0 or a number of tokens, got {window}"
+    if slopes is not None:
+        heads = q.shape[0] * q.shape[1] // max(B, 1)
+        if slopes.dtype != torch.float32 or not slopes.is_contiguous() or (B and slopes.numel() != heads):
+            return f"slopes must be {heads} contiguous float32 values"
+    return ""
+
+
+@_plain_positional
+def quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, batch_size,
+                                 num_kv_heads, sm_scale, soft_cap, window, slopes) -> None:
+    """paged_decode_attention over 8-bit pools, with capped scores, a window or
+    slopes.  The table's pages are divided over the card with scratch from
+    torch's allocator, whose OutOfMemoryError is the caller's; in a capture that
+    torch did not begin no scratch lasts, and every segment has a workgroup."""
+    lib = _lib or load_library()
+    if slopes is None:
+        index = _device_index(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len)
+    else:
+        index = _device_index(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, slopes)
+    if _current_device() != index:
+        with _on_device(torch.device("cuda", index)):
+            return quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices,
+                                                kv_last_page_len, batch_size, num_kv_heads, sm_scale, soft_cap, window,
+                                                slopes)
+    B, H = batch_size, num_kv_heads
+    wrong = _quant_attention_refusal(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B, H,
+                                     soft_cap, window, slopes)
+    if wrong:
+        raise RuntimeError("vortex_torch: " + wrong)
+    if B == 0:
+        return
+    rows, P, D = k_cache.shape
+    G = q.shape[0] * q.shape[1] // (B * H)
+    s0, s1 = (0 if n == 1 else t for n, t in zip(q.shape[:2], q.stride()))  # (one row's stride may be anything)
+    strides = _ThreeI64(s0, G * s1, s1) if q.shape[0] == B and q.shape[1] != G else _ThreeI64(H * s0, s0, s1)
+    stream = _stream_of(index)
+    floats = lib.vtx_quant_decode_attention_workspace_len(B, H, G, D, P, window, kv_indices.numel())
+    ws = None
+    if floats > 0 and _scratch_lasts(stream):
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device)
+    rc = lib.vtx_quant_decode_attention(
+        q.data_ptr(), strides, o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), rows,
+        kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr(), B, H, G, D, P,
+        _QUERY_DTYPES[q.dtype], _CODES[k_cache.dtype], sm_scale, soft_cap, window,
+        None if slopes is None else slopes.data_ptr(), None if ws is None else ws.data_ptr(),
+        0 if ws is None else floats, stream)
+    if rc:
+        _check(rc, "quant_paged_decode_attention")
 
 
 def bf16_rounding_check(device="cuda") -> tuple:

@@ -15,6 +15,10 @@ Requests that share leading pages (a system prompt, samples of one prompt):
 ``plan_shared_prefix`` finds what they share in a table, once per step, and
 ``shared_prefix_decode_attention`` reads those pages once for all of them, in
 every layer, with ``paged_decode_attention``'s result.
+
+``quant_paged_decode_attention`` (and its ``sparse_quant_decode_attention`` /
+``dense_quant_decode_attention``) reads an 8-bit cache (``cache.quant``), also
+with capped scores, a window, or a bias that grows with the distance.
 """
 from __future__ import annotations
 
@@ -117,5 +121,45 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     return o
 
 
+def quant_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                 kv_scales: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+                                 kv_last_page_len: torch.Tensor, batch_size: int, num_kv_heads: int,
+                                 sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                                 logits_soft_cap: Optional[float] = None, window: Optional[int] = None,
+                                 slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_decode_attention`` over 8-bit pools and their ``kv_scales``
+    (``cache.set_kv_buffer_quant``); q [B, H_q, D] or [B * H_kv, G, D], bf16 or
+    fp16, its rows dense, up to 16 query heads per kv head; returns q's type.
+
+    ``logits_soft_cap``: scores become cap * tanh(score / cap).  For tables in the
+    tokens' order (dense ones): ``window``, only the last so many tokens count;
+    ``slopes`` (fp32 [H_q]), the score of the token d before the newest one is
+    lowered by slope * d, after the cap."""
+    D = int(q.shape[-1])
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    _hip.quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len,
+                                      int(batch_size), int(num_kv_heads), scale, float(logits_soft_cap or 0.0),
+                                      int(window or 0), slopes)
+    return o
+
+
+def sparse_quant_decode_attention(q, k_cache, v_cache, kv_scales, ctx, sm_scale: Optional[float] = None, out=None,
+                                  logits_soft_cap: Optional[float] = None):
+    """Attention over the selected pages of an 8-bit cache (ctx's sparse table)."""
+    return quant_paged_decode_attention(q, k_cache, v_cache, kv_scales, ctx.sparse_kv_indptr, ctx.sparse_kv_indices,
+                                        ctx.kv_last_page_len, ctx.batch_size, ctx.num_kv_heads, sm_scale, out,
+                                        logits_soft_cap)
+
+
+def dense_quant_decode_attention(q, k_cache, v_cache, kv_scales, ctx, sm_scale: Optional[float] = None, out=None,
+                                 logits_soft_cap: Optional[float] = None, window: Optional[int] = None, slopes=None):
+    """Full attention over an 8-bit cache (ctx's dense table)."""
+    return quant_paged_decode_attention(q, k_cache, v_cache, kv_scales, ctx.dense_kv_indptr, ctx.dense_kv_indices,
+                                        ctx.kv_last_page_len, ctx.batch_size, ctx.num_kv_heads, sm_scale, out,
+                                        logits_soft_cap, window, slopes)
+
+
 __all__ = ["paged_decode_attention", "sparse_decode_attention", "dense_decode_attention", "SharedPrefixPlan",
-           "plan_shared_prefix", "shared_prefix_decode_attention"]
+           "plan_shared_prefix", "shared_prefix_decode_attention", "quant_paged_decode_attention",
+           "sparse_quant_decode_attention", "dense_quant_decode_attention"]
