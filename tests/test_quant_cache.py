@@ -812,9 +812,9 @@ def test_pool_and_reduction_refusals(no_gpu):
         with pytest.raises(RuntimeError, match=says):
             call(**kw)
     plain = as_vtensor(a["k_cache"], FORMAT.PAGED)
-    assert not hasattr(plain, "_kv_scales")
+    assert not hasattr(plain, "_quantized")
     pool = quantized_pool(a["k_cache"], a["kv_scales"], values=True)
-    assert pool._format == FORMAT.PAGED and pool.data_ptr() == a["k_cache"].data_ptr() and pool._kv_scales[1]
+    assert pool._format == FORMAT.PAGED and pool.data_ptr() == a["k_cache"].data_ptr()
 
 
 def _attention_args(**changes):

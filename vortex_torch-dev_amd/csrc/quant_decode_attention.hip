@@ -20,12 +20,13 @@
 // weight), and fp16 queries likewise (exactly): the matrix cores have time, the
 // launch waits for memory.
 //
-// 4 waves per workgroup, 32 tokens of a wave at a time.  The table's pages, all
-// segments after one another, are cut into equal ranges, a workgroup each, so
-// that ragged lengths and any number of segments fill the card evenly; a
-// workgroup meets the segments of its range one after another.  A segment inside
-// its range is finished there; the others' parts (at most two per workgroup) are
-// joined by a second launch.
+// 4 waves per workgroup, 32 tokens of a wave at a time; the next ones' keys are
+// requested behind the scores and their values behind the weighted sum, into the
+// registers that these leave.  The table's pages, all segments after one another,
+// are cut into equal ranges, a workgroup each, so that ragged lengths and any
+// number of segments fill the card evenly; a workgroup meets the segments of its
+// range one after another.  A segment inside its range is finished there; the
+// others' parts (at most two per workgroup) are joined by a second launch.
 #include "vtx_device.h"
 #include "vtx_host.h"
 #include "vtx_quant.h"
@@ -37,8 +38,27 @@ constexpr int kWaves = kThreads / vtx::kWave;
 constexpr int kHeads = 16;       // query heads of a matrix tile
 constexpr int kTile = 32;        // tokens of a wave at a time
 constexpr int kStage = 1024;     // page rows staged in LDS at a time
+constexpr int kBounds = 1024;    // bounds of a table that are brought to LDS whole
 constexpr int kMinTokens = 128;  // tokens of a range at least: a tile per wave
 constexpr float kLog2e = 1.4426950408889634f;
+
+// A divisor that the host knows: three scalar instructions and two corrections
+// for the compiler's division by an unknown, which takes a tenth of a microsecond
+// where nothing runs beside it.
+struct Divisor {
+  uint32_t d, m;  // m: 2^32 / d, rounded down (2^32 - 1 for 1)
+};
+__device__ __forceinline__ uint32_t divide(uint32_t x, Divisor v) {
+  uint32_t q = __umulhi(x, v.m), r = x - q * v.d;  // (one or two too small)
+  if (r >= v.d) {
+    ++q;
+    r -= v.d;
+  }
+  return r >= v.d ? q + 1 : q;
+}
+inline Divisor divisor(long long d) {
+  return Divisor{(uint32_t)d, d == 1 ? 0xffffffffu : (uint32_t)((1LL << 32) / d)};
+}
 
 struct QAttnArgs {
   const uint16_t* q;
@@ -54,56 +74,62 @@ struct QAttnArgs {
   const float* slopes;  // [H * G], or null
   int64_t q_batch, q_kv, q_head;  // strides in elements
   int32_t segments, H, G, P, p_shift;
+  Divisor by_segments, by_heads, by_workers, by_cus;
   int32_t window;  // the last tokens that count; 0: all
-  int32_t pitch;   // pages of a segment's place on the line of pages; 0: its own pages
   float c;         // scale log2 e; with a cap 2 scale log2 e / cap
   float cap;       // cap log2 e, or 0
   int32_t workers, least;  // ranges at most, pages of one at least; workers 0: a segment each, whole
-  float* acc;      // [2 workers, G, D]
-  float2* ml;      // [2 workers, G]
+  float* acc;       // [2 workers, G, D]
+  float2* ml;       // [2 workers, G]
+  int32_t* places;  // [segments + 1], of a packed line
 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// The line of pages and its ranges.
+// The line of pages and its ranges.  Where the pages divide evenly among the
+// segments (selected pages), a range is a whole number of segments or a whole part
+// of one if that costs the fullest compute unit no more than a quarter: fewer
+// parts to join, and a workgroup's waves start over less often (64 requests of 8
+// heads and 32 pages: 512 ranges of a segment each 20.5 us, 768 of 21.3 pages 27.9).
 struct Line {
   uint32_t total, per;  // pages, pages of a range
 };
-__device__ __forceinline__ Line line_of(const QAttnArgs& a, long long first, long long end) {
-  Line l;
-  if (a.pitch > 0) {
-    l.total = (uint32_t)a.segments * (uint32_t)a.pitch;  // (the host sees to it that this fits)
-  } else {
-    const long long all = end - first;
-    l.total = all < 0 ? 0u : (uint32_t)(all < a.indices_len ? all : a.indices_len);
+__device__ __forceinline__ Line line_of(const QAttnArgs& a, uint32_t total) {
+  Line l{total, divide(total + (uint32_t)a.workers - 1u, a.by_workers)};
+  if (l.per < (uint32_t)a.least) l.per = (uint32_t)a.least;
+  const uint32_t S = (uint32_t)a.segments, m = divide(total, a.by_segments);
+  if (m > 0 && m * S == total) {
+    // ranges of a segment, or segments of a range
+    const uint32_t many = m >= l.per ? m / l.per : (l.per - 1u) / m + 1u;
+    const uint32_t per = m >= l.per ? (m - 1u) / many + 1u : m * many;
+    const uint32_t ranges = m >= l.per ? S * many : (S - 1u) / many + 1u;
+    const uint64_t fullest = (uint64_t)(divide(ranges - 1u, a.by_cus) + 1u) * per;
+    if (4 * fullest <= 5 * (uint64_t)(divide(total - 1u, a.by_cus) + 1u)) l.per = per;
   }
-  const uint32_t even = (l.total + (uint32_t)a.workers - 1u) / (uint32_t)a.workers;
-  l.per = even > (uint32_t)a.least ? even : (uint32_t)a.least;
   return l;
 }
+__device__ __forceinline__ uint32_t table_pages(const QAttnArgs& a, int first, int end) {
+  const uint32_t all = end > first ? (uint32_t)end - (uint32_t)first : 0u, len = (uint32_t)a.indices_len;
+  return all < len ? all : len;
+}
 
-// A segment: its pages that count, and its place on the line.
+// A segment's pages that count.
 struct Segment {
-  long long start;     // of the pages that count, in the table
-  int pages, tokens;   // that count (tokens of the last page included), from the first of these pages on
-  int skip;            // tokens of the first page that the window leaves out
-  uint32_t at, end;    // on the line
+  int start;          // of them, in the table
+  int pages, tokens;  // tokens from the first of these pages on, the last page's included
+  int skip;           // tokens of the first page that the window leaves out
 };
-__device__ __forceinline__ Segment segment_of(const QAttnArgs& a, int s, long long first, long long p0, long long p1,
-                                              int last, uint32_t total) {
-  Segment g;
-  g.start = p0;
-  g.pages = g.tokens = g.skip = 0;
-  const long long m = p1 - p0;
-  if (m > 0 && p0 >= 0 && p1 <= a.indices_len && a.rows > 0) {
+__device__ __forceinline__ Segment segment_of(const QAttnArgs& a, int p0, int p1, int last) {
+  Segment g{p0, 0, 0, 0};
+  if (p0 >= 0 && p1 > p0 && (int64_t)p1 <= a.indices_len && a.rows > 0) {
     last = last < 0 ? 0 : (last > a.P ? a.P : last);
-    const long long n = (m - 1) * a.P + last;
+    const long long n = (long long)(p1 - p0 - 1) * a.P + last;
     if (n > 0 && n < (1LL << 30)) {
-      g.pages = (int)m;
+      g.pages = p1 - p0;
       g.tokens = (int)n;
-      if (a.window > 0 && n > a.window) {
-        const int lo = (int)n - a.window, pg = lo / a.P;
+      if (a.window > 0 && g.tokens > a.window) {
+        const int lo = g.tokens - a.window, pg = a.p_shift >= 0 ? lo >> a.p_shift : lo / a.P;
         g.start += pg;
         g.pages -= pg;
         g.tokens -= pg * a.P;
@@ -111,17 +137,36 @@ __device__ __forceinline__ Segment segment_of(const QAttnArgs& a, int s, long lo
       }
     }
   }
-  if (a.pitch > 0) {
-    g.at = (uint32_t)s * (uint32_t)a.pitch;
-    const uint32_t used = (uint32_t)g.pages < (uint32_t)a.pitch ? (uint32_t)g.pages : (uint32_t)a.pitch;
-    g.end = g.at + used;
-  } else {
-    const long long x = g.start - first, y = p1 - first;
-    const bool ok = x >= 0 && y >= x && y <= (long long)total && g.pages > 0;
-    g.at = ok ? (uint32_t)x : 0u;
-    g.end = ok ? (uint32_t)y : 0u;
-  }
   return g;
+}
+
+// Its place on the line: [at, end), both 0 where it has none.
+struct Place {
+  uint32_t at, end;
+};
+__device__ __forceinline__ Place place_of(const Segment& g, uint32_t at, uint32_t total) {
+  const bool ok = g.pages > 0 && at < total && (uint32_t)g.pages <= total - at;
+  return ok ? Place{at, at + (uint32_t)g.pages} : Place{0u, 0u};
+}
+
+// How many of the segments end at or before place v0 of the line, which is the
+// number of the first that does not: every wave by itself, 64 bounds at a time.
+// bound(j): the table's j-th.
+template <typename Bound>
+__device__ __forceinline__ int segments_before(int S, int first, uint32_t v0, Bound bound) {
+  int lo = 0, len = S;
+  while (true) {
+    const int step = (len + vtx::kWave - 1) / vtx::kWave;  // (0: nothing left)
+    const int j = lo + (vtx::lane_id() + 1) * step;
+    const bool in = step > 0 && j <= lo + len;
+    const int p = bound(in ? j : 0);
+    const uint64_t m = __ballot(in && (p <= first || (uint32_t)p - (uint32_t)first <= v0));
+    // (as many as the first bound past v0 leaves, also of a table that decreases)
+    const int c = m == ~0ull ? vtx::kWave : __builtin_ctzll(~m);
+    lo += c * step;
+    if (step <= 1) return vtx::uniform(lo);
+    len = min(step - 1, S - lo);
+  }
 }
 
 // What a wave holds of 16 query heads: their fragments, running maximum (base 2),
@@ -134,15 +179,40 @@ struct Heads {
   f32x4 o[kD / 16];
 };
 
-// 32 tokens' codes and factors on their way.
+// 32 tokens' keys on their way, and their values and factors.
 template <int kD>
-struct Tile {
+struct Keys {
   vtx::U4 k[2][kD / 64];
+};
+template <int kD>
+struct Values {
   uint32_t v[2][4][kD / 64];  // 16-token half, token, codes
   uint2 sc[2];                // (K, V) bytes of this lane's four tokens of a half
-  bool ok[2];                 // the half lies in the pool (P % 16 == 0)
-  uint32_t bad;               // tokens of this lane that do not count (otherwise): bit 4 half + i
 };
+
+// Loads of 16 tokens of one page by buffer loads: a lane's place among them is a
+// constant register, the tokens' address a scalar, and tokens past `bytes` cost
+// nothing and read as zeros, so the loop's loads stand behind no branch.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const unsigned char* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x27000);
+}
+constexpr int kStream = 2;  // read once: the non-temporal hint
+template <int N>
+__device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t r, int at, uint32_t (&to)[N]) {
+  if constexpr (N == 1) {
+    to[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, kStream);
+  } else if constexpr (N == 2) {
+    const auto t = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, kStream);
+    to[0] = t[0];
+    to[1] = t[1];
+  } else {
+    const auto t = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kStream);
+    to[0] = t[0];
+    to[1] = t[1];
+    to[2] = t[2];
+    to[3] = t[3];
+  }
+}
 
 template <int kD>
 __device__ __forceinline__ void load_v(const unsigned char* p, uint32_t (&to)[kD / 64]) {
@@ -167,10 +237,9 @@ __device__ __forceinline__ void load_v(const unsigned char* p, uint32_t (&to)[kD
 // the outputs stay as they are.
 constexpr float kGrowth = 8.f;
 
+// Scores of 32 tokens, without their factors.
 template <int kD, int kCodes, bool kHalf>
-__device__ __forceinline__ void attend(const QAttnArgs& a, Heads<kD, kHalf>& w, Tile<kD>& t, bool masked,
-                                       uint32_t bad, float far, float slope) {
-  f32x4 s[2];
+__device__ __forceinline__ void score(const Heads<kD, kHalf>& w, const Keys<kD>& t, f32x4 (&s)[2]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -193,6 +262,13 @@ __device__ __forceinline__ void attend(const QAttnArgs& a, Heads<kD, kHalf>& w, 
       }
     }
   }
+}
+
+// Their weights, and the values by these.  bad: tokens of this lane that do not
+// count (where masked); far: the distance of its first one; slope: base 2.
+template <int kD, int kCodes, bool kHalf>
+__device__ __forceinline__ void attend(const QAttnArgs& a, Heads<kD, kHalf>& w, const f32x4 (&s)[2], Values<kD>& t,
+                                       bool masked, uint32_t bad, float far, float slope) {
   if (masked) {  // uniform
     // tokens that do not count may be anything, NaN too: their values become zeros
 #pragma unroll
@@ -219,7 +295,7 @@ __device__ __forceinline__ void attend(const QAttnArgs& a, Heads<kD, kHalf>& w, 
     for (int i = 0; i < 8; ++i)  // cap tanh(y / cap), the argument doubled and in base 2
       x[i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[i]));
   }
-  if (a.slopes) {  // uniform; far: the distance of this lane's first token
+  if (a.slopes) {  // uniform
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = fmaf(-slope, far - (float)(16 * (i / 4) + i % 4), x[i]);
   }
@@ -299,196 +375,307 @@ __device__ __forceinline__ uint32_t round2(float a, float b) {
 __device__ __forceinline__ float inverse_sum(float L) { return L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN); }
 
 template <int kD, int kCodes, bool kHalf, bool kPages16>
-__global__ __launch_bounds__(kThreads, kD == 256 ? 2 : (kD == 128 ? 3 : 4)) void quant_attention_kernel(QAttnArgs a) {
+__global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_kernel(QAttnArgs a) {
   constexpr int kOut = kD + 4;  // floats of a head's outputs in LDS: 16 heads' pieces in all banks
-  __shared__ int32_t s_rows[kStage];
+  __shared__ int32_t s_ptr[kBounds], s_last[kBounds], s_rows[kStage];
   __shared__ float s_m[kWaves][kHeads], s_l[kWaves][kHeads];
   __shared__ alignas(16) float s_o[kWaves][kHeads][kOut];
-  __shared__ uint32_t s_count[kWaves];
 
   const int tid = threadIdx.x, lane = vtx::lane_id();
   const int wave = vtx::uniform(tid / vtx::kWave);
   const int c16 = lane % 16, g4 = lane / 16;
   const int S = a.segments, G = a.G, P = a.P;
 
-  // this workgroup's range of the line, and its first segment
-  long long first = 0;
+  // This workgroup's range of the line, and its first segment.  How the line is laid
+  // out: the table's own pages (also with a window where the table has too many
+  // segments for a sum over all of them: pages before the windows are passed over);
+  // with a window the pages that count, closely packed.  A table of few segments is
+  // brought to LDS whole, so that all its bounds cost one trip.
+  int first = 0, seg = (int)blockIdx.x;
   uint32_t total = 0, v0 = 0, v1 = 1;
-  int seg = (int)blockIdx.x;
-  const bool whole = a.workers == 0;  // uniform
+  const bool whole = a.workers == 0, few = !whole && S < kBounds, packed = few && a.window > 0;  // uniform
   if (!whole) {
-    first = a.indptr[0];
-    const Line l = line_of(a, first, a.indptr[S]);
-    total = l.total;
-    const unsigned long long at = (unsigned long long)blockIdx.x * l.per;
+    if (packed) {
+      constexpr int kEach = kBounds / kThreads;
+      uint32_t pages[kEach], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int j = tid * kEach + i;
+        pages[i] = j < S ? (uint32_t)segment_of(a, a.indptr[j], a.indptr[j + 1], a.last_len[j]).pages : 0u;
+        mine += pages[i];
+      }
+      uint32_t before = vtx::wave_prefix_sum(mine) - mine;
+      if (lane == vtx::kWave - 1) s_m[wave][0] = __uint_as_float(before + mine);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const uint32_t x = __float_as_uint(s_m[i][0]);
+        before += i < wave ? x : 0u;
+        total += x;
+      }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int j = tid * kEach + i;
+        if (j <= S) {
+          s_ptr[j] = (int32_t)before;
+          if (blockIdx.x == 0) a.places[j] = (int32_t)before;  // for the join
+        }
+        before += pages[i];
+      }
+      total = (uint32_t)vtx::uniform((int)total);
+      __syncthreads();
+    } else if (few) {
+#pragma unroll
+      for (int i = 0; i < kBounds; i += kThreads)
+        if (i + tid <= S) {
+          s_ptr[i + tid] = a.indptr[i + tid];
+          s_last[i + tid] = a.last_len[min(i + tid, S - 1)];
+        }
+      __syncthreads();
+      first = vtx::uniform(s_ptr[0]);
+      total = table_pages(a, first, vtx::uniform(s_ptr[S]));
+    } else {
+      first = a.indptr[0];
+      total = table_pages(a, first, a.indptr[S]);
+    }
+    const Line l = line_of(a, total);
+    const uint64_t at = (uint64_t)blockIdx.x * l.per;
     if (at >= total) return;  // uniform
     v0 = (uint32_t)at;
     v1 = total - v0 < l.per ? total : v0 + l.per;
-    if (a.pitch > 0) {
-      seg = (int)(v0 / (uint32_t)a.pitch);
-    } else {
-      // the segments that end at or before v0, of as many evenly spaced ones as
-      // there are threads first where they are many
-      const int step = S > 4 * kThreads ? (S + kThreads - 1) / kThreads : 1;
-      seg = 0;
-      for (int round = step > 1 ? 0 : 1; round < 2; ++round) {
-        const int n = round == 0 ? kThreads : (step > 1 ? step - 1 : S);
-        uint32_t mine = 0;
-        for (int i = tid; i < n; i += kThreads) {
-          const int j = round == 0 ? (i + 1) * step : seg + i + 1;  // ends of segment j - 1
-          mine += j <= S && (long long)a.indptr[j] - first <= (long long)v0 ? 1u : 0u;
-        }
-        mine = vtx::wave_sum(mine);
-        if (lane == 0) s_count[wave] = mine;
-        __syncthreads();
-        uint32_t all = 0;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) all += s_count[i];
-        seg = vtx::uniform(seg + (int)all * (round == 0 ? step : 1));
-        __syncthreads();
-      }
-    }
+    if (few) seg = segments_before(S, first, v0, [&](int j) { return s_ptr[j]; });
+    else seg = segments_before(S, first, v0, [&](int j) { return a.indptr[j]; });
   }
 
+  // What this workgroup has of a segment: pages pa .. pb of those that count.
+  struct Piece {
+    Segment s;
+    uint32_t at;
+    int seg, pa, pb;  // seg S: none
+    bool part;        // of a segment that lies in other ranges too
+  };
   int base_seg = -vtx::kWave - 1;  // the 64 segments whose bounds the lanes hold
   int b0 = 0, b1 = 0, bl = 0;
-  for (; seg < S; ++seg) {
-    if (seg - base_seg >= vtx::kWave || seg < base_seg) {  // uniform
-      base_seg = seg;
-      const int j = seg + lane < S ? seg + lane : S - 1;
-      b0 = a.indptr[j];
-      b1 = a.indptr[j + 1];
-      bl = a.last_len[j];
+  const bool bounds_here = few && !packed;
+  auto hold = [&](int s) {
+    if (s - base_seg >= vtx::kWave) {  // uniform
+      base_seg = s;
+      const int j = min(s + lane, S - 1);
+      bl = bounds_here ? s_last[j] : a.last_len[j];
+      b0 = bounds_here ? s_ptr[j] : a.indptr[j];
+      b1 = bounds_here ? s_ptr[j + 1] : a.indptr[j + 1];
     }
-    const int at = seg - base_seg;
-    const Segment sg =
-        segment_of(a, seg, first, (int)vtx::lane_value((uint32_t)b0, at), (int)vtx::lane_value((uint32_t)b1, at),
-                   (int)vtx::lane_value((uint32_t)bl, at), total);
-    int pa = 0, pb = sg.pages;  // this workgroup's pages of the segment
-    bool part = false;
-    int slot = 0;
-    if (!whole) {
-      // (an empty segment's place may lie anywhere: the bounds of the next decide)
-      if (a.pitch > 0 ? (unsigned long long)seg * (uint32_t)a.pitch >= v1
-                      : (long long)(int)vtx::lane_value((uint32_t)b0, at) - first >= (long long)v1)
+  };
+  auto piece_from = [&](int s) {  // the first from segment s on
+    Piece p;
+    p.seg = S;
+    for (; s < S; ++s) {
+      hold(s);
+      const int p0 = (int)vtx::lane_value((uint32_t)b0, s - base_seg);
+      p.s = segment_of(a, p0, (int)vtx::lane_value((uint32_t)b1, s - base_seg),
+                       (int)vtx::lane_value((uint32_t)bl, s - base_seg));
+      if (whole) {
+        p.at = 0;
+        p.seg = s;
+        p.pa = 0;
+        p.pb = p.s.pages;
+        p.part = false;
         break;
-      const uint32_t x = sg.at > v0 ? sg.at : v0, y = sg.end < v1 ? sg.end : v1;
+      }
+      const uint32_t begin = packed ? (uint32_t)vtx::uniform(s_ptr[s]) : (uint32_t)p0 - (uint32_t)first;
+      if (begin >= v1 && (packed || p0 > first)) break;
+      const Place l = place_of(p.s, packed ? begin : (uint32_t)p.s.start - (uint32_t)first, total);
+      const uint32_t x = l.at > v0 ? l.at : v0, y = l.end < v1 ? l.end : v1;
       if (x >= y) continue;  // (the join writes an empty segment's zeros)
-      pa = (int)(x - sg.at);
-      pb = (int)(y - sg.at);
-      part = sg.at < v0 || sg.end > v1;
-      slot = x == v0 ? 0 : 1;
+      p.at = l.at;
+      p.seg = s;
+      p.pa = (int)(x - l.at);
+      p.pb = (int)(y - l.at);
+      p.part = l.at < v0 || l.end > v1;
+      break;
     }
+    return p;
+  };
+  // the page rows of places staged .. staged_end, as far as they lie on the line
+  uint32_t staged = 0, staged_end = 0;
+  auto stage = [&](const Piece& p, uint32_t from, uint32_t end) {
+    staged = from;
+    staged_end = min(end, from + (uint32_t)kStage);
+    int s = p.seg;
+    for (uint32_t v = from + tid; v < staged_end; v += kThreads) {
+      int64_t at = whole ? (int64_t)p.s.start + v : (int64_t)first + v;
+      if (packed) {
+        while (s + 1 < S && (uint32_t)s_ptr[s + 1] <= v) ++s;
+        const Segment g = s == p.seg ? p.s : segment_of(a, a.indptr[s], a.indptr[s + 1], a.last_len[s]);
+        at = (int64_t)g.start + (v - (uint32_t)s_ptr[s]);
+      }
+      const int r = at >= 0 && at < a.indices_len ? a.indices[at] : -1;
+      s_rows[v - from] = r >= 0 && r < a.rows ? r : -1;
+    }
+    __syncthreads();
+  };
+  // the staged pages of a piece from page pc on: tokens numbered from the first of them
+  struct Stretch {
+    const int32_t* rows;
+    int pages, n;
+  };
+  auto stretch_of = [&](const Piece& p, int pc) {
+    const uint32_t v = p.at + (uint32_t)pc;
+    Stretch t{s_rows, 0, 0};
+    if (v >= staged && v < staged_end) {
+      t.rows += v - staged;
+      t.pages = min(p.pb - pc, (int)(staged_end - v));
+      t.n = (pc + t.pages == p.s.pages ? p.s.tokens : (pc + t.pages) * P) - pc * P;
+    }
+    return t;
+  };
 
+  // a tile's 16 tokens of one page (P % 16 == 0): their pool row, and how many of
+  // them there are (uniform); the tile whose codes are on their way
+  struct Half {
+    long long row;
+    int tokens;
+  };
+  auto half_of = [&](const Stretch& t, int i, int hf) {
+    const int t0 = i * kTile + hf * 16;
+    const int pg = a.p_shift >= 0 ? t0 >> a.p_shift : t0 / P;
+    const int r = vtx::uniform(t.rows[t0 < t.n ? pg : 0]);
+    return Half{(long long)r * P + (t0 - pg * P), t0 < t.n && r >= 0 ? min(t.n - t0, 16) : 0};
+  };
+
+  for (Piece cur = piece_from(seg); cur.seg < S; cur = piece_from(cur.seg + 1)) {
+    const int b = (int)divide((uint32_t)cur.seg, a.by_heads), h = cur.seg - b * a.H;
     Heads<kD, kHalf> w;
     w.m = -INFINITY;
     w.l = 0.f;
 #pragma unroll
     for (int d = 0; d < kD / 16; ++d) w.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int b = seg / a.H, h = seg - b * a.H;
+    // its query rows; heads past G take head 0's, and nobody takes their results
     {
-      // heads past G take head 0's queries, and nobody takes their results
       const uint16_t* q = a.q + b * a.q_batch + h * a.q_kv + (c16 < G ? c16 : 0) * a.q_head + g4 * 16;
 #pragma unroll
-      for (int j = 0; j < kD / 32; ++j) {
-        const vtx::U4 raw = vtx::ld16(q + (j / 2) * 64 + (j % 2) * 8);
-        if constexpr (kHalf) {
-          typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-          const f16x8 f = __builtin_bit_cast(f16x8, raw);
-          uint32_t x[4], y[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float u = (float)f[2 * e], v = (float)f[2 * e + 1];
-            x[e] = vtx::bf16_pair(u, v);
-            y[e] = vtx::bf16_pair(u - vtx::bf16_lo(x[e]), v - vtx::bf16_hi(x[e]));
-          }
-          w.q[j] = vtx::U4{x[0], x[1], x[2], x[3]};
-          w.ql[j] = vtx::U4{y[0], y[1], y[2], y[3]};
-        } else {
-          w.q[j] = raw;
-        }
-      }
+      for (int j = 0; j < kD / 32; ++j) w.q[j] = vtx::ld16(q + (j / 2) * 64 + (j % 2) * 8);
     }
     const float slope = a.slopes ? a.slopes[h * G + (c16 < G ? c16 : 0)] * kLog2e : 0.f;
 
-    for (int pc = pa; pc < pb; pc += kStage) {
-      const int np = min(kStage, pb - pc);
-      __syncthreads();  // (the staged rows before are done with)
-      for (int i = tid; i < np; i += kThreads) {
-        const int r = a.indices[sg.start + pc + i];
-        s_rows[i] = r >= 0 && r < a.rows ? r : -1;
+    for (int pc = cur.pa; pc < cur.pb;) {
+      Stretch st = stretch_of(cur, pc);
+      if (st.pages == 0) {  // uniform
+        if (staged_end > 0) __syncthreads();  // (the staged rows are done with)
+        stage(cur, cur.at + (uint32_t)pc, whole ? (uint32_t)cur.pb : v1);
+        st = stretch_of(cur, pc);
       }
-      __syncthreads();
-      // tokens of these pages, numbered from the first of them
-      const int n = (pc + np == sg.pages ? sg.tokens : (pc + np) * P) - pc * P;
-      const int skip = pc == 0 ? sg.skip : 0;
-      const int tiles = (n + kTile - 1) / kTile;
-      const float far0 = (float)(sg.tokens - 1 - pc * P - 4 * g4);
-
-      auto load = [&](int i, Tile<kD>& t) {
-        if constexpr (kPages16) {
+      const int skip = pc == 0 ? cur.s.skip : 0;
+      const int tiles = (st.n + kTile - 1) / kTile;
+      const float far0 = (float)(cur.s.tokens - 1 - pc * P - 4 * g4);
+      if constexpr (kHalf) {
+        if (pc == cur.pa) {  // fp16 queries as two bf16 values each
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const int t0 = i * kTile + hf * 16;  // uniform
-            const int pg = a.p_shift >= 0 ? t0 >> a.p_shift : t0 / P;
-            const int r = vtx::uniform(s_rows[pg < np ? pg : 0]);
-            t.ok[hf] = pg < np && r >= 0;
-            const long long row = (long long)(r >= 0 ? r : 0) * P + (pg < np ? t0 - pg * P : 0);
-            const unsigned char* kp = a.k + row * kD;
-            const unsigned char* vp = a.v + row * kD;
+          for (int j = 0; j < kD / 32; ++j) {
+            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+            const f16x8 f = __builtin_bit_cast(f16x8, w.q[j]);
+            uint32_t x[4], y[4];
 #pragma unroll
-            for (int j = 0; j < kD / 64; ++j) t.k[hf][j] = vtx::ld16_stream(kp + (c16 * kD + j * 64 + g4 * 16));
-#pragma unroll
-            for (int x = 0; x < 4; ++x) load_v<kD>(vp + ((4 * g4 + x) * kD + c16 * (kD / 16)), t.v[hf][x]);
-            t.sc[hf] = *reinterpret_cast<const uint2*>(a.scales + row * 2 + 8 * g4);
+            for (int e = 0; e < 4; ++e) {
+              const float u = (float)f[2 * e], v = (float)f[2 * e + 1];
+              x[e] = vtx::bf16_pair(u, v);
+              y[e] = vtx::bf16_pair(u - vtx::bf16_lo(x[e]), v - vtx::bf16_hi(x[e]));
+            }
+            w.q[j] = vtx::U4{x[0], x[1], x[2], x[3]};
+            w.ql[j] = vtx::U4{y[0], y[1], y[2], y[3]};
           }
-        } else {
-          t.bad = 0;
+        }
+      }
+      pc += st.pages;
+
+      if constexpr (kPages16) {
+        Half half[2];
+        Keys<kD> keys;
+        Values<kD> values;
+        auto aim = [&](int i) {
+          half[0] = half_of(st, i, 0);
+          half[1] = half_of(st, i, 1);
+        };
+        auto load_keys = [&]() {
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
-            auto row_of = [&](int tok, bool& ok) {
-              ok = tok < n;
-              const int pg = ok ? tok / P : 0;
-              const int r = s_rows[pg];
-              ok = ok && r >= 0;
-              return ok ? (long long)r * P + (tok - pg * P) : 0LL;
-            };
-            bool ok;
-            const unsigned char* kp = a.k + row_of(i * kTile + hf * 16 + c16, ok) * kD;
+            const auto r = buffer_of(a.k + half[hf].row * kD, (uint32_t)half[hf].tokens * kD);
 #pragma unroll
-            for (int j = 0; j < kD / 64; ++j) t.k[hf][j] = vtx::ld16_stream(kp + (j * 64 + g4 * 16));
+            for (int j = 0; j < kD / 64; ++j) {
+              uint32_t x[4];
+              load_words<4>(r, c16 * kD + g4 * 16 + j * 64, x);
+              keys.k[hf][j] = vtx::U4{x[0], x[1], x[2], x[3]};
+            }
+          }
+        };
+        auto load_values = [&]() {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t x[2];
+            // (all 16 slots': a load that reaches past the end gives nothing at all)
+            load_words<2>(buffer_of(a.scales + half[hf].row * 2, half[hf].tokens > 0 ? 32u : 0u), g4 * 8, x);
+            values.sc[hf] = uint2{x[0], x[1]};
+            const auto r = buffer_of(a.v + half[hf].row * kD, (uint32_t)half[hf].tokens * kD);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load_words<kD / 64>(r, 4 * g4 * kD + c16 * (kD / 16) + u * kD, values.v[hf][u]);
+          }
+        };
+        aim(wave);
+        load_keys();
+        load_values();
+        for (int i = wave; i < tiles; i += kWaves) {
+          f32x4 sc[2];
+          score<kD, kCodes, kHalf>(w, keys, sc);
+          const int n0 = half[0].tokens, n1 = half[1].tokens;
+          aim(i + kWaves);  // (none past the last: no loads)
+          load_keys();
+          const int out = skip - i * kTile;  // tokens before the window
+          uint32_t bad = 0;
+          const bool masked = n0 + n1 < kTile || out > 0;
+          if (masked) {  // uniform
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              bad |= 4 * g4 + x >= n0 || 4 * g4 + x < out ? 1u << x : 0u;
+              bad |= 4 * g4 + x >= n1 || 16 + 4 * g4 + x < out ? 16u << x : 0u;
+            }
+          }
+          attend<kD, kCodes, kHalf>(a, w, sc, values, masked, bad, far0 - (float)(i * kTile), slope);
+          load_values();
+        }
+      } else {
+        // the pool row of a token, and whether it counts (row 0 where not)
+        auto token_row = [&](int tok, bool& ok) {
+          ok = tok < st.n;
+          const int pg = ok ? tok / P : 0;
+          const int r = st.rows[pg];
+          ok = ok && r >= 0;
+          return ok ? (long long)r * P + (tok - pg * P) : 0LL;
+        };
+        for (int i = wave; i < tiles; i += kWaves) {
+          Keys<kD> keys;
+          Values<kD> values;
+          uint32_t bad = 0;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            bool ok;
+            const unsigned char* kp = a.k + token_row(i * kTile + hf * 16 + c16, ok) * kD + g4 * 16;
+#pragma unroll
+            for (int j = 0; j < kD / 64; ++j) keys.k[hf][j] = vtx::ld16_stream(kp + j * 64);
             uint32_t two[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const long long row = row_of(i * kTile + hf * 16 + 4 * g4 + x, ok);
-              load_v<kD>(a.v + row * kD + c16 * (kD / 16), t.v[hf][x]);
+              const int tok = i * kTile + hf * 16 + 4 * g4 + x;
+              const long long row = token_row(tok, ok);
+              load_v<kD>(a.v + row * kD + c16 * (kD / 16), values.v[hf][x]);
               two[x] = *reinterpret_cast<const uint16_t*>(a.scales + row * 2);
-              t.bad |= ok ? 0u : 1u << (4 * hf + x);
+              bad |= ok && tok >= skip ? 0u : 1u << (4 * hf + x);
             }
-            t.sc[hf] = uint2{two[0] | (two[1] << 16), two[2] | (two[3] << 16)};
+            values.sc[hf] = uint2{two[0] | (two[1] << 16), two[2] | (two[3] << 16)};
           }
+          f32x4 sc[2];
+          score<kD, kCodes, kHalf>(w, keys, sc);
+          attend<kD, kCodes, kHalf>(a, w, sc, values, __ballot(bad != 0) != 0, bad, far0 - (float)(i * kTile), slope);
         }
-      };
-      auto compute = [&](int i, Tile<kD>& t) {
-        uint32_t bad = 0;
-        bool masked = i * kTile + kTile > n || i * kTile < skip;
-        if constexpr (kPages16) masked = masked || !t.ok[0] || !t.ok[1];
-        else masked = masked || __ballot(t.bad != 0) != 0;
-        if (masked) {  // uniform
-          if constexpr (kPages16) bad = (t.ok[0] ? 0u : 0xfu) | (t.ok[1] ? 0u : 0xf0u);
-          else bad = t.bad;
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int tok = i * kTile + 16 * (x / 4) + 4 * g4 + x % 4;
-            bad |= tok >= n || tok < skip ? 1u << x : 0u;
-          }
-        }
-        attend<kD, kCodes, kHalf>(a, w, t, masked, bad, far0 - (float)(i * kTile), slope);
-      };
-      for (int i = wave; i < tiles; i += kWaves) {
-        Tile<kD> t;
-        load(i, t);
-        compute(i, t);
       }
     }
 
@@ -526,91 +713,102 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : (kD == 128 ? 3 : 4)) void
           O = float4{fmaf(y.x, f, O.x), fmaf(y.y, f, O.y), fmaf(y.z, f, O.z), fmaf(y.w, f, O.w)};
         }
       }
-      if (part) {  // uniform
-        const long long row = (2LL * blockIdx.x + slot) * G + g;
+      if (cur.part) {  // uniform
+        const long long row = (2LL * blockIdx.x + (cur.at + (uint32_t)cur.pa == v0 ? 0 : 1)) * G + g;
         *reinterpret_cast<float4*>(a.acc + row * kD + d) = O;
         if (d == 0) a.ml[row] = float2{M, L};
       } else {
         const float f = inverse_sum(L);
-        *reinterpret_cast<uint2*>(a.o + ((long long)seg * G + g) * kD + d) =
+        *reinterpret_cast<uint2*>(a.o + ((long long)cur.seg * G + g) * kD + d) =
             uint2{round2<kHalf>(O.x * f, O.y * f), round2<kHalf>(O.z * f, O.w * f)};
       }
     }
     if (whole) return;  // uniform
-    __syncthreads();  // (the next segment's results go to the same place)
+    __syncthreads();    // (the next segment's results go to the same place)
   }
 }
 
 // The parts of a segment that lies in several ranges, joined; zeros for one
 // without tokens.  A workgroup per segment: threads = (part of the parts, head,
 // four columns), each with a running maximum of its own.
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 256;
 template <int kD, bool kHalf>
 __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAttnArgs a) {
   constexpr int kAhead = 8;  // parts in flight
   __shared__ alignas(16) float s_o[kJoinThreads][4];
   __shared__ float2 s_ml[kJoinThreads];
   const int seg = blockIdx.x, tid = threadIdx.x, G = a.G, S = a.segments;
-  const long long first = a.indptr[0];
-  const Line l = line_of(a, first, a.indptr[S]);
-  const Segment sg = segment_of(a, seg, first, a.indptr[seg], a.indptr[seg + 1], a.last_len[seg], l.total);
-  int w0 = 0, n = 0;
+  const bool packed = S < kBounds && a.window > 0;
+  const int first = packed ? 0 : a.indptr[0];
+  const uint32_t total = packed ? (uint32_t)a.places[S] : table_pages(a, first, a.indptr[S]);
+  const Segment sg = segment_of(a, a.indptr[seg], a.indptr[seg + 1], a.last_len[seg]);
+  const Place at = place_of(sg, packed ? (uint32_t)a.places[seg] : (uint32_t)sg.start - (uint32_t)first, total);
+  const Line l = line_of(a, total);
+  uint32_t w0 = 0;
+  int n = 0;
   bool second = false;  // the first part lies behind another segment's
-  if (sg.end > sg.at) {
-    w0 = (int)(sg.at / l.per);
-    n = (int)((sg.end - 1) / l.per) - w0 + 1;
-    second = sg.at > (uint32_t)w0 * l.per;
-    if (n == 1) return;  // uniform: written by its workgroup
+  if (at.end > at.at) {
+    w0 = at.at / l.per;
+    if (at.end <= (w0 + 1) * l.per) return;  // uniform: written by its workgroup
+    n = (int)((at.end - 1) / l.per - w0) + 1;
+    second = at.at > w0 * l.per;
   }
   const int items = G * (kD / 4);
   for (int x0 = 0; x0 < items; x0 += kJoinThreads) {
-    // (items a multiple of 16: a group's size is a power of two times a head count)
-    const int here = min(items - x0, kJoinThreads), groups = kJoinThreads / here;
-    const int x = tid % here, grp = tid / here;
+    const int here = min(items - x0, kJoinThreads);
+    const int most = kJoinThreads / here, groups = n < most * 2 ? (n + 1) / 2 : most;
+    const int grp = tid / here, x = tid - grp * here;
     const int g = (x0 + x) / (kD / 4), d = ((x0 + x) % (kD / 4)) * 4;
     float M = -INFINITY, L = 0.f;
     float4 O{0.f, 0.f, 0.f, 0.f};
     if (grp < groups) {
+      // row of part i: 2 (w0 + i) G + g, the second of its range for the first where that
+      // lies behind another segment's
+      const float2* ml = a.ml + 2LL * w0 * G + g;
+      const float* acc = a.acc + (2LL * w0 * G + g) * kD + d;
       for (int i0 = grp; i0 < n; i0 += groups * kAhead) {
-        float2 ml[kAhead];
+        float2 z[kAhead];
         float4 y[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const int i = i0 + u * groups < n ? i0 + u * groups : i0;
-          const long long row = (2LL * (w0 + i) + (i == 0 && second ? 1 : 0)) * G + g;
-          ml[u] = a.ml[row];
-          y[u] = *reinterpret_cast<const float4*>(a.acc + row * kD + d);
+          const int i = i0 + u * groups, row = (i == 0 && second ? 1 : 2 * i) * G;
+          z[u] = float2{-INFINITY, 0.f};
+          y[u] = float4{0.f, 0.f, 0.f, 0.f};
+          if (i < n) {
+            z[u] = ml[row];
+            y[u] = *reinterpret_cast<const float4*>(acc + (long long)row * kD);
+          }
         }
         float nm = M;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) nm = fmaxf(nm, ml[u].x);
+        for (int u = 0; u < kAhead; ++u) nm = fmaxf(nm, z[u].x);
         if (nm == -INFINITY) continue;
         const float f = __builtin_amdgcn_exp2f(M - nm);
         L *= f;
         O = float4{O.x * f, O.y * f, O.z * f, O.w * f};
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const float e = i0 + u * groups < n ? __builtin_amdgcn_exp2f(ml[u].x - nm) : 0.f;
-          if (i0 + u * groups < n) {
-            L = fmaf(ml[u].y, e, L);
-            O = float4{fmaf(y[u].x, e, O.x), fmaf(y[u].y, e, O.y), fmaf(y[u].z, e, O.z), fmaf(y[u].w, e, O.w)};
-          }
+          const float e = __builtin_amdgcn_exp2f(z[u].x - nm);
+          L = fmaf(z[u].y, e, L);
+          O = float4{fmaf(y[u].x, e, O.x), fmaf(y[u].y, e, O.y), fmaf(y[u].z, e, O.z), fmaf(y[u].w, e, O.w)};
         }
         M = nm;
       }
     }
-    __syncthreads();
-    s_ml[tid] = float2{M, L};
-    *reinterpret_cast<float4*>(s_o[tid]) = O;
-    __syncthreads();
+    if (groups > 1) {  // uniform
+      __syncthreads();
+      s_ml[tid] = float2{M, L};
+      *reinterpret_cast<float4*>(s_o[tid]) = O;
+      __syncthreads();
+    }
     if (grp == 0) {
       for (int i = 1; i < groups; ++i) {
-        const float2 ml = s_ml[i * here + x];
+        const float2 z = s_ml[i * here + x];
         const float4 y = *reinterpret_cast<const float4*>(s_o[i * here + x]);
-        const float nm = fmaxf(M, ml.x);
+        const float nm = fmaxf(M, z.x);
         if (nm == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(M - nm), e = __builtin_amdgcn_exp2f(ml.x - nm);
-        L = L * f + ml.y * e;
+        const float f = __builtin_amdgcn_exp2f(M - nm), e = __builtin_amdgcn_exp2f(z.x - nm);
+        L = L * f + z.y * e;
         O = float4{O.x * f + y.x * e, O.y * f + y.y * e, O.z * f + y.z * e, O.w * f + y.w * e};
         M = nm;
       }
@@ -640,20 +838,21 @@ int launch_types(const QAttnArgs& a, int codes, bool half, hipStream_t s) {
 // Ranges of a call: as many workgroups as the card holds at once, and no more
 // than the buffer's pages can fill.
 struct Ranges {
-  long long workers, least, pitch;
+  long long workers, least, cus;
 };
-Ranges ranges_of(long long segments, int32_t head_dim, int32_t page_size, int32_t window, long long indices_len) {
-  const int cus = vtx::device_cu_count() > 0 ? vtx::device_cu_count() : 256;
+Ranges ranges_of(int32_t head_dim, int32_t page_size, long long indices_len) {
   Ranges r;
+  r.cus = vtx::device_cu_count() > 0 ? vtx::device_cu_count() : 256;
   r.least = (kMinTokens + (long long)page_size - 1) / page_size;
-  r.pitch = window > 0 ? ((long long)window + page_size - 1) / page_size + 1 : 0;
-  if (r.pitch * segments > 0x7fffffffLL) r.pitch = 0;  // (a window past any segment: the pages as they are)
-  const long long line = r.pitch > 0 ? r.pitch * segments : indices_len;
-  r.workers = (long long)cus * (head_dim == 256 ? 2 : (head_dim == 128 ? 3 : 4));
-  const long long need = (line + r.least - 1) / r.least;
+  r.workers = r.cus * (head_dim == 256 ? 2 : 3);
+  const long long need = (indices_len + r.least - 1) / r.least;
   if (r.workers > need) r.workers = need;
   if (r.workers < 1) r.workers = 1;
   return r;
+}
+// Floats of scratch: two parts a range, and a packed line's places.
+long long scratch_of(const Ranges& r, long long segments, int32_t group_size, int32_t head_dim, int32_t window) {
+  return 2 * r.workers * group_size * (head_dim + 2) + (window > 0 && segments < kBounds ? segments + 1 : 0);
 }
 
 }  // namespace
@@ -668,8 +867,8 @@ extern "C" int64_t vtx_quant_decode_attention_workspace_len(int32_t batch_size, 
   if (batch_size < 1 || num_kv_heads < 1 || page_size < 1 || window < 0 || kv_indices_len < 0 ||
       !vtx_quant_decode_attention_supported(head_dim, group_size))
     return 0;
-  const Ranges r = ranges_of((long long)batch_size * num_kv_heads, head_dim, page_size, window, kv_indices_len);
-  return 2 * r.workers * group_size * (head_dim + 2);
+  return scratch_of(ranges_of(head_dim, page_size, kv_indices_len), (long long)batch_size * num_kv_heads, group_size,
+                    head_dim, window);
 }
 
 extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_strides, void* o, const void* k_cache,
@@ -726,23 +925,28 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
   a.window = window;
   a.c = soft_cap > 0.f ? 2.f * kLog2e * (sm_scale / soft_cap) : sm_scale * kLog2e;
   a.cap = soft_cap * kLog2e;
-  a.pitch = 0;
   a.workers = 0;
   a.least = 1;
+  a.by_segments = divisor(segments);
+  a.by_heads = divisor(num_kv_heads);
+  a.by_workers = a.by_cus = divisor(1);
   a.acc = nullptr;
   a.ml = nullptr;
+  a.places = nullptr;
   if (workspace) {
-    const Ranges r = ranges_of(segments, head_dim, page_size, window, kv_indices_len);
-    const long long parts = 2 * r.workers * group_size;
-    if (workspace_len < parts * (head_dim + 2) || !vtx::aligned16(workspace))
+    const Ranges r = ranges_of(head_dim, page_size, kv_indices_len);
+    const long long parts = 2 * r.workers * group_size, need = scratch_of(r, segments, group_size, head_dim, window);
+    if (workspace_len < need || !vtx::aligned16(workspace))
       return vtx::fail(VTX_E_INVALID,
-                       "quant_decode_attention: workspace of %lld floats (16-byte aligned) needed, got %lld",
-                       parts * (long long)(head_dim + 2), (long long)workspace_len);
+                       "quant_decode_attention: workspace of %lld floats (16-byte aligned) needed, got %lld", need,
+                       (long long)workspace_len);
     a.workers = (int32_t)r.workers;
     a.least = (int32_t)r.least;
-    a.pitch = (int32_t)r.pitch;
+    a.by_workers = divisor(r.workers);
+    a.by_cus = divisor(r.cus);
     a.acc = workspace;
     a.ml = reinterpret_cast<float2*>(workspace + parts * head_dim);
+    a.places = reinterpret_cast<int32_t*>(workspace + parts * (head_dim + 2));
   }
   hipStream_t s = vtx::as_stream(stream);
   const bool half = dtype == VTX_DTYPE_F16;

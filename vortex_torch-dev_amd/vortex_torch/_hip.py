@@ -318,7 +318,7 @@ def device_cu_count(dev: torch.device) -> int:
     return _cu_counts[idx]
 
 
-_PLAIN_TYPES = frozenset({torch.Tensor, int, float, bool, type(None)})
+_PLAIN_TYPES = frozenset({torch.Tensor, int, float, bool, type(None), torch.dtype})
 
 
 def _plain_positional(fn):
@@ -1502,6 +1502,51 @@ def _quant_rows_refusal(k_cache, v_cache, kv_scales, k, v, loc, page_size, names
     return ""
 
 
+def _quant_pools_fit(k_cache, v_cache, kv_scales) -> bool:
+    """Whether the pools of an 8-bit cache are well-formed, in one look (otherwise
+    _quant_pools_refusal says what is wrong, if anything)."""
+    pools = k_cache.shape
+    if len(pools) != 3 or v_cache.shape != pools or k_cache.dtype not in _CODES or v_cache.dtype is not k_cache.dtype:
+        return False
+    scales = kv_scales.shape
+    return (len(scales) == 3 and scales[0] == pools[0] and scales[1] == pools[1] and scales[2] == 2
+            and kv_scales.dtype in _SCALES and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and kv_scales.is_contiguous())
+
+
+def _quant_new_rows(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size):
+    """vtx_set_kv_buffer_quant's arguments but for the stream, of a call that is
+    well-formed beyond doubt, in one look (None: _quant_rows_refusal says what is
+    wrong, if anything)."""
+    new, dtype = new_k.shape, new_k.dtype
+    if (len(new) != 3 or new_v.shape != new or dtype not in _ROPE_DTYPES or new_v.dtype is not dtype
+            or not _quant_pools_fit(k_cache, v_cache, kv_scales)):
+        return None
+    nnz, H, D = new
+    rows, P, cols = k_cache.shape
+    k0, k1, k2 = new_k.stride()
+    v0, v1, v2 = new_v.stride()
+    if (nnz < 1 or H < 1 or cols != D or P != page_size or rows % H or k2 != 1 or v2 != 1
+            or loc.dtype is not torch.int64 or not loc.is_contiguous() or loc.numel() < nnz):
+        return None
+    kp, vp, sp, k, v = (k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), new_k.data_ptr(),
+                        new_v.data_ptr())
+    pool, size = rows * P * D, 4 if dtype is torch.float32 else 2
+    k_end = k + size * ((nnz - 1) * k0 + (H - 1) * k1 + D)
+    v_end = v + size * ((nnz - 1) * v0 + (H - 1) * v1 + D)
+    s_end = sp + 2 * rows * P
+    if not ((kp + pool <= vp or vp + pool <= kp) and (kp + pool <= sp or s_end <= kp)
+            and (vp + pool <= sp or s_end <= vp) and _clear(k, k_end, kp, vp, pool) and _clear(v, v_end, kp, vp, pool)
+            and (k_end <= sp or s_end <= k) and (v_end <= sp or s_end <= v)):
+        return None
+    if nnz == 1:  # (one row's stride may be anything)
+        k0 = v0 = 0
+    if H == 1:
+        k1 = v1 = 0
+    return (kp, vp, sp, rows * P, k, v, _FourI64(k0, k1, v0, v1), loc.data_ptr(), nnz, H, D, _ROPE_DTYPES[dtype],
+            _CODES[k_cache.dtype], P)
+
+
 @_plain_positional
 def set_kv_buffer_quant(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size) -> None:
     """Quantises new_k / new_v [nnz, H, D] into 8-bit pools at the slots loc."""
@@ -1510,18 +1555,25 @@ def set_kv_buffer_quant(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_siz
     if _current_device() != index:
         with _on_device(torch.device("cuda", index)):
             return set_kv_buffer_quant(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size)
-    wrong = _quant_rows_refusal(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size, ("new_k", "new_v"), False)
-    if wrong:
-        raise RuntimeError("vortex_torch: " + wrong)
-    nnz, H, D = new_k.shape
-    k0, k1 = (0 if n == 1 else t for n, t in zip((nnz, H), new_k.stride()))
-    v0, v1 = (0 if n == 1 else t for n, t in zip((nnz, H), new_v.stride()))
-    rc = lib.vtx_set_kv_buffer_quant(
-        k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), k_cache.shape[0] * page_size, new_k.data_ptr(),
-        new_v.data_ptr(), _FourI64(k0, k1, v0, v1), loc.data_ptr(), nnz, H, D, _ROPE_DTYPES[new_k.dtype],
-        _CODES[k_cache.dtype], page_size, _stream_of(index))
+    args = _quant_new_rows(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size)
+    if args is None:
+        wrong = _quant_rows_refusal(k_cache, v_cache, kv_scales, new_k, new_v, loc, page_size, ("new_k", "new_v"),
+                                    False)
+        if wrong:
+            raise RuntimeError("vortex_torch: " + wrong)
+        args = _quant_rows_args(k_cache, v_cache, kv_scales, new_k, new_v, loc)
+    rc = lib.vtx_set_kv_buffer_quant(*args, _stream_of(index))
     if rc:
         _check(rc, "set_kv_buffer_quant")
+
+
+def _quant_rows_args(k_cache, v_cache, kv_scales, k, v, loc) -> tuple:
+    """vtx_set_kv_buffer_quant's and vtx_read_kv_buffer_quant's arguments but for the stream."""
+    nnz, H, D = k.shape
+    rows, P, _ = k_cache.shape
+    strides = [0 if n == 1 else st for t in (k, v) for n, st in zip((nnz, H), t.stride())]
+    return (k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), rows * P, k.data_ptr(), v.data_ptr(),
+            _FourI64(*strides), loc.data_ptr(), nnz, H, D, _ROPE_DTYPES[k.dtype], _CODES[k_cache.dtype], P)
 
 
 @_plain_positional
@@ -1529,84 +1581,115 @@ def read_kv_buffer_quant(k_cache, v_cache, kv_scales, loc, page_size, num_kv_hea
     """The values of 8-bit pools at the slots loc: k, v [nnz, H, D] (k_out and
     v_out, or new tensors of dtype)."""
     lib = _lib or load_library()
-    given = [t for t in (k_out, v_out) if t is not None]
-    index = _device_index(loc, k_cache, v_cache, kv_scales, *given)
+    if k_out is None and v_out is None:
+        index = _device_index(loc, k_cache, v_cache, kv_scales)
+    else:
+        index = _device_index(loc, k_cache, v_cache, kv_scales, *(t for t in (k_out, v_out) if t is not None))
     if _current_device() != index:
         with _on_device(torch.device("cuda", index)):
             return read_kv_buffer_quant(k_cache, v_cache, kv_scales, loc, page_size, num_kv_heads, dtype, k_out, v_out)
-    if len(given) == 1:
-        raise RuntimeError("vortex_torch: k_out and v_out go together")
-    if not given:
-        wrong = _quant_pools_refusal(k_cache, v_cache, kv_scales)
-        if not wrong and dtype not in _ROPE_DTYPES:
-            wrong = f"dtype must be bfloat16, float16 or float32, got {dtype}"
-        if not wrong and num_kv_heads < 1:
-            wrong = f"num_kv_heads must be positive, got {num_kv_heads}"
+    wrong, H = "", num_kv_heads
+    if (k_out is None) != (v_out is None):
+        wrong = "k_out and v_out go together"
+    elif k_out is None:
+        if not _quant_pools_fit(k_cache, v_cache, kv_scales):
+            wrong = _quant_pools_refusal(k_cache, v_cache, kv_scales)
         if wrong:
-            raise RuntimeError("vortex_torch: " + wrong)
-        shape = (loc.numel(), num_kv_heads, k_cache.shape[2])
-        k_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
-        v_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
-    elif k_out.dim() == 3 and (k_out.shape[0] != loc.numel() or k_out.shape[1] != num_kv_heads):
-        raise RuntimeError(
-            f"vortex_torch: k_out must be [{loc.numel()}, {num_kv_heads}, head_dim], got {tuple(k_out.shape)}")
-    wrong = _quant_rows_refusal(k_cache, v_cache, kv_scales, k_out, v_out, loc, page_size, ("k_out", "v_out"), True)
+            pass
+        elif dtype not in _ROPE_DTYPES:
+            wrong = f"dtype must be bfloat16, float16 or float32, got {dtype}"
+        elif H < 1:
+            wrong = f"num_kv_heads must be positive, got {H}"
+        else:
+            rows, P, D = k_cache.shape
+            nnz = loc.numel()
+            k_out = torch.empty((nnz, H, D), dtype=dtype, device=k_cache.device)
+            v_out = torch.empty((nnz, H, D), dtype=dtype, device=k_cache.device)
+            # (new tensors lie apart from everything)
+            if P == page_size and D > 0 and rows % H == 0 and loc.dtype is torch.int64 and loc.is_contiguous():
+                rc = lib.vtx_read_kv_buffer_quant(
+                    k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), rows * P, k_out.data_ptr(),
+                    v_out.data_ptr(), _FourI64(H * D, D, H * D, D), loc.data_ptr(), nnz, H, D, _ROPE_DTYPES[dtype],
+                    _CODES[k_cache.dtype], P, _stream_of(index))
+                if rc:
+                    _check(rc, "read_kv_buffer_quant")
+                return k_out, v_out
+    elif k_out.dim() == 3 and (k_out.shape[0] != loc.numel() or k_out.shape[1] != H):
+        wrong = f"k_out must be [{loc.numel()}, {H}, head_dim], got {tuple(k_out.shape)}"
+    wrong = wrong or _quant_rows_refusal(k_cache, v_cache, kv_scales, k_out, v_out, loc, page_size, ("k_out", "v_out"),
+                                         True)
     if wrong:
         raise RuntimeError("vortex_torch: " + wrong)
-    nnz, H, D = k_out.shape
-    k0, k1 = (0 if n == 1 else t for n, t in zip((nnz, H), k_out.stride()))
-    v0, v1 = (0 if n == 1 else t for n, t in zip((nnz, H), v_out.stride()))
-    rc = lib.vtx_read_kv_buffer_quant(
-        k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), k_cache.shape[0] * page_size, k_out.data_ptr(),
-        v_out.data_ptr(), _FourI64(k0, k1, v0, v1), loc.data_ptr(), nnz, H, D, _ROPE_DTYPES[k_out.dtype],
-        _CODES[k_cache.dtype], page_size, _stream_of(index))
+    rc = lib.vtx_read_kv_buffer_quant(*_quant_rows_args(k_cache, v_cache, kv_scales, k_out, v_out, loc),
+                                      _stream_of(index))
     if rc:
         _check(rc, "read_kv_buffer_quant")
     return k_out, v_out
 
 
-@_plain_args
 def page_reduce_quant(x, kv_scales, of_values, outs, reduce_types, loc, num_kv_heads: int, page_size: int,
                       dim: int) -> None:
     """page_reduce_multi (dim 1) over codes x with kv_scales' exponents of the
     keys (of_values: of the values)."""
-    lib = load_library()
-    outs, reduce_types = list(outs), [int(t) for t in reduce_types]
-    if not 1 <= len(outs) <= 4 or len(outs) != len(reduce_types):
+    lib = _lib or load_library()
+    x, kv_scales, loc, outs = _plain(x), _plain(kv_scales), _plain(loc), _plain(outs)
+    n = len(outs)
+    if not 1 <= n <= 4 or n != len(reduce_types):
         raise RuntimeError("vortex_torch: page_reduce_quant needs 1..4 outputs, one type each")
-    dev = _require_gpu(x, kv_scales, loc, *outs)
-    wrong = _quant_pools_refusal(x, x, kv_scales)
+    index = _device_index(x, kv_scales, loc, *outs)
+    if _current_device() != index:
+        with _on_device(torch.device("cuda", index)):
+            return page_reduce_quant(x, kv_scales, of_values, outs, reduce_types, loc, num_kv_heads, page_size, dim)
+    wrong = "" if _quant_pools_fit(x, x, kv_scales) else _quant_pools_refusal(x, x, kv_scales)
     if wrong:
         raise RuntimeError("vortex_torch: " + wrong)
     if dim != 1:
         raise RuntimeError(f"vortex_torch: pools of codes are reduced over a page's tokens (dim 1), not dim {dim}")
-    rows, P, D = (int(s) for s in x.shape)
+    rows, P, D = x.shape
     if P != page_size:
         raise RuntimeError(f"vortex_torch: x must be [rows, {page_size}, head_dim], got {tuple(x.shape)}")
     _req(loc, torch.int64, "loc")
-    out_rows = None
+    out_rows, ptrs, dts = rows, [], []
+    spans = [(x.data_ptr(), x.data_ptr() + rows * P * D), (kv_scales.data_ptr(), kv_scales.data_ptr() + 2 * rows * P)]
     for o in outs:
-        if o.dtype not in _OUT_DTYPES:
+        dts.append(_OUT_DTYPES.get(o.dtype))
+        if dts[-1] is None:
             raise RuntimeError(f"vortex_torch: reduce output must be bf16 or fp32, got {o.dtype}")
-        _req(o, o.dtype, "output")
-        if o.numel() % max(D, 1):
+        if not o.is_contiguous():
+            raise RuntimeError("vortex_torch: output must be contiguous")
+        size, first = o.numel(), o.data_ptr()
+        if D < 1 or size % D:
             raise RuntimeError("vortex_torch: page reduce output size is not a multiple of its row")
-        r = o.numel() // max(D, 1)
-        out_rows = r if out_rows is None else min(out_rows, r)
-    if not _apart(x, kv_scales, *outs):
-        raise RuntimeError("vortex_torch: outputs share memory with each other or the pool")
-    n = len(outs)
-    ptrs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
-    dts = (ctypes.c_int32 * n)(*[_OUT_DTYPES[o.dtype] for o in outs])
-    tys = (ctypes.c_int32 * n)(*reduce_types)
-    with _on_device(dev):
-        rc = lib.vtx_page_reduce_quant(
-            x.data_ptr(), kv_scales.data_ptr() + (1 if of_values else 0), rows, P, D, _CODES[x.dtype], n, ptrs, dts,
-            tys, out_rows, loc.data_ptr(), loc.numel(), int(num_kv_heads), _stream(dev))
-    _check(rc, "page_reduce_quant")
+        end = first + size * (4 if dts[-1] == DTYPE_F32 else 2)
+        for a, b in spans:
+            if first < b and a < end:
+                raise RuntimeError("vortex_torch: outputs share memory with each other or the pool")
+        spans.append((first, end))
+        out_rows = min(out_rows, size // D)
+        ptrs.append(first)
+    rc = lib.vtx_page_reduce_quant(
+        x.data_ptr(), kv_scales.data_ptr() + (1 if of_values else 0), rows, P, D, _CODES[x.dtype], n,
+        (_vp * n)(*ptrs), (_i32 * n)(*dts), (_i32 * n)(*reduce_types), out_rows, loc.data_ptr(), loc.numel(),
+        num_kv_heads, _stream_of(index))
+    if rc:
+        _check(rc, "page_reduce_quant")
 
 
 _QUERY_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+
+
+def _quant_attention_fits(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B, H, soft_cap,
+                          window, slopes) -> bool:
+    """Whether a call is well-formed beyond doubt, in one look (otherwise
+    _quant_attention_refusal says what is wrong, if anything)."""
+    rows = q.shape
+    if (slopes is not None or len(rows) != 3 or o.shape != rows or q.dtype not in _QUERY_DTYPES
+            or o.dtype is not q.dtype or B < 1 or H < 1 or not _quant_pools_fit(k_cache, v_cache, kv_scales)
+            or not _tables_fit(kv_indptr, kv_indices, kv_last_page_len)):
+        return False
+    return ((rows[0] == B and rows[1] % H == 0 or rows[0] == B * H) and rows[2] == k_cache.shape[2]
+            and q.stride(2) == 1 and o.is_contiguous() and kv_indptr.numel() > B * H
+            and kv_last_page_len.numel() >= B * H and 0.0 <= soft_cap < math.inf and 0 <= window <= 0x7fffffff)
 
 
 def _quant_attention_refusal(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B, H,
@@ -1646,12 +1729,15 @@ def _quant_attention_refusal(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_in
 
 @_plain_positional
 def quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, batch_size,
-                                 num_kv_heads, sm_scale, soft_cap, window, slopes) -> None:
+                                 num_kv_heads, sm_scale, soft_cap, window, slopes):
     """paged_decode_attention over 8-bit pools, with capped scores, a window or
-    slopes.  The table's pages are divided over the card with scratch from
-    torch's allocator, whose OutOfMemoryError is the caller's; in a capture that
-    torch did not begin no scratch lasts, and every segment has a workgroup."""
+    slopes, into o (None: a new tensor); returns it.  The table's pages are
+    divided over the card with scratch from torch's allocator, whose
+    OutOfMemoryError is the caller's; in a capture that torch did not begin no
+    scratch lasts, and every segment has a workgroup."""
     lib = _lib or load_library()
+    if o is None:
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if slopes is None:
         index = _device_index(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len)
     else:
@@ -1662,29 +1748,36 @@ def quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, k
                                                 kv_last_page_len, batch_size, num_kv_heads, sm_scale, soft_cap, window,
                                                 slopes)
     B, H = batch_size, num_kv_heads
-    wrong = _quant_attention_refusal(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B, H,
-                                     soft_cap, window, slopes)
-    if wrong:
-        raise RuntimeError("vortex_torch: " + wrong)
+    if not _quant_attention_fits(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B, H,
+                                 soft_cap, window, slopes):
+        wrong = _quant_attention_refusal(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B,
+                                         H, soft_cap, window, slopes)
+        if wrong:
+            raise RuntimeError("vortex_torch: " + wrong)
     if B == 0:
-        return
+        return o
     rows, P, D = k_cache.shape
-    G = q.shape[0] * q.shape[1] // (B * H)
-    s0, s1 = (0 if n == 1 else t for n, t in zip(q.shape[:2], q.stride()))  # (one row's stride may be anything)
-    strides = _ThreeI64(s0, G * s1, s1) if q.shape[0] == B and q.shape[1] != G else _ThreeI64(H * s0, s0, s1)
-    stream = _stream_of(index)
-    floats = lib.vtx_quant_decode_attention_workspace_len(B, H, G, D, P, window, kv_indices.numel())
+    n0, n1, _ = q.shape
+    G = n0 * n1 // (B * H)
+    s0, s1, _ = q.stride()
+    if n0 == 1:  # (one row's stride may be anything)
+        s0 = 0
+    if n1 == 1:
+        s1 = 0
+    strides = _ThreeI64(s0, G * s1, s1) if n0 == B and n1 != G else _ThreeI64(H * s0, s0, s1)
+    stream, entries = _stream_of(index), kv_indices.numel()
+    floats = lib.vtx_quant_decode_attention_workspace_len(B, H, G, D, P, window, entries)
     ws = None
     if floats > 0 and _scratch_lasts(stream):
         ws = torch.empty(floats, dtype=torch.float32, device=q.device)
     rc = lib.vtx_quant_decode_attention(
         q.data_ptr(), strides, o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), rows,
-        kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_last_page_len.data_ptr(), B, H, G, D, P,
+        kv_indptr.data_ptr(), kv_indices.data_ptr(), entries, kv_last_page_len.data_ptr(), B, H, G, D, P,
         _QUERY_DTYPES[q.dtype], _CODES[k_cache.dtype], sm_scale, soft_cap, window,
-        None if slopes is None else slopes.data_ptr(), None if ws is None else ws.data_ptr(),
-        0 if ws is None else floats, stream)
+        None if slopes is None else slopes.data_ptr(), None if ws is None else ws.data_ptr(), floats, stream)
     if rc:
         _check(rc, "quant_paged_decode_attention")
+    return o
 
 
 def bf16_rounding_check(device="cuda") -> tuple:

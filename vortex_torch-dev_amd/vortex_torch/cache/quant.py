@@ -54,8 +54,9 @@ def quantized_pool(codes: torch.Tensor, kv_scales: torch.Tensor, values: bool = 
     wrong = _hip._quant_pools_refusal(_hip._plain(codes), _hip._plain(codes), _hip._plain(kv_scales))
     if wrong:
         raise RuntimeError("vortex_torch: " + wrong.replace("k_cache and v_cache", "codes").replace("k_cache", "codes"))
-    pool = as_vtensor(_hip._plain(codes), FORMAT.PAGED)
-    pool._kv_scales = (_hip._plain(kv_scales), bool(values))
+    codes = _hip._plain(codes)
+    pool = as_vtensor(codes, FORMAT.PAGED)
+    pool._quantized = (codes, _hip._plain(kv_scales), bool(values))
     return pool
 
 

@@ -45,20 +45,21 @@ def _kernel_type(rt: ReduceType) -> int:
     return _KERNEL_TYPES[rt]
 
 
-def _scales_of(x):
-    """(kv_scales, whether the values' are meant) of a pool of codes, or None."""
-    return getattr(x, "_kv_scales", None)
+def _quantized(x):
+    """(codes, kv_scales, whether the values' are meant) of a pool of codes, or None."""
+    return getattr(x, "_quantized", None)
 
 
-def _reduce_quant(x, scales, outs, types, loc, ctx: Context, dim: int) -> None:
-    _hip.page_reduce_quant(x, scales[0], scales[1], outs, types, loc, ctx.head_num, ctx.page_size, dim)
+def _reduce_quant(pool, outs, types, loc, ctx: Context, dim: int) -> None:
+    _hip.page_reduce_quant(*pool, outs, types, loc, ctx.head_num, ctx.page_size, dim)
 
 
 def reduce_pp(x: torch.Tensor, output: torch.Tensor, loc: torch.Tensor, ctx: Context, dim: int,
               reduce_type: ReduceType) -> None:
     """(PAGED x, PAGED output): page-finish reduction triggered by loc."""
-    if _scales_of(x) is not None:
-        _reduce_quant(x, _scales_of(x), [output], [_kernel_type(reduce_type)], loc, ctx, dim)
+    pool = _quantized(x)
+    if pool is not None:
+        _reduce_quant(pool, [output], [_kernel_type(reduce_type)], loc, ctx, dim)
         return
     _hip.page_reduce(x, output, loc, ctx.head_num, ctx.page_size, dim, _kernel_type(reduce_type))
 
@@ -71,17 +72,16 @@ class _PendingPageReduce(_deferred.Pending):
 
     MAX_OUTPUTS = 4
 
-    def __init__(self, x: torch.Tensor, loc: torch.Tensor, ctx: Context, dim: int, scales=None):
+    def __init__(self, x: torch.Tensor, loc: torch.Tensor, ctx: Context, dim: int, quantized=None):
         super().__init__()
-        self.x, self.loc, self.ctx, self.dim, self.scales = x, loc, ctx, dim, scales
+        self.x, self.loc, self.ctx, self.dim, self.quantized = x, loc, ctx, dim, quantized
         self.outs, self.types = [], []
 
     def accepts(self, x: torch.Tensor, out: torch.Tensor, loc: torch.Tensor, ctx: Context, dim: int,
-                scales=None) -> bool:
+                quantized=None) -> bool:
         if self.done or ctx is not self.ctx or dim != self.dim or len(self.outs) >= self.MAX_OUTPUTS:
             return False
-        if (scales is None) != (self.scales is None) or (
-                scales is not None and (scales[0] is not self.scales[0] or scales[1] != self.scales[1])):
+        if quantized is not self.quantized:
             return False
         ptr = out.data_ptr()
         return (x.data_ptr() == self.x.data_ptr() and x.shape == self.x.shape and loc.data_ptr() == self.loc.data_ptr()
@@ -114,7 +114,7 @@ class _PendingPageReduce(_deferred.Pending):
         [rows, 1, D] pools."""
         if self.done or self.dim != 1 or self.loc.numel() > self.CARRY_MAX_LOC or self.carry_kind() is None:
             return False
-        if self.scales is not None:  # (the fused launches read bf16 pools)
+        if self.quantized is not None:  # (the fused launches read bf16 pools)
             return False
         x = self.x
         for out in self.outs:
@@ -129,8 +129,8 @@ class _PendingPageReduce(_deferred.Pending):
 
     def _run(self) -> None:
         c = self.ctx
-        if self.scales is not None:
-            _reduce_quant(self.x, self.scales, self.outs, self.types, self.loc, c, self.dim)
+        if self.quantized is not None:
+            _reduce_quant(self.quantized, self.outs, self.types, self.loc, c, self.dim)
         elif len(self.outs) == 1:
             _hip.page_reduce(self.x, self.outs[0], self.loc, c.head_num, c.page_size, self.dim, self.types[0])
         else:
@@ -147,11 +147,11 @@ def _record_page_reduce(x, output, loc, ctx: Context, dim: int, reduce_type: Red
         return False
     if not _recordable_operands(x, output, loc):
         return False
-    scales = _scales_of(x)
+    quantized = _quantized(x)
     xp, op, lp = _deferred.plain(x, output, loc)
     last = sc.pending[-1] if sc.pending else None
-    if not (isinstance(last, _PendingPageReduce) and last.accepts(xp, op, lp, ctx, dim, scales)):
-        last = _PendingPageReduce(xp, lp, ctx, dim, scales)
+    if not (isinstance(last, _PendingPageReduce) and last.accepts(xp, op, lp, ctx, dim, quantized)):
+        last = _PendingPageReduce(xp, lp, ctx, dim, quantized)
         sc.add(last)
     last.add(op, _kernel_type(reduce_type))
     return True
@@ -304,8 +304,9 @@ class MultiReduce(vOp):
         assert self._ready, f"{self._prefix()}called before profile()"
         _deferred.flush_all()  # recorded reductions first, in program order
         types = [_kernel_type(t) for t in self.reduce_types]
-        if _scales_of(x) is not None:
-            _reduce_quant(x, _scales_of(x), outputs, types, loc, ctx, self.dim)
+        pool = _quantized(x)
+        if pool is not None:
+            _reduce_quant(pool, outputs, types, loc, ctx, self.dim)
         else:
             _hip.page_reduce_multi(x, outputs, types, loc, ctx.head_num, ctx.page_size, self.dim)
         return list(outputs)

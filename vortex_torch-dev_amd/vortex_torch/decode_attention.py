@@ -135,13 +135,10 @@ def quant_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache
     tokens' order (dense ones): ``window``, only the last so many tokens count;
     ``slopes`` (fp32 [H_q]), the score of the token d before the newest one is
     lowered by slope * d, after the cap."""
-    D = int(q.shape[-1])
-    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    _hip.quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len,
-                                      int(batch_size), int(num_kv_heads), scale, float(logits_soft_cap or 0.0),
-                                      int(window or 0), slopes)
-    return o
+    scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
+    return _hip.quant_paged_decode_attention(q, out, k_cache, v_cache, kv_scales, kv_indptr, kv_indices,
+                                             kv_last_page_len, int(batch_size), int(num_kv_heads), scale,
+                                             float(logits_soft_cap or 0.0), int(window or 0), slopes)
 
 
 def sparse_quant_decode_attention(q, k_cache, v_cache, kv_scales, ctx, sm_scale: Optional[float] = None, out=None,
