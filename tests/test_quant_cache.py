@@ -273,7 +273,7 @@ def test_page_reductions_are_those_of_a_bf16_pool(gpu, H, P, D, codes):
 @pytest.mark.gpu
 def test_page_reductions_of_many_pages_and_of_rows_that_are_no_numbers(gpu):
     gen = torch.Generator().manual_seed(8)
-    H, P, D, pages = 8, 16, 128, 900
+    H, P, D, pages = 8, 16, 128, 2100
     kc, vc, sc = _random_pool(pages * H, P, D, E4M3, gen, gpu)
     loc = torch.arange(pages * P, device=gpu)
     out = torch.zeros((2, pages * H, 1, D), dtype=torch.bfloat16, device=gpu)
@@ -282,6 +282,10 @@ def test_page_reductions_of_many_pages_and_of_rows_that_are_no_numbers(gpu):
     plain = _values(kc, sc[..., 0].long()).bfloat16()
     _hip.page_reduce_multi(plain, list(want), [_hip.REDUCE_MAX, _hip.REDUCE_MIN], loc, H, P, 1)
     assert torch.equal(out, want)
+    for t in (_hip.REDUCE_MEAN, _hip.REDUCE_L2NORM):
+        _hip.page_reduce_quant(kc, sc, False, [out[0]], [t], loc, H, P, 1)
+        _hip.page_reduce(plain, want[0], loc, H, P, 1, t)
+        assert torch.equal(out[0], want[0])
     x = torch.randn((1, H, D), device=gpu)
     x[0, 3, 5] = math.inf
     set_kv_buffer_quant(kc, vc, sc, x, x, torch.tensor([40], device=gpu), P)

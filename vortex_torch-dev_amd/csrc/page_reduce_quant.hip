@@ -6,11 +6,14 @@
 // page_reduce.hip's order, so the outputs are bit for bit those of the same
 // reduction over a bf16 pool that holds the values.
 //
-// Bound by HBM for a burst of pages, by the launch and three dependent loads
-// (loc, codes, output) for a decode step.  As there, a workgroup scans 256 loc
-// entries and keeps the pages they close, and several share a block's tiles.  A
-// wave takes tiles one at a time: lane = (row group, 8 columns), all of a
-// 16-row tile's codes and factors loaded before the first is used.
+// Bound by HBM for a burst of pages (16,384 pages of 8 heads, Max + Min, 76 us, 4.5
+// TB/s), by the launch and two dependent loads (loc, codes) for a decode step (64
+// requests 3.8 us).  As there, a workgroup scans 256 loc entries and keeps the
+// pages they close, and several share a block's tiles.  Few tiles: a wave takes one
+// at a time, lane = (row group, 8 columns), the codes of 16 to 64 rows of a tile
+// loaded before the first is used.  Many (of up to 16 rows): lane = (tile, 8
+// columns), 64 / LPR tiles of a wave at a time, which a lane reduces alone, all its
+// rows in flight and nothing between the lanes.
 #include <algorithm>
 
 #include "vtx_device.h"
@@ -58,6 +61,13 @@ __device__ __forceinline__ int collect(const PageArgs& a, long long* first_row, 
   return total;
 }
 
+// 8 codes, read once (ld16_stream says why).
+__device__ __forceinline__ uint2 load8(const unsigned char* p) {
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  const v2u t = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(p));
+  return uint2{t.x, t.y};
+}
+
 template <int kCodes, int NEED>
 __device__ __forceinline__ void add8(Acc (&acc)[8], const uint2& w, uint32_t byte, bool in) {
   const float s = vtx::factor(byte);
@@ -70,43 +80,76 @@ __device__ __forceinline__ void add8(Acc (&acc)[8], const uint2& w, uint32_t byt
   for (int e = 0; e < 4; ++e) vtx::acc_add_if<NEED>(acc[4 + e], f[e] * s, in);
 }
 
+// Row groups kG0 .. kG0 + kN - 1 (group g: rows g, g + G, ..., in order) of a lane's
+// columns, folded pairwise as page_reduce.hip folds them: ((0 + 1) + (2 + 3)) + ..
+template <int kCodes, int G, int kG0, int kN, int NEED>
+__device__ __forceinline__ void fold_groups(const uint2 (&w)[16], const uint32_t (&b)[16], int R, Acc (&s)[8]) {
+  if constexpr (kN == 1) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vtx::acc_init<NEED>(s[e]);
+#pragma unroll
+    for (int r = kG0; r < 16; r += G) add8<kCodes, NEED>(s, w[r], b[r], r < R);
+  } else {
+    Acc lower[8];
+    fold_groups<kCodes, G, kG0, kN / 2, NEED>(w, b, R, lower);
+    fold_groups<kCodes, G, kG0 + kN / 2, kN / 2, NEED>(w, b, R, s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vtx::acc_fold<NEED>(lower[e], s[e]);
+  }
+}
+
 // C = 8 LPR, LPR | 64: page_reduce.hip's row groups (g: rows g, g + 64 / LPR, ..)
-// and their fold.
-template <int kCodes, int LPR, int NEED>
+// and their fold.  kBatch: rows of a group in flight; 0: a lane per column.
+template <int kCodes, int LPR, int NEED, int kBatch>
 __global__ __launch_bounds__(kThreads) void reduce_quant_kernel(PageArgs a) {
   constexpr int kGroups = vtx::kWave / LPR;
-  constexpr int kBatch = 16 / kGroups < 2 ? 2 : (16 / kGroups > 8 ? 8 : 16 / kGroups);
   __shared__ long long first_row[kThreads];
   __shared__ int wave_count[kWaves];
   const int pages = collect(a, first_row, wave_count);
   const int lane = vtx::lane_id(), grp = lane / LPR, cv = lane % LPR;
   const int wave = threadIdx.x / vtx::kWave;
-  const int R = a.r.rows_per_tile, tiles = pages * a.r.heads;
-  for (int t = blockIdx.y * kWaves + wave; t < tiles; t += gridDim.y * kWaves) {
+  const int R = a.r.rows_per_tile, C = a.r.cols, tiles = pages * a.r.heads;
+  constexpr int kAtOnce = kBatch == 0 ? kGroups : 1;
+  for (int t0 = (blockIdx.y * kWaves + wave) * kAtOnce; t0 < tiles; t0 += gridDim.y * kWaves * kAtOnce) {
+    const int t = kBatch == 0 ? t0 + grp : t0;
+    if (t >= tiles) continue;
     const long long row = first_row[t / a.r.heads] + (t % a.r.heads);
     if (!vtx::tile_in_range(a.r, row)) continue;
-    const unsigned char* base = a.codes + row * (long long)R * a.r.cols + cv * 8;
+    const unsigned char* base = a.codes + row * (long long)R * C + cv * 8;
     const unsigned char* sc = a.scales + row * (long long)R * 2;
     Acc acc[8];
+    if constexpr (kBatch == 0) {
+      uint2 w[16];
+      uint32_t b[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) vtx::acc_init<NEED>(acc[e]);
-    for (int r0 = grp; r0 < R; r0 += kBatch * kGroups) {
-      uint2 w[kBatch];
-      uint32_t b[kBatch];
+      for (int r = 0; r < 16; ++r) {
+        const int at = r < R ? r : R - 1;
+        w[r] = load8(base + at * C);
+        b[r] = sc[2 * at];
+      }
+      fold_groups<kCodes, kGroups, 0, kGroups, NEED>(w, b, R, acc);
+      vtx::tile_store_vec(a.r, row, cv, acc);
+    } else {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int r = r0 + u * kGroups, at = r < R ? r : R - 1;
-        w[u] = *reinterpret_cast<const uint2*>(base + (long long)at * a.r.cols);
-        b[u] = sc[2 * at];
+      for (int e = 0; e < 8; ++e) vtx::acc_init<NEED>(acc[e]);
+      for (int r0 = grp; r0 < R; r0 += kBatch * kGroups) {
+        uint2 w[kBatch];
+        uint32_t b[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int r = r0 + u * kGroups, at = r < R ? r : R - 1;
+          w[u] = load8(base + (long long)at * C);
+          b[u] = sc[2 * (long long)at];
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) add8<kCodes, NEED>(acc, w[u], b[u], r0 + u * kGroups < R);
       }
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) add8<kCodes, NEED>(acc, w[u], b[u], r0 + u * kGroups < R);
+      for (int d = LPR; d < vtx::kWave; d <<= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vtx::acc_merge_xor<NEED>(acc[e], d);
+      if (grp == 0) vtx::tile_store_vec(a.r, row, cv, acc);
     }
-#pragma unroll
-    for (int d = LPR; d < vtx::kWave; d <<= 1)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) vtx::acc_merge_xor<NEED>(acc[e], d);
-    if (grp == 0) vtx::tile_store_vec(a.r, row, cv, acc);
   }
 }
 
@@ -140,26 +183,46 @@ __global__ __launch_bounds__(kThreads) void reduce_quant_any_kernel(PageArgs a) 
   }
 }
 
+template <int kCodes, int LPR, int NEED>
+void launch_need(const PageArgs& a, int at_once, dim3 grid, hipStream_t s) {
+  constexpr int kGroups = vtx::kWave / LPR, kBatch = kGroups >= 8 ? 2 : 16 / kGroups > 8 ? 8 : 16 / kGroups;
+  if constexpr (vtx::lane_tiles_fit(LPR, NEED)) {
+    if (at_once > 1) {
+      reduce_quant_kernel<kCodes, LPR, NEED, 0><<<grid, kThreads, 0, s>>>(a);
+      return;
+    }
+  }
+  // (taller tiles: more rows in flight, as far as registers allow)
+  if (a.r.rows_per_tile > 16) reduce_quant_kernel<kCodes, LPR, NEED, 2 * kBatch><<<grid, kThreads, 0, s>>>(a);
+  else reduce_quant_kernel<kCodes, LPR, NEED, kBatch><<<grid, kThreads, 0, s>>>(a);
+}
+
+constexpr int kEnvelope = vtx::kNeedMax | vtx::kNeedMin;
+// Single reductions and Max + Min get their own code; other mixes accumulate every
+// statistic.
+constexpr int instance_need(int need) {
+  return need == vtx::kNeedSum || need == vtx::kNeedMax || need == vtx::kNeedMin || need == kEnvelope ? need
+                                                                                                     : vtx::kNeedAll;
+}
+
 template <int kCodes, int LPR>
-void launch_vec(const PageArgs& a, int need, dim3 grid, hipStream_t s) {
-  switch (need) {
-    case vtx::kNeedSum: reduce_quant_kernel<kCodes, LPR, vtx::kNeedSum><<<grid, kThreads, 0, s>>>(a); break;
-    case vtx::kNeedMax: reduce_quant_kernel<kCodes, LPR, vtx::kNeedMax><<<grid, kThreads, 0, s>>>(a); break;
-    case vtx::kNeedMin: reduce_quant_kernel<kCodes, LPR, vtx::kNeedMin><<<grid, kThreads, 0, s>>>(a); break;
-    case vtx::kNeedMax | vtx::kNeedMin:
-      reduce_quant_kernel<kCodes, LPR, vtx::kNeedMax | vtx::kNeedMin><<<grid, kThreads, 0, s>>>(a);
-      break;
-    default: reduce_quant_kernel<kCodes, LPR, vtx::kNeedAll><<<grid, kThreads, 0, s>>>(a); break;
+void launch_vec(const PageArgs& a, int need, int at_once, dim3 grid, hipStream_t s) {
+  switch (instance_need(need)) {
+    case vtx::kNeedSum: launch_need<kCodes, LPR, vtx::kNeedSum>(a, at_once, grid, s); break;
+    case vtx::kNeedMax: launch_need<kCodes, LPR, vtx::kNeedMax>(a, at_once, grid, s); break;
+    case vtx::kNeedMin: launch_need<kCodes, LPR, vtx::kNeedMin>(a, at_once, grid, s); break;
+    case kEnvelope: launch_need<kCodes, LPR, kEnvelope>(a, at_once, grid, s); break;
+    default: launch_need<kCodes, LPR, vtx::kNeedAll>(a, at_once, grid, s); break;
   }
 }
 
 template <int kCodes>
-void launch_codes(const PageArgs& a, int need, bool vec, dim3 grid, hipStream_t s) {
+void launch_codes(const PageArgs& a, int need, bool vec, int at_once, dim3 grid, hipStream_t s) {
   const int lpr = a.r.cols / 8;
-  if (vec && lpr == 8) launch_vec<kCodes, 8>(a, need, grid, s);
-  else if (vec && lpr == 16) launch_vec<kCodes, 16>(a, need, grid, s);
-  else if (vec && lpr == 32) launch_vec<kCodes, 32>(a, need, grid, s);
-  else if (vec && lpr == 64) launch_vec<kCodes, 64>(a, need, grid, s);
+  if (vec && lpr == 8) launch_vec<kCodes, 8>(a, need, at_once, grid, s);
+  else if (vec && lpr == 16) launch_vec<kCodes, 16>(a, need, at_once, grid, s);
+  else if (vec && lpr == 32) launch_vec<kCodes, 32>(a, need, at_once, grid, s);
+  else if (vec && lpr == 64) launch_vec<kCodes, 64>(a, need, at_once, grid, s);
   else reduce_quant_any_kernel<kCodes><<<grid, kThreads, 0, s>>>(a);
 }
 
@@ -213,16 +276,27 @@ extern "C" int vtx_page_reduce_quant(const void* x, const void* scales, int64_t 
   a.codes = static_cast<const unsigned char*>(x);
   a.scales = static_cast<const unsigned char*>(scales);
   a.last_page = x_rows / num_kv_heads - 1;
+  const bool vec = cols % 8 == 0 && aligned;
   // One round of the workgroups' waves takes a block's tiles of whole pages where
   // sixteen can, and sixteen share a block while the grid is under 512
   // (page_reduce.hip has the reasons).
   const long long tiles = (page_size < kThreads ? kThreads / page_size : 1) * (long long)num_kv_heads;
-  const long long share =
-      std::min<long long>(std::max((tiles + kWaves - 1) / kWaves, (512 + blocks - 1) / blocks), kMaxShare);
+  // Several tiles of a wave at a time pay where there are more than waves to take
+  // them, earlier with two statistics, whose fold across lanes is longer, or where a
+  // block has many; 256 columns have two a wave, which gain nothing.  One at a time /
+  // several, Mean, 128 columns: 8192 tiles 8.8 / 9.7 us, 16,384 13.5 / 13.1, 131,072
+  // 79.7 / 74.1; Max + Min: 512 tiles of 8 heads 6.0 / 5.5, 1024 of one head 4.5 /
+  // 5.9, 4096 7.1 / 6.1, 131,072 124 / 78; 256 columns, Mean, 131,072 122 / 130.
+  const int lpr = cols / 8, stats = __builtin_popcount(instance_need(need));
+  const bool lanes = vec && page_size <= 16 && (lpr == 8 || lpr == 16) &&
+                     vtx::lane_tiles_fit(lpr, instance_need(need)) &&
+                     (blocks * tiles >= (stats > 1 ? 4096 : 16384) || (stats > 1 && blocks >= 4 && tiles >= 64));
+  const int at_once = lanes ? vtx::kWave / lpr : 1;
+  const long long round = (tiles + kWaves * at_once - 1) / (kWaves * at_once);
+  const long long share = std::min<long long>(std::max(round, (512 + blocks - 1) / blocks), kMaxShare);
   const dim3 grid((unsigned)blocks, (unsigned)share);
-  const bool vec = cols % 8 == 0 && aligned;
   hipStream_t s = vtx::as_stream(stream);
-  if (codes == VTX_CODES_E4M3) launch_codes<VTX_CODES_E4M3>(a, need, vec, grid, s);
-  else launch_codes<VTX_CODES_INT8>(a, need, vec, grid, s);
+  if (codes == VTX_CODES_E4M3) launch_codes<VTX_CODES_E4M3>(a, need, vec, at_once, grid, s);
+  else launch_codes<VTX_CODES_INT8>(a, need, vec, at_once, grid, s);
   return vtx::check_launch("page_reduce_quant");
 }
