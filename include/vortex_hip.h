@@ -827,21 +827,23 @@ int vtx_page_reduce_quant(const void* x, const void* scales, int64_t x_rows, int
  * contents neither read nor kept across calls; calls that may overlap need one
  * each.  With it a table's pages are divided evenly over the card, and a second
  * launch joins the parts of segments that lie in several divisions: a request's
- * last bits follow the other requests of the table, and kv_indices_len.  NULL: a
- * workgroup per segment, one launch, the same bits in every batch.
+ * last bits follow the other requests of the table, and kv_indices_len.  NULL, or
+ * a length of 0: a workgroup per segment, one launch, the same bits in every batch.
+ * longest: tokens that no segment exceeds, if the caller knows (0: unknown); where
+ * the segments are short or many for it, that length is 0.  It steers speed alone.
  * head_dim 64, 128 or 256; group_size 1..16.
  */
 int vtx_quant_decode_attention_supported(int32_t head_dim, int32_t group_size);
 int64_t vtx_quant_decode_attention_workspace_len(int32_t batch_size, int32_t num_kv_heads, int32_t group_size,
                                                  int32_t head_dim, int32_t page_size, int32_t window,
-                                                 int64_t kv_indices_len);
+                                                 int32_t longest, int64_t kv_indices_len);
 int vtx_quant_decode_attention(const void* q, const int64_t* q_strides, void* o, const void* k_cache,
                                const void* v_cache, const void* scales, int64_t cache_rows, const int32_t* kv_indptr,
                                const int32_t* kv_indices, int64_t kv_indices_len, const int32_t* kv_last_page_len,
                                int32_t batch_size, int32_t num_kv_heads, int32_t group_size, int32_t head_dim,
                                int32_t page_size, int32_t dtype, int32_t codes, float sm_scale, float soft_cap,
-                               int32_t window, const float* slopes, float* workspace, int64_t workspace_len,
-                               void* stream);
+                               int32_t window, const float* slopes, int32_t longest, float* workspace,
+                               int64_t workspace_len, void* stream);
 
 /*
  * Bandwidth probes (measurement only; no counterpart in the reference).

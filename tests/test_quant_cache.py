@@ -439,6 +439,8 @@ def _uniform(tokens, H, G, D, P, device, window=0, codes_seed=1):
     ([1] * 700, 4, 64, 16, 0), ([5, 0, 64] * 500, 2, 128, 32, 0), ([40000, 9], 1, 256, 64, 0),
     ([9000, 1], 2, 128, 1, 0),
     ([20000, 30, 0, 7000], 2, 128, 16, 1000), ([3000] * 30, 4, 64, 16, 33), ([700, 9000], 1, 256, 5, 4096),
+    ([20000, 30, 0, 7000], 2, 128, 16, 3001), ([3000, 1, 0, 1600] * 8, 4, 64, 16, 1500), ([0, 9000, 0], 2, 64, 48, 8000),
+    ([5000, 0, 9000, 40] * 8, 8, 64, 24, 2500), ([16, 2000] * 150, 1, 128, 16, 2049),
     ([0, 0, 0], 2, 64, 16, 0), ([32769], 1, 64, 16, 0)], ids=lambda x: str(x)[:20])
 def test_attention_counts_every_token_once(gpu, tokens, H, D, P, window):
     _uniform(tokens, H, 2, D, P, gpu, window=window)
@@ -449,6 +451,16 @@ def test_attention_of_many_segments(gpu):
     """More segments than are looked through one by one, some of them empty."""
     r = random.Random(4)
     _uniform([r.choice([0, 1, 15, 16, 40, 200]) for _ in range(1500)], 2, 1, 64, 16, gpu)
+    _uniform([r.choice([0, 1, 300, 6000]) for _ in range(1100)], 1, 1, 64, 64, gpu, window=5000)
+    _uniform([r.choice([0, 1, 300, 600]) for _ in range(1100)], 1, 1, 64, 5, gpu, window=4500)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,tokens", [(8, [512] * 64), (2, [700] * 3), (3, [5, 900, 0, 33])])
+def test_attention_with_a_known_bound(gpu, H, tokens):
+    """max_tokens steers how the work is divided, also where it is wrong."""
+    for most in (None, 1, max(tokens), 1 << 40):
+        _case(tokens, H, 2, 128, 16, E4M3, torch.bfloat16, gpu, max_tokens=most)
 
 
 @pytest.mark.gpu
@@ -468,7 +480,7 @@ def test_attention_without_scratch_and_with_it(gpu, D, P):
         return lib.vtx_quant_decode_attention(
             q.data_ptr(), strides, out.data_ptr(), kc.data_ptr(), vc.data_ptr(), sc.data_ptr(), kc.shape[0],
             tables[0].data_ptr(), tables[1].data_ptr(), tables[1].numel(), tables[2].data_ptr(), B, H, G, D, P, 0, 0,
-            D ** -0.5, 0.0, window, None, ws, n, torch.cuda.current_stream().cuda_stream)
+            D ** -0.5, 0.0, window, None, 0, ws, n, torch.cuda.current_stream().cuda_stream)
 
     assert call(0, None, 0) == 0
     _near(out, want, off)
@@ -890,18 +902,21 @@ def test_c_refusals():
                                          (ctypes.c_int32 * 1)(rt), 64, p[4], nnz, H, None)
 
     for kw, says in ((dict(n_out=0), b"1..4"), (dict(n_out=5), b"1..4"), (dict(codes=7), b"codes"),
-                     (dict(P=0), b"sizes"), (dict(C=0), b"sizes"), (dict(H=0), b"sizes"), (dict(nnz=-1), b"sizes"), (dict(x=None), b"null"),
+                     (dict(P=0), b"sizes"), (dict(C=0), b"sizes"), (dict(H=0), b"sizes"), (dict(nnz=-1), b"sizes"),
+                     (dict(x=None), b"null"),
                      (dict(out=None), b"null"), (dict(dtype=2), b"dtype"), (dict(rt=4), b"reduce type"),
                      (dict(H=1 << 30), b"too many heads")):
         assert reduce(**kw) == -1 and says in lib.vtx_last_error(), (kw, lib.vtx_last_error())
     assert reduce(nnz=0) == 0
 
-    def attend(B=2, H=2, G=3, D=64, P=8, dtype=0, codes=0, cap=0.0, window=0, q=p[0], k=p[2], entries=8, st=three):
+    def attend(B=2, H=2, G=3, D=64, P=8, dtype=0, codes=0, cap=0.0, window=0, q=p[0], k=p[2], entries=8, st=three,
+               longest=0):
         return lib.vtx_quant_decode_attention(q, st, p[1], k, p[3], p[4], 32, p[5], p[6], entries, p[7], B, H, G, D, P,
-                                              dtype, codes, 0.1, cap, window, None, None, 0, None)
+                                              dtype, codes, 0.1, cap, window, None, longest, None, 0, None)
 
     for kw, says in ((dict(B=-1), b"sizes"), (dict(H=0), b"sizes"), (dict(P=0), b"sizes"), (dict(window=-1), b"sizes"),
-                     (dict(entries=-1), b"sizes"), (dict(D=96), b"not supported"), (dict(G=17), b"not supported"),
+                     (dict(entries=-1), b"sizes"), (dict(longest=-1), b"sizes"), (dict(D=96), b"not supported"),
+                     (dict(G=17), b"not supported"),
                      (dict(G=0), b"not supported"), (dict(dtype=1), b"element type"), (dict(codes=2), b"codes"),
                      (dict(cap=-1.0), b"cap"), (dict(cap=math.nan), b"cap"), (dict(cap=math.inf), b"cap"),
                      (dict(q=None), b"null"), (dict(q=p[0] + 8), b"aligned"), (dict(k=p[2] + 4), b"aligned"),
@@ -910,4 +925,8 @@ def test_c_refusals():
         assert attend(**kw) == -1 and says in lib.vtx_last_error(), (kw, lib.vtx_last_error())
     assert attend(B=0) == 0
     need = lib.vtx_quant_decode_attention_workspace_len
-    assert need(2, 2, 3, 64, 8, 0, 8) > 0 and need(0, 2, 3, 64, 8, 0, 8) == 0 and need(2, 2, 17, 64, 8, 0, 8) == 0
+    assert need(2, 2, 3, 64, 8, 0, 0, 1 << 20) > 0 and need(0, 2, 3, 64, 8, 0, 0, 1 << 20) == 0
+    assert need(2, 2, 17, 64, 8, 0, 0, 1 << 20) == 0
+    # where no segment can be long, none is divided
+    assert need(2, 2, 3, 64, 8, 0, 0, 8) == 0 and need(2, 2, 3, 64, 8, 0, 300, 1 << 20) == 0
+    assert need(2, 2, 3, 64, 8, 300, 0, 1 << 20) == 0 and need(2, 2, 3, 64, 8, 30000, 30000, 1 << 20) > 0

@@ -27,6 +27,8 @@
 // number of segments fill the card evenly; a workgroup meets the segments of its
 // range one after another.  A segment inside its range is finished there; the
 // others' parts (at most two per workgroup) are joined by a second launch.
+#include <algorithm>
+
 #include "vtx_device.h"
 #include "vtx_host.h"
 #include "vtx_quant.h"
@@ -74,11 +76,12 @@ struct QAttnArgs {
   const float* slopes;  // [H * G], or null
   int64_t q_batch, q_kv, q_head;  // strides in elements
   int32_t segments, H, G, P, p_shift;
-  Divisor by_segments, by_heads, by_workers, by_cus;
+  Divisor by_segments, by_heads, by_workers, by_cus, by_least, by_pitch;
   int32_t window;  // the last tokens that count; 0: all
+  int32_t pitch;   // places of a segment on a spaced line; 0: the line is another
   float c;         // scale log2 e; with a cap 2 scale log2 e / cap
   float cap;       // cap log2 e, or 0
-  int32_t workers, least;  // ranges at most, pages of one at least; workers 0: a segment each, whole
+  int32_t workers, least;  // ranges at most, pages of one at least; workers 0: a workgroup per segment
   float* acc;       // [2 workers, G, D]
   float2* ml;       // [2 workers, G]
   int32_t* places;  // [segments + 1], of a packed line
@@ -97,8 +100,11 @@ struct Line {
 };
 __device__ __forceinline__ Line line_of(const QAttnArgs& a, uint32_t total) {
   Line l{total, divide(total + (uint32_t)a.workers - 1u, a.by_workers)};
-  if (l.per < (uint32_t)a.least) l.per = (uint32_t)a.least;
   const uint32_t S = (uint32_t)a.segments, m = divide(total, a.by_segments);
+  // whole tiles of all waves, but no segments one after another where they are short
+  const uint32_t mean = m + (m * S < total ? 1u : 0u), least = (uint32_t)a.least;
+  if (mean < least) l.per = l.per < mean ? mean : l.per;
+  else l.per = divide(l.per + least - 1u, a.by_least) * least;
   if (m > 0 && m * S == total) {
     // ranges of a segment, or segments of a range
     const uint32_t many = m >= l.per ? m / l.per : (l.per - 1u) / m + 1u;
@@ -169,14 +175,30 @@ __device__ __forceinline__ int segments_before(int S, int first, uint32_t v0, Bo
   }
 }
 
-// What a wave holds of 16 query heads: their fragments, running maximum (base 2),
-// sum (of this lane's tokens) and output.
-template <int kD, bool kHalf>
+// What a wave holds of 16 query heads: running maximum (base 2), sum (of this
+// lane's tokens) and output.
+template <int kD>
 struct Heads {
-  vtx::U4 q[kD / 32];
-  vtx::U4 ql[kHalf ? kD / 32 : 1];  // what bf16 left of fp16 queries
   float m, l;
   f32x4 o[kD / 16];
+};
+
+// The heads' fragments: bf16 ones in registers, a copy in every wave; fp16 ones,
+// twice as many, in LDS, one copy for all waves (in registers they spilled: 128
+// columns, 32 requests of up to 8k tokens 77 us, so 66; bf16 ones in LDS cost 1 us
+// of 65).  After the tiles the waves' outputs take their place there.
+template <int kD, bool kHalf>
+struct Queries {
+  static constexpr int kOwn = kHalf ? (kD / 32 + kWaves - 1) / kWaves : kD / 32;  // of a wave
+  vtx::U4 raw[kOwn];
+};
+template <int kD, bool kHalf>
+struct Shared {
+  static constexpr int kOut = kD + 4;  // floats of a head's outputs: 16 heads' pieces in all banks
+  union {
+    vtx::U4 q[kHalf ? 2 : 1][kHalf ? kD / 32 : 1][vtx::kWave];  // rounded to bf16, and what that left
+    float o[kWaves][kHeads][kOut];
+  };
 };
 
 // 32 tokens' keys on their way, and their values and factors.
@@ -239,26 +261,36 @@ constexpr float kGrowth = 8.f;
 
 // Scores of 32 tokens, without their factors.
 template <int kD, int kCodes, bool kHalf>
-__device__ __forceinline__ void score(const Heads<kD, kHalf>& w, const Keys<kD>& t, f32x4 (&s)[2]) {
+__device__ __forceinline__ void score(const Shared<kD, kHalf>& sh, const Queries<kD, kHalf>& own, const Keys<kD>& t,
+                                      f32x4 (&s)[2]) {
+  int lane = vtx::lane_id();
+  if constexpr (kHalf) asm volatile("" : "+v"(lane));  // (read for every tile: kept out of the registers)
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int h = 0; h < 2; ++h) s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < kD / 64; ++j) {
+  for (int j = 0; j < kD / 64; ++j) {
+    vtx::U4 q[kHalf ? 4 : 2];
+#pragma unroll
+    for (int e = 0; e < (kHalf ? 4 : 2); ++e) {
+      if constexpr (kHalf) q[e] = sh.q[e / 2][2 * j + e % 2][lane];
+      else q[e] = own.raw[2 * j + e];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
       vtx::U4 f0, f1;
       vtx::decode_pairs<kCodes>(t.k[h][j].x, f0.x, f0.y);
       vtx::decode_pairs<kCodes>(t.k[h][j].y, f0.z, f0.w);
       vtx::decode_pairs<kCodes>(t.k[h][j].z, f1.x, f1.y);
       vtx::decode_pairs<kCodes>(t.k[h][j].w, f1.z, f1.w);
-      auto mul = [&](const vtx::U4& k, const vtx::U4& q) {
-        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q),
+      auto mul = [&](const vtx::U4& k, const vtx::U4& x) {
+        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, x),
                                                        s[h], 0, 0, 0);
       };
-      mul(f0, w.q[2 * j]);
-      mul(f1, w.q[2 * j + 1]);
+      mul(f0, q[0]);
+      mul(f1, q[1]);
       if constexpr (kHalf) {
-        mul(f0, w.ql[2 * j]);
-        mul(f1, w.ql[2 * j + 1]);
+        mul(f0, q[2]);
+        mul(f1, q[3]);
       }
     }
   }
@@ -266,8 +298,8 @@ __device__ __forceinline__ void score(const Heads<kD, kHalf>& w, const Keys<kD>&
 
 // Their weights, and the values by these.  bad: tokens of this lane that do not
 // count (where masked); far: the distance of its first one; slope: base 2.
-template <int kD, int kCodes, bool kHalf>
-__device__ __forceinline__ void attend(const QAttnArgs& a, Heads<kD, kHalf>& w, const f32x4 (&s)[2], Values<kD>& t,
+template <int kD, int kCodes>
+__device__ __forceinline__ void attend(const QAttnArgs& a, Heads<kD>& w, const f32x4 (&s)[2], Values<kD>& t,
                                        bool masked, uint32_t bad, float far, float slope) {
   if (masked) {  // uniform
     // tokens that do not count may be anything, NaN too: their values become zeros
@@ -374,12 +406,15 @@ __device__ __forceinline__ uint32_t round2(float a, float b) {
 // The result of sums O and L: zeros where nothing was seen, NaN where a score was.
 __device__ __forceinline__ float inverse_sum(float L) { return L > 0.f ? 1.f / L : (L == 0.f ? 0.f : NAN); }
 
+// Workgroups of a compute unit: as many as the registers let in.
+template <int kD>
+constexpr int kPerCu = kD == 256 ? 2 : (kD == 128 ? 3 : 4);
+
 template <int kD, int kCodes, bool kHalf, bool kPages16>
-__global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_kernel(QAttnArgs a) {
-  constexpr int kOut = kD + 4;  // floats of a head's outputs in LDS: 16 heads' pieces in all banks
+__global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(QAttnArgs a) {
   __shared__ int32_t s_ptr[kBounds], s_last[kBounds], s_rows[kStage];
   __shared__ float s_m[kWaves][kHeads], s_l[kWaves][kHeads];
-  __shared__ alignas(16) float s_o[kWaves][kHeads][kOut];
+  __shared__ alignas(16) Shared<kD, kHalf> sh;
 
   const int tid = threadIdx.x, lane = vtx::lane_id();
   const int wave = vtx::uniform(tid / vtx::kWave);
@@ -387,9 +422,9 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
   const int S = a.segments, G = a.G, P = a.P;
 
   // This workgroup's range of the line, and its first segment.  How the line is laid
-  // out: the table's own pages (also with a window where the table has too many
-  // segments for a sum over all of them: pages before the windows are passed over);
-  // with a window the pages that count, closely packed.  A table of few segments is
+  // out: the table's own pages; with a window the pages that count, closely packed,
+  // or where the segments are too many for a sum over all of them at equal distances
+  // (segments shorter than the window leave gaps).  A table of few segments is
   // brought to LDS whole, so that all its bounds cost one trip.
   int first = 0, seg = (int)blockIdx.x;
   uint32_t total = 0, v0 = 0, v1 = 1;
@@ -434,6 +469,8 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
       __syncthreads();
       first = vtx::uniform(s_ptr[0]);
       total = table_pages(a, first, vtx::uniform(s_ptr[S]));
+    } else if (a.pitch > 0) {
+      total = (uint32_t)S * (uint32_t)a.pitch;  // (the host sees to it that this fits)
     } else {
       first = a.indptr[0];
       total = table_pages(a, first, a.indptr[S]);
@@ -444,6 +481,7 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
     v0 = (uint32_t)at;
     v1 = total - v0 < l.per ? total : v0 + l.per;
     if (few) seg = segments_before(S, first, v0, [&](int j) { return s_ptr[j]; });
+    else if (a.pitch > 0) seg = (int)divide(v0, a.by_pitch);
     else seg = segments_before(S, first, v0, [&](int j) { return a.indptr[j]; });
   }
 
@@ -482,9 +520,11 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
         p.part = false;
         break;
       }
-      const uint32_t begin = packed ? (uint32_t)vtx::uniform(s_ptr[s]) : (uint32_t)p0 - (uint32_t)first;
-      if (begin >= v1 && (packed || p0 > first)) break;
-      const Place l = place_of(p.s, packed ? begin : (uint32_t)p.s.start - (uint32_t)first, total);
+      const bool laid = packed || a.pitch > 0;  // elsewhere than in the table
+      const uint32_t begin = packed ? (uint32_t)vtx::uniform(s_ptr[s])
+                                    : (laid ? (uint32_t)s * (uint32_t)a.pitch : (uint32_t)p0 - (uint32_t)first);
+      if (begin >= v1 && (laid || p0 > first)) break;
+      const Place l = place_of(p.s, laid ? begin : (uint32_t)p.s.start - (uint32_t)first, total);
       const uint32_t x = l.at > v0 ? l.at : v0, y = l.end < v1 ? l.end : v1;
       if (x >= y) continue;  // (the join writes an empty segment's zeros)
       p.at = l.at;
@@ -504,10 +544,11 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
     int s = p.seg;
     for (uint32_t v = from + tid; v < staged_end; v += kThreads) {
       int64_t at = whole ? (int64_t)p.s.start + v : (int64_t)first + v;
-      if (packed) {
-        while (s + 1 < S && (uint32_t)s_ptr[s + 1] <= v) ++s;
+      if (packed || a.pitch > 0) {
+        while (packed && s + 1 < S && (uint32_t)s_ptr[s + 1] <= v) ++s;
+        if (!packed) s = (int)divide(v, a.by_pitch);
         const Segment g = s == p.seg ? p.s : segment_of(a, a.indptr[s], a.indptr[s + 1], a.last_len[s]);
-        at = (int64_t)g.start + (v - (uint32_t)s_ptr[s]);
+        at = (int64_t)g.start + (v - (packed ? (uint32_t)s_ptr[s] : (uint32_t)s * (uint32_t)a.pitch));
       }
       const int r = at >= 0 && at < a.indices_len ? a.indices[at] : -1;
       s_rows[v - from] = r >= 0 && r < a.rows ? r : -1;
@@ -543,21 +584,81 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
     return Half{(long long)r * P + (t0 - pg * P), t0 < t.n && r >= 0 ? min(t.n - t0, 16) : 0};
   };
 
-  for (Piece cur = piece_from(seg); cur.seg < S; cur = piece_from(cur.seg + 1)) {
-    const int b = (int)divide((uint32_t)cur.seg, a.by_heads), h = cur.seg - b * a.H;
-    Heads<kD, kHalf> w;
+  Half half[2];  // of the tile on its way
+  Keys<kD> keys;
+  Values<kD> values;
+  auto aim = [&](const Stretch& t, int i) {
+    half[0] = half_of(t, i, 0);
+    half[1] = half_of(t, i, 1);
+  };
+  auto load_keys = [&]() {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const auto r = buffer_of(a.k + half[hf].row * kD, (uint32_t)half[hf].tokens * kD);
+#pragma unroll
+      for (int j = 0; j < kD / 64; ++j) {
+        uint32_t x[4];
+        load_words<4>(r, c16 * kD + g4 * 16 + j * 64, x);
+        keys.k[hf][j] = vtx::U4{x[0], x[1], x[2], x[3]};
+      }
+    }
+  };
+  auto load_values = [&]() {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      uint32_t x[2];
+      // (all 16 slots': a load that reaches past the end gives nothing at all)
+      load_words<2>(buffer_of(a.scales + half[hf].row * 2, half[hf].tokens > 0 ? 32u : 0u), g4 * 8, x);
+      values.sc[hf] = uint2{x[0], x[1]};
+      const auto r = buffer_of(a.v + half[hf].row * kD, (uint32_t)half[hf].tokens * kD);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) load_words<kD / 64>(r, 4 * g4 * kD + c16 * (kD / 16) + u * kD, values.v[hf][u]);
+    }
+  };
+  // a segment's query rows; heads past G take head 0's, and nobody takes their results
+  Queries<kD, kHalf> own;
+  float slope = 0.f;
+  auto load_queries = [&](int s) {
+    const int b = (int)divide((uint32_t)s, a.by_heads), h = s - b * a.H;
+    const uint16_t* q = a.q + b * a.q_batch + h * a.q_kv + (c16 < G ? c16 : 0) * a.q_head + g4 * 16;
+#pragma unroll
+    for (int i = 0; i < Queries<kD, kHalf>::kOwn; ++i) {
+      const int j = kHalf ? min(i * kWaves + wave, kD / 32 - 1) : i;
+      own.raw[i] = vtx::ld16(q + (j / 2) * 64 + (j % 2) * 8);
+    }
+    if (a.slopes) slope = a.slopes[h * G + (c16 < G ? c16 : 0)] * kLog2e;
+  };
+
+  Piece cur = piece_from(seg);
+  if (cur.seg >= S) return;  // uniform
+  load_queries(cur.seg);
+  bool ready = false;  // this wave's first tile of the segment is on its way
+  while (true) {
+    if constexpr (kHalf) {  // fp16 values as two bf16 ones, to LDS
+#pragma unroll
+      for (int i = 0; i < Queries<kD, kHalf>::kOwn; ++i) {
+        const int j = i * kWaves + wave;
+        if (j >= kD / 32) break;  // uniform
+        typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+        const f16x8 f = __builtin_bit_cast(f16x8, own.raw[i]);
+        uint32_t x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float u = (float)f[2 * e], v = (float)f[2 * e + 1];
+          x[e] = vtx::bf16_pair(u, v);
+          y[e] = vtx::bf16_pair(u - vtx::bf16_lo(x[e]), v - vtx::bf16_hi(x[e]));
+        }
+        sh.q[0][j][lane] = vtx::U4{x[0], x[1], x[2], x[3]};
+        sh.q[1][j][lane] = vtx::U4{y[0], y[1], y[2], y[3]};
+      }
+      // (where no staging with its barrier comes before the tiles)
+      if (stretch_of(cur, cur.pa).pages > 0) __syncthreads();
+    }
+    Heads<kD> w;
     w.m = -INFINITY;
     w.l = 0.f;
 #pragma unroll
     for (int d = 0; d < kD / 16; ++d) w.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // its query rows; heads past G take head 0's, and nobody takes their results
-    {
-      const uint16_t* q = a.q + b * a.q_batch + h * a.q_kv + (c16 < G ? c16 : 0) * a.q_head + g4 * 16;
-#pragma unroll
-      for (int j = 0; j < kD / 32; ++j) w.q[j] = vtx::ld16(q + (j / 2) * 64 + (j % 2) * 8);
-    }
-    const float slope = a.slopes ? a.slopes[h * G + (c16 < G ? c16 : 0)] * kLog2e : 0.f;
-
     for (int pc = cur.pa; pc < cur.pb;) {
       Stretch st = stretch_of(cur, pc);
       if (st.pages == 0) {  // uniform
@@ -568,66 +669,20 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
       const int skip = pc == 0 ? cur.s.skip : 0;
       const int tiles = (st.n + kTile - 1) / kTile;
       const float far0 = (float)(cur.s.tokens - 1 - pc * P - 4 * g4);
-      if constexpr (kHalf) {
-        if (pc == cur.pa) {  // fp16 queries as two bf16 values each
-#pragma unroll
-          for (int j = 0; j < kD / 32; ++j) {
-            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-            const f16x8 f = __builtin_bit_cast(f16x8, w.q[j]);
-            uint32_t x[4], y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float u = (float)f[2 * e], v = (float)f[2 * e + 1];
-              x[e] = vtx::bf16_pair(u, v);
-              y[e] = vtx::bf16_pair(u - vtx::bf16_lo(x[e]), v - vtx::bf16_hi(x[e]));
-            }
-            w.q[j] = vtx::U4{x[0], x[1], x[2], x[3]};
-            w.ql[j] = vtx::U4{y[0], y[1], y[2], y[3]};
-          }
-        }
-      }
       pc += st.pages;
 
       if constexpr (kPages16) {
-        Half half[2];
-        Keys<kD> keys;
-        Values<kD> values;
-        auto aim = [&](int i) {
-          half[0] = half_of(st, i, 0);
-          half[1] = half_of(st, i, 1);
-        };
-        auto load_keys = [&]() {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const auto r = buffer_of(a.k + half[hf].row * kD, (uint32_t)half[hf].tokens * kD);
-#pragma unroll
-            for (int j = 0; j < kD / 64; ++j) {
-              uint32_t x[4];
-              load_words<4>(r, c16 * kD + g4 * 16 + j * 64, x);
-              keys.k[hf][j] = vtx::U4{x[0], x[1], x[2], x[3]};
-            }
-          }
-        };
-        auto load_values = [&]() {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t x[2];
-            // (all 16 slots': a load that reaches past the end gives nothing at all)
-            load_words<2>(buffer_of(a.scales + half[hf].row * 2, half[hf].tokens > 0 ? 32u : 0u), g4 * 8, x);
-            values.sc[hf] = uint2{x[0], x[1]};
-            const auto r = buffer_of(a.v + half[hf].row * kD, (uint32_t)half[hf].tokens * kD);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) load_words<kD / 64>(r, 4 * g4 * kD + c16 * (kD / 16) + u * kD, values.v[hf][u]);
-          }
-        };
-        aim(wave);
-        load_keys();
-        load_values();
+        if (!ready) {  // uniform
+          aim(st, wave);
+          load_keys();
+          load_values();
+        }
+        ready = false;
         for (int i = wave; i < tiles; i += kWaves) {
           f32x4 sc[2];
-          score<kD, kCodes, kHalf>(w, keys, sc);
+          score<kD, kCodes, kHalf>(sh, own, keys, sc);
           const int n0 = half[0].tokens, n1 = half[1].tokens;
-          aim(i + kWaves);  // (none past the last: no loads)
+          aim(st, i + kWaves);  // (none past the last: no loads)
           load_keys();
           const int out = skip - i * kTile;  // tokens before the window
           uint32_t bad = 0;
@@ -639,7 +694,7 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
               bad |= 4 * g4 + x >= n1 || 16 + 4 * g4 + x < out ? 16u << x : 0u;
             }
           }
-          attend<kD, kCodes, kHalf>(a, w, sc, values, masked, bad, far0 - (float)(i * kTile), slope);
+          attend<kD, kCodes>(a, w, sc, values, masked, bad, far0 - (float)(i * kTile), slope);
           load_values();
         }
       } else {
@@ -652,8 +707,6 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
           return ok ? (long long)r * P + (tok - pg * P) : 0LL;
         };
         for (int i = wave; i < tiles; i += kWaves) {
-          Keys<kD> keys;
-          Values<kD> values;
           uint32_t bad = 0;
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
@@ -673,8 +726,25 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
             values.sc[hf] = uint2{two[0] | (two[1] << 16), two[2] | (two[3] << 16)};
           }
           f32x4 sc[2];
-          score<kD, kCodes, kHalf>(w, keys, sc);
-          attend<kD, kCodes, kHalf>(a, w, sc, values, __ballot(bad != 0) != 0, bad, far0 - (float)(i * kTile), slope);
+          score<kD, kCodes, kHalf>(sh, own, keys, sc);
+          attend<kD, kCodes>(a, w, sc, values, __ballot(bad != 0) != 0, bad, far0 - (float)(i * kTile), slope);
+        }
+      }
+    }
+
+    // the next segment's queries and first tiles, requested before this one's end
+    Piece nxt;
+    nxt.seg = S;
+    if (!whole) nxt = piece_from(cur.seg + 1);
+    if (nxt.seg < S) {  // uniform
+      load_queries(nxt.seg);
+      if constexpr (kPages16) {
+        const Stretch t = stretch_of(nxt, nxt.pa);
+        ready = t.pages > 0;
+        if (ready) {
+          aim(t, wave);
+          load_keys();
+          load_values();
         }
       }
     }
@@ -685,6 +755,7 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
     // (a maximum passes NaN scores by; where nothing else was seen it is still
     // -inf, which the joins take for no tokens)
     const float m = l != l ? 0.f : w.m;
+    if constexpr (kHalf) __syncthreads();  // (the queries are done with)
     if (c16 < G) {
       if (g4 == 0) {
         s_m[wave][c16] = m;
@@ -694,7 +765,7 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int x4 = 0; x4 < kD / 64; ++x4)
-          *reinterpret_cast<float4*>(&s_o[wave][c16][(4 * g4 + i) * (kD / 16) + 4 * x4]) =
+          *reinterpret_cast<float4*>(&sh.o[wave][c16][(4 * g4 + i) * (kD / 16) + 4 * x4]) =
               float4{w.o[4 * x4][i], w.o[4 * x4 + 1][i], w.o[4 * x4 + 2][i], w.o[4 * x4 + 3][i]};
     }
     __syncthreads();
@@ -708,7 +779,7 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) {
           const float f = __builtin_amdgcn_exp2f(s_m[i][g] - M);
-          const float4 y = *reinterpret_cast<const float4*>(&s_o[i][g][d]);
+          const float4 y = *reinterpret_cast<const float4*>(&sh.o[i][g][d]);
           L = fmaf(s_l[i][g], f, L);
           O = float4{fmaf(y.x, f, O.x), fmaf(y.y, f, O.y), fmaf(y.z, f, O.z), fmaf(y.w, f, O.w)};
         }
@@ -723,8 +794,9 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void quant_attention_k
             uint2{round2<kHalf>(O.x * f, O.y * f), round2<kHalf>(O.z * f, O.w * f)};
       }
     }
-    if (whole) return;  // uniform
-    __syncthreads();    // (the next segment's results go to the same place)
+    if (nxt.seg >= S) return;  // uniform
+    __syncthreads();           // (the next segment's results go to the same place)
+    cur = nxt;
   }
 }
 
@@ -739,10 +811,14 @@ __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAtt
   __shared__ float2 s_ml[kJoinThreads];
   const int seg = blockIdx.x, tid = threadIdx.x, G = a.G, S = a.segments;
   const bool packed = S < kBounds && a.window > 0;
-  const int first = packed ? 0 : a.indptr[0];
-  const uint32_t total = packed ? (uint32_t)a.places[S] : table_pages(a, first, a.indptr[S]);
+  const int first = a.indptr[0];
+  const uint32_t total = packed ? (uint32_t)a.places[S]
+                                : (a.pitch > 0 ? (uint32_t)S * (uint32_t)a.pitch : table_pages(a, first, a.indptr[S]));
   const Segment sg = segment_of(a, a.indptr[seg], a.indptr[seg + 1], a.last_len[seg]);
-  const Place at = place_of(sg, packed ? (uint32_t)a.places[seg] : (uint32_t)sg.start - (uint32_t)first, total);
+  const uint32_t begin = packed        ? (uint32_t)a.places[seg]
+                         : a.pitch > 0 ? (uint32_t)seg * (uint32_t)a.pitch
+                                       : (uint32_t)sg.start - (uint32_t)first;
+  const Place at = place_of(sg, begin, total);
   const Line l = line_of(a, total);
   uint32_t w0 = 0;
   int n = 0;
@@ -836,22 +912,46 @@ int launch_types(const QAttnArgs& a, int codes, bool half, hipStream_t s) {
 }
 
 // Ranges of a call: as many workgroups as the card holds at once, and no more
-// than the buffer's pages can fill.
+// than the buffer's pages can fill; or none, a workgroup per segment and one
+// launch, where no segment can be long.  known: tokens that no segment exceeds
+// (the window, the caller's word; 0: unknown).
+//
+// Segments of up to `few` tokens, by the buffer's size if all heads of a request
+// are alike: ranges / segments, 8 segments of 128 columns, 128 tokens 9.0 / 6.1 us,
+// 512 10.9 / 10.3, 768 11.1 / 13.1; 64 columns, 512 10.2 / 8.6, 768 10.4 / 10.7; 256
+// columns, 256 12.0 / 9.2, 512 12.3 / 13.3.  Known bounds: segments that fill the
+// card even out by themselves (512 of 128 columns, windows of 512 29 / 19, of 4096
+// 92 / 89; 256 of 2048 36 / 33, of 4096 52 / 57), and with a window the line costs
+// more to lay out (128 of 1024 22 / 19, of 2048 27 / 30; 256 columns, 64 of 768 22 /
+// 20, of 1024 22 / 24).
 struct Ranges {
-  long long workers, least, cus;
+  long long workers, least, cus, pitch;
 };
-Ranges ranges_of(int32_t head_dim, int32_t page_size, long long indices_len) {
-  Ranges r;
+Ranges ranges_of(long long segments, int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t window,
+                 int32_t longest, long long indices_len) {
+  Ranges r{0, 1, 1, 0};
   r.cus = vtx::device_cu_count() > 0 ? vtx::device_cu_count() : 256;
+  const long long few = 640 - head_dim;
+  const long long known = longest > 0 && (window == 0 || longest < window) ? longest : window;
+  const long long most = segments >= 2 * r.cus ? 4096
+                         : segments >= r.cus   ? 2048
+                         : window > 0          ? (head_dim == 256 ? 768 : 1024)
+                                               : few;
+  if (indices_len * page_size <= few * num_kv_heads || (known > 0 && known <= most)) return r;
   r.least = (kMinTokens + (long long)page_size - 1) / page_size;
-  r.workers = r.cus * (head_dim == 256 ? 2 : 3);
-  const long long need = (indices_len + r.least - 1) / r.least;
+  r.workers = r.cus * (head_dim == 256 ? kPerCu<256> : (head_dim == 128 ? kPerCu<128> : kPerCu<64>));
+  r.pitch = 0;
+  if (window > 0 && segments >= kBounds) {
+    const long long most = ((long long)window + page_size - 1) / page_size + 1;  // pages that a window touches
+    if (most * segments <= 0x7fffffffLL) r.pitch = most;
+  }
+  const long long need = std::max(segments, (indices_len + r.least - 1) / r.least);
   if (r.workers > need) r.workers = need;
-  if (r.workers < 1) r.workers = 1;
   return r;
 }
 // Floats of scratch: two parts a range, and a packed line's places.
 long long scratch_of(const Ranges& r, long long segments, int32_t group_size, int32_t head_dim, int32_t window) {
+  if (r.workers == 0) return 0;
   return 2 * r.workers * group_size * (head_dim + 2) + (window > 0 && segments < kBounds ? segments + 1 : 0);
 }
 
@@ -863,12 +963,13 @@ extern "C" int vtx_quant_decode_attention_supported(int32_t head_dim, int32_t gr
 
 extern "C" int64_t vtx_quant_decode_attention_workspace_len(int32_t batch_size, int32_t num_kv_heads,
                                                             int32_t group_size, int32_t head_dim, int32_t page_size,
-                                                            int32_t window, int64_t kv_indices_len) {
-  if (batch_size < 1 || num_kv_heads < 1 || page_size < 1 || window < 0 || kv_indices_len < 0 ||
+                                                            int32_t window, int32_t longest, int64_t kv_indices_len) {
+  if (batch_size < 1 || num_kv_heads < 1 || page_size < 1 || window < 0 || longest < 0 || kv_indices_len < 0 ||
       !vtx_quant_decode_attention_supported(head_dim, group_size))
     return 0;
-  return scratch_of(ranges_of(head_dim, page_size, kv_indices_len), (long long)batch_size * num_kv_heads, group_size,
-                    head_dim, window);
+  const long long segments = (long long)batch_size * num_kv_heads;
+  return scratch_of(ranges_of(segments, num_kv_heads, head_dim, page_size, window, longest, kv_indices_len), segments,
+                    group_size, head_dim, window);
 }
 
 extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_strides, void* o, const void* k_cache,
@@ -877,9 +978,11 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
                                           const int32_t* kv_last_page_len, int32_t batch_size, int32_t num_kv_heads,
                                           int32_t group_size, int32_t head_dim, int32_t page_size, int32_t dtype,
                                           int32_t codes, float sm_scale, float soft_cap, int32_t window,
-                                          const float* slopes, float* workspace, int64_t workspace_len, void* stream) {
+                                          const float* slopes, int32_t longest, float* workspace,
+                                          int64_t workspace_len, void* stream) {
   vtx::clear_error();
-  if (batch_size < 0 || num_kv_heads < 1 || page_size < 1 || cache_rows < 0 || kv_indices_len < 0 || window < 0)
+  if (batch_size < 0 || num_kv_heads < 1 || page_size < 1 || cache_rows < 0 || kv_indices_len < 0 || window < 0 ||
+      longest < 0)
     return vtx::fail(VTX_E_INVALID, "quant_decode_attention: bad sizes");
   if (!vtx_quant_decode_attention_supported(head_dim, group_size))
     return vtx::fail(VTX_E_INVALID, "quant_decode_attention: head_dim %d with %d query heads per kv head not supported",
@@ -929,21 +1032,25 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
   a.least = 1;
   a.by_segments = divisor(segments);
   a.by_heads = divisor(num_kv_heads);
-  a.by_workers = a.by_cus = divisor(1);
+  a.by_workers = a.by_cus = a.by_least = a.by_pitch = divisor(1);
+  a.pitch = 0;
   a.acc = nullptr;
   a.ml = nullptr;
   a.places = nullptr;
   if (workspace) {
-    const Ranges r = ranges_of(head_dim, page_size, kv_indices_len);
+    const Ranges r = ranges_of(segments, num_kv_heads, head_dim, page_size, window, longest, kv_indices_len);
     const long long parts = 2 * r.workers * group_size, need = scratch_of(r, segments, group_size, head_dim, window);
     if (workspace_len < need || !vtx::aligned16(workspace))
       return vtx::fail(VTX_E_INVALID,
                        "quant_decode_attention: workspace of %lld floats (16-byte aligned) needed, got %lld", need,
                        (long long)workspace_len);
-    a.workers = (int32_t)r.workers;
+    a.workers = (int32_t)r.workers;  // (0: as without a workspace)
     a.least = (int32_t)r.least;
-    a.by_workers = divisor(r.workers);
+    a.by_workers = divisor(r.workers > 0 ? r.workers : 1);
     a.by_cus = divisor(r.cus);
+    a.by_least = divisor(r.least);
+    a.pitch = (int32_t)r.pitch;
+    if (r.pitch > 0) a.by_pitch = divisor(r.pitch);
     a.acc = workspace;
     a.ml = reinterpret_cast<float2*>(workspace + parts * head_dim);
     a.places = reinterpret_cast<int32_t*>(workspace + parts * (head_dim + 2));

@@ -166,10 +166,10 @@ _SIGNATURES = {
         ctypes.c_int,
     ),
     "vtx_quant_decode_attention_supported": ([_i32, _i32], ctypes.c_int),
-    "vtx_quant_decode_attention_workspace_len": ([_i32, _i32, _i32, _i32, _i32, _i32, _i64], ctypes.c_int64),
+    "vtx_quant_decode_attention_workspace_len": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64], ctypes.c_int64),
     "vtx_quant_decode_attention": (
         [_vp, ctypes.POINTER(_i64), _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
-         _i32, ctypes.c_float, ctypes.c_float, _i32, _vp, _vp, _i64, _vp],
+         _i32, ctypes.c_float, ctypes.c_float, _i32, _vp, _i32, _vp, _i64, _vp],
         ctypes.c_int,
     ),
     "vtx_bf16_rounding_check": ([_vp, _vp], ctypes.c_int),
@@ -1729,12 +1729,13 @@ def _quant_attention_refusal(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_in
 
 @_plain_positional
 def quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, batch_size,
-                                 num_kv_heads, sm_scale, soft_cap, window, slopes):
+                                 num_kv_heads, sm_scale, soft_cap, window, slopes, longest):
     """paged_decode_attention over 8-bit pools, with capped scores, a window or
-    slopes, into o (None: a new tensor); returns it.  The table's pages are
-    divided over the card with scratch from torch's allocator, whose
-    OutOfMemoryError is the caller's; in a capture that torch did not begin no
-    scratch lasts, and every segment has a workgroup."""
+    slopes, into o (None: a new tensor); returns it.  longest: tokens that no
+    segment exceeds (0: unknown).  The table's pages are divided over the card
+    with scratch from torch's allocator, whose OutOfMemoryError is the caller's;
+    where segments are short, and in a capture that torch did not begin, in which
+    no scratch lasts, every segment has a workgroup."""
     lib = _lib or load_library()
     if o is None:
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -1746,7 +1747,7 @@ def quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, k
         with _on_device(torch.device("cuda", index)):
             return quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices,
                                                 kv_last_page_len, batch_size, num_kv_heads, sm_scale, soft_cap, window,
-                                                slopes)
+                                                slopes, longest)
     B, H = batch_size, num_kv_heads
     if not _quant_attention_fits(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B, H,
                                  soft_cap, window, slopes):
@@ -1766,7 +1767,7 @@ def quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, k
         s1 = 0
     strides = _ThreeI64(s0, G * s1, s1) if n0 == B and n1 != G else _ThreeI64(H * s0, s0, s1)
     stream, entries = _stream_of(index), kv_indices.numel()
-    floats = lib.vtx_quant_decode_attention_workspace_len(B, H, G, D, P, window, entries)
+    floats = lib.vtx_quant_decode_attention_workspace_len(B, H, G, D, P, window, longest, entries)
     ws = None
     if floats > 0 and _scratch_lasts(stream):
         ws = torch.empty(floats, dtype=torch.float32, device=q.device)
@@ -1774,7 +1775,7 @@ def quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, k
         q.data_ptr(), strides, o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(), rows,
         kv_indptr.data_ptr(), kv_indices.data_ptr(), entries, kv_last_page_len.data_ptr(), B, H, G, D, P,
         _QUERY_DTYPES[q.dtype], _CODES[k_cache.dtype], sm_scale, soft_cap, window,
-        None if slopes is None else slopes.data_ptr(), None if ws is None else ws.data_ptr(), floats, stream)
+        None if slopes is None else slopes.data_ptr(), longest, None if ws is None else ws.data_ptr(), floats, stream)
     if rc:
         _check(rc, "quant_paged_decode_attention")
     return o

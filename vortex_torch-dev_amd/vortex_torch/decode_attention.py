@@ -126,7 +126,8 @@ def quant_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache
                                  kv_last_page_len: torch.Tensor, batch_size: int, num_kv_heads: int,
                                  sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                                  logits_soft_cap: Optional[float] = None, window: Optional[int] = None,
-                                 slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+                                 slopes: Optional[torch.Tensor] = None,
+                                 max_tokens: Optional[int] = None) -> torch.Tensor:
     """``paged_decode_attention`` over 8-bit pools and their ``kv_scales``
     (``cache.set_kv_buffer_quant``); q [B, H_q, D] or [B * H_kv, G, D], bf16 or
     fp16, its rows dense, up to 16 query heads per kv head; returns q's type.
@@ -134,19 +135,24 @@ def quant_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache
     ``logits_soft_cap``: scores become cap * tanh(score / cap).  For tables in the
     tokens' order (dense ones): ``window``, only the last so many tokens count;
     ``slopes`` (fp32 [H_q]), the score of the token d before the newest one is
-    lowered by slope * d, after the cap."""
+    lowered by slope * d, after the cap.
+
+    ``max_tokens``: tokens that no request of the table has more of, where the
+    caller knows; it steers speed alone (short or many segments take one launch)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
     return _hip.quant_paged_decode_attention(q, out, k_cache, v_cache, kv_scales, kv_indptr, kv_indices,
                                              kv_last_page_len, int(batch_size), int(num_kv_heads), scale,
-                                             float(logits_soft_cap or 0.0), int(window or 0), slopes)
+                                             float(logits_soft_cap or 0.0), int(window or 0), slopes,
+                                             min(max(int(max_tokens or 0), 0), 0x7fffffff))
 
 
 def sparse_quant_decode_attention(q, k_cache, v_cache, kv_scales, ctx, sm_scale: Optional[float] = None, out=None,
                                   logits_soft_cap: Optional[float] = None):
     """Attention over the selected pages of an 8-bit cache (ctx's sparse table)."""
+    most = (ctx.topk_val + ctx.page_reserved_bos + ctx.page_reserved_eos) * ctx.page_size
     return quant_paged_decode_attention(q, k_cache, v_cache, kv_scales, ctx.sparse_kv_indptr, ctx.sparse_kv_indices,
                                         ctx.kv_last_page_len, ctx.batch_size, ctx.num_kv_heads, sm_scale, out,
-                                        logits_soft_cap)
+                                        logits_soft_cap, max_tokens=most)
 
 
 def dense_quant_decode_attention(q, k_cache, v_cache, kv_scales, ctx, sm_scale: Optional[float] = None, out=None,
