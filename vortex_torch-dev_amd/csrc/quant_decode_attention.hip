@@ -22,11 +22,15 @@
 //
 // 4 waves per workgroup, 32 tokens of a wave at a time; the next ones' keys are
 // requested behind the scores and their values behind the weighted sum, into the
-// registers that these leave.  The table's pages, all segments after one another,
-// are cut into equal ranges, a workgroup each, so that ragged lengths and any
-// number of segments fill the card evenly; a workgroup meets the segments of its
-// range one after another.  A segment inside its range is finished there; the
-// others' parts (at most two per workgroup) are joined by a second launch.
+// registers that these leave, and the next segment's first ones before the waves'
+// results are joined.  How a table's pages are divided among workgroups:
+// divide_pages; a segment that lies in several has its parts joined by a second
+// launch.
+//
+// Bound by HBM where there are many tokens (32 requests of up to 32k, 8 x 8 heads of
+// 128 columns, 213 us, 5.8 TB/s: the rate of a sequential read), by five dependent
+// trips to memory and the second launch where there are few (one request of 4096
+// tokens 11.9 us, of 128, in one launch, 6.1).
 #include <algorithm>
 
 #include "vtx_device.h"
@@ -76,44 +80,59 @@ struct QAttnArgs {
   const float* slopes;  // [H * G], or null
   int64_t q_batch, q_kv, q_head;  // strides in elements
   int32_t segments, H, G, P, p_shift;
-  Divisor by_segments, by_heads, by_workers, by_cus, by_least, by_pitch;
+  bool balanced;           // no compute unit has much more than its share of the segments
+  Divisor by_segments, by_heads, by_slots, by_cus, by_least, by_pitch;
   int32_t window;  // the last tokens that count; 0: all
   int32_t pitch;   // places of a segment on a spaced line; 0: the line is another
   float c;         // scale log2 e; with a cap 2 scale log2 e / cap
   float cap;       // cap log2 e, or 0
-  int32_t workers, least;  // ranges at most, pages of one at least; workers 0: a workgroup per segment
-  float* acc;       // [2 workers, G, D]
-  float2* ml;       // [2 workers, G]
+  int32_t workers, slots;  // workgroups (0: one per segment), and how many of them the card holds
+  int32_t least;           // pages of a range
+  float* acc;       // [2 slots, G, D]
+  float2* ml;       // [2 slots, G]
   int32_t* places;  // [segments + 1], of a packed line
 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// The line of pages and its ranges.  Where the pages divide evenly among the
-// segments (selected pages), a range is a whole number of segments or a whole part
-// of one if that costs the fullest compute unit no more than a quarter: fewer
-// parts to join, and a workgroup's waves start over less often (64 requests of 8
-// heads and 32 pages: 512 ranges of a segment each 20.5 us, 768 of 21.3 pages 27.9).
-struct Line {
-  uint32_t total, per;  // pages, pages of a range
+// How a table's pages are divided, from their total alone.
+//
+// Few long segments: all pages in a line, one segment's after another's, and a
+// range of the line for each workgroup that the card holds, whole tiles of all
+// waves; where the pages divide evenly among the segments a whole part of one, if
+// that costs the fullest compute unit no more than a quarter (fewer parts to join,
+// and a workgroup's waves start over less often).  A workgroup meets the segments
+// of its range one after another.
+//
+// Short segments, or many equal ones (chunk > 0): a workgroup each, and those longer
+// than a chunk, twice a workgroup's share and 1024 tokens at least, are cut into
+// equal parts, the first with that workgroup, the others with workgroups behind the
+// segments'.  Many uneven long ones stay on the line, which evens them out.
+// Line / chunks, 128 columns: 512 segments of up to 64 tokens 18.5 / 9.7 us, of up to
+// 1024 34.9 / 27.3, of up to 4096 66 / 75; 512 of 512 tokens each 21.2 / 20.0, 1024 of
+// 2048 109 / 96, 2048 of 512 62 / 56.
+struct Division {
+  uint32_t per;    // pages of a range
+  uint32_t chunk;  // pages of a part at most; 0: ranges
 };
-__device__ __forceinline__ Line line_of(const QAttnArgs& a, uint32_t total) {
-  Line l{total, divide(total + (uint32_t)a.workers - 1u, a.by_workers)};
+__device__ __forceinline__ Division divide_pages(const QAttnArgs& a, uint32_t total) {
+  const uint32_t even = divide(total + (uint32_t)a.slots - 1u, a.by_slots), least = (uint32_t)a.least;
   const uint32_t S = (uint32_t)a.segments, m = divide(total, a.by_segments);
-  // whole tiles of all waves, but no segments one after another where they are short
-  const uint32_t mean = m + (m * S < total ? 1u : 0u), least = (uint32_t)a.least;
-  if (mean < least) l.per = l.per < mean ? mean : l.per;
-  else l.per = divide(l.per + least - 1u, a.by_least) * least;
-  if (m > 0 && m * S == total) {
-    // ranges of a segment, or segments of a range
-    const uint32_t many = m >= l.per ? m / l.per : (l.per - 1u) / m + 1u;
-    const uint32_t per = m >= l.per ? (m - 1u) / many + 1u : m * many;
-    const uint32_t ranges = m >= l.per ? S * many : (S - 1u) / many + 1u;
-    const uint64_t fullest = (uint64_t)(divide(ranges - 1u, a.by_cus) + 1u) * per;
-    if (4 * fullest <= 5 * (uint64_t)(divide(total - 1u, a.by_cus) + 1u)) l.per = per;
+  const uint32_t mean = m + (m * S < total ? 1u : 0u);
+  if (mean < least || (mean < 2u * even && (mean <= 8u * least || (a.balanced && m * S == total))))
+    return Division{even, max(max(2u * even, 8u * least), mean)};
+  Division v{divide(max(even, least) + least - 1u, a.by_least) * least, 0u};
+  if (m >= v.per && m * S == total) {
+    const uint32_t many = m / v.per, per = (m - 1u) / many + 1u;  // ranges of a segment
+    const uint64_t fullest = (uint64_t)(divide(S * many - 1u, a.by_cus) + 1u) * per;
+    if (4 * fullest <= 5 * (uint64_t)(divide(total - 1u, a.by_cus) + 1u)) v.per = per;
   }
-  return l;
+  return v;
+}
+// Parts of a segment of so many pages.
+__device__ __forceinline__ uint32_t parts_of(int pages, uint32_t chunk) {
+  return (uint32_t)pages <= chunk ? 1u : ((uint32_t)pages - 1u) / chunk + 1u;
 }
 __device__ __forceinline__ uint32_t table_pages(const QAttnArgs& a, int first, int end) {
   const uint32_t all = end > first ? (uint32_t)end - (uint32_t)first : 0u, len = (uint32_t)a.indices_len;
@@ -153,6 +172,27 @@ struct Place {
 __device__ __forceinline__ Place place_of(const Segment& g, uint32_t at, uint32_t total) {
   const bool ok = g.pages > 0 && at < total && (uint32_t)g.pages <= total - at;
   return ok ? Place{at, at + (uint32_t)g.pages} : Place{0u, 0u};
+}
+
+__device__ __forceinline__ uint32_t parts_at(const QAttnArgs& a, int s, uint32_t chunk) {
+  return parts_of(segment_of(a, a.indptr[s], a.indptr[s + 1], a.last_len[s]).pages, chunk);
+}
+// The parts of the cut segments before segment s.  Every thread of the workgroup
+// calls it; sums: LDS, an entry per wave.
+template <int T>
+__device__ __forceinline__ uint32_t parts_before(const QAttnArgs& a, int s, uint32_t chunk, float* sums) {
+  uint32_t mine = 0;
+  for (int j = threadIdx.x; j < s; j += T) {
+    const uint32_t n = parts_at(a, j, chunk);
+    mine += n > 1u ? n : 0u;
+  }
+  mine = vtx::wave_sum(mine);
+  if (vtx::lane_id() == 0) sums[threadIdx.x / vtx::kWave] = __uint_as_float(mine);
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < T / vtx::kWave; ++i) all += __float_as_uint(sums[i]);
+  return (uint32_t)vtx::uniform((int)all);
 }
 
 // How many of the segments end at or before place v0 of the line, which is the
@@ -428,6 +468,9 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
   // brought to LDS whole, so that all its bounds cost one trip.
   int first = 0, seg = (int)blockIdx.x;
   uint32_t total = 0, v0 = 0, v1 = 1;
+  uint32_t chunk = 0;  // a segment's parts have at most so many pages (0: ranges of the line)
+  int nth = 0;         // which of them is this workgroup's
+  int part_row = 0;    // where its result goes
   const bool whole = a.workers == 0, few = !whole && S < kBounds, packed = few && a.window > 0;  // uniform
   if (!whole) {
     if (packed) {
@@ -475,16 +518,60 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
       first = a.indptr[0];
       total = table_pages(a, first, a.indptr[S]);
     }
-    const Line l = line_of(a, total);
-    const uint64_t at = (uint64_t)blockIdx.x * l.per;
-    if (at >= total) return;  // uniform
-    v0 = (uint32_t)at;
-    v1 = total - v0 < l.per ? total : v0 + l.per;
-    if (few) seg = segments_before(S, first, v0, [&](int j) { return s_ptr[j]; });
+    const Division dv = divide_pages(a, total);
+    chunk = dv.chunk;
+    if (chunk == 0) {
+      const uint64_t at = (uint64_t)blockIdx.x * dv.per;
+      if (at >= total) return;  // uniform
+      v0 = (uint32_t)at;
+      v1 = total - v0 < dv.per ? total : v0 + dv.per;
+    }
+    if (chunk > 0) {
+      if (seg >= S) {  // uniform: the (seg - S)-th part behind the segments' first ones
+        const uint32_t want = (uint32_t)(seg - S);
+        const int each = (S + kThreads - 1) / kThreads, j0 = min(tid * each, S), j1 = min(j0 + each, S);
+        uint32_t mine = 0, cut = 0;  // such parts of this thread's segments, and how many segments have them
+        for (int j = j0; j < j1; ++j) {
+          const uint32_t n = parts_at(a, j, chunk);
+          mine += n - 1u;
+          cut += n > 1u ? 1u : 0u;
+        }
+        uint32_t before = vtx::wave_prefix_sum(mine) - mine, rows = vtx::wave_prefix_sum(cut) - cut, all = 0;
+        if (lane == vtx::kWave - 1) {
+          s_m[wave][0] = __uint_as_float(before + mine);
+          s_m[wave][1] = __uint_as_float(rows + cut);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+          const uint32_t x = __float_as_uint(s_m[i][0]);
+          before += i < wave ? x : 0u;
+          rows += i < wave ? __float_as_uint(s_m[i][1]) : 0u;
+          all += x;
+        }
+        if (want >= all) return;  // uniform
+        if (want >= before && want < before + mine) {
+          int j = j0;
+          for (uint32_t n; want >= before + (n = parts_at(a, j, chunk) - 1u); ++j) {
+            before += n;
+            rows += n > 0u ? 1u : 0u;
+          }
+          s_l[0][0] = __int_as_float(j);
+          s_l[0][1] = __uint_as_float(want - before + 1u);
+          s_l[0][2] = __uint_as_float(want + 1u + rows);
+        }
+        __syncthreads();
+        seg = vtx::uniform(__float_as_int(s_l[0][0]));
+        nth = vtx::uniform(__float_as_int(s_l[0][1]));
+        part_row = vtx::uniform(__float_as_int(s_l[0][2]));
+        __syncthreads();
+      }
+    } else if (few) seg = segments_before(S, first, v0, [&](int j) { return s_ptr[j]; });
     else if (a.pitch > 0) seg = (int)divide(v0, a.by_pitch);
     else seg = segments_before(S, first, v0, [&](int j) { return a.indptr[j]; });
   }
 
+  const bool alone = whole || chunk > 0;  // this workgroup has one piece
   // What this workgroup has of a segment: pages pa .. pb of those that count.
   struct Piece {
     Segment s;
@@ -512,12 +599,13 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
       const int p0 = (int)vtx::lane_value((uint32_t)b0, s - base_seg);
       p.s = segment_of(a, p0, (int)vtx::lane_value((uint32_t)b1, s - base_seg),
                        (int)vtx::lane_value((uint32_t)bl, s - base_seg));
-      if (whole) {
+      if (alone) {
+        const int n = whole ? 1 : (int)parts_of(p.s.pages, chunk), each = (p.s.pages + n - 1) / n;
         p.at = 0;
         p.seg = s;
-        p.pa = 0;
-        p.pb = p.s.pages;
-        p.part = false;
+        p.pa = min(nth * each, p.s.pages);
+        p.pb = min(p.pa + each, p.s.pages);
+        p.part = n > 1;
         break;
       }
       const bool laid = packed || a.pitch > 0;  // elsewhere than in the table
@@ -543,8 +631,8 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
     staged_end = min(end, from + (uint32_t)kStage);
     int s = p.seg;
     for (uint32_t v = from + tid; v < staged_end; v += kThreads) {
-      int64_t at = whole ? (int64_t)p.s.start + v : (int64_t)first + v;
-      if (packed || a.pitch > 0) {
+      int64_t at = alone ? (int64_t)p.s.start + v : (int64_t)first + v;
+      if (!alone && (packed || a.pitch > 0)) {
         while (packed && s + 1 < S && (uint32_t)s_ptr[s + 1] <= v) ++s;
         if (!packed) s = (int)divide(v, a.by_pitch);
         const Segment g = s == p.seg ? p.s : segment_of(a, a.indptr[s], a.indptr[s + 1], a.last_len[s]);
@@ -631,6 +719,10 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
 
   Piece cur = piece_from(seg);
   if (cur.seg >= S) return;  // uniform
+  if (alone && cur.part && nth == 0) {  // uniform: behind the parts of the cut segments before this
+    part_row = (int)parts_before<kThreads>(a, seg, chunk, &s_l[0][0]);
+    __syncthreads();
+  }
   load_queries(cur.seg);
   bool ready = false;  // this wave's first tile of the segment is on its way
   while (true) {
@@ -663,7 +755,7 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
       Stretch st = stretch_of(cur, pc);
       if (st.pages == 0) {  // uniform
         if (staged_end > 0) __syncthreads();  // (the staged rows are done with)
-        stage(cur, cur.at + (uint32_t)pc, whole ? (uint32_t)cur.pb : v1);
+        stage(cur, cur.at + (uint32_t)pc, alone ? (uint32_t)cur.pb : v1);
         st = stretch_of(cur, pc);
       }
       const int skip = pc == 0 ? cur.s.skip : 0;
@@ -735,7 +827,7 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
     // the next segment's queries and first tiles, requested before this one's end
     Piece nxt;
     nxt.seg = S;
-    if (!whole) nxt = piece_from(cur.seg + 1);
+    if (!alone) nxt = piece_from(cur.seg + 1);
     if (nxt.seg < S) {  // uniform
       load_queries(nxt.seg);
       if constexpr (kPages16) {
@@ -785,7 +877,9 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
         }
       }
       if (cur.part) {  // uniform
-        const long long row = (2LL * blockIdx.x + (cur.at + (uint32_t)cur.pa == v0 ? 0 : 1)) * G + g;
+        const int at = alone ? part_row : 2 * (int)blockIdx.x + (cur.at + (uint32_t)cur.pa == v0 ? 0 : 1);
+        const long long row = (long long)at * G + g;
+        if (at >= 2 * a.slots) break;  // (a table that decreases, if at all)
         *reinterpret_cast<float4*>(a.acc + row * kD + d) = O;
         if (d == 0) a.ml[row] = float2{M, L};
       } else {
@@ -819,15 +913,20 @@ __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAtt
                          : a.pitch > 0 ? (uint32_t)seg * (uint32_t)a.pitch
                                        : (uint32_t)sg.start - (uint32_t)first;
   const Place at = place_of(sg, begin, total);
-  const Line l = line_of(a, total);
+  const Division dv = divide_pages(a, total);
   uint32_t w0 = 0;
   int n = 0;
   bool second = false;  // the first part lies behind another segment's
-  if (at.end > at.at) {
-    w0 = at.at / l.per;
-    if (at.end <= (w0 + 1) * l.per) return;  // uniform: written by its workgroup
-    n = (int)((at.end - 1) / l.per - w0) + 1;
-    second = at.at > w0 * l.per;
+  if (dv.chunk > 0) {
+    n = (int)parts_of(sg.pages, dv.chunk);
+    if (n == 1) return;  // uniform: written by its workgroup, zeros too
+    w0 = parts_before<kJoinThreads>(a, seg, dv.chunk, &s_o[0][0]);
+    if ((uint64_t)w0 + (uint32_t)n > 2u * (uint32_t)a.slots) n = 0;  // (a table that decreases, if at all)
+  } else if (at.end > at.at) {
+    w0 = at.at / dv.per;
+    if (at.end <= (w0 + 1) * dv.per) return;  // uniform: written by its workgroup
+    n = (int)((at.end - 1) / dv.per - w0) + 1;
+    second = at.at > w0 * dv.per;
   }
   const int items = G * (kD / 4);
   for (int x0 = 0; x0 < items; x0 += kJoinThreads) {
@@ -838,16 +937,18 @@ __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAtt
     float M = -INFINITY, L = 0.f;
     float4 O{0.f, 0.f, 0.f, 0.f};
     if (grp < groups) {
-      // row of part i: 2 (w0 + i) G + g, the second of its range for the first where that
-      // lies behind another segment's
-      const float2* ml = a.ml + 2LL * w0 * G + g;
-      const float* acc = a.acc + (2LL * w0 * G + g) * kD + d;
+      // part i of a cut segment is row w0 + i; of one in several ranges 2 (w0 + i), one
+      // more for the first where that lies behind another segment's
+      const int step = dv.chunk > 0 ? 1 : 2, row1 = second ? 1 : 0;
+      const long long row0 = (long long)w0 * step;
+      const float2* ml = a.ml + row0 * G + g;
+      const float* acc = a.acc + (row0 * G + g) * kD + d;
       for (int i0 = grp; i0 < n; i0 += groups * kAhead) {
         float2 z[kAhead];
         float4 y[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const int i = i0 + u * groups, row = (i == 0 && second ? 1 : 2 * i) * G;
+          const int i = i0 + u * groups, row = (i == 0 ? row1 : step * i) * G;
           z[u] = float2{-INFINITY, 0.f};
           y[u] = float4{0.f, 0.f, 0.f, 0.f};
           if (i < n) {
@@ -925,11 +1026,11 @@ int launch_types(const QAttnArgs& a, int codes, bool half, hipStream_t s) {
 // more to lay out (128 of 1024 22 / 19, of 2048 27 / 30; 256 columns, 64 of 768 22 /
 // 20, of 1024 22 / 24).
 struct Ranges {
-  long long workers, least, cus, pitch;
+  long long workers, slots, least, cus, pitch;
 };
 Ranges ranges_of(long long segments, int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t window,
                  int32_t longest, long long indices_len) {
-  Ranges r{0, 1, 1, 0};
+  Ranges r{0, 0, 1, 1, 0};
   r.cus = vtx::device_cu_count() > 0 ? vtx::device_cu_count() : 256;
   const long long few = 640 - head_dim;
   const long long known = longest > 0 && (window == 0 || longest < window) ? longest : window;
@@ -939,20 +1040,23 @@ Ranges ranges_of(long long segments, int32_t num_kv_heads, int32_t head_dim, int
                                                : few;
   if (indices_len * page_size <= few * num_kv_heads || (known > 0 && known <= most)) return r;
   r.least = (kMinTokens + (long long)page_size - 1) / page_size;
-  r.workers = r.cus * (head_dim == 256 ? kPerCu<256> : (head_dim == 128 ? kPerCu<128> : kPerCu<64>));
+  r.slots = r.cus * (head_dim == 256 ? kPerCu<256> : (head_dim == 128 ? kPerCu<128> : kPerCu<64>));
   r.pitch = 0;
   if (window > 0 && segments >= kBounds) {
     const long long most = ((long long)window + page_size - 1) / page_size + 1;  // pages that a window touches
     if (most * segments <= 0x7fffffffLL) r.pitch = most;
   }
   const long long need = std::max(segments, (indices_len + r.least - 1) / r.least);
-  if (r.workers > need) r.workers = need;
+  if (r.slots > need) r.slots = need;
+  // (a workgroup per segment, and no more parts behind them than chunks of twice a
+  // workgroup's share)
+  r.workers = std::max(r.slots, segments + r.slots / 2 + 1);
   return r;
 }
 // Floats of scratch: two parts a range, and a packed line's places.
 long long scratch_of(const Ranges& r, long long segments, int32_t group_size, int32_t head_dim, int32_t window) {
   if (r.workers == 0) return 0;
-  return 2 * r.workers * group_size * (head_dim + 2) + (window > 0 && segments < kBounds ? segments + 1 : 0);
+  return 2 * r.slots * group_size * (head_dim + 2) + (window > 0 && segments < kBounds ? segments + 1 : 0);
 }
 
 }  // namespace
@@ -1032,21 +1136,25 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
   a.least = 1;
   a.by_segments = divisor(segments);
   a.by_heads = divisor(num_kv_heads);
-  a.by_workers = a.by_cus = a.by_least = a.by_pitch = divisor(1);
+  a.slots = 0;
+  a.balanced = false;
+  a.by_slots = a.by_cus = a.by_least = a.by_pitch = divisor(1);
   a.pitch = 0;
   a.acc = nullptr;
   a.ml = nullptr;
   a.places = nullptr;
   if (workspace) {
     const Ranges r = ranges_of(segments, num_kv_heads, head_dim, page_size, window, longest, kv_indices_len);
-    const long long parts = 2 * r.workers * group_size, need = scratch_of(r, segments, group_size, head_dim, window);
+    const long long parts = 2 * r.slots * group_size, need = scratch_of(r, segments, group_size, head_dim, window);
     if (workspace_len < need || !vtx::aligned16(workspace))
       return vtx::fail(VTX_E_INVALID,
                        "quant_decode_attention: workspace of %lld floats (16-byte aligned) needed, got %lld", need,
                        (long long)workspace_len);
     a.workers = (int32_t)r.workers;  // (0: as without a workspace)
     a.least = (int32_t)r.least;
-    a.by_workers = divisor(r.workers > 0 ? r.workers : 1);
+    a.slots = (int32_t)r.slots;
+    a.balanced = 20 * ((segments + r.cus - 1) / r.cus * r.cus) <= 23 * segments;
+    a.by_slots = divisor(r.slots > 0 ? r.slots : 1);
     a.by_cus = divisor(r.cus);
     a.by_least = divisor(r.least);
     a.pitch = (int32_t)r.pitch;
