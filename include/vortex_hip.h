@@ -831,7 +831,7 @@ int vtx_page_reduce_quant(const void* x, const void* scales, int64_t x_rows, int
  * a length of 0: a workgroup per segment, one launch, the same bits in every batch.
  * longest: tokens that no segment exceeds, if the caller knows (0: unknown); where
  * the segments are short or many for it, that length is 0.  It steers speed alone.
- * head_dim 64, 128 or 256; group_size 1..16.
+ * head_dim 64, 128 or 256; group_size 1..16; at most 2^23 segments.
  */
 int vtx_quant_decode_attention_supported(int32_t head_dim, int32_t group_size);
 int64_t vtx_quant_decode_attention_workspace_len(int32_t batch_size, int32_t num_kv_heads, int32_t group_size,

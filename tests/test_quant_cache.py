@@ -439,8 +439,11 @@ def _uniform(tokens, H, G, D, P, device, window=0, codes_seed=1):
     ([1] * 700, 4, 64, 16, 0), ([5, 0, 64] * 500, 2, 128, 32, 0), ([40000, 9], 1, 256, 64, 0),
     ([9000, 1], 2, 128, 1, 0),
     ([20000, 30, 0, 7000], 2, 128, 16, 1000), ([3000] * 30, 4, 64, 16, 33), ([700, 9000], 1, 256, 5, 4096),
-    ([20000, 30, 0, 7000], 2, 128, 16, 3001), ([3000, 1, 0, 1600] * 8, 4, 64, 16, 1500), ([0, 9000, 0], 2, 64, 48, 8000),
+    ([20000, 30, 0, 7000], 2, 128, 16, 3001), ([3000, 1, 0, 1600] * 8, 4, 64, 16, 1500),
+    ([0, 9000, 0], 2, 64, 48, 8000),
     ([5000, 0, 9000, 40] * 8, 8, 64, 24, 2500), ([16, 2000] * 150, 1, 128, 16, 2049),
+    ([100] * 300 + [30000, 0, 5000], 2, 64, 16, 0), ([100] * 300 + [0, 9000], 2, 128, 5, 0),
+    ([3, 40000] + [90] * 500, 1, 256, 16, 0),
     ([0, 0, 0], 2, 64, 16, 0), ([32769], 1, 64, 16, 0)], ids=lambda x: str(x)[:20])
 def test_attention_counts_every_token_once(gpu, tokens, H, D, P, window):
     _uniform(tokens, H, 2, D, P, gpu, window=window)
@@ -921,7 +924,7 @@ def test_c_refusals():
                      (dict(cap=-1.0), b"cap"), (dict(cap=math.nan), b"cap"), (dict(cap=math.inf), b"cap"),
                      (dict(q=None), b"null"), (dict(q=p[0] + 8), b"aligned"), (dict(k=p[2] + 4), b"aligned"),
                      (dict(st=(ctypes.c_int64 * 3)(384, 192, 63)), b"aligned"), (dict(entries=1 << 31), b"entries"),
-                     (dict(B=1 << 20, H=1 << 12), b"too many")):
+                     (dict(B=1 << 20, H=1 << 12), b"too many"), (dict(B=(1 << 22) + 1), b"too many")):
         assert attend(**kw) == -1 and says in lib.vtx_last_error(), (kw, lib.vtx_last_error())
     assert attend(B=0) == 0
     need = lib.vtx_quant_decode_attention_workspace_len

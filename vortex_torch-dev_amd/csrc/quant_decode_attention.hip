@@ -1099,7 +1099,7 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
     return vtx::fail(VTX_E_INVALID, "quant_decode_attention: the cap must be finite and not negative");
   const long long segments = (long long)batch_size * num_kv_heads;
   if (segments == 0) return VTX_OK;
-  if (segments > 0x3fffffffLL || kv_indices_len > 0x7fffffffLL)
+  if (segments > (1LL << 23) || kv_indices_len > 0x7fffffffLL)  // (a launch has under 2^32 threads)
     return vtx::fail(VTX_E_INVALID, "quant_decode_attention: too many segments or table entries");
   if (!q || !q_strides || !o || !k_cache || !v_cache || !scales || !kv_indptr || !kv_last_page_len ||
       (kv_indices_len > 0 && !kv_indices))
