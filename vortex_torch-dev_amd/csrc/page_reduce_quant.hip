@@ -4,7 +4,8 @@
 // tile (loc / P) * H + h give one row of C statistics per output, rounded to
 // bf16.  Codes times a power of two are bf16 values, and the rows are taken in
 // page_reduce.hip's order, so the outputs are bit for bit those of the same
-// reduction over a bf16 pool that holds the values.
+// reduction over a bf16 pool that holds the values (e4m3 values under 2^-130 have
+// bits that bf16 has not; they are added as they are).
 //
 // Bound by HBM for a burst of pages (16,384 pages of 8 heads, Max + Min, 76 us, 4.5
 // TB/s), by the launch and two dependent loads (loc, codes) for a decode step (64

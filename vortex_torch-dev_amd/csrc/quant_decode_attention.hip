@@ -28,9 +28,9 @@
 // launch.
 //
 // Bound by HBM where there are many tokens (32 requests of up to 32k, 8 x 8 heads of
-// 128 columns, 213 us, 5.8 TB/s: the rate of a sequential read), by five dependent
+// 128 columns, 212 us, 5.9 TB/s: the rate of a sequential read), by five dependent
 // trips to memory and the second launch where there are few (one request of 4096
-// tokens 11.9 us, of 128, in one launch, 6.1).
+// tokens 12.1 us, of 128, in one launch, 6.1).
 #include <algorithm>
 
 #include "vtx_device.h"

@@ -39,8 +39,8 @@ def read_kv_buffer_quant(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scales
                          k_out: Optional[torch.Tensor] = None,
                          v_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values at the slots ``loc``, [nnz, H, D] each, rounded to
-    ``dtype`` (bf16, which holds every value, fp16 or fp32); zeros where a slot
-    lies outside the pool.  ``k_out`` / ``v_out``: tensors to write into, of any
+    ``dtype`` (bf16, which holds every value, of e4m3 from 2^-130 on, fp16 or
+    fp32); zeros where a slot lies outside the pool.  ``k_out`` / ``v_out``: tensors to write into, of any
     token and head strides, whose type then counts."""
     return _hip.read_kv_buffer_quant(k_cache, v_cache, kv_scales, loc, int(page_size), int(num_kv_heads), dtype, k_out,
                                      v_out)
