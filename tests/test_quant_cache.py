@@ -459,6 +459,15 @@ def test_attention_of_many_segments(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,H,G,D,P", [
+    ([40000], 1, 16, 128, 16), ([40000], 1, 3, 64, 16), ([9000], 1, 1, 64, 8), ([20000], 1, 11, 256, 16),
+    ([17000, 30], 2, 5, 128, 32), ([12000, 0, 9000], 1, 9, 256, 64), ([5000] * 6, 2, 16, 64, 16)])
+def test_attention_of_few_segments_in_many_parts(gpu, tokens, H, G, D, P):
+    """... which several workgroups each join some heads and columns of."""
+    _case(tokens, H, G, D, P, E4M3, torch.bfloat16, gpu, seed=len(tokens))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,tokens", [(8, [512] * 64), (2, [700] * 3), (3, [5, 900, 0, 33])])
 def test_attention_with_a_known_bound(gpu, H, tokens):
     """max_tokens steers how the work is divided, also where it is wrong."""

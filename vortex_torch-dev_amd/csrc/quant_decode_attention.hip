@@ -88,6 +88,7 @@ struct QAttnArgs {
   float cap;       // cap log2 e, or 0
   int32_t workers, slots;  // workgroups (0: one per segment), and how many of them the card holds
   int32_t least;           // pages of a range
+  int32_t join;            // (head, four columns) of a joining workgroup
   float* acc;       // [2 slots, G, D]
   float2* ml;       // [2 slots, G]
   int32_t* places;  // [segments + 1], of a packed line
@@ -895,12 +896,21 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
 }
 
 // The parts of a segment that lies in several ranges, joined; zeros for one
-// without tokens.  A workgroup per segment: threads = (part of the parts, head,
-// four columns), each with a running maximum of its own.
-constexpr int kJoinThreads = 256;
+// without tokens.  Threads = (part of the parts, head, four columns), each with a
+// running maximum of its own; a workgroup takes `join_items` of a segment's (head,
+// four columns): 256, or as many fewer (32, a row's 512 bytes, at least) as let its
+// threads take the parts that there are, on average, in one trip.  All by one
+// workgroup / so, 128 columns: 8 segments of up to 20k tokens and 16 heads 36.4 / 21.5
+// us, one of 32k and 8 heads 38.6 / 15.1, 13 of up to 30k and 8 heads 35.0 / 24.6.
+constexpr int kJoinThreads = 256, kJoinAhead = 8;  // parts of a thread in flight
+inline int join_items(long long segments, long long slots) {
+  int n = kJoinThreads;
+  while (n > 32 && n * slots > (long long)kJoinThreads * kJoinAhead * segments) n /= 2;
+  return n;
+}
 template <int kD, bool kHalf>
 __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAttnArgs a) {
-  constexpr int kAhead = 8;  // parts in flight
+  constexpr int kAhead = kJoinAhead;
   __shared__ alignas(16) float s_o[kJoinThreads][4];
   __shared__ float2 s_ml[kJoinThreads];
   const int seg = blockIdx.x, tid = threadIdx.x, G = a.G, S = a.segments;
@@ -928,71 +938,69 @@ __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAtt
     n = (int)((at.end - 1) / dv.per - w0) + 1;
     second = at.at > w0 * dv.per;
   }
-  const int items = G * (kD / 4);
-  for (int x0 = 0; x0 < items; x0 += kJoinThreads) {
-    const int here = min(items - x0, kJoinThreads);
-    const int most = kJoinThreads / here, groups = n < most * 2 ? (n + 1) / 2 : most;
-    const int grp = tid / here, x = tid - grp * here;
-    const int g = (x0 + x) / (kD / 4), d = ((x0 + x) % (kD / 4)) * 4;
-    float M = -INFINITY, L = 0.f;
-    float4 O{0.f, 0.f, 0.f, 0.f};
-    if (grp < groups) {
-      // part i of a cut segment is row w0 + i; of one in several ranges 2 (w0 + i), one
-      // more for the first where that lies behind another segment's
-      const int step = dv.chunk > 0 ? 1 : 2, row1 = second ? 1 : 0;
-      const long long row0 = (long long)w0 * step;
-      const float2* ml = a.ml + row0 * G + g;
-      const float* acc = a.acc + (row0 * G + g) * kD + d;
-      for (int i0 = grp; i0 < n; i0 += groups * kAhead) {
-        float2 z[kAhead];
-        float4 y[kAhead];
+  const int items = G * (kD / 4), x0 = (int)blockIdx.y * a.join;
+  const int here = min(items - x0, a.join);
+  const int most = kJoinThreads / here, groups = n < most * 2 ? (n + 1) / 2 : most;
+  const int grp = tid / here, x = tid - grp * here;
+  const int g = (x0 + x) / (kD / 4), d = ((x0 + x) % (kD / 4)) * 4;
+  float M = -INFINITY, L = 0.f;
+  float4 O{0.f, 0.f, 0.f, 0.f};
+  if (grp < groups) {
+    // part i of a cut segment is row w0 + i; of one in several ranges 2 (w0 + i), one
+    // more for the first where that lies behind another segment's
+    const int step = dv.chunk > 0 ? 1 : 2, row1 = second ? 1 : 0;
+    const long long row0 = (long long)w0 * step;
+    const float2* ml = a.ml + row0 * G + g;
+    const float* acc = a.acc + (row0 * G + g) * kD + d;
+    for (int i0 = grp; i0 < n; i0 += groups * kAhead) {
+      float2 z[kAhead];
+      float4 y[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const int i = i0 + u * groups, row = (i == 0 ? row1 : step * i) * G;
-          z[u] = float2{-INFINITY, 0.f};
-          y[u] = float4{0.f, 0.f, 0.f, 0.f};
-          if (i < n) {
-            z[u] = ml[row];
-            y[u] = *reinterpret_cast<const float4*>(acc + (long long)row * kD);
-          }
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * groups, row = (i == 0 ? row1 : step * i) * G;
+        z[u] = float2{-INFINITY, 0.f};
+        y[u] = float4{0.f, 0.f, 0.f, 0.f};
+        if (i < n) {
+          z[u] = ml[row];
+          y[u] = *reinterpret_cast<const float4*>(acc + (long long)row * kD);
         }
-        float nm = M;
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) nm = fmaxf(nm, z[u].x);
-        if (nm == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(M - nm);
-        L *= f;
-        O = float4{O.x * f, O.y * f, O.z * f, O.w * f};
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const float e = __builtin_amdgcn_exp2f(z[u].x - nm);
-          L = fmaf(z[u].y, e, L);
-          O = float4{fmaf(y[u].x, e, O.x), fmaf(y[u].y, e, O.y), fmaf(y[u].z, e, O.z), fmaf(y[u].w, e, O.w)};
-        }
-        M = nm;
       }
-    }
-    if (groups > 1) {  // uniform
-      __syncthreads();
-      s_ml[tid] = float2{M, L};
-      *reinterpret_cast<float4*>(s_o[tid]) = O;
-      __syncthreads();
-    }
-    if (grp == 0) {
-      for (int i = 1; i < groups; ++i) {
-        const float2 z = s_ml[i * here + x];
-        const float4 y = *reinterpret_cast<const float4*>(s_o[i * here + x]);
-        const float nm = fmaxf(M, z.x);
-        if (nm == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(M - nm), e = __builtin_amdgcn_exp2f(z.x - nm);
-        L = L * f + z.y * e;
-        O = float4{O.x * f + y.x * e, O.y * f + y.y * e, O.z * f + y.z * e, O.w * f + y.w * e};
-        M = nm;
+      float nm = M;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) nm = fmaxf(nm, z[u].x);
+      if (nm == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(M - nm);
+      L *= f;
+      O = float4{O.x * f, O.y * f, O.z * f, O.w * f};
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float e = __builtin_amdgcn_exp2f(z[u].x - nm);
+        L = fmaf(z[u].y, e, L);
+        O = float4{fmaf(y[u].x, e, O.x), fmaf(y[u].y, e, O.y), fmaf(y[u].z, e, O.z), fmaf(y[u].w, e, O.w)};
       }
-      const float f = inverse_sum(L);
-      *reinterpret_cast<uint2*>(a.o + ((long long)seg * G + g) * kD + d) =
-          uint2{round2<kHalf>(O.x * f, O.y * f), round2<kHalf>(O.z * f, O.w * f)};
+      M = nm;
     }
+  }
+  if (groups > 1) {  // uniform
+    __syncthreads();
+    s_ml[tid] = float2{M, L};
+    *reinterpret_cast<float4*>(s_o[tid]) = O;
+    __syncthreads();
+  }
+  if (grp == 0) {
+    for (int i = 1; i < groups; ++i) {
+      const float2 z = s_ml[i * here + x];
+      const float4 y = *reinterpret_cast<const float4*>(s_o[i * here + x]);
+      const float nm = fmaxf(M, z.x);
+      if (nm == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(M - nm), e = __builtin_amdgcn_exp2f(z.x - nm);
+      L = L * f + z.y * e;
+      O = float4{O.x * f + y.x * e, O.y * f + y.y * e, O.z * f + y.z * e, O.w * f + y.w * e};
+      M = nm;
+    }
+    const float f = inverse_sum(L);
+    *reinterpret_cast<uint2*>(a.o + ((long long)seg * G + g) * kD + d) =
+        uint2{round2<kHalf>(O.x * f, O.y * f), round2<kHalf>(O.z * f, O.w * f)};
   }
 }
 
@@ -1001,7 +1009,9 @@ int launch_one(const QAttnArgs& a, hipStream_t s) {
   const int grid = a.workers > 0 ? a.workers : a.segments;
   if (a.P % 16 == 0) quant_attention_kernel<kD, kCodes, kHalf, true><<<grid, kThreads, 0, s>>>(a);
   else quant_attention_kernel<kD, kCodes, kHalf, false><<<grid, kThreads, 0, s>>>(a);
-  if (a.workers > 0) quant_attention_join_kernel<kD, kHalf><<<a.segments, kJoinThreads, 0, s>>>(a);
+  if (a.workers > 0)
+    quant_attention_join_kernel<kD, kHalf>
+        <<<dim3(a.segments, (a.G * (kD / 4) + a.join - 1) / a.join), kJoinThreads, 0, s>>>(a);
   return vtx::check_launch("quant_decode_attention");
 }
 
@@ -1134,6 +1144,7 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
   a.cap = soft_cap * kLog2e;
   a.workers = 0;
   a.least = 1;
+  a.join = kJoinThreads;
   a.by_segments = divisor(segments);
   a.by_heads = divisor(num_kv_heads);
   a.slots = 0;
@@ -1152,6 +1163,7 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
                        (long long)workspace_len);
     a.workers = (int32_t)r.workers;  // (0: as without a workspace)
     a.least = (int32_t)r.least;
+    a.join = join_items(segments, r.slots);
     a.slots = (int32_t)r.slots;
     a.balanced = 20 * ((segments + r.cus - 1) / r.cus * r.cus) <= 23 * segments;
     a.by_slots = divisor(r.slots > 0 ? r.slots : 1);
