@@ -459,6 +459,21 @@ def test_attention_of_many_segments(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(max_tokens=128), dict(max_tokens=1), dict(window=70),
+                                dict(max_tokens=100, logits_soft_cap=20.0, slopes=True)], ids=str)
+@pytest.mark.parametrize("G,D,P,dtype", [(1, 64, 16, torch.bfloat16), (16, 128, 32, torch.float16),
+                                         (5, 256, 16, torch.bfloat16), (3, 256, 64, torch.float16)])
+def test_attention_of_many_tiny_segments(gpu, G, D, P, dtype, kw):
+    """... a few long ones among them, whatever the caller says of their length."""
+    r = random.Random(D + P)
+    tokens = [r.choice([0, 1, 7, 16, 17, 32, 33, 64]) for _ in range(530)]
+    for i, n in ((0, 129), (1, 513), (200, 2500), (529, 1040)):
+        tokens[i] = n
+    slopes = torch.rand(2 * G, generator=torch.Generator().manual_seed(G)).to(gpu) if kw.get("slopes") else None
+    _case(tokens, 2, G, D, P, E4M3, dtype, gpu, seed=G, **{**kw, "slopes": slopes})
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens,H,G,D,P", [
     ([40000], 1, 16, 128, 16), ([40000], 1, 3, 64, 16), ([9000], 1, 1, 64, 8), ([20000], 1, 11, 256, 16),
     ([17000, 30], 2, 5, 128, 32), ([12000, 0, 9000], 1, 9, 256, 64), ([5000] * 6, 2, 16, 64, 16)])

@@ -20,12 +20,12 @@
 // weight), and fp16 queries likewise (exactly): the matrix cores have time, the
 // launch waits for memory.
 //
-// 4 waves per workgroup, 32 tokens of a wave at a time; the next ones' keys are
-// requested behind the scores and their values behind the weighted sum, into the
-// registers that these leave, and the next segment's first ones before the waves'
-// results are joined.  How a table's pages are divided among workgroups:
-// divide_pages; a segment that lies in several has its parts joined by a second
-// launch.
+// 4 waves per workgroup (one where segments are many and tiny), 32 tokens of a wave
+// at a time; the next ones' keys are requested behind the scores and their values
+// behind the weighted sum, into the registers that these leave, and the next
+// segment's first ones before the waves' results are joined.  How a table's pages
+// are divided among workgroups: divide_pages, ranges_of; a segment that lies in
+// several has its parts joined by a second launch.
 //
 // Bound by HBM where there are many tokens (32 requests of up to 32k, 8 x 8 heads of
 // 128 columns, 212 us, 5.9 TB/s: the rate of a sequential read), by five dependent
@@ -39,13 +39,13 @@
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / vtx::kWave;
+constexpr int kAllWaves = 4;     // of a workgroup, but where segments are many and tiny (ranges_of): 1
 constexpr int kHeads = 16;       // query heads of a matrix tile
 constexpr int kTile = 32;        // tokens of a wave at a time
 constexpr int kStage = 1024;     // page rows staged in LDS at a time
 constexpr int kBounds = 1024;    // bounds of a table that are brought to LDS whole
 constexpr int kMinTokens = 128;  // tokens of a range at least: a tile per wave
+constexpr int kTiny = 256;       // tokens of a tiny segment
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A divisor that the host knows: three scalar instructions and two corrections
@@ -80,6 +80,7 @@ struct QAttnArgs {
   const float* slopes;  // [H * G], or null
   int64_t q_batch, q_kv, q_head;  // strides in elements
   int32_t segments, H, G, P, p_shift;
+  bool tiny;               // a wave each
   bool balanced;           // no compute unit has much more than its share of the segments
   Divisor by_segments, by_heads, by_slots, by_cus, by_least, by_pitch;
   int32_t window;  // the last tokens that count; 0: all
@@ -121,7 +122,7 @@ __device__ __forceinline__ Division divide_pages(const QAttnArgs& a, uint32_t to
   const uint32_t even = divide(total + (uint32_t)a.slots - 1u, a.by_slots), least = (uint32_t)a.least;
   const uint32_t S = (uint32_t)a.segments, m = divide(total, a.by_segments);
   const uint32_t mean = m + (m * S < total ? 1u : 0u);
-  if (mean < least || (mean < 2u * even && (mean <= 8u * least || (a.balanced && m * S == total))))
+  if (a.tiny || mean < least || (mean < 2u * even && (mean <= 8u * least || (a.balanced && m * S == total))))
     return Division{even, max(max(2u * even, 8u * least), mean)};
   Division v{divide(max(even, least) + least - 1u, a.by_least) * least, 0u};
   if (m >= v.per && m * S == total) {
@@ -228,12 +229,12 @@ struct Heads {
 // twice as many, in LDS, one copy for all waves (in registers they spilled: 128
 // columns, 32 requests of up to 8k tokens 77 us, so 66; bf16 ones in LDS cost 1 us
 // of 65).  After the tiles the waves' outputs take their place there.
-template <int kD, bool kHalf>
+template <int kD, bool kHalf, int kWaves>
 struct Queries {
   static constexpr int kOwn = kHalf ? (kD / 32 + kWaves - 1) / kWaves : kD / 32;  // of a wave
   vtx::U4 raw[kOwn];
 };
-template <int kD, bool kHalf>
+template <int kD, bool kHalf, int kWaves>
 struct Shared {
   static constexpr int kOut = kD + 4;  // floats of a head's outputs: 16 heads' pieces in all banks
   union {
@@ -301,9 +302,9 @@ __device__ __forceinline__ void load_v(const unsigned char* p, uint32_t (&to)[kD
 constexpr float kGrowth = 8.f;
 
 // Scores of 32 tokens, without their factors.
-template <int kD, int kCodes, bool kHalf>
-__device__ __forceinline__ void score(const Shared<kD, kHalf>& sh, const Queries<kD, kHalf>& own, const Keys<kD>& t,
-                                      f32x4 (&s)[2]) {
+template <int kD, int kCodes, bool kHalf, int kWaves>
+__device__ __forceinline__ void score(const Shared<kD, kHalf, kWaves>& sh, const Queries<kD, kHalf, kWaves>& own,
+                                      const Keys<kD>& t, f32x4 (&s)[2]) {
   int lane = vtx::lane_id();
   if constexpr (kHalf) asm volatile("" : "+v"(lane));  // (read for every tile: kept out of the registers)
 #pragma unroll
@@ -451,11 +452,15 @@ __device__ __forceinline__ float inverse_sum(float L) { return L > 0.f ? 1.f / L
 template <int kD>
 constexpr int kPerCu = kD == 256 ? 2 : (kD == 128 ? 3 : 4);
 
-template <int kD, int kCodes, bool kHalf, bool kPages16>
-__global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(QAttnArgs a) {
-  __shared__ int32_t s_ptr[kBounds], s_last[kBounds], s_rows[kStage];
+// kWaves 1: a workgroup per segment, or per part of one (Division's chunks).
+template <int kD, int kCodes, bool kHalf, bool kPages16, int kWaves>
+__global__ __launch_bounds__(kWaves* vtx::kWave, kPerCu<kD>) void quant_attention_kernel(QAttnArgs a) {
+  constexpr int kThreads = kWaves * vtx::kWave;
+  constexpr bool kLine = kWaves > 1;
+  constexpr int kStage = kLine ? ::kStage : 128;
+  __shared__ int32_t s_ptr[kLine ? kBounds : 1], s_last[kLine ? kBounds : 1], s_rows[kStage];
   __shared__ float s_m[kWaves][kHeads], s_l[kWaves][kHeads];
-  __shared__ alignas(16) Shared<kD, kHalf> sh;
+  __shared__ alignas(16) Shared<kD, kHalf, kWaves> sh;
 
   const int tid = threadIdx.x, lane = vtx::lane_id();
   const int wave = vtx::uniform(tid / vtx::kWave);
@@ -472,10 +477,10 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
   uint32_t chunk = 0;  // a segment's parts have at most so many pages (0: ranges of the line)
   int nth = 0;         // which of them is this workgroup's
   int part_row = 0;    // where its result goes
-  const bool whole = a.workers == 0, few = !whole && S < kBounds, packed = few && a.window > 0;  // uniform
+  const bool whole = a.workers == 0, few = kLine && !whole && S < kBounds, packed = few && a.window > 0;  // uniform
   if (!whole) {
     if (packed) {
-      constexpr int kEach = kBounds / kThreads;
+      constexpr int kEach = kLine ? kBounds / kThreads : 1;
       uint32_t pages[kEach], mine = 0;
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
@@ -505,7 +510,7 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
       __syncthreads();
     } else if (few) {
 #pragma unroll
-      for (int i = 0; i < kBounds; i += kThreads)
+      for (int i = 0; i < (kLine ? kBounds : 0); i += kThreads)
         if (i + tid <= S) {
           s_ptr[i + tid] = a.indptr[i + tid];
           s_last[i + tid] = a.last_len[min(i + tid, S - 1)];
@@ -521,15 +526,24 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
     }
     const Division dv = divide_pages(a, total);
     chunk = dv.chunk;
-    if (chunk == 0) {
+    if (kLine && chunk == 0) {
       const uint64_t at = (uint64_t)blockIdx.x * dv.per;
       if (at >= total) return;  // uniform
       v0 = (uint32_t)at;
       v1 = total - v0 < dv.per ? total : v0 + dv.per;
     }
-    if (chunk > 0) {
+    if (!kLine || chunk > 0) {
       if (seg >= S) {  // uniform: the (seg - S)-th part behind the segments' first ones
         const uint32_t want = (uint32_t)(seg - S);
+        if constexpr (!kLine) {  // mostly none is cut: a look at the table first
+          bool any = false;
+#pragma unroll 8
+          for (int j = lane; j < S; j += vtx::kWave) {
+            const int p0 = a.indptr[j], p1 = a.indptr[j + 1];
+            any |= p1 > p0 && (uint32_t)p1 - (uint32_t)p0 > chunk;
+          }
+          if (!__any(any)) return;  // uniform
+        }
         const int each = (S + kThreads - 1) / kThreads, j0 = min(tid * each, S), j1 = min(j0 + each, S);
         uint32_t mine = 0, cut = 0;  // such parts of this thread's segments, and how many segments have them
         for (int j = j0; j < j1; ++j) {
@@ -572,7 +586,7 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
     else seg = segments_before(S, first, v0, [&](int j) { return a.indptr[j]; });
   }
 
-  const bool alone = whole || chunk > 0;  // this workgroup has one piece
+  const bool alone = !kLine || whole || chunk > 0;  // this workgroup has one piece
   // What this workgroup has of a segment: pages pa .. pb of those that count.
   struct Piece {
     Segment s;
@@ -705,13 +719,13 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
     }
   };
   // a segment's query rows; heads past G take head 0's, and nobody takes their results
-  Queries<kD, kHalf> own;
+  Queries<kD, kHalf, kWaves> own;
   float slope = 0.f;
   auto load_queries = [&](int s) {
     const int b = (int)divide((uint32_t)s, a.by_heads), h = s - b * a.H;
     const uint16_t* q = a.q + b * a.q_batch + h * a.q_kv + (c16 < G ? c16 : 0) * a.q_head + g4 * 16;
 #pragma unroll
-    for (int i = 0; i < Queries<kD, kHalf>::kOwn; ++i) {
+    for (int i = 0; i < Queries<kD, kHalf, kWaves>::kOwn; ++i) {
       const int j = kHalf ? min(i * kWaves + wave, kD / 32 - 1) : i;
       own.raw[i] = vtx::ld16(q + (j / 2) * 64 + (j % 2) * 8);
     }
@@ -729,7 +743,7 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
   while (true) {
     if constexpr (kHalf) {  // fp16 values as two bf16 ones, to LDS
 #pragma unroll
-      for (int i = 0; i < Queries<kD, kHalf>::kOwn; ++i) {
+      for (int i = 0; i < Queries<kD, kHalf, kWaves>::kOwn; ++i) {
         const int j = i * kWaves + wave;
         if (j >= kD / 32) break;  // uniform
         typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -773,7 +787,7 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
         ready = false;
         for (int i = wave; i < tiles; i += kWaves) {
           f32x4 sc[2];
-          score<kD, kCodes, kHalf>(sh, own, keys, sc);
+          score<kD, kCodes>(sh, own, keys, sc);
           const int n0 = half[0].tokens, n1 = half[1].tokens;
           aim(st, i + kWaves);  // (none past the last: no loads)
           load_keys();
@@ -819,7 +833,7 @@ __global__ __launch_bounds__(kThreads, kPerCu<kD>) void quant_attention_kernel(Q
             values.sc[hf] = uint2{two[0] | (two[1] << 16), two[2] | (two[3] << 16)};
           }
           f32x4 sc[2];
-          score<kD, kCodes, kHalf>(sh, own, keys, sc);
+          score<kD, kCodes>(sh, own, keys, sc);
           attend<kD, kCodes>(a, w, sc, values, __ballot(bad != 0) != 0, bad, far0 - (float)(i * kTile), slope);
         }
       }
@@ -1007,8 +1021,9 @@ __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAtt
 template <int kD, int kCodes, bool kHalf>
 int launch_one(const QAttnArgs& a, hipStream_t s) {
   const int grid = a.workers > 0 ? a.workers : a.segments;
-  if (a.P % 16 == 0) quant_attention_kernel<kD, kCodes, kHalf, true><<<grid, kThreads, 0, s>>>(a);
-  else quant_attention_kernel<kD, kCodes, kHalf, false><<<grid, kThreads, 0, s>>>(a);
+  if (a.P % 16 != 0) quant_attention_kernel<kD, kCodes, kHalf, false, kAllWaves><<<grid, kAllWaves * vtx::kWave, 0, s>>>(a);
+  else if (a.tiny) quant_attention_kernel<kD, kCodes, kHalf, true, 1><<<grid, vtx::kWave, 0, s>>>(a);
+  else quant_attention_kernel<kD, kCodes, kHalf, true, kAllWaves><<<grid, kAllWaves * vtx::kWave, 0, s>>>(a);
   if (a.workers > 0)
     quant_attention_join_kernel<kD, kHalf>
         <<<dim3(a.segments, (a.G * (kD / 4) + a.join - 1) / a.join), kJoinThreads, 0, s>>>(a);
@@ -1035,12 +1050,22 @@ int launch_types(const QAttnArgs& a, int codes, bool half, hipStream_t s) {
 // 92 / 89; 256 of 2048 36 / 33, of 4096 52 / 57), and with a window the line costs
 // more to lay out (128 of 1024 22 / 19, of 2048 27 / 30; 256 columns, 64 of 768 22 /
 // 20, of 1024 22 / 24).
+//
+// Tiny segments, more than workgroups that the card holds: a wave each, since four
+// share a tile or two and then wait for each other (by the longest they can have or,
+// unknown, by the buffer's size; those that are long all the same are cut from 64
+// tokens x 8 on).  Four waves / one, 128 columns, 1024 segments of 16 tokens 13.6 /
+// 7.7 us, 2048 of 64 25.8 / 14.8, of 128 29.8 / 20.7, of 256 38.5 / 32.7, of 512 57.5
+// / 56.3, of up to 1000 74.0 / 83.6; 64 columns, 2048 of 64 20.1 / 11.7, of 256 26.8 /
+// 23.3, of up to 500 30.8 / 33.2; 256 columns, 1024 of 64 21.4 / 12.5, of 256 33.5 /
+// 29.1.
 struct Ranges {
   long long workers, slots, least, cus, pitch;
+  bool tiny;
 };
 Ranges ranges_of(long long segments, int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t window,
                  int32_t longest, long long indices_len) {
-  Ranges r{0, 0, 1, 1, 0};
+  Ranges r{0, 0, 1, 1, 0, false};
   r.cus = vtx::device_cu_count() > 0 ? vtx::device_cu_count() : 256;
   const long long few = 640 - head_dim;
   const long long known = longest > 0 && (window == 0 || longest < window) ? longest : window;
@@ -1048,9 +1073,13 @@ Ranges ranges_of(long long segments, int32_t num_kv_heads, int32_t head_dim, int
                          : segments >= r.cus   ? 2048
                          : window > 0          ? (head_dim == 256 ? 768 : 1024)
                                                : few;
+  const int per_cu = head_dim == 256 ? kPerCu<256> : (head_dim == 128 ? kPerCu<128> : kPerCu<64>);
+  r.tiny = page_size % 16 == 0 && segments > r.cus * per_cu &&
+           ((known > 0 && known <= kTiny) || (window == 0 && indices_len * page_size <= kTiny * segments));
   if (indices_len * page_size <= few * num_kv_heads || (known > 0 && known <= most)) return r;
-  r.least = (kMinTokens + (long long)page_size - 1) / page_size;
-  r.slots = r.cus * (head_dim == 256 ? kPerCu<256> : (head_dim == 128 ? kPerCu<128> : kPerCu<64>));
+  r.least = ((r.tiny ? kMinTokens / 2 : kMinTokens) + (long long)page_size - 1) / page_size;
+  r.slots = r.cus * per_cu * (r.tiny ? kAllWaves : 1);
+  if (r.tiny) r.slots = std::min(r.slots, segments);
   r.pitch = 0;
   if (window > 0 && segments >= kBounds) {
     const long long most = ((long long)window + page_size - 1) / page_size + 1;  // pages that a window touches
@@ -1058,9 +1087,9 @@ Ranges ranges_of(long long segments, int32_t num_kv_heads, int32_t head_dim, int
   }
   const long long need = std::max(segments, (indices_len + r.least - 1) / r.least);
   if (r.slots > need) r.slots = need;
-  // (a workgroup per segment, and no more parts behind them than chunks of twice a
-  // workgroup's share)
-  r.workers = std::max(r.slots, segments + r.slots / 2 + 1);
+  // (a workgroup per segment, and no more parts behind them than chunks, of twice a
+  // workgroup's share and of eight times the least)
+  r.workers = std::max(r.slots, segments + std::min(r.slots / 2, indices_len / (8 * r.least)) + 1);
   return r;
 }
 // Floats of scratch: two parts a range, and a packed line's places.
@@ -1143,6 +1172,7 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
   a.c = soft_cap > 0.f ? 2.f * kLog2e * (sm_scale / soft_cap) : sm_scale * kLog2e;
   a.cap = soft_cap * kLog2e;
   a.workers = 0;
+  a.tiny = false;
   a.least = 1;
   a.join = kJoinThreads;
   a.by_segments = divisor(segments);
@@ -1154,8 +1184,9 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
   a.acc = nullptr;
   a.ml = nullptr;
   a.places = nullptr;
+  const Ranges r = ranges_of(segments, num_kv_heads, head_dim, page_size, window, longest, kv_indices_len);
+  a.tiny = r.tiny && (workspace || r.workers == 0);
   if (workspace) {
-    const Ranges r = ranges_of(segments, num_kv_heads, head_dim, page_size, window, longest, kv_indices_len);
     const long long parts = 2 * r.slots * group_size, need = scratch_of(r, segments, group_size, head_dim, window);
     if (workspace_len < need || !vtx::aligned16(workspace))
       return vtx::fail(VTX_E_INVALID,
