@@ -1021,9 +1021,10 @@ __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAtt
 template <int kD, int kCodes, bool kHalf>
 int launch_one(const QAttnArgs& a, hipStream_t s) {
   const int grid = a.workers > 0 ? a.workers : a.segments;
-  if (a.P % 16 != 0) quant_attention_kernel<kD, kCodes, kHalf, false, kAllWaves><<<grid, kAllWaves * vtx::kWave, 0, s>>>(a);
+  constexpr int all = kAllWaves, threads = all * vtx::kWave;
+  if (a.P % 16 != 0) quant_attention_kernel<kD, kCodes, kHalf, false, all><<<grid, threads, 0, s>>>(a);
   else if (a.tiny) quant_attention_kernel<kD, kCodes, kHalf, true, 1><<<grid, vtx::kWave, 0, s>>>(a);
-  else quant_attention_kernel<kD, kCodes, kHalf, true, kAllWaves><<<grid, kAllWaves * vtx::kWave, 0, s>>>(a);
+  else quant_attention_kernel<kD, kCodes, kHalf, true, all><<<grid, threads, 0, s>>>(a);
   if (a.workers > 0)
     quant_attention_join_kernel<kD, kHalf>
         <<<dim3(a.segments, (a.G * (kD / 4) + a.join - 1) / a.join), kJoinThreads, 0, s>>>(a);
