@@ -9,7 +9,7 @@
 //
 // Bound by HBM for a burst of pages (16,384 pages of 8 heads, Max + Min, 76 us, 4.5
 // TB/s), by the launch and two dependent loads (loc, codes) for a decode step (64
-// requests 3.8 us).  As there, a workgroup scans 256 loc entries and keeps the
+// requests 3.5 us).  As there, a workgroup scans 256 loc entries and keeps the
 // pages they close, and several share a block's tiles.  Few tiles: a wave takes one
 // at a time, lane = (row group, 8 columns), the codes of 16 to 64 rows of a tile
 // loaded before the first is used.  Many (of up to 16 rows): lane = (tile, 8
