@@ -814,8 +814,9 @@ int vtx_page_reduce_quant(const void* x, const void* scales, int64_t x_rows, int
  * vtx_paged_decode_attention over the 8-bit pools, sparse tables or dense ones:
  *   o[s * G + g] = sum_t softmax_t(f(sm_scale * q . K[t]) - slopes[h * G + g] * (n - 1 - t)) V[t]
  * over the n tokens of segment s = b * H + h, t counted in the table's order; with
- * f(y) = soft_cap * tanh(y / soft_cap), or y for a soft_cap of 0; slopes (fp32,
- * H * G, may be NULL: none); and with window > 0 only the last `window` tokens.
+ * f(y) = soft_cap * tanh(y / soft_cap), within 2^-20 of itself for every finite cap,
+ * or y for a soft_cap of 0; slopes (fp32, H * G, may be NULL: none); and with window >
+ * 0 only the last `window` tokens.
  * Products and sums are fp32, the weights exact to 2^-17.  q: bf16 or fp16 (dtype)
  * rows q + b * q_strides[0] + h * q_strides[1] + g * q_strides[2] (elements); o the
  * same type, [B * H * G, head_dim], dense.  A segment without tokens gets zeros,

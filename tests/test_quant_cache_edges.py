@@ -1,0 +1,49 @@
+"""The 8-bit paged cache at the edges of what it accepts, against the formulas and
+by the tolerances of test_quant_cache."""
+import pytest
+import torch
+
+from test_quant_cache import E4M3, INT8, _near, _plain, _random_pool, _table
+from vortex_torch.decode_attention import quant_paged_decode_attention
+
+
+# --------------------------------------------------------------------- caps
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,P", [(64, 16), (128, 5), (256, 32)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("cap", [1e3, 1e4, 1e5, 1e6, 1e9, 1e20, 3e38])
+def test_large_caps(gpu, cap, dtype, D, P):
+    """The bound follows the scores, not the cap: that of uncapped ones, whose sum of
+    products is allowed D 2^-23 sum |q k|, twice what D fp32 additions are off by.  The
+    other half, at least 2^-18 of the score, has room for the cap's steps: 2^-20 of it.
+    (Between the two formulas lies y (y / cap)^2 / 3, 2^-19 |y| for |y| <= 2 at 1e3.)"""
+    H, G, tokens = 2, 4, [700, 1, 33, 0, 2000]
+    gen = torch.Generator().manual_seed(D)
+    indptr, indices, last, pages = _table(tokens, P, H, 3)
+    kc, vc, sc = _random_pool(pages * H, P, D, E4M3, gen, gpu, spread=1)
+    q = (torch.randn((5, H * G, D), generator=gen) * 2.5).to(dtype).to(gpu)
+    got = quant_paged_decode_attention(q, kc, vc, sc, *(t.to(gpu) for t in (indptr, indices, last)), 5, H,
+                                       logits_soft_cap=cap)
+    want, _ = _plain(q, kc, vc, sc, indptr, indices, last, 5, H, cap=cap)
+    _, off = _plain(q, kc, vc, sc, indptr, indices, last, 5, H)
+    _near(got, want, off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e-3, 1e-20, 1e-37, 1e-40, 1e-46, 1e-300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_small_caps(gpu, dtype, cap):
+    """... down to where every score is almost the same, scores of zero among them;
+    a cap that fp32 holds as 0 is a cap all the same."""
+    H, G, D, P, tokens = 2, 2, 64, 16, [300, 17]
+    gen = torch.Generator().manual_seed(1)
+    indptr, indices, last, pages = _table(tokens, P, H, 3)
+    kc, vc, sc = _random_pool(pages * H, P, D, INT8, gen, gpu)
+    q = torch.randn((2, H * G, D), generator=gen).to(dtype).to(gpu)
+    q[:, 1] = 0
+    got = quant_paged_decode_attention(q, kc, vc, sc, *(t.to(gpu) for t in (indptr, indices, last)), 2, H,
+                                       logits_soft_cap=cap)
+    # a score is at most the cap, and off by 2^-20 of it
+    want, _ = _plain(q, kc, vc, sc, indptr, indices, last, 2, H, cap=cap)
+    _, off = _plain(q * 0, kc, vc, sc, indptr, indices, last, 2, H)
+    _near(got, want, off + 2.0 ** -19 * cap)

@@ -32,6 +32,7 @@
 // trips to memory and the second launch where there are few (one request of 4096
 // tokens 12.1 us, of 128, in one launch, 6.1).
 #include <algorithm>
+#include <cfloat>
 
 #include "vtx_device.h"
 #include "vtx_host.h"
@@ -85,8 +86,9 @@ struct QAttnArgs {
   Divisor by_segments, by_heads, by_slots, by_cus, by_least, by_pitch;
   int32_t window;  // the last tokens that count; 0: all
   int32_t pitch;   // places of a segment on a spaced line; 0: the line is another
-  float c;         // scale log2 e; with a cap 2 scale log2 e / cap
+  float c;         // scale log2 e
   float cap;       // cap log2 e, or 0
+  float by_cap;    // 1 over that
   int32_t workers, slots;  // workgroups (0: one per segment), and how many of them the card holds
   int32_t least;           // pages of a range
   int32_t join;            // (head, four columns) of a joining workgroup
@@ -338,6 +340,22 @@ __device__ __forceinline__ void score(const Shared<kD, kHalf, kWaves>& sh, const
   }
 }
 
+// cap tanh(y / cap), to 2^-20 of itself whatever the cap, with z = y / cap: under 0.75
+// by five terms of Lambert's continued fraction of tanh(z) / z, (1 + u / 9 + u^2 / 945)
+// / (1 + 4 u / 9 + u^2 / 63) with u = z^2 (2^-27 off), which is 1 for a cap that nothing
+// comes near; from there on by (e - 1) / (e + 1), e = 2^(2 z log2 e), where e - 1 loses
+// nothing that counts.  A NaN stays one.  cap - 2 cap / (e + 1) is shorter and off by
+// 2^-22 of the cap, however small y is: 48 requests of up to 8k tokens, 256 columns,
+// 68.0 us, so 68.8; skipped where no score of a tile needs e, 68.6.
+__device__ __forceinline__ float capped(float y, float cap, float by_cap) {
+  const float z = y * by_cap, u = z * z;
+  const bool small = !(fabsf(z) >= 0.75f);
+  const float e = __builtin_amdgcn_exp2f(fminf(fmaxf(z, -12.f), 12.f) * (2.f * kLog2e));
+  const float n = small ? fmaf(u, fmaf(u, 1.f / 945.f, 1.f / 9.f), 1.f) : e - 1.f;
+  const float d = small ? fmaf(u, fmaf(u, 1.f / 63.f, 4.f / 9.f), 1.f) : e + 1.f;
+  return (small ? y : cap) * (n * __builtin_amdgcn_rcpf(d));
+}
+
 // Their weights, and the values by these.  bad: tokens of this lane that do not
 // count (where masked); far: the distance of its first one; slope: base 2.
 template <int kD, int kCodes>
@@ -366,8 +384,7 @@ __device__ __forceinline__ void attend(const QAttnArgs& a, Heads<kD>& w, const f
   }
   if (a.cap != 0.f) {  // uniform
 #pragma unroll
-    for (int i = 0; i < 8; ++i)  // cap tanh(y / cap), the argument doubled and in base 2
-      x[i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[i]));
+    for (int i = 0; i < 8; ++i) x[i] = capped(x[i], a.cap, a.by_cap);
   }
   if (a.slopes) {  // uniform
 #pragma unroll
@@ -1170,8 +1187,9 @@ extern "C" int vtx_quant_decode_attention(const void* q, const int64_t* q_stride
   a.P = page_size;
   a.p_shift = vtx::log2_exact(page_size);
   a.window = window;
-  a.c = soft_cap > 0.f ? 2.f * kLog2e * (sm_scale / soft_cap) : sm_scale * kLog2e;
-  a.cap = soft_cap * kLog2e;
+  a.c = sm_scale * kLog2e;
+  a.cap = std::min(soft_cap * kLog2e, FLT_MAX);
+  a.by_cap = soft_cap > 0.f ? std::min(1.f / a.cap, FLT_MAX) : 0.f;
   a.workers = 0;
   a.tiny = false;
   a.least = 1;
