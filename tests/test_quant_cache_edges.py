@@ -1,9 +1,12 @@
 """The 8-bit paged cache at the edges of what it accepts, against the formulas and
 by the tolerances of test_quant_cache."""
+import ctypes
+
 import pytest
 import torch
 
 from test_quant_cache import E4M3, INT8, _near, _plain, _random_pool, _table
+from vortex_torch import _hip
 from vortex_torch.decode_attention import quant_paged_decode_attention
 
 
@@ -47,3 +50,33 @@ def test_small_caps(gpu, dtype, cap):
     want, _ = _plain(q, kc, vc, sc, indptr, indices, last, 2, H, cap=cap)
     _, off = _plain(q * 0, kc, vc, sc, indptr, indices, last, 2, H)
     _near(got, want, off + 2.0 ** -19 * cap)
+
+
+# ---------------------------------------------------------- malformed tables
+@pytest.mark.gpu
+def test_overlapping_segments_of_more_parts_than_32_bits_count(gpu):
+    """20,000 segments of which every other one is the whole table, 2^25 pages in 2^19
+    parts each: nothing is written but the outputs and the workspace."""
+    S, D, P, pages = 20000, 64, 16, 1 << 25
+    lib = _hip.load_library()
+    kc, vc, sc = _random_pool(1, P, D, INT8, torch.Generator().manual_seed(1), gpu)
+    indices = torch.zeros(pages, dtype=torch.int32, device=gpu)
+    indptr = torch.zeros(S + 1, dtype=torch.int32, device=gpu)
+    indptr[1::2] = pages
+    indptr[S] = 1
+    last = torch.full((S,), P, dtype=torch.int32, device=gpu)
+    q = torch.randn((S, D), generator=torch.Generator().manual_seed(2)).bfloat16().to(gpu)
+    need = lib.vtx_quant_decode_attention_workspace_len(S, 1, 1, D, P, 0, 0, pages)
+    assert need > 0
+    room = 1 << 20
+    ws = torch.full((need + 2 * room,), 7.0, device=gpu)
+    out = torch.full((S * D + 2 * room,), 7.0, dtype=torch.bfloat16, device=gpu)
+    rc = lib.vtx_quant_decode_attention(
+        q.data_ptr(), (ctypes.c_int64 * 3)(D, D, D), out[room:].data_ptr(), kc.data_ptr(), vc.data_ptr(),
+        sc.data_ptr(), 1, indptr.data_ptr(), indices.data_ptr(), pages, last.data_ptr(), S, 1, 1, D, P, 0,
+        _hip.CODES_INT8, D ** -0.5, 0.0, 0, None, 0, ws[room:].data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    for t in (ws, out):
+        assert bool((t[:room] == 7).all()) and bool((t[-room:] == 7).all())
+    assert int(out[room:-room].view(S, D)[1:-1:2].count_nonzero()) == 0  # segments without pages

@@ -181,6 +181,11 @@ __device__ __forceinline__ Place place_of(const Segment& g, uint32_t at, uint32_
 __device__ __forceinline__ uint32_t parts_at(const QAttnArgs& a, int s, uint32_t chunk) {
   return parts_of(segment_of(a, a.indptr[s], a.indptr[s + 1], a.last_len[s]).pages, chunk);
 }
+// A thread's sum of parts, held below kMostParts, which is more than there are rows
+// for (ranges_of: a few thousand): in a table that decreases segments overlap, their
+// parts are any number, and 32 bits of a workgroup's sum are to hold it all the same.
+constexpr uint32_t kMostParts = 1u << 22;
+__device__ __forceinline__ uint32_t add_parts(uint32_t sum, uint32_t n) { return min(sum + n, kMostParts); }
 // The parts of the cut segments before segment s.  Every thread of the workgroup
 // calls it; sums: LDS, an entry per wave.
 template <int T>
@@ -188,7 +193,7 @@ __device__ __forceinline__ uint32_t parts_before(const QAttnArgs& a, int s, uint
   uint32_t mine = 0;
   for (int j = threadIdx.x; j < s; j += T) {
     const uint32_t n = parts_at(a, j, chunk);
-    mine += n > 1u ? n : 0u;
+    mine = add_parts(mine, n > 1u ? n : 0u);
   }
   mine = vtx::wave_sum(mine);
   if (vtx::lane_id() == 0) sums[threadIdx.x / vtx::kWave] = __uint_as_float(mine);
@@ -565,7 +570,7 @@ __global__ __launch_bounds__(kWaves* vtx::kWave, kPerCu<kD>) void quant_attentio
         uint32_t mine = 0, cut = 0;  // such parts of this thread's segments, and how many segments have them
         for (int j = j0; j < j1; ++j) {
           const uint32_t n = parts_at(a, j, chunk);
-          mine += n - 1u;
+          mine = add_parts(mine, n - 1u);
           cut += n > 1u ? 1u : 0u;
         }
         uint32_t before = vtx::wave_prefix_sum(mine) - mine, rows = vtx::wave_prefix_sum(cut) - cut, all = 0;
