@@ -80,3 +80,13 @@ def test_overlapping_segments_of_more_parts_than_32_bits_count(gpu):
     for t in (ws, out):
         assert bool((t[:room] == 7).all()) and bool((t[-room:] == 7).all())
     assert int(out[room:-room].view(S, D)[1:-1:2].count_nonzero()) == 0  # segments without pages
+
+
+def test_reductions_refuse_heads_whose_tiles_pass_an_int():
+    """256 pages of a block times the heads, and a round of the workgroups more."""
+    lib, p = _hip.load_library(), [0x10000 * (i + 1) for i in range(4)]
+    for heads in ((1 << 31) // 256 - 1, (1 << 31) // 256 - 4):
+        assert lib.vtx_page_reduce_quant(p[0], p[1], 1 << 31, 1, 1, _hip.CODES_INT8, 1, (ctypes.c_void_p * 1)(p[2]),
+                                         (ctypes.c_int32 * 1)(0), (ctypes.c_int32 * 1)(_hip.REDUCE_MEAN), 1 << 31, p[3],
+                                         256, heads, None) == -1
+        assert b"too many heads" in lib.vtx_last_error()

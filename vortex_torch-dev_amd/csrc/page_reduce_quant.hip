@@ -26,7 +26,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / vtx::kWave;
-constexpr int kMaxShare = 16;  // workgroups that share one block of entries
+constexpr int kMaxShare = 16;  // workgroups that share one block of entries; of few blocks twice as many
+constexpr int kMostAtOnce = 2 * kMaxShare * kWaves * 8;  // tiles of them at a time, 8 of a wave
 using vtx::Acc;
 
 struct PageArgs {
@@ -240,7 +241,8 @@ extern "C" int vtx_page_reduce_quant(const void* x, const void* scales, int64_t 
     return vtx::fail(VTX_E_INVALID, "page_reduce_quant: bad sizes");
   if (codes != VTX_CODES_E4M3 && codes != VTX_CODES_INT8)
     return vtx::fail(VTX_E_INVALID, "page_reduce_quant: unknown codes %d", codes);
-  if (num_kv_heads > 0x7fffffff / kThreads) return vtx::fail(VTX_E_INVALID, "page_reduce_quant: too many heads");
+  // (a block's tiles, and a round of its workgroups past them, are counted in an int)
+  if (num_kv_heads > (0x7fffffff - kMostAtOnce) / kThreads) return vtx::fail(VTX_E_INVALID, "page_reduce_quant: too many heads");
   PageArgs a;
   bool aligned = reinterpret_cast<uintptr_t>(x) % 8 == 0;
   int need = 0;
