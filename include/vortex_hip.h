@@ -803,7 +803,9 @@ int vtx_read_kv_buffer_quant(const void* k_cache, const void* v_cache, const voi
  * vtx_page_reduce_multi, dim 1, over a pool of codes: x [x_rows, page_size, cols],
  * its bytes scales[(row * page_size + slot) * 2] (pass scales + 1 for V's).  The
  * outputs are those of the same reductions of a bf16 pool that holds the values,
- * bit for bit where cols is 64, 128, 256 or 512 (else the sums' order may differ).
+ * bit for bit where cols is 64, 128, 256 or 512 (else the sums' order may differ),
+ * but for values that are NaN: every output that sees one is NaN, MAX and MIN too
+ * (vtx_page_reduce_multi's pass it by), so that a page's bounds hold or are none.
  */
 int vtx_page_reduce_quant(const void* x, const void* scales, int64_t x_rows, int32_t page_size, int32_t cols,
                           int32_t codes, int32_t n_out, void* const* outs, const int32_t* out_dtypes,

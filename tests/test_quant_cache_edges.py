@@ -1,12 +1,14 @@
 """The 8-bit paged cache at the edges of what it accepts, against the formulas and
 by the tolerances of test_quant_cache."""
 import ctypes
+import math
 
 import pytest
 import torch
 
-from test_quant_cache import E4M3, INT8, _near, _plain, _random_pool, _table
+from test_quant_cache import CODES, E4M3, INT8, _near, _plain, _random_pool, _table
 from vortex_torch import _hip
+from vortex_torch.cache import set_kv_buffer_quant
 from vortex_torch.decode_attention import quant_paged_decode_attention
 
 
@@ -90,3 +92,41 @@ def test_reductions_refuse_heads_whose_tiles_pass_an_int():
                                          (ctypes.c_int32 * 1)(0), (ctypes.c_int32 * 1)(_hip.REDUCE_MEAN), 1 << 31, p[3],
                                          256, heads, None) == -1
         assert b"too many heads" in lib.vtx_last_error()
+
+
+# --------------------------------------------------- rows that are no numbers
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", CODES, ids=str)
+@pytest.mark.parametrize("H,P,D,pages", [(2, 16, 128, 9), (2, 16, 64, 9), (1, 64, 256, 5), (2, 33, 512, 5),
+                                         (3, 5, 128, 9), (2, 16, 80, 9), (1, 7, 3, 9), (8, 16, 128, 700),
+                                         (8, 16, 64, 2100)])
+def test_page_reductions_of_rows_that_are_no_numbers(gpu, H, P, D, pages, codes):
+    """Every statistic of a page with such a row is NaN, the extremes among them,
+    and of every other page what it was; a NaN code is one of its column."""
+    gen = torch.Generator().manual_seed(D)
+    kc, vc, sc = _random_pool(pages * H, P, D, codes, gen, gpu)
+    loc = torch.arange(pages * P, device=gpu)
+    types = [_hip.REDUCE_MEAN, _hip.REDUCE_MAX, _hip.REDUCE_MIN, _hip.REDUCE_L2NORM]
+
+    def reduce(kinds):
+        outs = [torch.zeros((pages * H, 1, D), dtype=torch.bfloat16, device=gpu) for _ in kinds]
+        _hip.page_reduce_quant(kc, sc, False, outs, kinds, loc, H, P, 1)
+        return outs
+
+    sets = [[t] for t in types] + [[_hip.REDUCE_MAX, _hip.REDUCE_MIN], types]
+    before = [reduce(kinds) for kinds in sets]
+    x = torch.randn((3, H, D), generator=gen).to(gpu)
+    x[0, 0, 0], x[1, H - 1, D - 1], x[2, 0, D // 2] = math.inf, math.nan, -math.inf
+    # the first, a middle and the last token of three pages
+    set_kv_buffer_quant(kc, vc, sc, x, x, torch.tensor([0, P + P // 2, 3 * P - 1], device=gpu), P)
+    bad = torch.zeros((pages * H, 1, D), dtype=torch.bool, device=gpu)
+    bad[[0, 2 * H - 1, 2 * H]] = True
+    if codes == E4M3:
+        kc.view(torch.uint8)[4 * H, P // 3, 1] = 0x7F
+        bad[4 * H, 0, 1] = True
+    keep = torch.ones(pages * H, dtype=torch.bool, device=gpu)
+    keep[:3 * H], keep[4 * H] = False, codes != E4M3
+    for kinds, old in zip(sets, before):
+        for got, was in zip(reduce(kinds), old):
+            assert torch.equal(got.isnan(), bad), kinds
+            assert torch.equal(got[keep], was[keep])

@@ -5,9 +5,11 @@
 // bf16.  Codes times a power of two are bf16 values, and the rows are taken in
 // page_reduce.hip's order, so the outputs are bit for bit those of the same
 // reduction over a bf16 pool that holds the values (e4m3 values under 2^-130 have
-// bits that bf16 has not; they are added as they are).
+// bits that bf16 has not; they are added as they are) - but where rows are no numbers:
+// Max and Min, which there pass a NaN by, are NaN, since a row with an infinity is held
+// as NaN here, and a bound that left it out would not bound the page.
 //
-// Bound by HBM for a burst of pages (16,384 pages of 8 heads, Max + Min, 76 us, 4.5
+// Bound by HBM for a burst of pages (16,384 pages of 8 heads, Max + Min, 71 us, 4.8
 // TB/s), by the launch and two dependent loads (loc, codes) for a decode step (64
 // requests 3.5 us).  As there, a workgroup scans 256 loc entries and keeps the
 // pages they close, and several share a block's tiles.  Few tiles: a wave takes one
@@ -76,10 +78,10 @@ __device__ __forceinline__ void add8(Acc (&acc)[8], const uint2& w, uint32_t byt
   float f[4];
   vtx::decode4<kCodes>(w.x, f);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) vtx::acc_add_if<NEED>(acc[e], f[e] * s, in);
+  for (int e = 0; e < 4; ++e) vtx::acc_add_if<NEED | vtx::kKeepNan>(acc[e], f[e] * s, in);
   vtx::decode4<kCodes>(w.y, f);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) vtx::acc_add_if<NEED>(acc[4 + e], f[e] * s, in);
+  for (int e = 0; e < 4; ++e) vtx::acc_add_if<NEED | vtx::kKeepNan>(acc[4 + e], f[e] * s, in);
 }
 
 // Row groups kG0 .. kG0 + kN - 1 (group g: rows g, g + G, ..., in order) of a lane's
@@ -96,7 +98,7 @@ __device__ __forceinline__ void fold_groups(const uint2 (&w)[16], const uint32_t
     fold_groups<kCodes, G, kG0, kN / 2, NEED>(w, b, R, lower);
     fold_groups<kCodes, G, kG0 + kN / 2, kN / 2, NEED>(w, b, R, s);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) vtx::acc_fold<NEED>(lower[e], s[e]);
+    for (int e = 0; e < 8; ++e) vtx::acc_fold<NEED | vtx::kKeepNan>(lower[e], s[e]);
   }
 }
 
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void reduce_quant_kernel(PageArgs a) {
 #pragma unroll
       for (int d = LPR; d < vtx::kWave; d <<= 1)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) vtx::acc_merge_xor<NEED>(acc[e], d);
+        for (int e = 0; e < 8; ++e) vtx::acc_merge_xor<NEED | vtx::kKeepNan>(acc[e], d);
       if (grp == 0) vtx::tile_store_vec(a.r, row, cv, acc);
     }
   }
@@ -172,7 +174,7 @@ __global__ __launch_bounds__(kThreads) void reduce_quant_any_kernel(PageArgs a) 
       for (int r = 0; r < R; ++r) {
         float f[4];
         vtx::decode4<kCodes>(a.codes[(row * R + r) * C + c], f);
-        vtx::acc_add(acc, f[0] * vtx::factor(a.scales[(row * R + r) * 2]));
+        vtx::acc_add<vtx::kNeedAll | vtx::kKeepNan>(acc, f[0] * vtx::factor(a.scales[(row * R + r) * 2]));
       }
 #pragma unroll
       for (int o = 0; o < vtx::kPageReduceMaxOut; ++o)
@@ -242,7 +244,8 @@ extern "C" int vtx_page_reduce_quant(const void* x, const void* scales, int64_t 
   if (codes != VTX_CODES_E4M3 && codes != VTX_CODES_INT8)
     return vtx::fail(VTX_E_INVALID, "page_reduce_quant: unknown codes %d", codes);
   // (a block's tiles, and a round of its workgroups past them, are counted in an int)
-  if (num_kv_heads > (0x7fffffff - kMostAtOnce) / kThreads) return vtx::fail(VTX_E_INVALID, "page_reduce_quant: too many heads");
+  if (num_kv_heads > (0x7fffffff - kMostAtOnce) / kThreads)
+    return vtx::fail(VTX_E_INVALID, "page_reduce_quant: too many heads");
   PageArgs a;
   bool aligned = reinterpret_cast<uintptr_t>(x) % 8 == 0;
   int need = 0;

@@ -34,12 +34,26 @@ struct Acc {
 // Statistics a launch needs (bit mask): only these are accumulated and
 // folded across lanes.
 constexpr int kNeedSum = 1, kNeedMax = 2, kNeedMin = 4, kNeedSq = 8, kNeedAll = 15;
+// With this bit a NaN is the largest and the smallest value that there can be, as it
+// is part of every sum; without it Max and Min pass it by.
+constexpr int kKeepNan = 16;
 
 __host__ __device__ constexpr int need_of(int type) {
   return type == VTX_REDUCE_MEAN ? kNeedSum
          : type == VTX_REDUCE_MAX ? kNeedMax
          : type == VTX_REDUCE_MIN ? kNeedMin
                                   : kNeedSq;
+}
+
+template <int NEED>
+__device__ __forceinline__ float larger(float a, float b) {
+  if constexpr ((NEED & kKeepNan) != 0) return __builtin_elementwise_maximum(a, b);
+  else return fmaxf(a, b);
+}
+template <int NEED>
+__device__ __forceinline__ float smaller(float a, float b) {
+  if constexpr ((NEED & kKeepNan) != 0) return __builtin_elementwise_minimum(a, b);
+  else return fminf(a, b);
 }
 
 template <int NEED = kNeedAll>
@@ -53,23 +67,23 @@ template <int NEED = kNeedAll>
 __device__ __forceinline__ void acc_add(Acc& a, float v) {
   if constexpr ((NEED & kNeedSum) != 0) a.sum += v;
   if constexpr ((NEED & kNeedSq) != 0) a.sq = fmaf(v, v, a.sq);
-  if constexpr ((NEED & kNeedMax) != 0) a.mx = fmaxf(a.mx, v);
-  if constexpr ((NEED & kNeedMin) != 0) a.mn = fminf(a.mn, v);
+  if constexpr ((NEED & kNeedMax) != 0) a.mx = larger<NEED>(a.mx, v);
+  if constexpr ((NEED & kNeedMin) != 0) a.mn = smaller<NEED>(a.mn, v);
 }
 // acc_add when `in`, else the accumulator unchanged (bit for bit)
 template <int NEED = kNeedAll>
 __device__ __forceinline__ void acc_add_if(Acc& a, float v, bool in) {
   if constexpr ((NEED & kNeedSum) != 0) a.sum = in ? a.sum + v : a.sum;
   if constexpr ((NEED & kNeedSq) != 0) a.sq = in ? fmaf(v, v, a.sq) : a.sq;
-  if constexpr ((NEED & kNeedMax) != 0) a.mx = in ? fmaxf(a.mx, v) : a.mx;
-  if constexpr ((NEED & kNeedMin) != 0) a.mn = in ? fminf(a.mn, v) : a.mn;
+  if constexpr ((NEED & kNeedMax) != 0) a.mx = in ? larger<NEED>(a.mx, v) : a.mx;
+  if constexpr ((NEED & kNeedMin) != 0) a.mn = in ? smaller<NEED>(a.mn, v) : a.mn;
 }
 template <int NEED = kNeedAll>
 __device__ __forceinline__ void acc_merge_xor(Acc& a, int d) {
   if constexpr ((NEED & kNeedSum) != 0) a.sum += xshfl(a.sum, d);
   if constexpr ((NEED & kNeedSq) != 0) a.sq += xshfl(a.sq, d);
-  if constexpr ((NEED & kNeedMax) != 0) a.mx = fmaxf(a.mx, xshfl(a.mx, d));
-  if constexpr ((NEED & kNeedMin) != 0) a.mn = fminf(a.mn, xshfl(a.mn, d));
+  if constexpr ((NEED & kNeedMax) != 0) a.mx = larger<NEED>(a.mx, xshfl(a.mx, d));
+  if constexpr ((NEED & kNeedMin) != 0) a.mn = smaller<NEED>(a.mn, xshfl(a.mn, d));
 }
 // Final value of reduction `type` over `count` elements, rounded to bf16 bits.
 __device__ __forceinline__ uint32_t acc_value(const Acc& a, int type, int count) {
@@ -167,8 +181,8 @@ template <int NEED>
 __device__ __forceinline__ void acc_fold(const Acc& lower, Acc& higher) {
   if constexpr ((NEED & kNeedSum) != 0) higher.sum = lower.sum + higher.sum;
   if constexpr ((NEED & kNeedSq) != 0) higher.sq = lower.sq + higher.sq;
-  if constexpr ((NEED & kNeedMax) != 0) higher.mx = fmaxf(lower.mx, higher.mx);
-  if constexpr ((NEED & kNeedMin) != 0) higher.mn = fminf(lower.mn, higher.mn);
+  if constexpr ((NEED & kNeedMax) != 0) higher.mx = larger<NEED>(lower.mx, higher.mx);
+  if constexpr ((NEED & kNeedMin) != 0) higher.mn = smaller<NEED>(lower.mn, higher.mn);
 }
 
 // Statistics of row groups kG0 .. kG0 + kN - 1 (group g: rows g, g + G,

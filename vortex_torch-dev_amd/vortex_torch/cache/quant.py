@@ -50,7 +50,8 @@ def quantized_pool(codes: torch.Tensor, kv_scales: torch.Tensor, values: bool = 
     """``codes`` (a pool of keys; of values with ``values``) as a PAGED vTensor
     that ``cache.Mean`` / ``Max`` / ``Min`` / ``L2Norm`` / ``MultiReduce`` (dim 1)
     reduce with its factors: a flow's ``cache["k"]``, for example.  Nothing is
-    copied; the results are those of a bf16 pool of the same values."""
+    copied; the results are those of a bf16 pool of the same values, but that a row
+    which is no number makes its page's Max and Min NaN as well."""
     wrong = _hip._quant_pools_refusal(_hip._plain(codes), _hip._plain(codes), _hip._plain(kv_scales))
     if wrong:
         raise RuntimeError("vortex_torch: " + wrong.replace("k_cache and v_cache", "codes").replace("k_cache", "codes"))
