@@ -54,6 +54,31 @@ def test_small_caps(gpu, dtype, cap):
     _near(got, want, off + 2.0 ** -19 * cap)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,P", [(64, 16), (128, 5), (256, 32)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_an_infinite_query_under_a_cap(gpu, dtype, D, P):
+    """Its scores are infinities by the keys' signs, which a cap makes +-cap."""
+    H, G, n, cap = 1, 2, 200, 3.0
+    gen = torch.Generator().manual_seed(D)
+    indptr, indices, last, pages = _table([n], P, H, 3)
+    kc, vc, sc = _random_pool(pages * H, P, D, INT8, gen, gpu)
+    kc[kc == 0] = 1
+    q = torch.randn((1, G, D), generator=gen).to(dtype).to(gpu)
+    q[0, :, 7] = torch.tensor([math.inf, -math.inf])
+    got = quant_paged_decode_attention(q, kc, vc, sc, *(t.to(gpu) for t in (indptr, indices, last)), 1, H,
+                                       logits_soft_cap=cap)
+    at = indices.long()[torch.arange(n) // P] * P + torch.arange(n) % P
+    sign = kc.view(-1, D).cpu()[at, 7].double().sign()
+    v = vc.view(-1, D).cpu()[at].double() * torch.exp2(sc.view(-1, 2).cpu()[at, 1].double() - 127)[:, None]
+    p = torch.softmax(torch.stack([sign, -sign]) * cap, -1)
+    # +-cap is exact to 2^-20 of it; the weights' and the sums' errors as ever
+    off = (2 * math.expm1(2.0 ** -20 * cap + 2.0 ** -22) + 2.0 ** -16 + n * 2.0 ** -24) * (p @ v.abs())
+    _near(got, p @ v, off)
+    got = quant_paged_decode_attention(q, kc, vc, sc, *(t.to(gpu) for t in (indptr, indices, last)), 1, H)
+    assert bool(got.isnan().all())
+
+
 # ---------------------------------------------------------- malformed tables
 @pytest.mark.gpu
 def test_overlapping_segments_of_more_parts_than_32_bits_count(gpu):

@@ -774,8 +774,11 @@ __global__ __launch_bounds__(kWaves* vtx::kWave, kPerCu<kD>) void quant_attentio
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float u = (float)f[2 * e], v = (float)f[2 * e + 1];
+          // (under a cap an infinity leaves nothing, so that its scores become +-cap;
+          // without one they are no weights, and its NaN says so)
           x[e] = vtx::bf16_pair(u, v);
-          y[e] = vtx::bf16_pair(u - vtx::bf16_lo(x[e]), v - vtx::bf16_hi(x[e]));
+          y[e] = vtx::bf16_pair(a.cap != 0.f && fabsf(u) == INFINITY ? 0.f : u - vtx::bf16_lo(x[e]),
+                                a.cap != 0.f && fabsf(v) == INFINITY ? 0.f : v - vtx::bf16_hi(x[e]));
         }
         sh.q[0][j][lane] = vtx::U4{x[0], x[1], x[2], x[3]};
         sh.q[1][j][lane] = vtx::U4{y[0], y[1], y[2], y[3]};
