@@ -824,6 +824,7 @@ int vtx_page_reduce_quant(const void* x, const void* scales, int64_t x_rows, int
  * same type, [B * H * G, head_dim], dense.  A segment without tokens gets zeros,
  * and so does one whose range lies outside kv_indices; entries outside the pool
  * count as no tokens.  A NaN among a segment's scores or values gives NaN.
+ * Segments have under 2^30 tokens; a longer one gets NaN, whatever the window.
  * kv_indptr is not to decrease (otherwise the results are undefined, but no access
  * leaves a buffer).
  * workspace: vtx_quant_decode_attention_workspace_len floats, 16-byte aligned, its

@@ -79,6 +79,33 @@ def test_an_infinite_query_under_a_cap(gpu, dtype, D, P):
     assert bool(got.isnan().all())
 
 
+# ------------------------------------------------------------------ lengths
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_the_longest_segments_and_longer_ones(gpu, D):
+    """Tables of one page over and over: 2^30 - 1024 tokens are attended to (weights of
+    one and values of 64, every sum exact), 2^30 give NaN, not the zeros of a segment
+    without tokens; those beside them are as ever."""
+    P, most = 1024, 1 << 20
+    kc, vc, sc = _random_pool(2, P, D, INT8, torch.Generator().manual_seed(1), gpu)
+    vc.fill_(64)
+    sc.fill_(127)
+    q = torch.zeros((3, 2, D), dtype=torch.bfloat16, device=gpu)
+    for pages, window, far in ((most, 0, True), (most, 5000, True), (most + 7, 0, True), (most - 1, 0, False)):
+        if not far and D != 64:
+            continue
+        indices = torch.ones(pages + 3, dtype=torch.int32, device=gpu)
+        indptr = torch.tensor([0, 2, 2 + pages, 3 + pages], dtype=torch.int32, device=gpu)
+        last = torch.tensor([5, P, 9], dtype=torch.int32, device=gpu)
+        for known in (None, 100):  # divided over the card, and a workgroup each
+            if known and not far:
+                continue
+            got = quant_paged_decode_attention(q, kc, vc, sc, indptr, indices, last, 3, 1, window=window,
+                                               max_tokens=known)
+            assert bool((got[[0, 2]] == 64).all())
+            assert bool(got[1].isnan().all() if far else (got[1] == 64).all())
+
+
 # ---------------------------------------------------------- malformed tables
 @pytest.mark.gpu
 def test_overlapping_segments_of_more_parts_than_32_bits_count(gpu):
@@ -98,10 +125,11 @@ def test_overlapping_segments_of_more_parts_than_32_bits_count(gpu):
     room = 1 << 20
     ws = torch.full((need + 2 * room,), 7.0, device=gpu)
     out = torch.full((S * D + 2 * room,), 7.0, dtype=torch.bfloat16, device=gpu)
+    stream = torch.cuda.current_stream().cuda_stream
     rc = lib.vtx_quant_decode_attention(
         q.data_ptr(), (ctypes.c_int64 * 3)(D, D, D), out[room:].data_ptr(), kc.data_ptr(), vc.data_ptr(),
         sc.data_ptr(), 1, indptr.data_ptr(), indices.data_ptr(), pages, last.data_ptr(), S, 1, 1, D, P, 0,
-        _hip.CODES_INT8, D ** -0.5, 0.0, 0, None, 0, ws[room:].data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        _hip.CODES_INT8, D ** -0.5, 0.0, 0, None, 0, ws[room:].data_ptr(), need, stream)
     assert rc == 0
     torch.cuda.synchronize()
     for t in (ws, out):

@@ -148,13 +148,15 @@ struct Segment {
   int start;          // of them, in the table
   int pages, tokens;  // tokens from the first of these pages on, the last page's included
   int skip;           // tokens of the first page that the window leaves out
+  bool over;          // more tokens than an int counts, with the requests past the end: none of them do
 };
 __device__ __forceinline__ Segment segment_of(const QAttnArgs& a, int p0, int p1, int last) {
-  Segment g{p0, 0, 0, 0};
+  Segment g{p0, 0, 0, 0, false};
   if (p0 >= 0 && p1 > p0 && (int64_t)p1 <= a.indices_len && a.rows > 0) {
     last = last < 0 ? 0 : (last > a.P ? a.P : last);
     const long long n = (long long)(p1 - p0 - 1) * a.P + last;
-    if (n > 0 && n < (1LL << 30)) {
+    g.over = n >= (1LL << 30);
+    if (n > 0 && !g.over) {
       g.pages = p1 - p0;
       g.tokens = (int)n;
       if (a.window > 0 && g.tokens > a.window) {
@@ -923,7 +925,7 @@ __global__ __launch_bounds__(kWaves* vtx::kWave, kPerCu<kD>) void quant_attentio
         *reinterpret_cast<float4*>(a.acc + row * kD + d) = O;
         if (d == 0) a.ml[row] = float2{M, L};
       } else {
-        const float f = inverse_sum(L);
+        const float f = cur.s.over ? NAN : inverse_sum(L);
         *reinterpret_cast<uint2*>(a.o + ((long long)cur.seg * G + g) * kD + d) =
             uint2{round2<kHalf>(O.x * f, O.y * f), round2<kHalf>(O.z * f, O.w * f)};
       }
@@ -1037,7 +1039,7 @@ __global__ __launch_bounds__(kJoinThreads) void quant_attention_join_kernel(QAtt
       O = float4{O.x * f + y.x * e, O.y * f + y.y * e, O.z * f + y.z * e, O.w * f + y.w * e};
       M = nm;
     }
-    const float f = inverse_sum(L);
+    const float f = sg.over ? NAN : inverse_sum(L);
     *reinterpret_cast<uint2*>(a.o + ((long long)seg * G + g) * kD + d) =
         uint2{round2<kHalf>(O.x * f, O.y * f), round2<kHalf>(O.z * f, O.w * f)};
   }

@@ -130,7 +130,8 @@ def quant_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache
                                  max_tokens: Optional[int] = None) -> torch.Tensor:
     """``paged_decode_attention`` over 8-bit pools and their ``kv_scales``
     (``cache.set_kv_buffer_quant``); q [B, H_q, D] or [B * H_kv, G, D], bf16 or
-    fp16, its rows dense, up to 16 query heads per kv head; returns q's type.
+    fp16, its rows dense, up to 16 query heads per kv head; returns q's type.  A
+    request of 2^30 tokens or more gets NaN.
 
     ``logits_soft_cap``: scores become cap * tanh(score / cap).  For tables in the
     tokens' order (dense ones): ``window``, only the last so many tokens count;
