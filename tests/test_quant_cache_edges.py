@@ -183,3 +183,17 @@ def test_page_reductions_of_rows_that_are_no_numbers(gpu, H, P, D, pages, codes)
         for got, was in zip(reduce(kinds), old):
             assert torch.equal(got.isnan(), bad), kinds
             assert torch.equal(got[keep], was[keep])
+
+
+# ------------------------------------------------------------- known bounds
+@pytest.mark.parametrize("segments,D,window,most", [
+    (256, 64, 0, 2048), (256, 128, 0, 2048), (256, 256, 0, 1024), (512, 128, 0, 2048), (2048, 64, 0, 2048),
+    (512, 128, 1, 2048), (512, 256, 1, 1024), (1024, 128, 1, 4096), (2048, 256, 1, 4096), (8, 128, 0, 512),
+    (8, 128, 1, 1024), (8, 256, 1, 768)])
+def test_known_bounds_up_to_which_every_segment_has_a_workgroup(segments, D, window, most):
+    """Past them the table is looked at, which needs the workspace: ragged batches of
+    longer requests are slower with a workgroup each."""
+    need = _hip.load_library().vtx_quant_decode_attention_workspace_len
+    for tokens, divided in ((most, False), (most + 1, True)):
+        asked = (tokens, 0) if window else (0, tokens)
+        assert (need(segments, 1, 2, D, 16, *asked, 1 << 20) > 0) == divided

@@ -1073,11 +1073,29 @@ int launch_types(const QAttnArgs& a, int codes, bool half, hipStream_t s) {
 // Segments of up to `few` tokens, by the buffer's size if all heads of a request
 // are alike: ranges / segments, 8 segments of 128 columns, 128 tokens 9.0 / 6.1 us,
 // 512 10.9 / 10.3, 768 11.1 / 13.1; 64 columns, 512 10.2 / 8.6, 768 10.4 / 10.7; 256
-// columns, 256 12.0 / 9.2, 512 12.3 / 13.3.  Known bounds: segments that fill the
-// card even out by themselves (512 of 128 columns, windows of 512 29 / 19, of 4096
-// 92 / 89; 256 of 2048 36 / 33, of 4096 52 / 57), and with a window the line costs
-// more to lay out (128 of 1024 22 / 19, of 2048 27 / 30; 256 columns, 64 of 768 22 /
-// 20, of 1024 22 / 24).
+// columns, 256 12.0 / 9.2, 512 12.3 / 13.3.
+//
+// Known bounds, of fewer segments than compute units: with a window the line costs
+// more to lay out (128 of 1024 22 / 19, of 2048 27 / 30; 256 columns, 64 of 768 22 / 20,
+// of 1024 22 / 24).  Of more, which fill the card by themselves, it depends on the
+// table.  Ranges / segments, all equal; between an eighth of the bound and it; anything
+// under it; one in eight as long, the others a sixteenth:
+//   128 columns, 256 of 1024  21 / 18, 24 / 17, 39 / 15, 18 / 16
+//                256 of 2048  33 / 31, 31 / 29, 56 / 28, 18 / 27
+//                512 of 2048  52 / 50, 49 / 42, 39 / 40, 36 / 38
+//                512 of 4096  95 / 93, 68 / 76, 93 / 73, 39 / 71
+//               1024 of 4096  184 / 181, 114 / 150, 121 / 124, 69 / 105
+//   64 columns,  512 of 2048  34 / 30, 30 / 27, 62 / 27, 25 / 27
+//                512 of 4096  57 / 54, 41 / 49, 71 / 48, 28 / 48
+//   256 columns, 512 of 1024  50 / 47, 41 / 39, 38 / 36, 39 / 36
+//                512 of 2048  90 / 88, 65 / 73, 71 / 66, 62 / 66
+//                320 of 2048  64 / 77, 47 / 65, 46 / 62, 42 / 65
+// (ranges lose where a few requests of a page or two share one, whose segments a
+// workgroup takes one by one, segments where a few long ones come last).  So up to 2048
+// tokens, or 1024 of 256 columns, where segments lose less than ranges would; past that
+// divide_pages looks at the table.  With windows of a spaced line, whose places are all
+// alike, that comes to segments as well, and the second launch on top (1024 of 4096 183
+// / 180, 126 / 124): up to 4096.
 //
 // Tiny segments, more than workgroups that the card holds: a wave each, since four
 // share a tile or two and then wait for each other (by the longest they can have or,
@@ -1097,10 +1115,9 @@ Ranges ranges_of(long long segments, int32_t num_kv_heads, int32_t head_dim, int
   r.cus = vtx::device_cu_count() > 0 ? vtx::device_cu_count() : 256;
   const long long few = 640 - head_dim;
   const long long known = longest > 0 && (window == 0 || longest < window) ? longest : window;
-  const long long most = segments >= 2 * r.cus ? 4096
-                         : segments >= r.cus   ? 2048
-                         : window > 0          ? (head_dim == 256 ? 768 : 1024)
-                                               : few;
+  const long long most = segments < r.cus ? (window == 0 ? few : (head_dim == 256 ? 768 : 1024))
+                         : window > 0 && segments >= kBounds ? 4096
+                                                             : (head_dim == 256 ? 1024 : 2048);
   const int per_cu = head_dim == 256 ? kPerCu<256> : (head_dim == 128 ? kPerCu<128> : kPerCu<64>);
   r.tiny = page_size % 16 == 0 && segments > r.cus * per_cu &&
            ((known > 0 && known <= kTiny) || (window == 0 && indices_len * page_size <= kTiny * segments));
