@@ -2,11 +2,12 @@
 by the tolerances of test_quant_cache."""
 import ctypes
 import math
+import random
 
 import pytest
 import torch
 
-from test_quant_cache import CODES, E4M3, INT8, _near, _plain, _random_pool, _table
+from test_quant_cache import CODES, E4M3, INT8, _case, _near, _plain, _random_pool, _table
 from vortex_torch import _hip
 from vortex_torch.cache import set_kv_buffer_quant
 from vortex_torch.decode_attention import quant_paged_decode_attention
@@ -104,6 +105,45 @@ def test_the_longest_segments_and_longer_ones(gpu, D):
                                                max_tokens=known)
             assert bool((got[[0, 2]] == 64).all())
             assert bool(got[1].isnan().all() if far else (got[1] == 64).all())
+
+
+# ------------------------------------------------- windows on divided tables
+def _windowed(tokens, H, G, D, P, window, codes, dtype, device, **kw):
+    need = _hip.load_library().vtx_quant_decode_attention_workspace_len
+    entries = H * sum(-(-t // P) for t in tokens)
+    assert need(len(tokens), H, G, D, P, window, 0, entries) > 0  # (not a workgroup per segment)
+    if kw.pop("slopes", False):
+        kw["slopes"] = torch.exp2(-2.0 - torch.arange(H * G, dtype=torch.float32)).to(device)
+    _case(tokens, H, G, D, P, codes, dtype, device, seed=window, window=window, **kw)
+
+
+SCORES = [dict(), dict(slopes=True), dict(logits_soft_cap=2.0), dict(logits_soft_cap=8.0, slopes=True, sm_scale=0.2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", SCORES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("D,P,window", [(64, 16, 1500), (128, 16, 3001), (256, 32, 2050), (128, 5, 1025),
+                                        (64, 48, 5000)])
+def test_windows_on_a_packed_line(gpu, D, P, window, dtype, kw):
+    """Segments cut by ranges and by the window, whose parts have maxima of their own;
+    shorter ones and empty ones between them."""
+    _windowed([9000, 30, 0, 7001, 1, 2600, window, window + 1, 17], 2, 3, D, P, window, INT8 if D == 64 else E4M3,
+              dtype, gpu, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", SCORES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("count,D,P,window", [(600, 64, 16, 2500), (300, 256, 16, 1100), (1030, 64, 32, 4200),
+                                              (1030, 128, 5, 4500)])
+def test_windows_on_tables_of_many_segments(gpu, count, D, P, window, dtype, kw):
+    """... packed ones of under 1024 segments, spaced ones of more."""
+    r = random.Random(count)
+    tokens = [r.choice([0, 1, 16, 33, 200]) for _ in range(count)]
+    for i, n in ((0, window + 700), (3, 9000), (count // 2, window), (count - 1, 2 * window + 5)):
+        tokens[i] = n
+    _windowed(tokens, 1, 2, D, P, window, E4M3, dtype, gpu, **kw)
 
 
 # ---------------------------------------------------------- malformed tables
