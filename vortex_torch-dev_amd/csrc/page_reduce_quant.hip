@@ -287,14 +287,16 @@ extern "C" int vtx_page_reduce_quant(const void* x, const void* scales, int64_t 
   // sixteen can, and sixteen share a block while the grid is under 512
   // (page_reduce.hip has the reasons); of up to 16 blocks, decode steps, 32, so that
   // no wave takes two tiles one after the other (8 heads, sixteen / 32: 256 entries
-  // 8.0 / 5.3 us, Max + Min 10.1 / 6.3, 4096 8.7 / 6.9).
+  // 7.6 / 5.1 us, Max + Min 9.1 / 5.8, 4096 9.6 / 7.0).
   const long long tiles = (page_size < kThreads ? kThreads / page_size : 1) * (long long)num_kv_heads;
   // Several tiles of a wave at a time pay where there are more than waves to take
-  // them, earlier with two statistics, whose fold across lanes is longer, or where a
-  // block has many; 256 columns have two a wave, which gain nothing.  One at a time /
-  // several, Mean, 128 columns: 8192 tiles 8.8 / 9.7 us, 16,384 13.5 / 13.1, 131,072
-  // 79.7 / 74.1; Max + Min: 512 tiles of 8 heads 6.0 / 5.5, 1024 of one head 4.5 /
-  // 5.9, 4096 7.1 / 6.1, 131,072 124 / 78; 256 columns, Mean, 131,072 122 / 130.
+  // them, earlier with two statistics, whose fold across lanes is longer; 256 columns
+  // have two a wave, which gain nothing.  One at a time / several, Mean, 128 columns:
+  // 8192 tiles 8.8 / 9.8 us, 16,384 14.0 / 12.7, 131,072 79.5 / 74.2; Max + Min: 4096
+  // tiles 7.7 / 6.1, 131,072 108 / 72, 1024 of one head 4.4 / 5.8; 256 columns, Mean,
+  // 131,072 122 / 130.  Two statistics of 1024 entries and more, of 8 heads, which may
+  // be a burst's or a decode step's: a burst 4.2 / 5.6, of 2048 5.1 / 5.9, steps 6.7 /
+  // 5.2 and 6.8 / 5.3, so several, which are never far off.
   const int lpr = cols / 8, stats = __builtin_popcount(instance_need(need));
   const bool lanes = vec && page_size <= 16 && (lpr == 8 || lpr == 16) &&
                      vtx::lane_tiles_fit(lpr, instance_need(need)) &&

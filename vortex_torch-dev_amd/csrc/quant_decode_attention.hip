@@ -28,9 +28,9 @@
 // several has its parts joined by a second launch.
 //
 // Bound by HBM where there are many tokens (32 requests of up to 32k, 8 x 8 heads of
-// 128 columns, 212 us, 5.9 TB/s: the rate of a sequential read), by five dependent
-// trips to memory and the second launch where there are few (one request of 4096
-// tokens 12.1 us, of 128, in one launch, 6.1).
+// 128 columns, 213 us, 5.8 TB/s; a large copy, which writes half of it, reaches 4.9 to
+// 5.0), by five dependent trips to memory and the second launch where there are few
+// (one request of 4096 tokens 12.0 us, of 128, in one launch, 6.1).
 #include <algorithm>
 #include <cfloat>
 
@@ -115,7 +115,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // segments'.  Many uneven long ones stay on the line, which evens them out.
 // Line / chunks, 128 columns: 512 segments of up to 64 tokens 18.5 / 9.7 us, of up to
 // 1024 34.9 / 27.3, of up to 4096 66 / 75; 512 of 512 tokens each 21.2 / 20.0, 1024 of
-// 2048 109 / 96, 2048 of 512 62 / 56.
+// 2048 109 / 96, 2048 of 512 62 / 56.  (Where single requests of a few tokens lie among
+// long ones the line is the slower one: ranges_of has figures.)
 struct Division {
   uint32_t per;    // pages of a range
   uint32_t chunk;  // pages of a part at most; 0: ranges
