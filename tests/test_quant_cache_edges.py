@@ -17,7 +17,7 @@ from vortex_torch.decode_attention import quant_paged_decode_attention
 @pytest.mark.gpu
 @pytest.mark.parametrize("D,P", [(64, 16), (128, 5), (256, 32)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
-@pytest.mark.parametrize("cap", [1e3, 1e4, 1e5, 1e6, 1e9, 1e20, 3e38])
+@pytest.mark.parametrize("cap", [1e3, 1e4, 1e5, 1e6, 1e9, 1e20, 3e38, 1e39, 1e300])
 def test_large_caps(gpu, cap, dtype, D, P):
     """The bound follows the scores, not the cap: that of uncapped ones, whose sum of
     products is allowed D 2^-23 sum |q k|, twice what D fp32 additions are off by.  The

@@ -1675,7 +1675,7 @@ def page_reduce_quant(x, kv_scales, of_values, outs, reduce_types, loc, num_kv_h
         _check(rc, "page_reduce_quant")
 
 
-_F32_TINY = torch.finfo(torch.float32).tiny
+_F32 = torch.finfo(torch.float32)
 _QUERY_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 
 
@@ -1750,8 +1750,8 @@ def quant_paged_decode_attention(q, o, k_cache, v_cache, kv_scales, kv_indptr, k
                                                 kv_last_page_len, batch_size, num_kv_heads, sm_scale, soft_cap, window,
                                                 slopes, longest)
     B, H = batch_size, num_kv_heads
-    if 0.0 < soft_cap < _F32_TINY:  # (in fp32 it could become 0, which is no cap)
-        soft_cap = _F32_TINY
+    if 0.0 < soft_cap < math.inf:  # (in fp32 it could become 0, which is no cap, or an infinity)
+        soft_cap = min(max(soft_cap, _F32.tiny), _F32.max)
     if not _quant_attention_fits(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B, H,
                                  soft_cap, window, slopes):
         wrong = _quant_attention_refusal(q, o, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, kv_last_page_len, B,
